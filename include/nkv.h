@@ -742,6 +742,95 @@ int nkv_build_step_metadata(const int32_t* packed, int32_t n_seqs, int32_t block
                             int32_t* block_tables, int64_t bt_row_stride, int32_t bt_width,
                             void* stream);
 
+/*
+ * Pages of a paged K/V cache that sequences share: a reference count per page
+ * (0: free), a length and a block table per row (sequence), all on the
+ * device, so that taking, freeing, forking and moving pages needs no host
+ * data and can be captured in a HIP graph. An array of pointers and sizes,
+ * 8 bytes each:
+ *   kv_cache      the pool, [n_planes, n_pages, block_size, row_bytes] bytes
+ *                 (planes: K and V of every layer), 16-byte aligned; rows a
+ *                 multiple of 16 bytes
+ *   ref_counts    int32 [n_pages], 16-byte aligned
+ *   context_lens  int32 [n_rows]
+ *   block_tables  int32 [n_rows, bt_row_stride], max_blocks entries each; -1
+ *                 past a row's ceil(length / block_size) pages
+ *   workspace     nkv_pages_workspace_bytes(n_pages) bytes, 16-byte aligned
+ * At most 8192 rows, 8192 entries in a list, 2^20 pages; slots and lengths fit
+ * 32 bits. A row's last page, where it is filled in part, belongs to that row
+ * alone: the calls keep it so, and appended tokens never land in a page that
+ * another row holds. Code that writes rows in place (the compression step)
+ * needs pages of the sequence's own: fork it with share_pages = 0.
+ *
+ * Lists are taken as the state before the call has it. An entry of -1 is
+ * padding; a row named twice counts where it is named first. Pages are taken
+ * lowest first, in the list's order: an entry is granted if the pages of all
+ * entries up to it are free before the call, else it is refused and changes
+ * nothing. status[i] is 1 for an entry that was carried out, else 0. Calls on
+ * the same pages must be ordered on a stream.
+ *
+ * Replaces: BlockManager's bookkeeping (nanokvllm/engine/block_manager.py:
+ *           13-138) for callers that keep it on the device; forks, moves and
+ *           copies of pages have no counterpart there.
+ */
+typedef struct nkv_pages {
+  void* kv_cache;
+  int64_t n_planes, n_pages, block_size, row_bytes;
+  int32_t *ref_counts, *context_lens, *block_tables;
+  int64_t bt_row_stride, max_blocks, n_rows;
+  void* workspace;
+  int64_t workspace_bytes;
+} nkv_pages;
+size_t nkv_pages_workspace_bytes(int64_t n_pages);
+
+/*
+ * New tokens for n rows: one each (cu_seqlens_q NULL, n_tokens = n), or
+ * cu_seqlens_q[i+1] - cu_seqlens_q[i] for row rows[i] (int32 [n+1], from >= 0,
+ * nondecreasing, up to n_tokens; every entry is refused otherwise). Rows get the
+ * pages they need and their new lengths; slot_mapping[t] (int32 [n_tokens]) the
+ * slot of every new token, in the list's order, -1 for those of refused
+ * entries and outside cu_seqlens_q. An entry past max_blocks pages is refused.
+ * Replaces: BlockManager.allocate / may_append (block_manager.py:52-113) and
+ *           the slots of prepare_step (model_runner.py:160-219).
+ */
+int nkv_pages_append(const nkv_pages* pages, const int32_t* rows, int32_t n,
+                     const int32_t* cu_seqlens_q, int64_t n_tokens, int32_t* slot_mapping,
+                     int32_t* status, void* stream);
+
+/*
+ * Row rows[i] keeps its first keep_lens[i] tokens (0: the sequence is freed;
+ * more than it has, or fewer than 0: refused). Pages behind them lose a
+ * reference and the table entries become -1. A page that stays in part while
+ * other rows hold it too (its count before the call is above 1) is replaced by
+ * a copy of its kept rows in a free page. Then every page of page_ids (int32
+ * [n_page_ids], -1: none) loses a reference, as for the pages that a compression
+ * step's events list. Counts do not go below 0.
+ * Replaces: BlockManager.deallocate / truncate_blocks (block_manager.py:82-92,
+ *           117-138).
+ */
+int nkv_pages_truncate(const nkv_pages* pages, const int32_t* rows, const int32_t* keep_lens,
+                       int32_t n, const int32_t* page_ids, int64_t n_page_ids, int32_t* status,
+                       void* stream);
+
+/*
+ * Row children[i], which must be empty, becomes a copy of row parents[i]. Its
+ * full pages are the parent's (one more reference each) and the one filled in
+ * part is copied; with share_pages = 0 all pages are copied. A child whose
+ * parent is empty stays empty. No counterpart in the reference.
+ */
+int nkv_pages_fork(const nkv_pages* pages, const int32_t* parents, const int32_t* children,
+                   int32_t n, int32_t share_pages, int32_t* status, void* stream);
+
+/*
+ * Moves pages in use to the pool's lower end: with n_live pages in use, the
+ * k-th lowest free page below n_live takes the k-th highest page in use, for
+ * the first max_moves of them; all tables and counts follow. info[0] = n_live,
+ * info[1] = the moves made; moves (int32 [max_moves, 2], 8-byte aligned) lists
+ * them as (from, to), padded with -1. No counterpart in the reference.
+ */
+int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info, int32_t* moves,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

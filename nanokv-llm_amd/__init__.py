@@ -5,6 +5,7 @@ Host side in Python on PyTorch-ROCm; all compute in libnkv_amd.so
 directory name is not a Python identifier; import it with
 ``importlib.import_module("nanokv-llm_amd")``.
 """
+from .engine.pages import PagedSequences
 from .layers.attention import (Attention, paged_decode, release_retired_decode_workspaces,
                                reserve_decode_workspace, store_kvcache, varlen_prefill)
 from .layers.compress_utils import MyCompressCompact
@@ -17,5 +18,5 @@ __all__ = [
     "release_retired_decode_workspaces", "varlen_prefill",
     "MyCompressCompact",
     "SnapKV", "Context", "get_context", "set_context", "reset_context", "RotaryEmbedding",
-    "get_rope", "qk_norm_rope_store",
+    "get_rope", "qk_norm_rope_store", "PagedSequences",
 ]

@@ -10,6 +10,7 @@ library binds to; the streams handed over are torch's own.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -125,6 +126,12 @@ SIGNATURES = {
                                         _p, _p]),
     "nkv_build_step_metadata": (C.c_int, [_p, _i32, _i32, _i32, _i64, _i32, _p, _i64, _i32, _i32,
                                           _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _p]),
+    # the first argument: a packed nkv_pages
+    "nkv_pages_workspace_bytes": (_sz, [_i64]),
+    "nkv_pages_append": (C.c_int, [C.c_char_p, _p, _i32, _p, _i64, _p, _p, _p]),
+    "nkv_pages_truncate": (C.c_int, [C.c_char_p, _p, _p, _i32, _p, _i64, _p, _p]),
+    "nkv_pages_fork": (C.c_int, [C.c_char_p, _p, _p, _i32, _i32, _p, _p]),
+    "nkv_pages_compact": (C.c_int, [C.c_char_p, _i32, _p, _p, _p]),
 }
 
 _LIB = None
@@ -195,6 +202,15 @@ def need(cond: bool, msg: str) -> None:
     """Argument check that survives ``python -O``: raises ValueError(msg)."""
     if not cond:
         raise ValueError(msg)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def device_of(index: int):
+    """A context in which device ``index`` is the current one: the library takes launch sizes from
+    the current device, and a null stream belongs to it."""
+    return _SAME_DEVICE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def stream_of(t: torch.Tensor) -> int:

@@ -1,0 +1,323 @@
+"""PagedSequences against the sequential oracle: state, statuses, slots and every copied byte.
+
+All outputs are whole numbers or copied rows, so every comparison is for equality.
+"""
+import importlib
+import random
+
+import pytest
+import torch
+
+from oracle.attention_ref import paged_decode_ref
+from oracle.pages_ref import PagedSequencesRef
+
+pytestmark = pytest.mark.gpu
+
+nkv = importlib.import_module("nanokv-llm_amd")
+I32 = torch.int32
+
+
+def ints(x, dev):
+    return torch.tensor(x, dtype=I32, device=dev)
+
+
+class Pair:
+    """The operators and the oracle over equal pools; every call is made on both and compared."""
+
+    def __init__(self, dev, layers=2, pages=40, block=16, heads=2, dim=64, rows=8, width=6,
+                 dtype=torch.bfloat16, seed=0):
+        g = torch.Generator().manual_seed(seed)
+        raw = torch.randint(-100, 100, (2, layers, pages, block, heads, dim), generator=g)
+        self.bits = torch.int8 if dtype == torch.float8_e4m3fn else torch.int16
+        self.ref = PagedSequencesRef(raw.to(self.bits), rows, width)
+        self.kv = raw.to(self.bits).to(dev).view(dtype)
+        self.seqs = nkv.PagedSequences(self.kv, rows, width)
+        self.dev, self.S, self.B = dev, rows, block
+
+    def check(self, got, want):
+        assert got.cpu().tolist() == list(want)
+        assert torch.equal(self.seqs.state.cpu(), self.ref.state())
+        assert torch.equal(self.kv.view(self.bits).cpu(), self.ref.kv)
+
+    def append(self, rows, counts=None):
+        if counts is None:
+            slots, status = self.seqs.append(ints(rows, self.dev))
+            want_slots, want = self.ref.append(rows)
+        else:
+            cu = [0]
+            for c in counts:
+                cu.append(cu[-1] + c)
+            return self.append_cu(rows, cu, cu[-1])
+        assert slots.cpu().tolist() == want_slots
+        self.check(status, want)
+        return want
+
+    def append_cu(self, rows, cu, n_tokens):
+        slots, status = self.seqs.append(ints(rows, self.dev), ints(cu, self.dev), n_tokens)
+        want_slots, want = self.ref.append(rows, cu=cu, n_tokens=n_tokens)
+        assert slots.cpu().tolist() == want_slots
+        self.check(status, want)
+        return want
+
+    def truncate(self, rows, lens, pages=None):
+        got = self.seqs.truncate(ints(rows, self.dev), ints(lens, self.dev),
+                                 None if pages is None else ints(pages, self.dev))
+        want = self.ref.truncate(rows, lens, pages or ())
+        self.check(got, want)
+        return want
+
+    def fork(self, parents, children, share=True):
+        got = self.seqs.fork(ints(parents, self.dev), ints(children, self.dev), share)
+        want = self.ref.fork(parents, children, share)
+        self.check(got, want)
+        return want
+
+    def compact(self, max_moves):
+        info, moves = self.seqs.compact(max_moves)
+        want_info, want_moves = self.ref.compact(max_moves)
+        assert moves.cpu().tolist() == want_moves
+        self.check(info, want_info)
+        return want_info
+
+
+def test_append_one_token_each(dev):
+    p = Pair(dev)
+    for _ in range(40):
+        p.append(list(range(8)))
+    assert p.ref.lens == [40] * 8
+
+
+def test_append_lengths_around_a_page(dev):
+    p = Pair(dev, rows=6, width=4)
+    assert p.append([0, 1, 2, 3, 4, 5], [0, 1, 15, 16, 17, 64]) == [1] * 6
+    assert p.append([5, 4, 0], [1, 0, 3]) == [0, 1, 1]  # row 5 is at its table's width
+    assert p.append([1, 2, 3], [16, 1, 32]) == [1, 1, 1]
+
+
+def test_append_refuses_in_order_when_pages_run_out(dev):
+    p = Pair(dev, pages=5, rows=5, width=6)
+    assert p.append([0, 1, 2, 3], [32, 20, 33, 1]) == [1, 1, 0, 0]
+    assert p.append([1, 2, 0], [10, 1, 1]) == [1, 1, 0]  # row 1 has room in its page
+    assert p.append([3, 1], [0, 2]) == [1, 1]
+
+
+def test_lists_with_padding_repeats_and_rows_outside(dev):
+    p = Pair(dev)
+    assert p.append([-1, 3, 3, 8, 2, -7, 2 ** 30], [4, 5, 6, 7, 8, 1, 1]) == [0, 1, 0, 0, 1, 0, 0]
+    assert p.append([3, -1, 3]) == [1, 0, 0]
+    assert p.fork([3, 3, 2, 9, -1], [4, 4, -1, 5, 6]) == [1, 0, 0, 0, 0]
+    assert p.truncate([-1, 2, 2, 77], [0, 3, 1, 0]) == [0, 1, 0, 0]
+
+
+@pytest.mark.parametrize("cu,n_tokens", [([0, 5, 3, 9], 9), ([-1, 2, 3, 4], 9),
+                                         ([0, 2, 5, 10], 9), ([0, 0, 2 ** 30, 4], 9)])
+def test_append_refuses_cu_seqlens_out_of_order_or_range(dev, cu, n_tokens):
+    assert Pair(dev).append_cu([0, 1, 2], cu, n_tokens) == [0, 0, 0]
+
+
+def test_append_slots_outside_cu_seqlens_are_padding(dev):
+    p = Pair(dev)
+    assert p.append_cu([0, 1], [3, 5, 25], 31) == [1, 1]
+    assert p.append_cu([], [0], 7) == []
+    assert p.append([]) == []
+    assert p.append([0, 1], [0, 0]) == [1, 1]
+
+
+def test_truncate_frees_and_rolls_back(dev):
+    p = Pair(dev)
+    p.append([0, 1, 2], [50, 33, 16])
+    assert p.truncate([0, 1, 2], [51, -1, 16]) == [0, 0, 1]  # more than there is; nothing dropped
+    assert p.truncate([0, 1], [17, 32]) == [1, 1]
+    assert p.truncate([2, 0], [0, 0]) == [1, 1]
+    assert p.append([3], [60]) == [1]
+
+
+def test_truncate_inside_a_shared_page_copies_it(dev):
+    p = Pair(dev)
+    p.append([0], [40])
+    p.fork([0, 0], [1, 2])
+    assert p.truncate([1], [20]) == [1]      # its page of its own now
+    assert p.truncate([0, 2], [7, 7]) == [1, 1]  # both leave the page they share
+    p.append([0, 1, 2], [30, 30, 30])
+    p.truncate([0, 1, 2], [0, 0, 0])
+    assert sum(p.ref.refs) == 0
+
+
+def test_truncate_refuses_a_copy_without_a_free_page(dev):
+    p = Pair(dev, pages=3, rows=4)
+    p.append([0], [32])
+    p.fork([0], [1])
+    assert p.append([2]) == [1]  # the last free page
+    assert p.truncate([0, 1, 2], [20, 16, 0]) == [0, 1, 1]
+    assert p.truncate([0, 1], [20, 0]) == [1, 1]
+
+
+def test_truncate_drops_listed_pages(dev):
+    p = Pair(dev)
+    p.append([0, 1], [64, 40])
+    t = p.ref.tables
+    # freed by a compression step: listed pages, padding, one twice, one free, ids outside the pool
+    assert p.truncate([1], [3], [t[0][3], -1, t[0][3], 39, 40, -9, 2 ** 30]) == [1]
+    assert p.truncate([], [], [t[0][2]]) == []
+    p.truncate([], [], [])
+
+
+def test_fork_shares_full_pages_and_copies_the_last(dev):
+    p = Pair(dev)
+    p.append([0, 1, 2], [35, 32, 5])
+    assert p.fork([0, 1, 2, 0], [3, 4, 5, 6]) == [1] * 4
+    assert p.fork([3, 7, 0], [0, 7, 1]) == [0, 1, 0]  # children in use; an empty parent
+    for _ in range(20):
+        p.append([0, 1, 2, 3, 4, 5, 6])
+
+
+def test_fork_without_sharing_copies_every_page(dev):
+    p = Pair(dev)
+    p.append([0, 1], [70, 16])
+    assert p.fork([0, 1], [2, 3], share=False) == [1, 1]
+    assert all(c <= 1 for c in p.ref.refs)
+
+
+def test_fork_of_an_empty_child_in_the_same_call(dev):
+    p = Pair(dev)
+    p.append([0], [20])
+    assert p.fork([0, 1], [1, 2]) == [1, 1]  # row 1 is empty before the call, so row 2 stays empty
+    assert p.ref.lens[:3] == [20, 20, 0]
+
+
+@pytest.mark.parametrize("max_moves", [0, 1, 5, 100])
+def test_compact_moves_the_highest_pages_down(dev, max_moves):
+    p = Pair(dev, rows=9)
+    p.append(list(range(8)), [80, 16, 64, 3, 50, 33, 20, 41])
+    p.fork([4], [8])
+    p.truncate([0, 2, 5], [0, 10, 0])
+    p.compact(max_moves)
+    p.append([0, 2, 5], [30, 30, 30])
+    assert p.compact(max_moves)[1] == 0 or max_moves < 100
+
+
+def test_compact_of_empty_full_and_packed_pools(dev):
+    p = Pair(dev, pages=8, rows=3, width=8)
+    assert p.compact(8) == [0, 0]
+    p.append([0, 1], [64, 64])
+    assert p.compact(8) == [8, 0]
+    p.truncate([1], [0])
+    assert p.compact(8) == [4, 0]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("layers,block,heads,dim", [(1, 16, 1, 64), (3, 48, 2, 128), (2, 256, 8, 128),
+                                                    (5, 32, 3, 64)])
+def test_random_programs(dev, dtype, layers, block, heads, dim):
+    rng = random.Random(layers * 1000 + block)
+    p = Pair(dev, layers, 37, block, heads, dim, rows=11, width=7, dtype=dtype, seed=block)
+    for _ in range(40):
+        rows = [rng.randrange(-2, 13) for _ in range(rng.randint(0, 9))]
+        op = rng.choice(["one", "many", "many", "truncate", "truncate", "fork", "fork", "copy",
+                         "compact"])
+        if op == "one":
+            p.append(rows)
+        elif op == "many":
+            p.append(rows, [rng.choice([0, 1, block - 1, block, rng.randint(0, 3 * block)])
+                            for _ in rows])
+        elif op == "truncate":
+            keep = [rng.randint(-1, p.ref.lens[r] + 1) if 0 <= r < 11 else 0 for r in rows]
+            p.truncate(rows, keep)
+        elif op == "compact":
+            p.compact(rng.choice([0, 1, 3, 50]))
+        else:
+            p.fork([rng.randrange(-1, 12) for _ in rows], rows, op == "fork")
+
+
+def test_many_rows_and_pages(dev):
+    """More list entries than the plan has threads, and more pages than one step of its walk."""
+    p = Pair(dev, layers=1, pages=40_000, block=16, heads=1, dim=8, rows=3000, width=20)
+    rng = random.Random(3)
+    rows = list(range(3000))
+    rng.shuffle(rows)
+    p.append(rows, [rng.randint(0, 200) for _ in rows])
+    p.append(rows)
+    p.truncate(rows[:1500], [rng.choice([0, p.ref.lens[r] // 2]) for r in rows[:1500]])
+    p.compact(3000)
+    p.compact(40_000)
+    empty = [r for r in range(3000) if p.ref.lens[r] == 0]
+    p.fork([rng.choice(rows) for _ in empty], empty)
+    p.append([r for r in rows for _ in (0, 1)])  # every row twice: 6000 entries
+
+
+def test_a_pool_object_and_a_kept_state(dev):
+    pool = nkv.layers.kv_cache.KVCachePool(2, 2, 64, 16, num_blocks=10, device=dev)
+    pool.kv_cache.zero_()
+    seqs = nkv.PagedSequences(pool, 4, 5)
+    seqs.append(ints([0, 1], dev), ints([0, 20, 25], dev), 25)
+    kept = seqs.state.clone()
+    seqs.truncate(ints([0], dev), ints([0], dev))
+    again = nkv.PagedSequences(pool, 4, 5, state=kept)
+    assert again.context_lens.tolist() == [20, 5, 0, 0]
+    assert again.ref_counts.tolist() == [1, 1, 1] + [0] * 7
+    assert again.block_tables[:2].tolist() == [[0, 1, -1, -1, -1], [2, -1, -1, -1, -1]]
+    assert seqs.context_lens.tolist() == [0, 5, 0, 0]
+
+
+def test_calls_on_another_stream(dev):
+    p = Pair(dev)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        p.append([0, 1, 2], [30, 40, 50])
+        p.fork([0, 2], [3, 4])
+        p.truncate([0, 2], [9, 33])
+        p.compact(10)
+    s.synchronize()
+
+
+def test_a_decode_step_captured_in_a_graph(dev):
+    """append, store, attention in one graph, replayed with eager calls between: each replay's
+    slots, state and outputs are those of the same steps made one after another."""
+    H, Hk, D, B, S = 4, 2, 64, 16, 5
+    g = torch.Generator().manual_seed(4)
+    p = Pair(dev, layers=1, pages=30, block=B, heads=Hk, dim=D, rows=S, width=6)
+    p.kv.copy_(torch.randn(p.kv.shape, generator=g).to(torch.bfloat16))
+    p.ref.kv = p.kv.view(torch.int16).cpu()
+    rows = ints([3, 0, -1, 2, 1], dev)
+    q = torch.randn(S, H, D, generator=g).to(torch.bfloat16).to(dev)
+    k, v = (torch.randn(S, Hk, D, generator=g).to(torch.bfloat16).to(dev) for _ in range(2))
+    kc, vc = p.kv[0, 0], p.kv[1, 0]
+    p.append([0, 1, 2, 3, 4], [14, 33, 1, 15, 8])
+    ws = nkv.layers.attention.paged_decode_workspace(q, kc, p.seqs.block_tables)
+
+    def step():
+        slots, status = p.seqs.append(rows)
+        nkv.store_kvcache(k, v, kc, vc, slots)
+        out = nkv.paged_decode(q, kc, vc, p.seqs.context_lens, p.seqs.block_tables, D ** -0.5,
+                               workspace=ws)
+        return slots, status, out
+
+    kept, kv = p.seqs.state.clone(), p.kv.clone()
+    step()  # warm-up
+    torch.cuda.synchronize()
+    p.seqs.state.copy_(kept)
+    p.kv.copy_(kv)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        slots, status, out = step()
+    for i in range(6):
+        graph.replay()
+        torch.cuda.synchronize()
+        want_slots, want = p.ref.append([3, 0, -1, 2, 1])
+        assert slots.cpu().tolist() == want_slots and status.cpu().tolist() == want
+        flat = p.ref.kv.view(2, -1, Hk, D)
+        for t, s in enumerate(want_slots):
+            if s >= 0:
+                flat[0, s], flat[1, s] = k[t].view(torch.int16).cpu(), v[t].view(torch.int16).cpu()
+        p.check(status, want)
+        refs = p.ref.kv.view(torch.bfloat16)
+        lens = torch.tensor(p.ref.lens, dtype=I32)
+        ref = paged_decode_ref(q.float().cpu(), refs[0, 0], refs[1, 0], lens,
+                               torch.tensor(p.ref.tables, dtype=I32), D ** -0.5)
+        # weights and the output rounded to bf16 (half a step 2^-9 of values up to 4 each)
+        assert (out.float().cpu() - ref).abs().max() <= 2 * 4 * 2.0 ** -8
+        if i == 2:  # eager work between the replays
+            p.truncate([0, 3], [5, 16])
+        if i == 3:
+            p.fork([1], [4]) if p.ref.lens[4] == 0 else p.truncate([4], [0])

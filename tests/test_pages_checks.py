@@ -1,0 +1,131 @@
+"""PagedSequences: the oracle's own rules, and the refusals that need no GPU."""
+import importlib
+import random
+import struct
+
+import pytest
+import torch
+
+from oracle.pages_ref import PagedSequencesRef
+
+pages = importlib.import_module("nanokv-llm_amd.engine.pages")
+_lib = importlib.import_module("nanokv-llm_amd._lib")
+P = 0x10000
+
+
+def test_oracle_keeps_counts_tables_and_contents():
+    """Random programs: counts are the tables' entries, a partly filled page has one holder, and
+    every row reads back the tokens that were written for it, whatever was moved or copied."""
+    rng = random.Random(1)
+    B, S = 4, 7
+    ref = PagedSequencesRef(torch.zeros(2, 1, 25, B, 1, 1, dtype=torch.int64), S, 6)
+    want, clock = [[] for _ in range(S)], 0
+    for _ in range(600):
+        rows = rng.sample(range(S), rng.randint(1, 4))
+        op = rng.choice(["append", "append", "truncate", "fork", "copy", "compact"])
+        if op == "append":
+            n = [rng.randint(0, 9) for _ in rows]
+            cu = [sum(n[:i]) for i in range(len(n) + 1)]
+            slots, ok = ref.append(rows, cu=cu, n_tokens=cu[-1])
+            for i, r in enumerate(rows):
+                for t in slots[cu[i]:cu[i + 1]]:
+                    clock += 1
+                    assert (t >= 0) == bool(ok[i])
+                    if ok[i]:
+                        ref.kv.view(2, -1)[:, t] = clock
+                        want[r].append(clock)
+        elif op == "truncate":
+            keep = [rng.randint(0, ref.lens[r]) for r in rows]
+            for r, k, ok in zip(rows, keep, ref.truncate(rows, keep)):
+                want[r] = want[r][:k] if ok else want[r]
+        elif op == "compact":
+            ref.compact(rng.choice([1, 3, 25]))
+        else:
+            parents = [rng.randrange(S) for _ in rows]
+            before = [list(want[p]) for p in parents]
+            for r, b, ok in zip(rows, before, ref.fork(parents, rows, op == "fork")):
+                want[r] = b if ok else want[r]
+        held = [x for t in ref.tables for x in t if x >= 0]
+        assert ref.refs == [held.count(x) for x in range(25)]
+        for r in range(S):
+            n = ref.lens[r]
+            assert [x >= 0 for x in ref.tables[r]] == [j * B < n for j in range(6)]
+            got = [int(ref.kv[0, 0, ref.tables[r][t // B], t % B]) for t in range(n)]
+            assert got == want[r] and n == len(want[r])
+            assert n % B == 0 or ref.refs[ref.tables[r][n // B]] == 1
+
+
+def test_constructor_refuses_bad_pools_and_states():
+    kv = torch.zeros(2, 1, 4, 16, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="expected GPU"):
+        pages.PagedSequences(kv, 2, 2)
+    with pytest.raises(ValueError, match="contiguous"):
+        pages.PagedSequences(kv.transpose(2, 3), 2, 2)
+    with pytest.raises(ValueError, match="contiguous"):
+        pages.PagedSequences(kv[0], 2, 2)
+
+
+def _args(**kw):
+    a = dict(kv=P, planes=4, pages=10, block=16, row=256, refs=P, lens=P, tables=P, stride=8,
+             width=8, rows=5, ws=P, wsb=1 << 30)
+    a.update(kw)
+    return struct.pack("13q", *a.values())
+
+
+BAD = [
+    (dict(planes=0), -1, b"bad sizes"), (dict(pages=0), -1, b"bad sizes"),
+    (dict(block=0), -1, b"bad sizes"), (dict(rows=0), -1, b"bad sizes"),
+    (dict(stride=7), -1, b"bad sizes"), (dict(row=24), -4, b"multiple of 16"),
+    (dict(rows=8193), -4, b"at most"), (dict(pages=(1 << 20) + 1), -4, b"at most"),
+    (dict(planes=65536), -4, b"at most"), (dict(pages=1 << 20, block=2048), -4, b"32 bits"),
+    (dict(width=1 << 28, stride=1 << 28), -4, b"32 bits"), (dict(row=1 << 32), -4, b"32 bits"),
+    (dict(kv=0), -1, b"null"), (dict(refs=0), -1, b"null"), (dict(lens=0), -1, b"null"),
+    (dict(tables=0), -1, b"null"), (dict(kv=P + 8), -1, b"aligned"),
+    (dict(refs=P + 4), -1, b"aligned"), (dict(ws=0), -3, b"workspace"),
+    (dict(ws=P + 8), -3, b"workspace"), (dict(wsb=1000), -3, b"workspace"),
+]
+
+
+@pytest.mark.parametrize("kw,code,msg", BAD)
+def test_entry_points_refuse_bad_pages(kw, code, msg):
+    lib = _lib.lib()
+    a = _args(**kw)
+    for rc in (lib.nkv_pages_append(a, P, 1, None, 1, P, P, None),
+               lib.nkv_pages_truncate(a, P, P, 1, None, 0, P, None),
+               lib.nkv_pages_fork(a, P, P, 1, 1, P, None),
+               lib.nkv_pages_compact(a, 1, P, P, None)):
+        assert rc == code and msg in lib.nkv_last_error(), lib.nkv_last_error()
+
+
+@pytest.mark.parametrize("call,args,code,msg", [
+    ("append", (P, -1, None, -1, P, P), -1, b"rows"),
+    ("append", (P, 8193, None, 8193, P, P), -1, b"rows"),
+    ("append", (P, 3, None, 4, P, P), -1, b"one token a row"),
+    ("append", (P, 3, P, 1 << 31, P, P), -1, b"2^31"),
+    ("append", (None, 3, None, 3, P, P), -1, b"null"),
+    ("append", (P, 3, P, 4, None, P), -1, b"null"),
+    ("append", (None, 0, None, 0, None, None), 0, b""),
+    ("truncate", (P, P, -1, None, 0, P), -1, b"rows"),
+    ("truncate", (P, P, 1, None, 1, P), -1, b"null"),
+    ("truncate", (P, None, 1, None, 0, P), -1, b"null"),
+    ("truncate", (P, P, 1, P, 1 << 30, P), -1, b"page ids"),
+    ("truncate", (None, None, 0, None, 0, None), 0, b""),
+    ("fork", (P, P, 8193, 1, P), -1, b"rows"),
+    ("fork", (P, None, 1, 1, P), -1, b"null"),
+    ("fork", (None, None, 0, 0, None), 0, b""),
+    ("compact", (-1, P, P), -1, b"max_moves"),
+    ("compact", (1, None, P), -1, b"needed"),
+    ("compact", (1, P, P + 4), -1, b"8-byte"),
+    ("compact", (1, P, None), -1, b"needed"),
+])
+def test_entry_points_refuse_bad_lists(call, args, code, msg):
+    lib = _lib.lib()
+    rc = getattr(lib, "nkv_pages_" + call)(_args(), *args, None)
+    assert rc == code and msg in lib.nkv_last_error(), lib.nkv_last_error()
+    assert getattr(lib, "nkv_pages_" + call)(None, *args, None) == -1
+
+
+def test_workspace_bytes():
+    f = _lib.lib().nkv_pages_workspace_bytes
+    assert f(0) == f(-1) == f((1 << 20) + 1) == 0
+    assert f(1000) == 64 + 16 * 8192 + 24 * 1000
