@@ -831,6 +831,36 @@ int nkv_pages_fork(const nkv_pages* pages, const int32_t* parents, const int32_t
 int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info, int32_t* moves,
                       void* stream);
 
+/*
+ * Differential attention over the same caches. Heads stand in pairs: query
+ * pair h (heads 2h, 2h+1 of q) reads KV pair p = h / (n_q_heads / n_kv_heads),
+ * K heads 2p, 2p+1 and one value of 2*head_dim, V heads 2p and 2p+1 side by
+ * side; n_q_heads and n_kv_heads are those of q and of the cache, both even.
+ *   A_m = softmax(scale * q_{2h+m} . K_{2p+m}) [V_2p | V_2p+1]     m = 0, 1
+ *   lambda = exp(l[0].l[1]) - exp(l[2].l[3]) + lambda_init
+ *   o   = A_0 - lambda * A_1
+ *   out[., h, :] = (1 - lambda_init) * o / sqrt(mean(o^2) + eps) * norm_weight
+ * lambdas: fp32 [4, head_dim]; norm_weight: [2*head_dim] in q's type, or NULL
+ * for ones; out rows hold n_q_heads/2 heads of 2*head_dim (8-byte aligned, row
+ * stride a multiple of 4). A row that sees no key gives zeros. head_dim 64 or
+ * 128, at most NKV_DIFF_MAX_GROUP query pairs to a KV pair. kv_type: one of
+ * NKV_KV_*, the caches' type; q, norm_weight and out are bf16, or fp16 with
+ * fp16 caches; k_scale and v_scale are used for fp8 caches. The other arguments
+ * are as for nkv_paged_decode (one new token per sequence).
+ * No counterpart in the reference (beside nanokvllm/layers/attention.py:104-107).
+ */
+#define NKV_DIFF_MAX_GROUP 64
+size_t nkv_diff_decode_workspace_bytes(int32_t batch, int32_t n_q_heads, int32_t head_dim,
+                                       int32_t max_blocks_per_seq, int32_t block_size);
+int nkv_diff_decode(int32_t kv_type, const void* q, int64_t q_row_stride, const void* k_cache,
+                    const void* v_cache, const int32_t* block_tables, int64_t bt_row_stride,
+                    const int32_t* context_lens, int32_t batch, int32_t n_q_heads,
+                    int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+                    int32_t max_blocks_per_seq, int64_t n_blocks, float scale, float k_scale,
+                    float v_scale, const float* lambdas, float lambda_init,
+                    const void* norm_weight, float eps, void* out, int64_t out_row_stride,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,7 +16,6 @@ constexpr int kMinChunks = 4;            // chunks per wave range that grids are
 // (4 x 32), and one, so that a table of 512 chunks splits into ranges of 4
 constexpr int kMaxSlots = 129;
 constexpr int kWinBlocks = 64;           // block ids held per window (one per lane)
-constexpr int kBufferFlags = 0x00020000; // raw buffer resource word 3 (dword data)
 constexpr int kStreamPolicy = 2;         // cache policy "nt": K/V are read exactly once
 constexpr int kWavesPerCU = 8;           // resident split waves per CU (2 per SIMD)
 // floats per partial row: O, m, l, 2 pad (528 B at D = 128)
@@ -138,13 +137,19 @@ __device__ __forceinline__ int stage_off(int dim) {
 // HP*G are computed and dropped. D: head_dim (64, 128 or 256); a wave's piece of
 // a token row (HP*D elements) is 128 to 512 bytes.
 //
+// DIFF (differential attention): a "KV head" of D dims is a pair of K heads of D/2 and the pair's
+// value of D, and query head h (rows of D/2) is map h % 2 of its pair: its scores are against that
+// half of the K row. Each half's products are made for all columns and a column takes its own, as
+// many MFMAs as one product over D dims; a zero in the other half's place would turn an infinity
+// there into NaN.
+//
 // One wave's work: wave `wid` of `n_waves`; `lbuf` is its own LDS, decode_lds_elems of it.
 template <bool F8, int HP, int D>
 constexpr int decode_lds_elems() {
   constexpr int kRows = HP * kChunk * (D + 16);
   return 2 * kRows * 2 >= 20480 ? kRows : 2 * kRows;
 }
-template <bool F8, int HP, int D, bool H16, typename Seqs>
+template <bool F8, int HP, int D, bool H16, bool DIFF = false, typename Seqs>
 __device__ __forceinline__ void decode_stream(
     const Seqs seqs, const int wid, const int n_waves, bf16_t* lbuf,
     const bf16_t* __restrict__ q, int64_t q_row_stride,
@@ -158,6 +163,7 @@ __device__ __forceinline__ void decode_stream(
   constexpr int kSeg = HP * D * kEl;           // bytes a wave reads of each token row
   static_assert(kSeg >= 64 && kSeg <= 512, "a wave's piece of a row is 64..512 bytes");
   constexpr int kKs = D / 32;                  // k-steps of S^T (32 dims each)
+  constexpr int kQ = DIFF ? kKs / 2 : kKs;     // those of a row of q
   constexpr int kDb = D / 16;                  // 16-dim blocks of O^T
   constexpr int kVRow = D + 16;                // LDS row stride of a staged chunk (elements)
   constexpr int kPartRow = part_row(D);
@@ -254,13 +260,13 @@ __device__ __forceinline__ void decode_stream(
 
     // q^T as the MFMA B operand: lane l -> query head kvh0*G + l%16 (columns
     // >= HP*G re-read the first head and are discarded), dims 8*(l/16) + 32*ks
-    u32x4_t qreg[kKs];
+    u32x4_t qreg[kQ];
     {
       const int hc = col < HPG ? col : 0;
       const u32x4_t* qp = reinterpret_cast<const u32x4_t*>(
-          q + seqs.row(b) * q_row_stride + (int64_t)(qh0 + hc) * D + g4 * 8);
+          q + seqs.row(b) * q_row_stride + (int64_t)(qh0 + hc) * (kQ * 32) + g4 * 8);
 #pragma unroll
-      for (int ks = 0; ks < kKs; ++ks) qreg[ks] = qp[ks * 4];
+      for (int ks = 0; ks < kQ; ++ks) qreg[ks] = qp[ks * 4];
     }
     const char* kbase = static_cast<const char*>(k_cache) + (int64_t)kvh0 * D * kEl;
     const char* vbase = static_cast<const char*>(v_cache) + (int64_t)kvh0 * D * kEl;
@@ -349,12 +355,18 @@ __device__ __forceinline__ void decode_stream(
 #pragma unroll
         for (int hh = 0; hh < HP; ++hh) {
           f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+          [[maybe_unused]] f32x4_t a1 = {0.f, 0.f, 0.f, 0.f};  // DIFF: the second half's
 #pragma unroll
           for (int ks = 0; ks < kKs; ++ks) {
             const u32x4_t ka =
                 *reinterpret_cast<const u32x4_t*>(
                     &kbuf[hh][col * kVRow + stage_off<F8, D>(g4 * 8 + ks * 32)]);
-            a = mfma_16x16x32<H16>(ka, qreg[ks], a);
+            if (DIFF && ks >= kQ) a1 = mfma_16x16x32<H16>(ka, qreg[ks - kQ], a1);
+            else a = mfma_16x16x32<H16>(ka, qreg[ks], a);
+          }
+          if constexpr (DIFF) {  // column 0 is an even query head
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a[r] = (col & 1) ? a1[r] : a[r];
           }
           st[hh] = a;
         }
@@ -467,11 +479,18 @@ __device__ __forceinline__ void decode_stream(
 // s % WAVES == w (in its lane s / WAVES), and merge once more through LDS: a context that many
 // waves shared has up to kMaxSlots, and one wave took 10.3 us over a 23001-token sequence's 120
 // (a round trip for every eight rows), four waves with 32 rows in flight each 4.2 us.
-template <int D, bool H16, int WAVES, typename Seqs>
-__device__ __forceinline__ void decode_combine(
+// Wave `wave` of those WAVES; true in the wave that then holds o and l (the output is o / l, zero
+// where l is).
+template <int D, int WAVES>
+struct MergeLds {
+  float so[WAVES][D / 64][64];
+  float2 sml[WAVES];
+};
+template <int D, int WAVES, typename Seqs>
+__device__ __forceinline__ bool decode_merge(
     const Seqs seqs, const int b, const int h, int32_t Hq, int32_t Hk, int32_t NCG,
-    const float* __restrict__ part, const i32x4v_t* __restrict__ desc,
-    bf16_t* __restrict__ out, int64_t out_row_stride) {
+    const float* __restrict__ part, const i32x4v_t* __restrict__ desc, const int wave,
+    [[maybe_unused]] MergeLds<D, WAVES>* lds, float (&o)[D / 64], float& L) {
   static_assert(decode_dim_ok(D), "head_dim 64, 128 or 256");
   static_assert(WAVES == 1 || !Seqs::kZeroInvalid, "each wave would weigh the keys past the table");
   constexpr int N = D / 64;
@@ -479,7 +498,6 @@ __device__ __forceinline__ void decode_combine(
   constexpr int kPer = (kMaxSlots + 64 * WAVES - 1) / (64 * WAVES);  // (m, l) pairs a lane holds
   constexpr int kFirst = WAVES > 1 ? 32 : 16;  // rows in flight with the (m, l) pairs
   const int lane = threadIdx.x & 63;
-  const int wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : 0;
   const int G = Hq / Hk;
   // The context length and the KV head's descriptor first (one round trip), then every
   // (m, l) pair and the first partial rows at once (the second).
@@ -487,16 +505,12 @@ __device__ __forceinline__ void decode_combine(
   const int hq = h % G;                         // query head within the KV head's group
   const int cg = NCG > 1 ? hq / kMaxCols : 0;    // its column group (0 unless G > 16)
   const i32x4v_t d = desc[((int64_t)b * Hk + h / G) * NCG + cg];
-  bf16_t* op = out + seqs.row(b) * out_row_stride + (int64_t)h * D + N * lane;
-  float o[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.f;
+  L = 0.f;
   // the descriptor is written by this call for every sequence with ctx > 0
   const int n_all = ctx > 0 ? min(d.y, kMaxSlots) : 0;
-  if (n_all == 0) {  // uniform
-    if (wave == 0) store_dims<N, H16>(op, o, 0.f);
-    return;
-  }
+  if (n_all == 0) return wave == 0;  // uniform
   // this wave's partials: s = wave + WAVES * j, j < ns
   const int ns = (n_all - wave + WAVES - 1) / WAVES;
   const int64_t stride = (int64_t)d.z * kPartRow * WAVES;  // floats between them
@@ -532,7 +546,7 @@ __device__ __forceinline__ void decode_combine(
     past = max(ctx - seqs.max_tokens, 0);
     if (past > 0) M = fmaxf(M, 0.f);
   }
-  float w[kPer], L = 0.f;
+  float w[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
     w[k] = (ml[k].x == -INFINITY) ? 0.f : fast_exp2(ml[k].x - M);
@@ -567,28 +581,62 @@ __device__ __forceinline__ void decode_combine(
     }
   }
   if constexpr (WAVES > 1) {
-    __shared__ float so[WAVES][N][64];
-    __shared__ float2 sml[WAVES];
 #pragma unroll
-    for (int i = 0; i < N; ++i) so[wave][i][lane] = o[i];
-    if (lane == 0) sml[wave] = float2{M, L};
+    for (int i = 0; i < N; ++i) lds->so[wave][i][lane] = o[i];
+    if (lane == 0) lds->sml[wave] = float2{M, L};
     __syncthreads();
-    if (wave > 0) return;
+    if (wave > 0) return false;
 #pragma unroll
-    for (int x = 1; x < WAVES; ++x) M = fmaxf(M, sml[x].x);
+    for (int x = 1; x < WAVES; ++x) M = fmaxf(M, lds->sml[x].x);
     L = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = 0.f;
 #pragma unroll
     for (int x = 0; x < WAVES; ++x) {
-      const float2 p = sml[x];
+      const float2 p = lds->sml[x];
       const float wx = p.x == -INFINITY ? 0.f : fast_exp2(p.x - M);
       L = fmaf(wx, p.y, L);
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = fmaf(wx, so[x][i][lane], o[i]);
+      for (int i = 0; i < N; ++i) o[i] = fmaf(wx, lds->so[x][i][lane], o[i]);
     }
   }
-  store_dims<N, H16>(op, o, L > 0.f ? 1.f / L : 0.f);
+  return true;
 }
+
+// The merged row of out.
+template <int D, bool H16, int WAVES, typename Seqs>
+__device__ __forceinline__ void decode_combine(
+    const Seqs seqs, const int b, const int h, int32_t Hq, int32_t Hk, int32_t NCG,
+    const float* __restrict__ part, const i32x4v_t* __restrict__ desc,
+    bf16_t* __restrict__ out, int64_t out_row_stride) {
+  constexpr int N = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : 0;
+  bf16_t* op = out + seqs.row(b) * out_row_stride + (int64_t)h * D + N * lane;
+  float o[N], L;
+  MergeLds<D, WAVES>* lds = nullptr;
+  if constexpr (WAVES > 1) {
+    __shared__ MergeLds<D, WAVES> s;
+    lds = &s;
+  }
+  if (decode_merge<D, WAVES>(seqs, b, h, Hq, Hk, NCG, part, desc, wave, lds, o, L))
+    store_dims<N, H16>(op, o, L > 0.f ? 1.f / L : 0.f);
+}
+
+// A decode split over pairs of K heads (DIFF), by kv_type, and where its partials are (the host's
+// part: paged_decode.hip). n_pairs KV heads of value_dim dims; q's n_q_heads heads have half.
+struct DecodeParts {
+  const float* part;
+  const i32x4v_t* desc;
+  int ncg;
+  bool wide;  // the combine's rows may have many partials
+};
+int decode_split_pairs(int32_t kv_type, const void* q, int64_t q_row_stride, const void* k_cache,
+                       const void* v_cache, const int32_t* block_tables, int64_t bt_row_stride,
+                       const int32_t* context_lens, int32_t batch, int32_t n_q_heads,
+                       int32_t n_pairs, int32_t value_dim, int32_t block_size,
+                       int32_t max_blocks_per_seq, int64_t n_blocks, float scale, float k_scale,
+                       float v_scale, void* workspace, size_t workspace_bytes, void* stream,
+                       DecodeParts* parts);
 
 }  // namespace nkv

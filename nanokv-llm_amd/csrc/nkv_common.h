@@ -228,6 +228,8 @@ __device__ __forceinline__ void store_dims(bf16_t* op, const float (&o)[N], floa
   }
 }
 
+constexpr int kBufferFlags = 0x00020000;  // raw buffer resource word 3 (dword data)
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }

@@ -54,7 +54,7 @@
 
 namespace nkv {
 
-template <bool F8, int HP, int D, bool H16 = false>
+template <bool F8, int HP, int D, bool H16 = false, bool DIFF = false>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2)))
 void paged_decode_split_kernel(
     const bf16_t* __restrict__ q, int64_t q_row_stride,
@@ -64,7 +64,7 @@ void paged_decode_split_kernel(
     int32_t NCG, int32_t block_size, int32_t max_blocks, int64_t n_blocks, int32_t min_chunks,
     float scale_log2, float v_scale, float* __restrict__ part, i32x4v_t* __restrict__ desc) {
   __shared__ __attribute__((aligned(16))) bf16_t lbuf[decode_lds_elems<F8, HP, D>()];
-  decode_stream<F8, HP, D, H16>(DecodeSeqs{context_lens, batch}, (int)blockIdx.x,
+  decode_stream<F8, HP, D, H16, DIFF>(DecodeSeqs{context_lens, batch}, (int)blockIdx.x,
                                 (int)gridDim.x, lbuf, q, q_row_stride, k_cache, v_cache,
                                 block_tables, bt_row_stride, Hk, G, NCG, block_size, max_blocks,
                                 n_blocks, min_chunks, scale_log2, v_scale, part, desc);
@@ -85,7 +85,7 @@ static int decode_check(const void* q, const void* k_cache, const void* v_cache,
                         const int32_t* block_tables, const int32_t* context_lens, int32_t batch,
                         int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
                         int32_t block_size, int32_t max_blocks_per_seq, int64_t q_row_stride,
-                        int64_t bt_row_stride) {
+                        int64_t bt_row_stride, int32_t q_dim) {
   NKV_REQUIRE(batch >= 0 && n_kv_heads > 0 && n_q_heads > 0, NKV_EINVAL,
               "paged_decode: bad sizes (batch=%d, Hq=%d, Hk=%d)", batch, n_q_heads, n_kv_heads);
   NKV_REQUIRE(decode_dim_ok(head_dim), NKV_EUNSUPPORTED,
@@ -104,7 +104,7 @@ static int decode_check(const void* q, const void* k_cache, const void* v_cache,
               "paged_decode: max_blocks_per_seq * block_size too large");
   NKV_REQUIRE((int64_t)block_size * n_kv_heads * head_dim * 2 < (1ll << 31), NKV_EUNSUPPORTED,
               "paged_decode: cache block too large for 32-bit buffer offsets");
-  NKV_REQUIRE(q_row_stride >= (int64_t)n_q_heads * head_dim && q_row_stride % 8 == 0,
+  NKV_REQUIRE(q_row_stride >= (int64_t)n_q_heads * q_dim && q_row_stride % 8 == 0,
               NKV_EINVAL, "paged_decode: q row stride must be >= Hq*D and a multiple of 8");
   NKV_REQUIRE(q && k_cache && v_cache && block_tables && context_lens, NKV_EINVAL,
               "paged_decode: null pointer");
@@ -245,7 +245,8 @@ extern "C" size_t nkv_paged_decode_workspace_bytes(int32_t batch, int32_t n_q_he
 }
 
 namespace nkv {
-template <bool F8, bool H16 = false>
+// DIFF: n_kv_heads pairs of K heads, head_dim the two heads' dims together (q's heads have half).
+template <bool F8, bool H16 = false, bool DIFF = false>
 static int decode_split(const void* q, int64_t q_row_stride, const void* k_cache,
                         const void* v_cache, const int32_t* block_tables, int64_t bt_row_stride,
                         const int32_t* context_lens, int32_t batch, int32_t n_q_heads,
@@ -254,7 +255,7 @@ static int decode_split(const void* q, int64_t q_row_stride, const void* k_cache
                         float v_scale, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = decode_check(q, k_cache, v_cache, block_tables, context_lens, batch, n_q_heads,
                         n_kv_heads, head_dim, block_size, max_blocks_per_seq, q_row_stride,
-                        bt_row_stride);
+                        bt_row_stride, DIFF ? head_dim / 2 : head_dim);
   if (rc) return rc;
   if (batch == 0) return NKV_OK;
   NKV_REQUIRE(k_scale > 0.f && v_scale > 0.f, NKV_EINVAL, "paged_decode: scales must be > 0");
@@ -276,15 +277,17 @@ static int decode_split(const void* q, int64_t q_row_stride, const void* k_cache
   const float scale_log2 = scale * k_scale * kLog2e;
   hipStream_t s = as_stream(stream);
 #define NKV_DECODE_LAUNCH(HP, D)                                                               \
-  hipLaunchKernelGGL((paged_decode_split_kernel<F8, HP, D, H16>), dim3(p.grid), dim3(64), 0, s, \
+  hipLaunchKernelGGL((paged_decode_split_kernel<F8, HP, D, H16, DIFF>), dim3(p.grid), dim3(64), 0, s, \
                      (const bf16_t*)q, q_row_stride, k_cache, v_cache, block_tables,           \
                      bt_row_stride, context_lens, batch, n_kv_heads, g, p.ncg, block_size,     \
                      max_blocks_per_seq, n_blocks, p.min_chunks, scale_log2, v_scale, part,    \
                      desc)
   if (head_dim == 64) {
-    if (p.hp == 4) NKV_DECODE_LAUNCH(4, 64);
-    else if (p.hp == 2) NKV_DECODE_LAUNCH(2, 64);
-    else NKV_DECODE_LAUNCH(1, 64);
+    if constexpr (!DIFF) {
+      if (p.hp == 4) NKV_DECODE_LAUNCH(4, 64);
+      else if (p.hp == 2) NKV_DECODE_LAUNCH(2, 64);
+      else NKV_DECODE_LAUNCH(1, 64);
+    }
   } else if (head_dim == 128) {
     if (p.hp == 4) {
       if constexpr (F8) NKV_DECODE_LAUNCH(4, 128);
@@ -355,6 +358,33 @@ static int decode_combine(const int32_t* context_lens, int32_t batch, int32_t n_
 #undef NKV_COMBINE_LAUNCH
 #undef NKV_COMBINE_LAUNCH_W
   return check_launch("nkv_paged_decode_combine");
+}
+
+int decode_split_pairs(int32_t kv_type, const void* q, int64_t q_row_stride, const void* k_cache,
+                       const void* v_cache, const int32_t* block_tables, int64_t bt_row_stride,
+                       const int32_t* context_lens, int32_t batch, int32_t n_q_heads,
+                       int32_t n_pairs, int32_t value_dim, int32_t block_size,
+                       int32_t max_blocks_per_seq, int64_t n_blocks, float scale, float k_scale,
+                       float v_scale, void* workspace, size_t workspace_bytes, void* stream,
+                       DecodeParts* parts) {
+  auto* fn = kv_type == NKV_KV_FP8   ? decode_split<true, false, true>
+             : kv_type == NKV_KV_F16 ? decode_split<false, true, true>
+                                     : decode_split<false, false, true>;
+  const int rc = fn(q, q_row_stride, k_cache, v_cache, block_tables, bt_row_stride, context_lens,
+                    batch, n_q_heads, n_pairs, value_dim, block_size, max_blocks_per_seq,
+                    n_blocks, scale, k_scale, v_scale, workspace, workspace_bytes, stream);
+  if (rc || batch == 0) return rc;
+  const int ncg = decode_ncg(n_q_heads / n_pairs);
+  const int64_t max_chunks = decode_max_chunks(max_blocks_per_seq, block_size);
+  parts->ncg = ncg;
+  parts->desc = static_cast<const i32x4v_t*>(workspace);
+  parts->part = reinterpret_cast<const float*>(static_cast<const char*>(workspace) +
+                                               decode_desc_bytes(batch, n_pairs * ncg));
+  parts->wide = combine_wide(batch, n_pairs, ncg, max_chunks,
+                             decode_min_chunks(max_chunks,
+                                               decode_range_floor(batch, value_dim, false)),
+                             (int64_t)device_cus() * kWavesPerCU);
+  return NKV_OK;
 }
 }  // namespace nkv
 
@@ -487,7 +517,7 @@ extern "C" int nkv_paged_decode_noalloc(const void* q, int64_t q_row_stride, con
   clear_error();
   int rc = decode_check(q, k_cache, v_cache, block_tables, context_lens, batch, n_q_heads,
                         n_kv_heads, head_dim, block_size, max_blocks_per_seq, q_row_stride,
-                        bt_row_stride);
+                        bt_row_stride, head_dim);
   if (rc) return rc;
   if (batch == 0) return NKV_OK;
   // the bytes this call's plan needs, against the array's fixed size

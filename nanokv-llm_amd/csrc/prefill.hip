@@ -45,6 +45,7 @@
 //    workgroups of their own, as the decode kernel does.
 #include "decode_stream.h"
 #include "launch_rules.h"
+#include "lds_tiles.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -66,18 +67,7 @@ constexpr int prefill_tile_rows(int D, bool F8) { return 64 * prefill_row_groups
 // largest GQA group, the same for every instance of a head_dim: each tile holds at least
 // one query for all g heads of its KV head
 constexpr int prefill_max_group(int D) { return D == 256 ? 64 : 128; }
-// XOR applied to the 16-byte chunk index of LDS row r (even: chunk pairs stay together).
-// Keeps the K row reads and the V transpose reads free of bank conflicts: 2*(r & 7) for
-// 256- and 512-byte rows, 2*((r >> 1) & 3) for 128-byte rows (two rows per bank line).
-template <int D>
-__device__ __forceinline__ int chunk_swz(int r) {
-  if constexpr (D == 64) return 2 * ((r >> 1) & 3);
-  else return 2 * (r & 7);
-}
 constexpr float kLazy = 8.f;              // log2 headroom before the running max is raised
-
-typedef __attribute__((address_space(3))) u32x4_t lds_u32x4_t;
-typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 
 // Output pair: bf16 with the round-to-nearest-even of pack_bf16x2, or fp16.
 template <bool H16>
@@ -85,23 +75,6 @@ __device__ __forceinline__ uint32_t out_pack(float a, float b) {
   if constexpr (H16) return cvt_pk16<true>(a, b);
   else return pack_bf16x2(a, b);
 }
-// Raw buffer descriptor over [base, base + bytes): loads past `bytes` return 0.
-__device__ __forceinline__ i32x4_t buffer_desc(const void* base, uint32_t bytes) {
-  const uint64_t a = (uint64_t)(uintptr_t)base;
-  return i32x4_t{__builtin_amdgcn_readfirstlane((int32_t)(uint32_t)a),
-                 __builtin_amdgcn_readfirstlane((int32_t)((a >> 32) & 0xffffu)),
-                 __builtin_amdgcn_readfirstlane((int32_t)bytes), kBufferFlags};
-}
-// 16 bytes per lane from desc+voff into LDS at lds_addr + 16 * lane. Written as
-// asm so that the compiler does not add a wait for it before every barrier;
-// the ring's own s_waitcnt (vmcnt) orders it.
-__device__ __forceinline__ void load_to_lds(i32x4_t desc, uint32_t lds_addr, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(lds_addr), "v"(voff), "s"(desc)
-               : "memory");
-}
-
 // ---------------------------------------------------------------- split keys
 // What the split launch adds to the plain one's arguments.
 struct SplitArgs {

@@ -1,0 +1,224 @@
+"""Differential attention of single tokens over paged caches against the definition in 64 bits.
+
+The tolerance of an output row, from the roundings that the kernel makes. A rounding to the 16-bit
+type is off by at most u = eps / 2 of the value (bf16 2^-8, fp16 2^-11). The weights are rounded once to 16 bits, each by at most u of itself, and the row's sum is that of
+the unrounded ones, so A_m is off by at most u * sum_k p_k |v_k| <= u * max|v|; fp32 sums and exp2
+add far less (2^-20). o = A_0 - lambda A_1 is then off by at most d = u (1 + |lambda|) max|v| in every
+dimension. With r = sqrt(mean(o^2) + eps), o / r is off by at most 2 d / r (d in the numerator, and the
+norm, an average of values each off by at most d, by at most d of r again, times |o|/r, bounded by its own
+value): |err| <= (d / r) (1 + |o / r|). The factors (1 - init) w multiply it; the output rounds by u of
+its value. One more eighth for the terms of second order.
+"""
+import importlib
+
+import pytest
+import torch
+
+from oracle.diff_attention_ref import diff_attention_ref, gather_rows
+
+pytestmark = pytest.mark.gpu
+
+nkv = importlib.import_module("nanokv-llm_amd")
+BF, F16, FP8 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+I32 = torch.int32
+KS, VS = 0.02, 0.03
+
+
+def tolerance(ref, vmax, lambdas, init, weight, eps, dtype):
+    """The bound above for reference rows [..., 2 D] (float64)."""
+    u = torch.finfo(dtype).eps / 2
+    l = lambdas.double()
+    lam = (l[0] @ l[1]).exp() - (l[2] @ l[3]).exp() + init
+    w = (1 - init) * (torch.ones(ref.size(-1), dtype=torch.float64) if weight is None
+                      else weight.double())
+    unit = torch.where(w == 0, 0.0, ref / w)              # o / r
+    # mean((o/r)^2) = 1 - eps / r^2
+    r2 = eps / (1 - unit.square().mean(-1, keepdim=True)).clamp(min=1e-12)
+    d = u * (1 + abs(float(lam))) * vmax
+    return 1.125 * ((d / r2.sqrt()) * (1 + unit.abs()) * w.abs() + u * ref.abs()) + 1e-6
+
+
+def make(dev, lens, hq, hk, d, B=16, dtype=BF, kv=None, seed=0, width=None, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    counts = [-(-n // B) for n in lens]
+    NB = sum(counts) + 2
+    ids = torch.randperm(NB, generator=g)
+    width = width or max(counts) + 1
+    bt, at = torch.full((len(lens), width), -1, dtype=I32), 0
+    for i, c in enumerate(counts):
+        bt[i, :c] = ids[at:at + c]
+        at += c
+    q = (torch.randn(len(lens), hq, d, generator=g) * spread).to(dtype)
+    k = torch.randn(NB, B, hk, d, generator=g)
+    v = torch.randn(NB, B, hk, d, generator=g) + 0.3
+    if kv is FP8:
+        k, v = (k / KS).to(FP8), (v / VS).to(FP8)
+    else:
+        k, v = k.to(dtype), v.to(dtype)
+    lambdas = torch.randn(4, d, generator=g) * 0.1
+    weight = (1 + 0.2 * torch.randn(2 * d, generator=g)).to(dtype)
+    return dict(q=q, k=k, v=v, bt=bt, lens=torch.tensor(lens, dtype=I32), lambdas=lambdas,
+                weight=weight, init=0.43, scale=d ** -0.5, B=B, fp8=kv is FP8, dev=dev)
+
+
+def run(c, **kw):
+    dev = c["dev"]
+    ks, vs = (KS, VS) if c["fp8"] else (1.0, 1.0)
+    kw.setdefault("norm_weight", c["weight"].to(dev))
+    return nkv.diff_paged_decode(c["q"].to(dev), c["k"].to(dev), c["v"].to(dev),
+                                 c["lens"].to(dev), c["bt"].to(dev), c["scale"],
+                                 c["lambdas"].to(dev), c["init"], k_scale=ks, v_scale=vs, **kw)
+
+
+def reference(c, weight="own", eps=1e-5):
+    ks, vs = (KS, VS) if c["fp8"] else (1.0, 1.0)
+    weight = c["weight"] if isinstance(weight, str) else weight
+    outs, tols = [], []
+    for i, n in enumerate(c["lens"].tolist()):
+        k = gather_rows(c["k"], c["bt"][i], n, c["B"], scale=ks)
+        v = gather_rows(c["v"], c["bt"][i], n, c["B"], scale=vs)
+        # every key of the rows left is visible
+        o = diff_attention_ref(c["q"][i:i + 1], k, v, c["scale"], c["lambdas"], c["init"], weight,
+                               eps)
+        outs.append(o)
+        vmax = float(v.abs().max()) if len(v) else 0.0
+        tols.append(tolerance(o, vmax, c["lambdas"], c["init"], weight, eps, c["q"].dtype))
+    return torch.cat(outs), torch.cat(tols)
+
+
+def check(out, c, **kw):
+    ref, tol = reference(c, **kw)
+    err = (out.double().cpu() - ref).abs()
+    assert out.shape == ref.shape and bool((err <= tol).all()), \
+        f"off by up to {float((err / tol).max()):.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("dtype,kv", [(BF, None), (F16, None), (BF, FP8)])
+@pytest.mark.parametrize("hq,hk,d", [(2, 2, 64), (4, 2, 128), (16, 8, 64), (32, 8, 128), (6, 6, 64),
+                                     (40, 8, 128), (20, 2, 64), (12, 2, 128), (128, 2, 64)])
+def test_types_heads_and_lengths(dev, dtype, kv, hq, hk, d):
+    c = make(dev, [1, 0, 15, 16, 17, 100, 333], hq, hk, d, dtype=dtype, kv=kv, seed=hq + d)
+    check(run(c), c)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("B", [16, 48, 256])
+def test_a_long_sequence_beside_short_ones(dev, d, B):
+    c = make(dev, [4097, 3, 900, 1], 8, 4, d, B=B, seed=B)
+    check(run(c), c)
+
+
+def test_many_sequences(dev):
+    """More sequences than lanes of a cursor, and several head pairs a wave."""
+    c = make(dev, [(7 * i) % 90 for i in range(150)], 8, 8, 64, seed=5)
+    check(run(c), c)
+
+
+def test_sharp_maps(dev):
+    """Scores of tens: weights that underflow, one key that carries a row."""
+    c = make(dev, [300, 40], 8, 4, 64, seed=6, spread=12.0)
+    check(run(c), c)
+
+
+def test_without_a_norm_weight_and_other_eps(dev):
+    c = make(dev, [50, 7], 4, 2, 64, seed=7)
+    check(run(c, norm_weight=None, eps=0.5), c, weight=None, eps=0.5)
+
+
+def test_empty_rows_are_zero(dev):
+    c = make(dev, [0, 0, 5], 4, 2, 128, seed=8)
+    out = run(c)
+    assert bool((out[:2] == 0).all())
+    check(out, c)
+
+
+def test_equal_maps_cancel(dev):
+    """lambda = 1 and the same q and k in both maps: o is zero but for roundings, the output bounded by
+    what eps leaves of it."""
+    c = make(dev, [77], 4, 2, 64, seed=9)
+    c["q"][:, 1::2] = c["q"][:, 0::2]
+    c["k"][:, :, 1::2] = c["k"][:, :, 0::2]
+    c["lambdas"].zero_()
+    c["init"] = 1.0
+    assert bool((run(c) == 0).all())  # (1 - init) = 0
+    c["init"], c["lambdas"][0, 0], c["lambdas"][1, 0] = 0.0, 1.0, float(torch.log(torch.tensor(2.)))
+    # lambda = exp(ln 2) - exp(0) + 0 = 1 to within fp32; both maps' weights are the same numbers
+    assert run(c, eps=1.0).abs().max() <= 1e-5
+
+
+def test_infinity_in_one_map_stays_in_it(dev):
+    """A key whose second head scores -inf has weight zero there and its own in the first map."""
+    c = make(dev, [33], 4, 2, 64, seed=10)
+    c["q"][:, 1::2] = c["q"][:, 1::2].abs()
+    c["k"][c["bt"][0, 0], 5, 1] = -float("inf")
+    check(run(c), c)
+
+
+def test_rows_behind_a_context_are_not_read(dev):
+    """NaN in the pages' rows past each context, and in pages of nobody."""
+    c = make(dev, [5, 18, 31], 4, 2, 64, seed=11)
+    c["k"][:], clean = float("nan"), c["k"].clone()
+    v_clean = c["v"].clone()
+    c["v"][:] = float("nan")
+    for i, n in enumerate(c["lens"].tolist()):
+        for t in range(n):
+            b = int(c["bt"][i, t // 16])
+            c["k"][b, t % 16], c["v"][b, t % 16] = clean[b, t % 16], v_clean[b, t % 16]
+    check(run(c), c)
+
+
+def test_invalid_blocks_and_lengths_past_the_table(dev):
+    c = make(dev, [60, 64, 33], 4, 2, 64, seed=12, width=4)
+    c["bt"][0, 1], c["bt"][1, 2], c["bt"][2, 0] = -1, 10 ** 6, -5
+    c["bt"][2, 3] = c["bt"][0, 0]
+    c["lens"][2] = 500  # the table holds 64
+    ref = dict(c, lens=torch.tensor([60, 64, 64], dtype=I32))
+    out = run(c)
+    check(out, ref)
+
+
+def test_strided_q_out_and_tables(dev):
+    c = make(dev, [90, 14], 8, 4, 64, seed=13)
+    fused = torch.zeros(2, 8 * 64 + 128, dtype=BF, device=dev)
+    fused[:, 64:64 + 512] = c["q"].reshape(2, -1).to(dev)
+    q = fused[:, 64:64 + 512].unflatten(1, (8, 64))
+    bt = torch.full((2, 40), -1, dtype=I32, device=dev)
+    bt[:, 3:3 + c["bt"].size(1)] = c["bt"].to(dev)
+    out = torch.full((3, 4 * 128 + 4), 7.0, dtype=BF, device=dev)
+    view = out[:2, 4:].unflatten(1, (4, 128))
+    got = nkv.diff_paged_decode(q, c["k"].to(dev), c["v"].to(dev), c["lens"].to(dev),
+                                bt[:, 3:3 + c["bt"].size(1)], c["scale"], c["lambdas"].to(dev),
+                                c["init"], norm_weight=c["weight"].to(dev), out=view)
+    assert got.data_ptr() == view.data_ptr()
+    check(got, c)
+    assert bool((out[2] == 7).all()) and bool((out[:, :4] == 7).all())
+
+
+def test_equal_results_call_after_call_and_on_a_stream(dev):
+    c = make(dev, [700, 90, 1500], 16, 8, 128, seed=14)
+    first = run(c)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        again = run(c)
+    s.synchronize()
+    assert torch.equal(first, again) and torch.equal(first, run(c))
+
+
+def test_a_cache_past_4_gib(dev):
+    """Pages whose byte offset passes 32 bits."""
+    B, hk, d = 256, 8, 128
+    NB = (5 << 30) // (B * hk * d * 2)
+    g = torch.Generator().manual_seed(15)
+    k = torch.empty(NB, B, hk, d, dtype=BF, device=dev)
+    v = torch.empty(NB, B, hk, d, dtype=BF, device=dev)
+    bt = torch.tensor([[NB - 1, 0, NB - 2]], dtype=I32)
+    rows = torch.randn(2, 3, B, hk, d, generator=g).to(BF)
+    k[bt[0].long().to(dev)], v[bt[0].long().to(dev)] = rows[0].to(dev), rows[1].to(dev)
+    q = torch.randn(1, 16, d, generator=g).to(BF)
+    lambdas = torch.randn(4, d, generator=g) * 0.1
+    out = nkv.diff_paged_decode(q.to(dev), k, v, torch.tensor([700], dtype=I32, device=dev),
+                                bt.to(dev), d ** -0.5, lambdas.to(dev), 0.2)
+    kk, vv = rows[0].flatten(0, 1)[:700], rows[1].flatten(0, 1)[:700]
+    ref = diff_attention_ref(q, kk, vv, d ** -0.5, lambdas, 0.2)
+    tol = tolerance(ref, float(vv.abs().max()), lambdas, 0.2, None, 1e-5, BF)
+    assert bool(((out.double().cpu() - ref).abs() <= tol).all())
