@@ -861,6 +861,32 @@ int nkv_diff_decode(int32_t kv_type, const void* q, int64_t q_row_stride, const 
                     const void* norm_weight, float eps, void* out, int64_t out_row_stride,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Differential attention (as nkv_diff_decode) of total_q query rows, cu_seqlens_q/k
+ * as for nkv_prefill_varlen: query j of a sequence with Lq queries and Lk keys
+ * sees keys 0 .. Lk-Lq+j, over the paged caches, or with block_tables NULL over
+ * contiguous rows of k and v (bf16 or fp16; n_rows of them, each with its own row
+ * stride). n_rows: the rows of k and v (paged: blocks * block_size). Keys of
+ * invalid blocks and past the table are zeros, as there. Without a workspace a
+ * query tile's keys stay with one workgroup; with one of
+ * nkv_diff_prefill_workspace_bytes (0: no use) they are split where few tiles
+ * would leave the chip idle. max_seqlen_k: an upper bound of the key lengths,
+ * which that choice goes by (results do not depend on it beyond rounding).
+ * No counterpart in the reference (beside nanokvllm/layers/attention.py:96-102).
+ */
+size_t nkv_diff_prefill_workspace_bytes(int32_t n_seqs, int64_t total_q, int64_t max_seqlen_k,
+                                        int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim);
+int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_stride, int64_t total_q,
+                     const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride,
+                     const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                     const int32_t* block_tables, int64_t bt_row_stride,
+                     int32_t max_blocks_per_seq, int32_t n_seqs, int64_t max_seqlen_k,
+                     int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+                     int64_t n_rows, float scale, float k_scale, float v_scale,
+                     const float* lambdas, float lambda_init, const void* norm_weight, float eps,
+                     void* out, int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,7 +10,8 @@ from .layers.attention import (Attention, paged_decode, release_retired_decode_w
                                reserve_decode_workspace, store_kvcache, varlen_prefill)
 from .layers.compress_utils import MyCompressCompact
 from .layers.CompressMethod import SnapKV
-from .layers.diff_attention import diff_paged_decode
+from .layers.diff_attention import (DifferentialAttention, diff_paged_decode,
+                                    diff_varlen_prefill, lambda_init_of)
 from .layers.rotary_embedding import RotaryEmbedding, get_rope, qk_norm_rope_store
 from .utils.context import Context, get_context, set_context, reset_context
 
@@ -20,5 +21,5 @@ __all__ = [
     "MyCompressCompact",
     "SnapKV", "Context", "get_context", "set_context", "reset_context", "RotaryEmbedding",
     "get_rope", "qk_norm_rope_store", "PagedSequences",
-    "diff_paged_decode",
+    "DifferentialAttention", "diff_paged_decode", "diff_varlen_prefill", "lambda_init_of",
 ]

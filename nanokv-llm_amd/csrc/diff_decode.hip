@@ -72,9 +72,9 @@ int diff_check(const char* what, int32_t kv_type, int32_t n_q_heads, int32_t n_k
   NKV_REQUIRE(n_q_heads / n_kv_heads <= NKV_DIFF_MAX_GROUP, NKV_EUNSUPPORTED,
               "%s: %d query pairs to a KV pair, above %d", what, n_q_heads / n_kv_heads,
               NKV_DIFF_MAX_GROUP);
-  NKV_REQUIRE(isfinite(scale) && k_scale > 0.f && v_scale > 0.f && isfinite(k_scale) &&
+  NKV_REQUIRE(scale > 0.f && isfinite(scale) && k_scale > 0.f && v_scale > 0.f && isfinite(k_scale) &&
                   isfinite(v_scale),
-              NKV_EINVAL, "%s: scales must be finite, k_scale and v_scale > 0", what);
+              NKV_EINVAL, "%s: scales must be finite and > 0", what);
   NKV_REQUIRE(isfinite(lambda_init) && eps > 0.f && isfinite(eps), NKV_EINVAL,
               "%s: lambda_init must be finite and eps > 0", what);
   NKV_REQUIRE(lambdas && (reinterpret_cast<uintptr_t>(lambdas) & 3u) == 0 &&

@@ -1,0 +1,726 @@
+// Differential attention of many query rows (prompts, chunks of them, decode rows among them)
+// over the paged K/V cache or contiguous K/V: bf16/fp16 MFMA, fp32 softmax. The formulas are in
+// diff_common.h; causal, aligned to the bottom right. No counterpart in the reference; it stands
+// beside the varlen attention of nanokvllm/layers/attention.py:96-102 over the same cache.
+//
+// MI355X design (MFMA-bound):
+//  * Workgroup = (sequence, tile of queries, KV pair, range of keys). A tile's R rows are its
+//    queries for all G query pairs of the KV pair, query-major, and each row is computed twice, once
+//    for each map: the first half of the waves takes map 0, the other half map 1 of the same rows.
+//    Both read the same V tile (the pair's value of 2 D dims), and each its own half of every K row, so
+//    that K and V are fetched once for both maps and no product is made with the other map's keys.
+//  * Keys advance in steps of 64. A step's K and V rows (2 D dims each: the pair's two heads lie
+//    beside each other) go straight into LDS, one step ahead, with the chunk permutation of
+//    lds_tiles.h; fp8 codes pass through registers and are widened on the way.
+//  * S^T = K Q^T (A: 16 keys from LDS, B: the wave's Q^T, held in registers) leaves a lane with one
+//    row's scores of 4 keys in every 16; the weights, packed to 16 bits, are the B operand of
+//    O^T += V^T P^T, its A operand read transposed from LDS. A row's running maximum is raised only
+//    when it grows by more than kLazy (log2), its sum is over the rounded weights.
+//  * The end of a tile: map 1's waves leave A_1 in LDS (the tiles' ring, free by then), map 0's
+//    waves subtract, take the mean square over the row's 2 D dims (in the row's 4 lanes), normalise and
+//    store. Nothing but the output is written.
+//  * Few tiles: the keys of each tile are split into up to n_splits ranges of at least min_steps
+//    steps, a partial row (O, m, l) is written for each and map, and a second kernel merges and ends
+//    them. Tiles of one range are ended by the first kernel.
+// Tiles are numbered over the batch without gaps (their number per sequence is known on the device
+// only), each sequence's last ones first: they see the most keys.
+#include "decode_stream.h"
+#include "diff_common.h"
+#include "lds_tiles.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace nkv {
+
+constexpr int kDiffStep = 64;        // keys per step
+constexpr float kDiffLazy = 8.f;     // log2 headroom before a running maximum is raised
+constexpr int kDiffMinSteps = 8;     // shortest range of a split tile
+constexpr int kDiffMergeWaves = 4;
+
+// Waves of a workgroup, and 16-row groups of a wave. At head_dim 128 a step's tiles take 64 KiB, so
+// one workgroup is resident and brings both waves of each SIMD itself.
+constexpr int diff_waves(int D) { return D == 128 ? 8 : 4; }
+constexpr int diff_groups(int D) { return D == 128 ? 2 : 3; }
+constexpr int diff_rows(int D) { return 8 * diff_waves(D) * diff_groups(D); }  // of a tile
+constexpr int diff_part_row(int D) { return 2 * D + 4; }  // floats: O, m, l, 2 pad
+
+struct DiffPrefillArgs {
+  const bf16_t* q;
+  int64_t q_row_stride;
+  const void *k, *v;
+  int64_t k_row_stride, v_row_stride;
+  const int32_t *cu_q, *cu_k, *block_tables;
+  int64_t bt_row_stride;
+  int32_t P, G, block_size, max_blocks, n_limit, n_seqs, total_q;
+  int32_t n_splits, min_steps;
+  float scale_log2, v_scale;
+  DiffArgs diff;
+  bf16_t* out;
+  int64_t out_row_stride;
+  float* part;
+};
+
+// A tile of the batch: queries j0 .. of a sequence (row q0 of q), and its ranges of keys.
+struct DiffTile {
+  int seq, q0, Lq, kb0, Lk, j0;
+  int n_steps, ranges;
+};
+
+// Tile `t` of the batch, QT queries each; false past the last one. By the whole wave.
+__device__ __forceinline__ bool diff_tile(const DiffPrefillArgs& a, int QT, int t, DiffTile& d) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int cb = 0; cb < a.n_seqs; cb += 64) {  // uniform
+    const int s = cb + lane;
+    int q0 = 0, Lq = 0, kb0 = 0, Lk = 0;
+    if (s < a.n_seqs) {
+      q0 = a.cu_q[s];
+      Lq = a.cu_q[s + 1] - q0;
+      kb0 = a.cu_k[s];
+      Lk = a.cu_k[s + 1] - kb0;
+      NKV_DBG(t == 0 && (Lq < 0 || Lk < 0 || Lq > Lk || q0 < 0 || q0 + Lq > a.total_q),
+              NKV_DEBUG_LENGTH);
+      if (q0 < 0 || q0 > a.total_q - Lq) Lq = 0;  // rows outside q
+    }
+    const int nt = Lq > 0 ? (Lq - 1) / QT + 1 : 0;
+    const int incl = wave_incl_scan(nt);
+    const int total = __builtin_amdgcn_readlane(incl, 63);
+    if (t < base + total) {
+      const int ln =
+          __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(base + incl > t)));
+      d.seq = cb + ln;
+      d.q0 = __builtin_amdgcn_readlane(q0, ln);
+      d.Lq = __builtin_amdgcn_readlane(Lq, ln);
+      d.kb0 = __builtin_amdgcn_readlane(kb0, ln);
+      d.Lk = max(__builtin_amdgcn_readlane(Lk, ln), 0);
+      // the sequence's last tile first
+      d.j0 = (base + __builtin_amdgcn_readlane(incl, ln) - 1 - t) * QT;
+      const int last = min(d.Lk - 1, d.Lk - d.Lq + min(d.Lq, d.j0 + QT) - 1);
+      d.n_steps = last >= 0 ? last / kDiffStep + 1 : 0;
+      d.ranges = min(a.n_splits, max(1, d.n_steps / a.min_steps));
+      return true;
+    }
+    base += total;
+  }
+  return false;
+}
+
+// The partial rows of range `sp` of (tile t, pair p), map 0's then map 1's.
+template <int D>
+__device__ __forceinline__ float* diff_part(const DiffPrefillArgs& a, int t, int p, int sp) {
+  return a.part + (((int64_t)t * a.P + p) * a.n_splits + sp) *
+                      (2 * diff_rows(D) * diff_part_row(D));
+}
+
+template <bool F8, int D, bool H16, bool PAGED>
+__global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
+    const DiffPrefillArgs a) {
+  static_assert(!(F8 && (H16 || !PAGED)), "fp8 caches are paged and read with bf16 queries");
+  constexpr int kWaves = diff_waves(D), kRG = diff_groups(D);
+  constexpr int kV = 2 * D;                     // dims of a K or V row of the pair
+  constexpr int kEl = F8 ? 1 : 2;               // bytes per cache element
+  constexpr int kRB = kV * 2;                   // bytes of a staged (16-bit) row
+  constexpr int kNC = kV / 8;                   // 16-byte chunks per staged row
+  constexpr int kTileB = kDiffStep * kRB;       // bytes of a K or V tile
+  constexpr int kStageB = 2 * kTileB;
+  constexpr int kKs = D / 32;                   // k-steps of S^T (of one map's K head)
+  constexpr int kDb = kV / 16;                  // 16-dim blocks of O^T
+  constexpr int kWR = kDiffStep / kWaves;       // rows of a tile that a wave brings
+  constexpr int kRpl = 1024 / kRB;              // rows per 1 KiB load into LDS
+  constexpr int kNl = kWR / kRpl;               // such loads per wave per tile
+  constexpr int kLpr8 = kV / 16;                // F8: lanes per row (16 codes each)
+  constexpr int kRpl8 = 64 / kLpr8;             // F8: rows per load
+  constexpr int kNl8 = kWR / kRpl8;             // F8: loads per wave per tile
+  static_assert(kNl >= 1 && kNl8 >= 1, "a wave brings whole loads");
+  static_assert(kWaves / 2 * kRG * kDb * 1024 <= 2 * kStageB, "A_1 fits the ring");
+  __shared__ __attribute__((aligned(1024))) char ring[2 * kStageB];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g4 = lane >> 4;
+  const int col = lane & 15;
+  const int map = wave / (kWaves / 2);
+  const int wi = wave % (kWaves / 2);  // which rows
+  const int G = a.G, P = a.P;
+  const int QT = diff_rows(D) / G;     // queries per tile
+
+  const int p = blockIdx.x % P;
+  const int sp = blockIdx.x / P % a.n_splits;
+  const int t = blockIdx.x / P / a.n_splits;
+  DiffTile d;
+  if (!diff_tile(a, QT, t, d) || sp >= d.ranges) return;  // uniform
+  const int j0 = d.j0, Lq = d.Lq, Lk = d.Lk;
+  const int n_rows = min(QT, Lq - j0) * G;
+  const int s_lo = (int)((int64_t)d.n_steps * sp / d.ranges);
+  const int s_end = (int)((int64_t)d.n_steps * (sp + 1) / d.ranges);
+  const int diag = Lk - Lq;  // query j sees keys <= diag + j
+
+  // ---- the wave's share of a step's K and V rows: kWR consecutive keys, which lie in one block
+  const uint32_t row_b = (uint32_t)a.k_row_stride * kEl;
+  const uint32_t row_bv = (uint32_t)a.v_row_stride * kEl;
+  const int lrow = lane / kNC;
+  uint32_t vol[kNl];
+#pragma unroll
+  for (int h = 0; h < kNl; ++h) {
+    const int r = kRpl * h + lrow;
+    vol[h] = (uint32_t)r * row_b + (uint32_t)p * kRB +
+             (uint32_t)((lane % kNC) ^ chunk_swz<kV>(r + kWR * wave)) * 16u;
+  }
+  const uint32_t ring_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)ring +
+                             (uint32_t)wave * (kWR * kRB);
+  const int f8_row0 = lane / kLpr8;
+  const int f8_c = lane % kLpr8;
+  [[maybe_unused]] u32x4_t kq[kNl8], vq[kNl8];  // F8: the next step's codes
+
+  const int32_t* bt = PAGED ? a.block_tables + (int64_t)d.seq * a.bt_row_stride : nullptr;
+  int bt_base = 0;   // lane i holds entry bt_base + i of the table row
+  int bt_lane = -1;
+  auto load_window = [&]() {
+    const int e = bt_base + lane;
+    const int id = e < a.max_blocks ? bt[e] : -1;
+    NKV_DBG((int64_t)e * a.block_size < Lk && (e >= a.max_blocks || id < 0 || id >= a.n_limit),
+            e >= a.max_blocks ? NKV_DEBUG_LENGTH : NKV_DEBUG_BLOCK);
+    bt_lane = (id >= 0 && id < a.n_limit) ? id : -1;
+  };
+  int c_t0 = s_lo * kDiffStep + kWR * wave;  // first key of the rows loaded next
+  int c_blk = 0, c_off = 0;                  // their block and place in it
+  if constexpr (PAGED) {
+    c_blk = c_t0 / a.block_size;
+    c_off = c_t0 - c_blk * a.block_size;
+    bt_base = c_blk & ~63;
+    load_window();
+  }
+  const int k_lim = min(Lk, s_end * kDiffStep);
+  auto issue = [&](int stage) {
+    int nv = min(kWR, k_lim - c_t0);
+    int64_t row0;
+    if constexpr (PAGED) {
+      const int pb = __builtin_amdgcn_readlane(bt_lane, c_blk - bt_base);
+      nv = pb < 0 ? 0 : nv;
+      row0 = (int64_t)pb * a.block_size + c_off;
+    } else {
+      const int r0 = d.kb0 + c_t0;
+      NKV_DBG(nv > 0 && (r0 < 0 || r0 > a.n_limit - nv), NKV_DEBUG_BLOCK);
+      nv = (r0 < 0 || r0 > a.n_limit - nv) ? 0 : nv;  // outside the K/V rows
+      row0 = r0;
+    }
+    nv = max(nv, 0);
+    row0 = nv > 0 ? row0 : 0;
+    const char* kp = static_cast<const char*>(a.k) + row0 * a.k_row_stride * kEl;
+    const char* vp = static_cast<const char*>(a.v) + row0 * a.v_row_stride * kEl;
+    if constexpr (F8) {  // into registers; widened into the stage by commit()
+      (void)stage;
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)kp, (short)0, (uint32_t)nv * row_b, kBufferFlags);
+      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)vp, (short)0, (uint32_t)nv * row_bv, kBufferFlags);
+#pragma unroll
+      for (int f = 0; f < kNl8; ++f) {
+        const uint32_t r = (uint32_t)(kRpl8 * f + f8_row0);
+        const uint32_t c = (uint32_t)p * kV + (uint32_t)f8_c * 16u;
+        kq[f] = __builtin_bit_cast(
+            u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, r * row_b + c, 0, 0));
+        vq[f] = __builtin_bit_cast(
+            u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rv, r * row_bv + c, 0, 0));
+      }
+    } else {
+      const i32x4_t dk = buffer_desc(kp, (uint32_t)nv * row_b);
+      const i32x4_t dv = buffer_desc(vp, (uint32_t)nv * row_bv);
+      const uint32_t at = ring_base + (uint32_t)stage * kStageB;
+#pragma unroll
+      for (int h = 0; h < kNl; ++h) load_to_lds(dk, at + 1024u * h, vol[h]);
+#pragma unroll
+      for (int h = 0; h < kNl; ++h)
+        load_to_lds(dv, at + kTileB + 1024u * h,
+                    vol[h] + (uint32_t)(kRpl * h + lrow) * (row_bv - row_b));
+    }
+    c_t0 += kDiffStep;
+    if constexpr (PAGED) {  // blocks crossed: at most 4 (blocks are a multiple of 16)
+      const int B = a.block_size, v = c_off + kDiffStep;
+      const int n = (v >= B) + (v >= 2 * B) + (v >= 3 * B) + (v >= 4 * B);
+      c_off = v - n * B;
+      c_blk = __builtin_amdgcn_readfirstlane(c_blk + n);
+    }
+  };
+  auto refill_window = [&]() {  // uniform; once per 64 blocks
+    if constexpr (PAGED) {
+      if (c_blk - bt_base >= 64) {
+        bt_base = c_blk & ~63;
+        load_window();
+      }
+    }
+  };
+  // F8: the codes of the last issue(), widened into their rows of stage `stage`. Lanes in the
+  // second half of a row write their pair's second chunk first, so that each 16-byte write
+  // instruction covers distinct banks.
+  const bool f8_swap = f8_c >= kLpr8 / 2;
+  auto commit = [&](int stage) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    char* at = ring + stage * kStageB + wave * (kWR * kRB);
+#pragma unroll
+    for (int f = 0; f < kNl8; ++f) {
+      const int r = kRpl8 * f + f8_row0;
+      const int off = r * kRB + ((2 * f8_c) ^ chunk_swz<kV>(r + kWR * wave)) * 16;
+      const int o1 = off + (f8_swap ? 16 : 0), o2 = off + (f8_swap ? 0 : 16);
+      u32x4_t lo, hi;
+      u32x4_t c = kq[f];
+      if (f8_swap) c = u32x4_t{c[2], c[3], c[0], c[1]};
+      fp8x16_to_bf16(c, lo, hi);
+      *reinterpret_cast<u32x4_t*>(at + o1) = lo;
+      *reinterpret_cast<u32x4_t*>(at + o2) = hi;
+      c = vq[f];
+      if (f8_swap) c = u32x4_t{c[2], c[3], c[0], c[1]};
+      fp8x16_to_bf16(c, lo, hi);
+      *reinterpret_cast<u32x4_t*>(at + kTileB + o1) = lo;
+      *reinterpret_cast<u32x4_t*>(at + kTileB + o2) = hi;
+    }
+  };
+  auto landed = [&](int stage) {  // the wave's rows of the stage are in LDS
+    if constexpr (F8) commit(stage);
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
+
+  if (s_lo < s_end) {
+    issue(0);
+    refill_window();
+  }
+
+  // ---- the wave's rows: query pair and query of this lane's row in each group (query-major; rows
+  // past the tile's are attended like its first one and never stored)
+  const bool active = wi * (16 * kRG) < n_rows;  // uniform over the wave
+  int pair[kRG], jrow[kRG];
+  u32x4_t qreg[kRG][kKs];
+#pragma unroll
+  for (int rr = 0; rr < kRG; ++rr) {
+    const int r = (wi * kRG + rr) * 16 + col;
+    const bool real = r < n_rows;
+    pair[rr] = real ? r % G : 0;
+    jrow[rr] = real ? j0 + r / G : Lq;
+    const u32x4_t* qp = reinterpret_cast<const u32x4_t*>(
+        a.q + (int64_t)(d.q0 + (real ? jrow[rr] : j0)) * a.q_row_stride +
+        (int64_t)(2 * (p * G + pair[rr]) + map) * D + g4 * 8);
+#pragma unroll
+    for (int ks = 0; ks < kKs; ++ks) qreg[rr][ks] = qp[ks * 4];
+  }
+
+  // LDS read offsets (bytes from a tile's start). K A operand, 16-key quarter h: row 16h + col,
+  // dims map * D + 32 ks + 8 g4.
+  uint32_t ko[kKs];
+#pragma unroll
+  for (int ks = 0; ks < kKs; ++ks)
+    ko[ks] = (uint32_t)col * kRB +
+             (uint32_t)((map * (D / 8) + g4 + 4 * ks) ^ chunk_swz<kV>(col)) * 16u;
+  // V^T by ds_read_b64_tr_b16: lane 16g + 4r + c reads row 4g + r (and +16), dims 16 db + 4c .. +3
+  const int vrow = 4 * g4 + (col >> 2);
+  uint32_t vo[kDb];
+#pragma unroll
+  for (int db = 0; db < kDb; ++db)
+    vo[db] = (uint32_t)vrow * kRB + (uint32_t)(db ^ (chunk_swz<kV>(vrow) >> 1)) * 32u +
+             (uint32_t)(col & 3) * 8u;
+
+  f32x4_t acc[kRG][kDb];  // O^T: lane l -> row l%16, dims 16 db + 4(l/16) .. +3
+  float m_run[kRG], l_run[kRG], mb_run[kRG];  // mb_run: m_run, or 0 while the row sees no key
+#pragma unroll
+  for (int rr = 0; rr < kRG; ++rr) {
+#pragma unroll
+    for (int db = 0; db < kDb; ++db) acc[rr][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    m_run[rr] = -INFINITY;
+    l_run[rr] = 0.f;
+    mb_run[rr] = 0.f;
+  }
+  // the uses pin the loads of Q here, so that no wait for them lands inside the loop
+#pragma unroll
+  for (int rr = 0; rr < kRG; ++rr)
+#pragma unroll
+    for (int ks = 0; ks < kKs; ++ks) asm volatile("" ::"v"(qreg[rr][ks]));
+  if (s_lo < s_end) landed(0);
+  __syncthreads();
+
+  const char* lds = (const char*)(__attribute__((address_space(3))) char*)ring;
+  auto step = [&](auto stage_c, int s, bool more) {
+    constexpr int ST = decltype(stage_c)::value;
+    if constexpr (F8) issue(ST ^ 1);
+    const char* kt = lds + ST * kStageB;
+    const char* vt = kt + kTileB;
+    f32x4_t st[kRG][4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      u32x4_t ka[kKs];
+#pragma unroll
+      for (int ks = 0; ks < kKs; ++ks)
+        ka[ks] = *reinterpret_cast<const u32x4_t*>(kt + h * (16 * kRB) + ko[ks]);
+      if constexpr (!F8) {
+        if (h == 2) issue(ST ^ 1);
+      }
+#pragma unroll
+      for (int rr = 0; rr < kRG; ++rr) {
+        f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < kKs; ++ks) x = mfma_16x16x32<H16>(ka[ks], qreg[rr][ks], x);
+        st[rr][h] = x;
+      }
+    }
+    const bool edge = (s * kDiffStep + kDiffStep - 1 > diag + j0) ||
+                      (s * kDiffStep + kDiffStep > Lk);  // uniform
+    float sv[kRG][16];
+#pragma unroll
+    for (int rr = 0; rr < kRG; ++rr)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sv[rr][e] = st[rr][e / 4][e % 4];
+    if (edge) {
+#pragma unroll
+      for (int rr = 0; rr < kRG; ++rr) {
+        const int lim = min(diag + jrow[rr], Lk - 1);  // the row's last visible key
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (s * kDiffStep + 16 * (e / 4) + 4 * g4 + e % 4 > lim) sv[rr][e] = -INFINITY;
+      }
+    }
+    // a lane tests its own scores against the headroom; only when some lane's exceed it does the
+    // wave take the rows' maxima and rescale
+    float lmax[kRG];
+    bool lraise = false;
+#pragma unroll
+    for (int rr = 0; rr < kRG; ++rr) {
+      const float* x = sv[rr];
+      lmax[rr] = fmax3(fmax3(fmax3(x[0], x[1], x[2]), fmax3(x[3], x[4], x[5]),
+                             fmax3(x[6], x[7], x[8])),
+                       fmax3(x[9], x[10], x[11]),
+                       fmax3(fmax3(x[12], x[13], x[14]), x[15], -INFINITY));
+      lraise = lraise || (lmax[rr] * a.scale_log2 > m_run[rr] + kDiffLazy);
+    }
+    if (__builtin_amdgcn_ballot_w64(lraise) != 0) {
+#pragma unroll
+      for (int rr = 0; rr < kRG; ++rr) {
+        const float cm = col_max4(lmax[rr]) * a.scale_log2;
+        const bool raise = cm > m_run[rr] + kDiffLazy;
+        const float alpha = raise ? fast_exp2(m_run[rr] - cm) : 1.f;
+        m_run[rr] = raise ? cm : m_run[rr];
+        mb_run[rr] = m_run[rr] == -INFINITY ? 0.f : m_run[rr];
+        l_run[rr] *= alpha;
+#pragma unroll
+        for (int db = 0; db < kDb; ++db) acc[rr][db] *= alpha;
+      }
+    }
+    // 32 keys at a time: k-slot j of lane group g is key 32c+4g+j (j<4), or 32c+16+4g+(j-4)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      u32x4_t pb[kRG];
+#pragma unroll
+      for (int rr = 0; rr < kRG; ++rr) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          w[e] = fast_exp2(fmaf(sv[rr][8 * c + e], a.scale_log2, -mb_run[rr]));  // -inf -> 0
+        pb[rr] = u32x4_t{cvt_pk16<H16>(w[0], w[1]), cvt_pk16<H16>(w[2], w[3]),
+                         cvt_pk16<H16>(w[4], w[5]), cvt_pk16<H16>(w[6], w[7])};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) l_run[rr] = sum2_16<H16>(pb[rr][e], l_run[rr]);
+      }
+#pragma unroll
+      for (int db = 0; db < kDb; ++db) {
+        const char* vc = vt + c * (32 * kRB) + vo[db];
+        const i16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)vc);
+        const i16x4_t v1 =
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(vc + 16 * kRB));
+        const u32x4_t va = {__builtin_bit_cast(uint2, v0).x, __builtin_bit_cast(uint2, v0).y,
+                            __builtin_bit_cast(uint2, v1).x, __builtin_bit_cast(uint2, v1).y};
+#pragma unroll
+        for (int rr = 0; rr < kRG; ++rr)
+          acc[rr][db] = mfma_16x16x32<H16>(va, pb[rr], acc[rr][db]);
+      }
+    }
+    // the next step's rows landed (each wave waits for its own), then the barrier publishes them and
+    // frees this stage
+    if (!F8 || more) landed(ST ^ 1);
+    __syncthreads();
+    refill_window();
+  };
+  if (active) {
+    for (int s = s_lo; s < s_end; s += 2) {
+      step(std::integral_constant<int, 0>{}, s, s + 1 < s_end);
+      if (s + 1 >= s_end) break;
+      step(std::integral_constant<int, 1>{}, s + 1, s + 2 < s_end);
+    }
+  } else {  // a wave without rows only brings its share of the tiles
+    for (int s = s_lo; s < s_end; ++s) {
+      const int next = (s - s_lo + 1) & 1;
+      issue(next);
+      landed(next);
+      __syncthreads();
+      refill_window();
+    }
+  }
+
+  // ---- the end
+  float l[kRG];
+#pragma unroll
+  for (int rr = 0; rr < kRG; ++rr) l[rr] = col_sum4(l_run[rr]);
+  if (d.ranges > 1) {  // a part: O, m and l as they are
+    if (!active) return;
+    float* rows = diff_part<D>(a, t, p, sp) + (int64_t)map * (diff_rows(D) * diff_part_row(D));
+#pragma unroll
+    for (int rr = 0; rr < kRG; ++rr) {
+      if (jrow[rr] >= Lq) continue;
+      float* pr = rows + ((wi * kRG + rr) * 16 + col) * diff_part_row(D);
+#pragma unroll
+      for (int db = 0; db < kDb; ++db)
+        *reinterpret_cast<f32x4_t*>(pr + db * 16 + g4 * 4) = acc[rr][db];
+      if (g4 == 0) *reinterpret_cast<float2*>(pr + kV) = float2{m_run[rr], l[rr]};
+    }
+    return;
+  }
+  float inv[kRG];
+#pragma unroll
+  for (int rr = 0; rr < kRG; ++rr) inv[rr] = l[rr] > 0.f ? a.v_scale / l[rr] : 0.f;
+  // the last step's barrier has freed the ring: A_1, lane by lane as it is held
+  f32x4_t* other = reinterpret_cast<f32x4_t*>(ring) + wi * (kRG * kDb * 64) + lane;
+  if (map == 1 && active) {
+#pragma unroll
+    for (int rr = 0; rr < kRG; ++rr)
+#pragma unroll
+      for (int db = 0; db < kDb; ++db) other[(rr * kDb + db) * 64] = acc[rr][db] * inv[rr];
+  }
+  __syncthreads();
+  if (map == 1 || !active) return;
+  const float lambda = diff_lambda<D>(a.diff);
+#pragma unroll
+  for (int rr = 0; rr < kRG; ++rr) {
+    float ss = 0.f;
+#pragma unroll
+    for (int db = 0; db < kDb; ++db) {
+      const f32x4_t x = acc[rr][db] * inv[rr] - other[(rr * kDb + db) * 64] * lambda;
+      acc[rr][db] = x;
+      ss += (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
+    }
+    inv[rr] = (1.f - a.diff.init) / sqrtf(col_sum4(ss) * (1.f / kV) + a.diff.eps);
+  }
+#pragma unroll
+  for (int db = 0; db < kDb; ++db) {
+    float w[4];
+    const int dim = db * 16 + g4 * 4;
+    diff_weight<4, H16>(a.diff.weight ? a.diff.weight + dim : nullptr, w);
+#pragma unroll
+    for (int rr = 0; rr < kRG; ++rr) {
+      if (jrow[rr] >= Lq) continue;
+      bf16_t* op = a.out + (int64_t)(d.q0 + jrow[rr]) * a.out_row_stride +
+                   (int64_t)(p * G + pair[rr]) * kV + dim;
+      float o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = acc[rr][db][e] * w[e];
+      store_dims<4, H16>(op, o, inv[rr]);
+    }
+  }
+}
+
+// Merges and ends the rows of tiles that have several ranges: one row a wave, lane l dims N*l ..,
+// both maps' partials of four ranges in flight.
+template <int D, bool H16>
+__global__ __launch_bounds__(64 * kDiffMergeWaves) void diff_merge_kernel(
+    const DiffPrefillArgs a) {
+  constexpr int N = D / 32;
+  constexpr int kV = 2 * D;
+  constexpr int kRow = diff_part_row(D);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int G = a.G, P = a.P;
+  const int QT = diff_rows(D) / G;
+  const int p = blockIdx.x % P;
+  const int t = blockIdx.x / P;
+  const int r = (int)blockIdx.y * kDiffMergeWaves + wave;
+  DiffTile d;
+  if (!diff_tile(a, QT, t, d) || d.ranges < 2 || r >= min(QT, d.Lq - d.j0) * G) return;
+  const float* part = diff_part<D>(a, t, p, 0) + (int64_t)r * kRow;
+  const int64_t map_f = (int64_t)diff_rows(D) * kRow;
+  float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f}, o[2][N] = {};
+  for (int s0 = 0; s0 < d.ranges; s0 += 4) {
+    float2 ml[4][2];
+    float v[4][2][N];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const float* row = part + (2 * (int64_t)min(s0 + u, d.ranges - 1) + m) * map_f;
+        ml[u][m] = *reinterpret_cast<const float2*>(row + kV);
+        load_dims<N>(row + N * lane, v[u][m]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        if (s0 + u >= d.ranges || ml[u][m].x == -INFINITY) continue;  // uniform
+        const float top = fmaxf(M[m], ml[u][m].x);
+        const float alpha = fast_exp2(M[m] - top), w = fast_exp2(ml[u][m].x - top);
+        M[m] = top;
+        L[m] = fmaf(w, ml[u][m].y, L[m] * alpha);
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[m][e] = fmaf(w, v[u][m][e], o[m][e] * alpha);
+      }
+    }
+  }
+  const float lambda = diff_lambda<D>(a.diff);
+  float w[N], x[N], ss = 0.f;
+  const float i0 = L[0] > 0.f ? a.v_scale / L[0] : 0.f;
+  const float i1 = L[1] > 0.f ? a.v_scale / L[1] : 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    x[e] = fmaf(-lambda, o[1][e] * i1, o[0][e] * i0);
+    ss = fmaf(x[e], x[e], ss);
+  }
+  const float norm = (1.f - a.diff.init) / sqrtf(wave_sum(ss) * (1.f / kV) + a.diff.eps);
+  diff_weight<N, H16>(a.diff.weight ? a.diff.weight + N * lane : nullptr, w);
+#pragma unroll
+  for (int e = 0; e < N; ++e) x[e] *= w[e];
+  store_dims<N, H16>(a.out + (int64_t)(d.q0 + d.j0 + r / G) * a.out_row_stride +
+                         (int64_t)(p * G + r % G) * kV + N * lane,
+                     x, norm);
+}
+
+// Tiles that a batch can have, and the ranges that a tile is cut into.
+static int64_t diff_max_tiles(int64_t total_q, int64_t n_seqs, int qt) {
+  return total_q / qt + n_seqs;
+}
+static int diff_splits(int64_t total_q, int64_t n_seqs, int64_t max_seqlen_k, int pairs, int G,
+                       int D) {
+  const int64_t groups = diff_max_tiles(total_q, n_seqs, diff_rows(D) / G) * pairs;
+  const int64_t resident = (int64_t)device_cus() * (D == 128 ? 1 : 2);
+  const int64_t most = max_seqlen_k / (kDiffStep * kDiffMinSteps);
+  return (int)std::max<int64_t>(1, std::min(most, (2 * resident + groups - 1) / groups));
+}
+
+template <bool F8, int D, bool H16, bool PAGED>
+static void diff_launch(const DiffPrefillArgs& a, int64_t tiles, hipStream_t s) {
+  hipLaunchKernelGGL((diff_prefill_kernel<F8, D, H16, PAGED>),
+                     dim3((unsigned)(tiles * a.P * a.n_splits)), dim3(64 * diff_waves(D)), 0, s,
+                     a);
+  if (a.n_splits > 1)
+    hipLaunchKernelGGL((diff_merge_kernel<D, H16>),
+                       dim3((unsigned)(tiles * a.P), diff_rows(D) / kDiffMergeWaves),
+                       dim3(64 * kDiffMergeWaves), 0, s, a);
+}
+
+}  // namespace nkv
+
+extern "C" size_t nkv_diff_prefill_workspace_bytes(int32_t n_seqs, int64_t total_q,
+                                                   int64_t max_seqlen_k, int32_t n_q_heads,
+                                                   int32_t n_kv_heads, int32_t head_dim) {
+  using namespace nkv;
+  if (n_seqs <= 0 || total_q <= 0 || n_kv_heads <= 0 || n_kv_heads % 2 || n_q_heads <= 0 ||
+      n_q_heads % n_kv_heads || n_q_heads / n_kv_heads > NKV_DIFF_MAX_GROUP ||
+      (head_dim != 64 && head_dim != 128))
+    return 0;
+  const int G = n_q_heads / n_kv_heads, P = n_kv_heads / 2;
+  const int splits = diff_splits(total_q, n_seqs, max_seqlen_k, P, G, head_dim);
+  if (splits < 2) return 0;
+  return (size_t)diff_max_tiles(total_q, n_seqs, diff_rows(head_dim) / G) * P * splits * 2 *
+         diff_rows(head_dim) * diff_part_row(head_dim) * sizeof(float);
+}
+
+extern "C" int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_stride,
+                                int64_t total_q, const void* k, const void* v,
+                                int64_t k_row_stride, int64_t v_row_stride,
+                                const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                const int32_t* block_tables, int64_t bt_row_stride,
+                                int32_t max_blocks_per_seq, int32_t n_seqs, int64_t max_seqlen_k,
+                                int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                int32_t block_size, int64_t n_rows, float scale, float k_scale,
+                                float v_scale, const float* lambdas, float lambda_init,
+                                const void* norm_weight, float eps, void* out,
+                                int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  using namespace nkv;
+  clear_error();
+  int rc = diff_check("diff_prefill", kv_type, n_q_heads, n_kv_heads, head_dim, scale, k_scale,
+                      v_scale, lambdas, lambda_init, norm_weight, eps);
+  if (rc) return rc;
+  const bool paged = block_tables != nullptr, f8 = kv_type == NKV_KV_FP8;
+  const int G = n_q_heads / n_kv_heads, P = n_kv_heads / 2;
+  const int64_t row = (int64_t)n_kv_heads * head_dim;
+  NKV_REQUIRE(n_seqs >= 0 && total_q >= 0 && n_rows >= 0 && total_q < (1ll << 31), NKV_EINVAL,
+              "diff_prefill: bad sizes (n_seqs=%d, total_q=%lld, n_rows=%lld)", n_seqs,
+              (long long)total_q, (long long)n_rows);
+  if (n_seqs == 0 || total_q == 0) return NKV_OK;
+  NKV_REQUIRE(q && k && v && cu_seqlens_q && cu_seqlens_k && out, NKV_EINVAL,
+              "diff_prefill: null pointer");
+  NKV_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) &&
+                  (reinterpret_cast<uintptr_t>(out) & 7u) == 0,
+              NKV_EINVAL, "diff_prefill: q, k and v must be 16-byte aligned, out 8-byte");
+  NKV_REQUIRE(q_row_stride >= (int64_t)n_q_heads * head_dim && q_row_stride % 8 == 0 &&
+                  out_row_stride >= (int64_t)n_q_heads * head_dim && out_row_stride % 4 == 0,
+              NKV_EINVAL, "diff_prefill: row strides must be >= Hq*D, q's a multiple of 8, out's "
+              "of 4");
+  NKV_REQUIRE(k_row_stride >= row && v_row_stride >= row && k_row_stride % 8 == 0 &&
+                  v_row_stride % 8 == 0 && k_row_stride < (1 << 24) && v_row_stride < (1 << 24),
+              NKV_EINVAL, "diff_prefill: k and v row strides must be multiples of 8 from Hk*D to "
+              "2^24");
+  if (paged) {
+    NKV_REQUIRE(block_size > 0 && block_size % 16 == 0, NKV_EUNSUPPORTED,
+                "diff_prefill: block_size must be a multiple of 16 (got %d)", block_size);
+    NKV_REQUIRE(max_blocks_per_seq > 0 && bt_row_stride >= max_blocks_per_seq, NKV_EINVAL,
+                "diff_prefill: bad block table width/stride (%d, %lld)", max_blocks_per_seq,
+                (long long)bt_row_stride);
+    NKV_REQUIRE(k_row_stride == row && v_row_stride == row, NKV_EINVAL,
+                "diff_prefill: paged rows are Hk*D apart");
+    // fp8 rows are read 16 codes at a time
+    NKV_REQUIRE(n_rows / block_size < (1ll << 31), NKV_EUNSUPPORTED,
+                "diff_prefill: too many blocks");
+  } else {
+    NKV_REQUIRE(!f8, NKV_EUNSUPPORTED, "diff_prefill: fp8 rows must be paged");
+    NKV_REQUIRE(n_rows < (1ll << 31), NKV_EUNSUPPORTED, "diff_prefill: too many K/V rows");
+  }
+  DiffPrefillArgs a{};
+  a.n_splits = 1;
+  if (workspace) {
+    const size_t need = nkv_diff_prefill_workspace_bytes(n_seqs, total_q, max_seqlen_k, n_q_heads,
+                                                         n_kv_heads, head_dim);
+    NKV_REQUIRE(workspace_bytes >= need && aligned16(workspace), NKV_EWORKSPACE,
+                "diff_prefill: workspace needs %zu bytes, 16-byte aligned (got %zu)", need,
+                workspace_bytes);
+    a.n_splits = diff_splits(total_q, n_seqs, max_seqlen_k, P, G, head_dim);
+  }
+  const int64_t tiles = diff_max_tiles(total_q, n_seqs, diff_rows(head_dim) / G);
+  NKV_REQUIRE(tiles * P * a.n_splits < (1ll << 31), NKV_EUNSUPPORTED,
+              "diff_prefill: too many tiles");
+  a.q = (const bf16_t*)q;
+  a.q_row_stride = q_row_stride;
+  a.k = k;
+  a.v = v;
+  a.k_row_stride = k_row_stride;
+  a.v_row_stride = v_row_stride;
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.block_tables = block_tables;
+  a.bt_row_stride = bt_row_stride;
+  a.P = P;
+  a.G = G;
+  a.block_size = block_size;
+  a.max_blocks = max_blocks_per_seq;
+  a.n_limit = (int32_t)(paged ? n_rows / block_size : n_rows);
+  a.n_seqs = n_seqs;
+  a.total_q = (int32_t)total_q;
+  a.min_steps = kDiffMinSteps;
+  a.scale_log2 = scale * (f8 ? k_scale : 1.f) * kLog2e;
+  a.v_scale = f8 ? v_scale : 1.f;
+  a.diff = DiffArgs{lambdas, (const bf16_t*)norm_weight, lambda_init, eps};
+  a.out = (bf16_t*)out;
+  a.out_row_stride = out_row_stride;
+  a.part = static_cast<float*>(workspace);
+  hipStream_t s = as_stream(stream);
+#define NKV_DIFF_LAUNCH(D)                                            \
+  do {                                                                \
+    if (f8) diff_launch<true, D, false, true>(a, tiles, s);           \
+    else if (kv_type == NKV_KV_F16)                                   \
+      paged ? diff_launch<false, D, true, true>(a, tiles, s)          \
+            : diff_launch<false, D, true, false>(a, tiles, s);        \
+    else                                                              \
+      paged ? diff_launch<false, D, false, true>(a, tiles, s)         \
+            : diff_launch<false, D, false, false>(a, tiles, s);       \
+  } while (0)
+  if (head_dim == 64) NKV_DIFF_LAUNCH(64);
+  else NKV_DIFF_LAUNCH(128);
+#undef NKV_DIFF_LAUNCH
+  return check_launch("nkv_diff_prefill");
+}

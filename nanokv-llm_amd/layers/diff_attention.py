@@ -120,3 +120,131 @@ def diff_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     if rc:
         _lib.check(rc, what)
     return out
+
+
+def diff_prefill_workspace(q: torch.Tensor, k: torch.Tensor, n_seqs: int,
+                           max_seqlen_k: int) -> torch.Tensor | None:
+    """The workspace for splitting diff_varlen_prefill's keys where that is of use (few query tiles
+    over long contexts), else None. Sized by the chip and the tiles, not by the lengths; None
+    too where the device has no such memory left, since nothing else needs any."""
+    nbytes = _lib.lib().nkv_diff_prefill_workspace_bytes(n_seqs, q.size(0), int(max_seqlen_k),
+                                                         q.size(1), k.size(-2), q.size(2))
+    try:
+        return torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    except torch.OutOfMemoryError:
+        return None
+
+
+def diff_varlen_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                        cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor,
+                        max_seqlen_q: int, scale: float, lambdas: torch.Tensor,
+                        lambda_init: float, norm_weight: torch.Tensor | None = None,
+                        eps: float = 1e-5, block_tables: torch.Tensor | None = None,
+                        out: torch.Tensor | None = None, max_seqlen_k: int | None = None,
+                        k_scale: float = 1.0, v_scale: float = 1.0,
+                        workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Varlen causal (bottom-right) differential attention: q [sum Lq, Hq, D] -> [sum Lq, Hq/2,
+    2 D].
+
+    With ``block_tables`` k and v are the paged caches [NB, B, Hk, D] (q's dtype, or fp8 with bf16
+    q); without, they are [sum Lk, Hk, D] rows, each with its own row stride. ``lambdas`` and
+    ``norm_weight`` are ``diff_paged_decode``'s, the rest ``varlen_prefill``'s (``max_seqlen_q`` is
+    not needed here: the rows of q say how many tiles there are). Given ``max_seqlen_k``, the keys
+    are split over the chip where few tiles would leave it idle, in ``workspace``
+    (diff_prefill_workspace) or in memory taken for the call; without, nothing but the output is
+    allocated. A row that sees no key gives zeros.
+    """
+    what = "diff_varlen_prefill"
+    paged = block_tables is not None
+    N, Hq, D, Hk, kv_type = _check(what, q, k, v, lambdas, norm_weight, out, paged,
+                                   cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k,
+                                   block_tables=block_tables, workspace=workspace)
+    _int32_rows(what, "cu_seqlens_q", cu_seqlens_q)
+    _int32_rows(what, "cu_seqlens_k", cu_seqlens_k)
+    n_seqs = cu_seqlens_q.numel() - 1
+    _lib.need(n_seqs >= 0 and cu_seqlens_k.numel() == n_seqs + 1,
+              f"{what}: cu_seqlens_q and cu_seqlens_k need one entry per sequence + 1")
+    if paged:
+        _int32_rows(what, "block_tables", block_tables, 2)
+        _lib.need(block_tables.size(0) >= n_seqs,
+                  f"{what}: block_tables needs a row for each of the {n_seqs} sequences")
+        B, rows = k.size(1), k.size(0) * k.size(1)
+        k_stride = v_stride = Hk * D
+        bt, bt_stride, width = (block_tables.data_ptr(), block_tables.stride(0),
+                                block_tables.size(1))
+    else:
+        B, rows, k_stride, v_stride = 0, k.size(0), k.stride(0), v.stride(0)
+        bt, bt_stride, width = None, 0, 0
+    if out is None:
+        out = torch.empty(N, Hq // 2, 2 * D, dtype=q.dtype, device=q.device)
+    _lib.need(workspace is None or (workspace.dtype == torch.uint8 and workspace.is_contiguous()),
+              f"{what}: workspace must be contiguous uint8")
+    with _lib.device_of(q.get_device()):
+        if workspace is None and max_seqlen_k is not None:
+            workspace = diff_prefill_workspace(q, k, n_seqs, max_seqlen_k)
+        rc = _lib.lib().nkv_diff_prefill(
+            kv_type, q.data_ptr(), q.stride(0), N, k.data_ptr(), v.data_ptr(), k_stride, v_stride,
+            cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), bt, bt_stride, width, n_seqs,
+            0 if max_seqlen_k is None else int(max_seqlen_k), Hq, Hk, D, B, rows, scale, k_scale,
+            v_scale, lambdas.data_ptr(), lambda_init, _lib.ptr(norm_weight), eps, out.data_ptr(),
+            out.stride(0), _lib.ptr(workspace), 0 if workspace is None else workspace.numel(),
+            _lib.stream_of(q))
+    if rc:
+        _lib.check(rc, what)
+    return out
+
+
+class DifferentialAttention(nn.Module):
+    """One layer's differential attention: store, then prefill or decode, by the context that
+    ``Attention`` goes by (same ``k_cache``/``v_cache`` attributes, assigned by
+    ``KVCachePool.bind`` or the model runner).
+
+    ``num_heads`` and ``num_kv_heads`` count q's and the cache's heads (both even, two to a pair).
+    ``lambdas`` (float32 [4, head_dim]) and ``norm_weight`` ([2 head_dim], the model's dtype)
+    are parameters to load; gradients are not computed. There is no compression of such a cache.
+    """
+
+    def __init__(self, num_heads: int, head_dim: int, scale: float, num_kv_heads: int,
+                 lambda_init: float, norm_eps: float = 1e-5):
+        super().__init__()
+        _lib.need(head_dim in (64, 128),
+                  f"DifferentialAttention: head_dim {head_dim} is not 64 or 128")
+        _lib.need(num_heads > 0 and num_kv_heads > 0 and num_heads % 2 == 0
+                  and num_kv_heads % 2 == 0 and num_heads % num_kv_heads == 0
+                  and num_heads // num_kv_heads <= MAX_GROUP,
+                  f"DifferentialAttention: {num_heads} query and {num_kv_heads} KV heads are not "
+                  f"pairs with 1 to {MAX_GROUP} query pairs to a KV pair")
+        _lib.need(scale > 0 and norm_eps > 0,
+                  "DifferentialAttention: scale and norm_eps must be > 0")
+        self.num_heads, self.head_dim, self.num_kv_heads = num_heads, head_dim, num_kv_heads
+        self.scale, self.lambda_init, self.norm_eps = scale, lambda_init, norm_eps
+        self.lambdas = nn.Parameter(torch.zeros(4, head_dim, dtype=torch.float32),
+                                    requires_grad=False)
+        self.norm_weight = nn.Parameter(torch.ones(2 * head_dim), requires_grad=False)
+        self.k_cache = self.v_cache = torch.tensor([])
+        self.k_scale = self.v_scale = 1.0
+
+    def forward(self, q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None, Layer=None,
+                kv_stored: bool = False):
+        """q [N, Hq, D], k and v [N, Hk, D] -> [N, Hq/2, 2 D] (decode: [N, 1, Hq/2, 2 D], as
+        ``Attention``). ``kv_stored=True``: k and v are in the cache already."""
+        ctx = get_context()
+        _lib.need(not ctx.is_compress_step, "DifferentialAttention: its cache takes no part in "
+                  "compression steps")
+        kc, vc = self.k_cache, self.v_cache
+        if kc.numel() and not kv_stored:
+            store_kvcache(k, v, kc, vc, ctx.slot_mapping, self.k_scale, self.v_scale)
+        weights = (self.lambdas, self.lambda_init, self.norm_weight, self.norm_eps)
+        if ctx.use_decode_kernel:
+            bt = ctx.block_tables
+            workspace = shared_decode_workspace(q.device, diff_decode_workspace_bytes(
+                q.size(0), q.size(1), bt.size(1), kc.size(1), q.size(2)))
+            return diff_paged_decode(q, kc, vc, ctx.context_lens, bt, self.scale, *weights,
+                                     workspace=workspace, k_scale=self.k_scale,
+                                     v_scale=self.v_scale).unsqueeze(1)
+        if ctx.block_tables is not None:
+            k, v = kc, vc
+        return diff_varlen_prefill(q, k, v, ctx.cu_seqlens_q, ctx.cu_seqlens_k, ctx.max_seqlen_q,
+                                   self.scale, *weights, block_tables=ctx.block_tables,
+                                   max_seqlen_k=ctx.max_seqlen_k, k_scale=self.k_scale,
+                                   v_scale=self.v_scale)
