@@ -10,8 +10,11 @@
 //    Both read the same V tile (the pair's value of 2 D dims), and each its own half of every K row, so
 //    that K and V are fetched once for both maps and no product is made with the other map's keys.
 //  * Keys advance in steps of 64. A step's K and V rows (2 D dims each: the pair's two heads lie
-//    beside each other) go straight into LDS, one step ahead, with the chunk permutation of
-//    lds_tiles.h; fp8 codes pass through registers and are widened on the way.
+//    beside each other) go straight into LDS, one step ahead or more, with the chunk permutation
+//    of lds_tiles.h; fp8 codes pass through registers and are widened on the way.
+//  * head_dim 64: four waves of three row groups, two workgroups a CU, which drift apart by
+//    themselves. head_dim 128: eight waves of two row groups, one workgroup a CU, the maps' waves
+//    half a step apart (see the half steps below).
 //  * S^T = K Q^T (A: 16 keys from LDS, B: the wave's Q^T, held in registers) leaves a lane with one
 //    row's scores of 4 keys in every 16; the weights, packed to 16 bits, are the B operand of
 //    O^T += V^T P^T, its A operand read transposed from LDS. A row's running maximum is raised only
@@ -118,12 +121,14 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
     const DiffPrefillArgs a) {
   static_assert(!(F8 && (H16 || !PAGED)), "fp8 caches are paged and read with bf16 queries");
   constexpr int kWaves = diff_waves(D), kRG = diff_groups(D);
+  constexpr bool kPing = kWaves == 8;
   constexpr int kV = 2 * D;                     // dims of a K or V row of the pair
   constexpr int kEl = F8 ? 1 : 2;               // bytes per cache element
   constexpr int kRB = kV * 2;                   // bytes of a staged (16-bit) row
   constexpr int kNC = kV / 8;                   // 16-byte chunks per staged row
   constexpr int kTileB = kDiffStep * kRB;       // bytes of a K or V tile
-  constexpr int kStageB = 2 * kTileB;
+  constexpr int kTiles = kPing ? 5 : 4;         // places in the ring
+  [[maybe_unused]] constexpr int kStageB = 2 * kTileB;  // a step's K and V tiles
   constexpr int kKs = D / 32;                   // k-steps of S^T (of one map's K head)
   constexpr int kDb = kV / 16;                  // 16-dim blocks of O^T
   constexpr int kWR = kDiffStep / kWaves;       // rows of a tile that a wave brings
@@ -133,8 +138,8 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   constexpr int kRpl8 = 64 / kLpr8;             // F8: rows per load
   constexpr int kNl8 = kWR / kRpl8;             // F8: loads per wave per tile
   static_assert(kNl >= 1 && kNl8 >= 1, "a wave brings whole loads");
-  static_assert(kWaves / 2 * kRG * kDb * 1024 <= 2 * kStageB, "A_1 fits the ring");
-  __shared__ __attribute__((aligned(1024))) char ring[2 * kStageB];
+  static_assert(kWaves / 2 * kRG * kDb * 1024 <= kTiles * kTileB, "A_1 fits the ring");
+  __shared__ __attribute__((aligned(1024))) char ring[kTiles * kTileB];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -172,6 +177,7 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
                              (uint32_t)wave * (kWR * kRB);
   const int f8_row0 = lane / kLpr8;
   const int f8_c = lane % kLpr8;
+  const uint32_t f8_off = (uint32_t)p * kV + (uint32_t)f8_c * 16u;
   [[maybe_unused]] u32x4_t kq[kNl8], vq[kNl8];  // F8: the next step's codes
 
   const int32_t* bt = PAGED ? a.block_tables + (int64_t)d.seq * a.bt_row_stride : nullptr;
@@ -193,9 +199,11 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
     load_window();
   }
   const int k_lim = min(Lk, s_end * kDiffStep);
-  auto issue = [&](int stage) {
-    int nv = min(kWR, k_lim - c_t0);
-    int64_t row0;
+  // The rows of the next step: their K into the tile at byte `at` of the ring, and then their V.
+  int64_t row0 = 0;
+  int nv = 0;  // valid ones of the wave's rows
+  auto issue_k = [&](uint32_t at) {
+    nv = min(kWR, k_lim - c_t0);
     if constexpr (PAGED) {
       const int pb = __builtin_amdgcn_readlane(bt_lane, c_blk - bt_base);
       nv = pb < 0 ? 0 : nv;
@@ -209,32 +217,19 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
     nv = max(nv, 0);
     row0 = nv > 0 ? row0 : 0;
     const char* kp = static_cast<const char*>(a.k) + row0 * a.k_row_stride * kEl;
-    const char* vp = static_cast<const char*>(a.v) + row0 * a.v_row_stride * kEl;
     if constexpr (F8) {  // into registers; widened into the stage by commit()
-      (void)stage;
       const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
           (void*)kp, (short)0, (uint32_t)nv * row_b, kBufferFlags);
-      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)vp, (short)0, (uint32_t)nv * row_bv, kBufferFlags);
 #pragma unroll
-      for (int f = 0; f < kNl8; ++f) {
-        const uint32_t r = (uint32_t)(kRpl8 * f + f8_row0);
-        const uint32_t c = (uint32_t)p * kV + (uint32_t)f8_c * 16u;
+      for (int f = 0; f < kNl8; ++f)
         kq[f] = __builtin_bit_cast(
-            u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, r * row_b + c, 0, 0));
-        vq[f] = __builtin_bit_cast(
-            u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rv, r * row_bv + c, 0, 0));
-      }
+            u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                         rk, (uint32_t)(kRpl8 * f + f8_row0) * row_b + f8_off, 0, 0));
     } else {
       const i32x4_t dk = buffer_desc(kp, (uint32_t)nv * row_b);
-      const i32x4_t dv = buffer_desc(vp, (uint32_t)nv * row_bv);
-      const uint32_t at = ring_base + (uint32_t)stage * kStageB;
-#pragma unroll
-      for (int h = 0; h < kNl; ++h) load_to_lds(dk, at + 1024u * h, vol[h]);
 #pragma unroll
       for (int h = 0; h < kNl; ++h)
-        load_to_lds(dv, at + kTileB + 1024u * h,
-                    vol[h] + (uint32_t)(kRpl * h + lrow) * (row_bv - row_b));
+        load_to_lds(dk, ring_base + at + 1024u * h, vol[h]);
     }
     c_t0 += kDiffStep;
     if constexpr (PAGED) {  // blocks crossed: at most 4 (blocks are a multiple of 16)
@@ -242,6 +237,24 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
       const int n = (v >= B) + (v >= 2 * B) + (v >= 3 * B) + (v >= 4 * B);
       c_off = v - n * B;
       c_blk = __builtin_amdgcn_readfirstlane(c_blk + n);
+    }
+  };
+  auto issue_v = [&](uint32_t at) {
+    const char* vp = static_cast<const char*>(a.v) + row0 * a.v_row_stride * kEl;
+    if constexpr (F8) {
+      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)vp, (short)0, (uint32_t)nv * row_bv, kBufferFlags);
+#pragma unroll
+      for (int f = 0; f < kNl8; ++f)
+        vq[f] = __builtin_bit_cast(
+            u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                         rv, (uint32_t)(kRpl8 * f + f8_row0) * row_bv + f8_off, 0, 0));
+    } else {
+      const i32x4_t dv = buffer_desc(vp, (uint32_t)nv * row_bv);
+#pragma unroll
+      for (int h = 0; h < kNl; ++h)
+        load_to_lds(dv, ring_base + at + 1024u * h,
+                    vol[h] + (uint32_t)(kRpl * h + lrow) * (row_bv - row_b));
     }
   };
   auto refill_window = [&]() {  // uniform; once per 64 blocks
@@ -252,38 +265,26 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
       }
     }
   };
-  // F8: the codes of the last issue(), widened into their rows of stage `stage`. Lanes in the
-  // second half of a row write their pair's second chunk first, so that each 16-byte write
-  // instruction covers distinct banks.
+  // F8: codes in registers, widened into the wave's rows of an LDS tile. Lanes in the second half of
+  // a row write their pair's second chunk first, so that each 16-byte write instruction covers
+  // distinct banks.
   const bool f8_swap = f8_c >= kLpr8 / 2;
-  auto commit = [&](int stage) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    char* at = ring + stage * kStageB + wave * (kWR * kRB);
+  auto commit = [&](const u32x4_t (&codes)[kNl8], char* tile) {
+    char* at = tile + wave * (kWR * kRB);
 #pragma unroll
     for (int f = 0; f < kNl8; ++f) {
       const int r = kRpl8 * f + f8_row0;
       const int off = r * kRB + ((2 * f8_c) ^ chunk_swz<kV>(r + kWR * wave)) * 16;
-      const int o1 = off + (f8_swap ? 16 : 0), o2 = off + (f8_swap ? 0 : 16);
-      u32x4_t lo, hi;
-      u32x4_t c = kq[f];
+      u32x4_t lo, hi, c = codes[f];
       if (f8_swap) c = u32x4_t{c[2], c[3], c[0], c[1]};
       fp8x16_to_bf16(c, lo, hi);
-      *reinterpret_cast<u32x4_t*>(at + o1) = lo;
-      *reinterpret_cast<u32x4_t*>(at + o2) = hi;
-      c = vq[f];
-      if (f8_swap) c = u32x4_t{c[2], c[3], c[0], c[1]};
-      fp8x16_to_bf16(c, lo, hi);
-      *reinterpret_cast<u32x4_t*>(at + kTileB + o1) = lo;
-      *reinterpret_cast<u32x4_t*>(at + kTileB + o2) = hi;
+      *reinterpret_cast<u32x4_t*>(at + off + (f8_swap ? 16 : 0)) = lo;
+      *reinterpret_cast<u32x4_t*>(at + off + (f8_swap ? 0 : 16)) = hi;
     }
   };
-  auto landed = [&](int stage) {  // the wave's rows of the stage are in LDS
-    if constexpr (F8) commit(stage);
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  };
-
   if (s_lo < s_end) {
-    issue(0);
+    issue_k(0);
+    issue_v(kTileB);
     refill_window();
   }
 
@@ -306,19 +307,15 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   }
 
   // LDS read offsets (bytes from a tile's start). K A operand, 16-key quarter h: row 16h + col,
-  // dims map * D + 32 ks + 8 g4.
-  uint32_t ko[kKs];
-#pragma unroll
-  for (int ks = 0; ks < kKs; ++ks)
-    ko[ks] = (uint32_t)col * kRB +
-             (uint32_t)((map * (D / 8) + g4 + 4 * ks) ^ chunk_swz<kV>(col)) * 16u;
-  // V^T by ds_read_b64_tr_b16: lane 16g + 4r + c reads row 4g + r (and +16), dims 16 db + 4c .. +3
+  // dims map * D + 32 ks + 8 g4: chunk map * D/8 + 4 ks + g4 before the permutation, an XOR like
+  // the place of ks in it, so that one register holds them all.
+  const uint32_t ko = (uint32_t)col * kRB +
+                      (uint32_t)((map * (D / 8) + g4) ^ chunk_swz<kV>(col)) * 16u;
+  // V^T by ds_read_b64_tr_b16: lane 16g + 4r + c reads row 4g + r (and +16), dims 16 db + 4c .. +3:
+  // chunk 2 db + c/2, half c%2. The low three bits of db likewise; the rows' permutation has no more.
   const int vrow = 4 * g4 + (col >> 2);
-  uint32_t vo[kDb];
-#pragma unroll
-  for (int db = 0; db < kDb; ++db)
-    vo[db] = (uint32_t)vrow * kRB + (uint32_t)(db ^ (chunk_swz<kV>(vrow) >> 1)) * 32u +
-             (uint32_t)(col & 3) * 8u;
+  const uint32_t vo = (uint32_t)vrow * kRB + (uint32_t)chunk_swz<kV>(vrow) * 16u +
+                      (uint32_t)(col & 3) * 8u;
 
   f32x4_t acc[kRG][kDb];  // O^T: lane l -> row l%16, dims 16 db + 4(l/16) .. +3
   float m_run[kRG], l_run[kRG], mb_run[kRG];  // mb_run: m_run, or 0 while the row sees no key
@@ -335,40 +332,50 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   for (int rr = 0; rr < kRG; ++rr)
 #pragma unroll
     for (int ks = 0; ks < kKs; ++ks) asm volatile("" ::"v"(qreg[rr][ks]));
-  if (s_lo < s_end) landed(0);
-  __syncthreads();
-
   const char* lds = (const char*)(__attribute__((address_space(3))) char*)ring;
-  auto step = [&](auto stage_c, int s, bool more) {
-    constexpr int ST = decltype(stage_c)::value;
-    if constexpr (F8) issue(ST ^ 1);
-    const char* kt = lds + ST * kStageB;
-    const char* vt = kt + kTileB;
-    f32x4_t st[kRG][4];
+  float sv[kRG][16];     // a step's scores
+  u32x4_t pb[2][kRG];    // and its weights, 32 keys at a time
+  // S^T of a K tile; `between` runs among its products. Two k-steps' reads are issued before the
+  // products of the two before, and the barriers keep them there: the compiler would wait for each
+  // read right after it.
+  auto scores = [&](uint32_t kt, auto between) {
+    constexpr int kN = 4 * kKs / 2;
+    u32x4_t ka[2][2];
+    auto read = [&](int i, u32x4_t (&x)[2]) {
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      u32x4_t ka[kKs];
+      for (int j = 0; j < 2; ++j)
+        x[j] = *reinterpret_cast<const u32x4_t*>(lds + ((kt + ko) ^ (2 * i % kKs + j) * 64u) +
+                                                 2 * i / kKs * (16 * kRB));
+    };
+    read(0, ka[0]);
+    f32x4_t x[kRG];
 #pragma unroll
-      for (int ks = 0; ks < kKs; ++ks)
-        ka[ks] = *reinterpret_cast<const u32x4_t*>(kt + h * (16 * kRB) + ko[ks]);
-      if constexpr (!F8) {
-        if (h == 2) issue(ST ^ 1);
+    for (int i = 0; i < kN; ++i) {
+      if (i + 1 < kN) read(i + 1, ka[(i + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i == 2) between();
+      if (2 * i % kKs == 0) {
+#pragma unroll
+        for (int rr = 0; rr < kRG; ++rr) x[rr] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       }
 #pragma unroll
-      for (int rr = 0; rr < kRG; ++rr) {
-        f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int ks = 0; ks < kKs; ++ks) x = mfma_16x16x32<H16>(ka[ks], qreg[rr][ks], x);
-        st[rr][h] = x;
+        for (int rr = 0; rr < kRG; ++rr)
+          x[rr] = mfma_16x16x32<H16>(ka[i & 1][j], qreg[rr][2 * i % kKs + j], x[rr]);
+      if (2 * (i + 1) % kKs == 0) {
+#pragma unroll
+        for (int rr = 0; rr < kRG; ++rr)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sv[rr][2 * i / kKs * 4 + e] = x[rr][e];
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  // masks step s and raises the running maxima
+  auto maxima = [&](int s) {
     const bool edge = (s * kDiffStep + kDiffStep - 1 > diag + j0) ||
                       (s * kDiffStep + kDiffStep > Lk);  // uniform
-    float sv[kRG][16];
-#pragma unroll
-    for (int rr = 0; rr < kRG; ++rr)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sv[rr][e] = st[rr][e / 4][e % 4];
     if (edge) {
 #pragma unroll
       for (int rr = 0; rr < kRG; ++rr) {
@@ -404,53 +411,172 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
         for (int db = 0; db < kDb; ++db) acc[rr][db] *= alpha;
       }
     }
-    // 32 keys at a time: k-slot j of lane group g is key 32c+4g+j (j<4), or 32c+16+4g+(j-4)
+  };
+  // the weights of 32 keys: k-slot j of lane group g is key 32c+4g+j (j<4), or 32c+16+4g+(j-4)
+  auto weights = [&](int c) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      u32x4_t pb[kRG];
+    for (int rr = 0; rr < kRG; ++rr) {
+      float w[8];
 #pragma unroll
-      for (int rr = 0; rr < kRG; ++rr) {
-        float w[8];
+      for (int e = 0; e < 8; ++e)
+        w[e] = fast_exp2(fmaf(sv[rr][8 * c + e], a.scale_log2, -mb_run[rr]));  // -inf -> 0
+      pb[c][rr] = u32x4_t{cvt_pk16<H16>(w[0], w[1]), cvt_pk16<H16>(w[2], w[3]),
+                          cvt_pk16<H16>(w[4], w[5]), cvt_pk16<H16>(w[6], w[7])};
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          w[e] = fast_exp2(fmaf(sv[rr][8 * c + e], a.scale_log2, -mb_run[rr]));  // -inf -> 0
-        pb[rr] = u32x4_t{cvt_pk16<H16>(w[0], w[1]), cvt_pk16<H16>(w[2], w[3]),
-                         cvt_pk16<H16>(w[4], w[5]), cvt_pk16<H16>(w[6], w[7])};
+      for (int e = 0; e < 4; ++e) l_run[rr] = sum2_16<H16>(pb[c][rr][e], l_run[rr]);
+    }
+  };
+  // O^T += V^T P^T: V^T of kVg 16-dim blocks at a time, the next ones' reads in flight
+  constexpr int kVg = 4;
+  auto values = [&](uint32_t vt) {
+    u32x4_t va[2][kVg];
+    auto read = [&](int g, u32x4_t (&x)[kVg]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) l_run[rr] = sum2_16<H16>(pb[rr][e], l_run[rr]);
+      for (int i = 0; i < kVg; ++i) {
+        const int db = (g * kVg + i) % kDb;
+        const char* at = lds + ((vt + vo) ^ (db & 7) * 32u) + (db & 8) * 32 +
+                         g * kVg / kDb * (32 * kRB);
+        const i16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)at);
+        const i16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(at + 16 * kRB));
+        x[i] = u32x4_t{__builtin_bit_cast(uint2, v0).x, __builtin_bit_cast(uint2, v0).y,
+                       __builtin_bit_cast(uint2, v1).x, __builtin_bit_cast(uint2, v1).y};
       }
+    };
+    read(0, va[0]);
 #pragma unroll
-      for (int db = 0; db < kDb; ++db) {
-        const char* vc = vt + c * (32 * kRB) + vo[db];
-        const i16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)vc);
-        const i16x4_t v1 =
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(vc + 16 * kRB));
-        const u32x4_t va = {__builtin_bit_cast(uint2, v0).x, __builtin_bit_cast(uint2, v0).y,
-                            __builtin_bit_cast(uint2, v1).x, __builtin_bit_cast(uint2, v1).y};
+    for (int g = 0; g < 2 * kDb / kVg; ++g) {
+      if (g + 1 < 2 * kDb / kVg) read(g + 1, va[(g + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kVg; ++i)
 #pragma unroll
         for (int rr = 0; rr < kRG; ++rr)
-          acc[rr][db] = mfma_16x16x32<H16>(va, pb[rr], acc[rr][db]);
+          acc[rr][(g * kVg + i) % kDb] = mfma_16x16x32<H16>(
+              va[g & 1][i], pb[g * kVg / kDb][rr], acc[rr][(g * kVg + i) % kDb]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  const int n = s_end - s_lo;
+  if constexpr (kPing) {
+    // Half steps, a barrier after each. Waves w and w + 4, on one SIMD, are of different maps, and
+    // map 1's are half a step behind: while one's softmax keeps the vector unit busy, the other's
+    // products have the matrix cores. Tiles are numbered K 0, V 0, K 1, V 1 ..: in half step h the
+    // waves of map 0 work on tile h (scores of a K tile, products of a V tile), those of map 1 on
+    // tile h - 1. Tile i lies in place i % kTiles of the ring, which is free from half step
+    // i + 2 - kTiles on, and is fetched from then on until the end of half step i - 1: three half
+    // steps with five places; fp8 codes, which wait in registers, two. Four chunks of up to 2048 tokens
+    // over up to 6000 (Hq 32, Hk 8): whole steps with a barrier each 690 us, half steps and four
+    // places 685, five 665; without the fetches 600, and without the softmax too 555.
+    constexpr int kAhead = F8 ? 2 : 3;
+    auto next = [](uint32_t at) { return at + kTileB == kTiles * kTileB ? 0u : at + kTileB; };
+    uint32_t rd = 0, wr = 2 * kTileB;  // places read and fetched next
+    [[maybe_unused]] uint32_t cm = 0;  // F8: and written next
+    auto fetch = [&](auto v_c) {
+      if constexpr (decltype(v_c)::value) {
+        issue_v(wr);
+      } else {
+        issue_k(wr);
+      }
+      wr = next(wr);
+    };
+    // the tile after the one that map 0 has now is in LDS; kAhead - 1 fetches may be in flight
+    auto landed = [&](auto v_c) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kAhead - 1) * (F8 ? kNl8 : kNl)) : "memory");
+      if constexpr (F8) {
+        commit(decltype(v_c)::value ? vq : kq, ring + cm);
+        cm = next(cm);
+      }
+    };
+    using K = std::integral_constant<bool, false>;
+    using V = std::integral_constant<bool, true>;
+    using First = std::conditional_t<kAhead == 2, K, V>;  // what an even half step fetches
+    using Second = std::conditional_t<kAhead == 2, V, K>;
+    if (n > 0) {
+      if constexpr (kAhead == 3) fetch(K{});
+      refill_window();
+      landed(K{});
+      __syncthreads();
+      if (map == 1) {  // half step 0
+        fetch(First{});
+        refill_window();
+        landed(V{});
+        __syncthreads();
+      }
+      auto run = [&](auto map_c) {
+        using Scores = std::conditional_t<decltype(map_c)::value == 0, First, Second>;
+        using Values = std::conditional_t<decltype(map_c)::value == 0, Second, First>;
+        using Next = std::conditional_t<decltype(map_c)::value == 0, V, K>;  // lands with scores
+        using After = std::conditional_t<decltype(map_c)::value == 0, K, V>;
+        for (int s = s_lo; s < s_end; ++s) {
+          if (active) {
+            scores(rd, [&] { fetch(Scores{}); });
+            maxima(s);
+            weights(0);
+            weights(1);
+          } else {
+            fetch(Scores{});
+          }
+          rd = next(rd);
+          refill_window();
+          landed(Next{});
+          __syncthreads();
+          fetch(Values{});
+          if (active) values(rd);
+          rd = next(rd);
+          refill_window();
+          landed(After{});
+          __syncthreads();
+        }
+      };
+      if (map == 0) {
+        run(std::integral_constant<int, 0>{});
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // map 1's last half step
+      } else {
+        run(std::integral_constant<int, 1>{});
       }
     }
-    // the next step's rows landed (each wave waits for its own), then the barrier publishes them and
-    // frees this stage
-    if (!F8 || more) landed(ST ^ 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into LDS is left in flight
     __syncthreads();
-    refill_window();
-  };
-  if (active) {
-    for (int s = s_lo; s < s_end; s += 2) {
-      step(std::integral_constant<int, 0>{}, s, s + 1 < s_end);
-      if (s + 1 >= s_end) break;
-      step(std::integral_constant<int, 1>{}, s + 1, s + 2 < s_end);
-    }
-  } else {  // a wave without rows only brings its share of the tiles
-    for (int s = s_lo; s < s_end; ++s) {
-      const int next = (s - s_lo + 1) & 1;
-      issue(next);
-      landed(next);
+  } else {
+    auto landed = [&](int stage) {  // the wave's rows of the stage are in LDS
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if constexpr (F8) {
+        commit(kq, ring + stage * kStageB);
+        commit(vq, ring + stage * kStageB + kTileB);
+      }
+    };
+    if (n > 0) landed(0);
+    __syncthreads();
+    auto step = [&](auto stage_c, int s) {
+      constexpr int ST = decltype(stage_c)::value;
+      constexpr uint32_t kt = ST * kStageB;
+      auto fetch = [&] {
+        issue_k((ST ^ 1) * kStageB);
+        issue_v((ST ^ 1) * kStageB + kTileB);
+      };
+      if constexpr (F8) fetch();
+      if (active) {
+        scores(kt, [&] {
+          if constexpr (!F8) fetch();
+        });
+        maxima(s);
+        weights(0);
+        weights(1);
+        values(kt + kTileB);
+      } else if constexpr (!F8) {
+        fetch();
+      }
+      // the next step's rows landed (each wave waits for its own), then the barrier publishes them
+      // and frees this stage
+      landed(ST ^ 1);
       __syncthreads();
       refill_window();
+    };
+    for (int s = s_lo; s < s_end; s += 2) {
+      step(std::integral_constant<int, 0>{}, s);
+      if (s + 1 >= s_end) break;
+      step(std::integral_constant<int, 1>{}, s + 1);
     }
   }
 
@@ -475,7 +601,7 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   float inv[kRG];
 #pragma unroll
   for (int rr = 0; rr < kRG; ++rr) inv[rr] = l[rr] > 0.f ? a.v_scale / l[rr] : 0.f;
-  // the last step's barrier has freed the ring: A_1, lane by lane as it is held
+  // the ring is free: A_1, lane by lane as it is held
   f32x4_t* other = reinterpret_cast<f32x4_t*>(ring) + wi * (kRG * kDb * 64) + lane;
   if (map == 1 && active) {
 #pragma unroll
