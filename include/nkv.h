@@ -869,19 +869,24 @@ int nkv_diff_decode(int32_t kv_type, const void* q, int64_t q_row_stride, const 
  * stride). n_rows: the rows of k and v (paged: blocks * block_size). Keys of
  * invalid blocks and past the table are zeros, as there. Without a workspace a
  * query tile's keys stay with one workgroup; with one of
- * nkv_diff_prefill_workspace_bytes (0: no use) they are split where few tiles
- * would leave the chip idle. max_seqlen_k: an upper bound of the key lengths,
- * which that choice goes by (results do not depend on it beyond rounding).
+ * nkv_diff_prefill_workspace_bytes (same arguments; 0: no use) they are split
+ * where few tiles would leave the chip idle, and sequences that bring one token
+ * to paged caches are streamed as by nkv_diff_decode. max_seqlen_q and
+ * max_seqlen_k: upper bounds of the lengths (0: not known), which those choices
+ * go by; results do not depend on them beyond rounding.
  * No counterpart in the reference (beside nanokvllm/layers/attention.py:96-102).
  */
-size_t nkv_diff_prefill_workspace_bytes(int32_t n_seqs, int64_t total_q, int64_t max_seqlen_k,
-                                        int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim);
+size_t nkv_diff_prefill_workspace_bytes(int32_t kv_type, int32_t n_seqs, int64_t total_q,
+                                        int64_t max_seqlen_q, int64_t max_seqlen_k,
+                                        int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                        int32_t paged);
 int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_stride, int64_t total_q,
                      const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride,
                      const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
                      const int32_t* block_tables, int64_t bt_row_stride,
-                     int32_t max_blocks_per_seq, int32_t n_seqs, int64_t max_seqlen_k,
-                     int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+                     int32_t max_blocks_per_seq, int32_t n_seqs, int64_t max_seqlen_q,
+                     int64_t max_seqlen_k, int32_t n_q_heads, int32_t n_kv_heads,
+                     int32_t head_dim, int32_t block_size,
                      int64_t n_rows, float scale, float k_scale, float v_scale,
                      const float* lambdas, float lambda_init, const void* norm_weight, float eps,
                      void* out, int64_t out_row_stride, void* workspace, size_t workspace_bytes,

@@ -130,10 +130,11 @@ SIGNATURES = {
     "nkv_diff_decode": (C.c_int, [_i32, _p, _i64, _p, _p, _p, _i64, _p, _i32, _i32, _i32, _i32,
                                   _i32, _i32, _i64, _f32, _f32, _f32, _p, _f32, _p, _f32, _p,
                                   _i64, _p, _sz, _p]),
-    "nkv_diff_prefill_workspace_bytes": (_sz, [_i32, _i64, _i64, _i32, _i32, _i32]),
+    "nkv_diff_prefill_workspace_bytes": (_sz, [_i32, _i32, _i64, _i64, _i64, _i32, _i32, _i32,
+                                               _i32]),
     "nkv_diff_prefill": (C.c_int, [_i32, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p, _i64,
-                                   _i32, _i32, _i64, _i32, _i32, _i32, _i32, _i64, _f32, _f32,
-                                   _f32, _p, _f32, _p, _f32, _p, _i64, _p, _sz, _p]),
+                                   _i32, _i32, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _f32,
+                                   _f32, _f32, _p, _f32, _p, _f32, _p, _i64, _p, _sz, _p]),
     # the first argument: a packed nkv_pages
     "nkv_pages_workspace_bytes": (_sz, [_i64]),
     "nkv_pages_append": (C.c_int, [C.c_char_p, _p, _i32, _p, _i64, _p, _p, _p]),

@@ -6,7 +6,7 @@
 //   out = (1 - lambda_init) * o / sqrt(mean(o^2) + eps) * w
 #pragma once
 
-#include "nkv_common.h"
+#include "decode_stream.h"
 
 namespace nkv {
 
@@ -42,6 +42,61 @@ __device__ __forceinline__ void diff_weight(const bf16_t* w, float (&v)[N]) {
     v[i] = w ? e16_lo<H16>(x) : 1.f;
     v[i + 1] = w ? e16_hi<H16>(x) : 1.f;
   }
+}
+
+// o = A_0 - lambda A_1 held N dims a lane, D in all: normalised and stored by the whole wave.
+template <int D, bool H16>
+__device__ __forceinline__ void diff_store(const DiffArgs& d, const float (&o)[D / 64],
+                                           const float (&w)[D / 64], bf16_t* op) {
+  constexpr int N = D / 64;
+  float ss = 0.f, x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    ss = fmaf(o[i], o[i], ss);
+    x[i] = o[i] * w[i];
+  }
+  store_dims<N, H16>(op, x, (1.f - d.init) / sqrtf(wave_sum(ss) * (1.f / D) + d.eps));
+}
+
+// The end of one (sequence b, query pair h) of a decode stream over pairs (DIFF): the partials of
+// its two maps, merged by 2 x WAVES waves (`wave` of them) of a workgroup that all call it, those with
+// live = false for nothing but the barrier.
+template <int D, int WAVES>
+struct DiffLds {
+  MergeLds<D, WAVES> merge[2];
+  float second[D / 64][64];
+};
+template <int D, bool H16, int WAVES, typename Seqs>
+__device__ __forceinline__ void diff_combine(const Seqs seqs, const int b, const int h,
+                                             const bool live, const int wave, int32_t Hq,
+                                             int32_t P, int32_t NCG,
+                                             const float* __restrict__ part,
+                                             const i32x4v_t* __restrict__ desc,
+                                             const DiffArgs& diff, bf16_t* __restrict__ out,
+                                             int64_t out_row_stride, DiffLds<D, WAVES>& lds) {
+  constexpr int N = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int map = wave / WAVES;
+  float lambda = 0.f, w[N], o[N], l = 0.f;
+  bool holds = false;
+  if (live) {
+    if (wave == 0) {
+      lambda = diff_lambda<D / 2>(diff);
+      diff_weight<N, H16>(diff.weight ? diff.weight + N * lane : nullptr, w);
+    }
+    holds = decode_merge<D, WAVES>(seqs, b, 2 * h + map, Hq, P, NCG, part, desc, wave % WAVES,
+                                   &lds.merge[map], o, l);
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (holds && map == 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) lds.second[i][lane] = o[i] * inv;
+  }
+  __syncthreads();
+  if (!live || wave > 0) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = fmaf(-lambda, lds.second[i][lane], o[i] * inv);
+  diff_store<D, H16>(diff, o, w, out + seqs.row(b) * out_row_stride + (int64_t)h * D + N * lane);
 }
 
 // The checks of both entry points; `what` begins their messages.

@@ -10,7 +10,6 @@
 // attentions (two maps, each over both halves of the value) K and V would be read twice.
 // The combine merges the partials of a pair's two rows in the halves of one workgroup, and
 // subtracts, normalises and scales them in the wave that holds the first.
-#include "decode_stream.h"
 #include "diff_common.h"
 
 #include <math.h>
@@ -24,38 +23,11 @@ __global__ __launch_bounds__(128 * WAVES) void diff_decode_combine_kernel(
     const int32_t* __restrict__ context_lens, int32_t Hq, int32_t P, int32_t NCG,
     const float* __restrict__ part, const i32x4v_t* __restrict__ desc, const DiffArgs diff,
     bf16_t* __restrict__ out, int64_t out_row_stride) {
-  constexpr int N = D / 64;
-  __shared__ MergeLds<D, WAVES> lds[2];
-  __shared__ float second[N][64];
-  const int lane = threadIdx.x & 63;
+  __shared__ DiffLds<D, WAVES> lds;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int map = wave / WAVES;
-  const int b = (int)blockIdx.x / (Hq / 2), h = (int)blockIdx.x % (Hq / 2);
-  float lambda = 0.f, w[N];
-  if (wave == 0) {
-    lambda = diff_lambda<D / 2>(diff);
-    diff_weight<N, H16>(diff.weight ? diff.weight + N * lane : nullptr, w);
-  }
-  float o[N], l;
-  const bool holds = decode_merge<D, WAVES>(DecodeSeqs{context_lens, 0}, b, 2 * h + map, Hq, P,
-                                            NCG, part, desc, wave % WAVES, &lds[map], o, l);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  if (holds && map == 1) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) second[i][lane] = o[i] * inv;
-  }
-  __syncthreads();
-  if (wave > 0) return;
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    o[i] = fmaf(-lambda, second[i][lane], o[i] * inv);
-    ss = fmaf(o[i], o[i], ss);
-  }
-  const float norm = (1.f - diff.init) / sqrtf(wave_sum(ss) * (1.f / D) + diff.eps);
-#pragma unroll
-  for (int i = 0; i < N; ++i) o[i] *= w[i];
-  store_dims<N, H16>(out + b * out_row_stride + (int64_t)h * D + N * lane, o, norm);
+  diff_combine<D, H16, WAVES>(DecodeSeqs{context_lens, 0}, (int)blockIdx.x / (Hq / 2),
+                              (int)blockIdx.x % (Hq / 2), true, wave, Hq, P, NCG, part, desc, diff,
+                              out, out_row_stride, lds);
 }
 
 int diff_check(const char* what, int32_t kv_type, int32_t n_q_heads, int32_t n_kv_heads,

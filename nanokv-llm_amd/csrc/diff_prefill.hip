@@ -22,13 +22,16 @@
 //  * The end of a tile: map 1's waves leave A_1 in LDS (the tiles' ring, free by then), map 0's
 //    waves subtract, take the mean square over the row's 2 D dims (in the row's 4 lanes), normalise and
 //    store. Nothing but the output is written.
-//  * Few tiles: the keys of each tile are split into up to n_splits ranges of at least min_steps
-//    steps, a partial row (O, m, l) is written for each and map, and a second kernel merges and ends
-//    them. Tiles of one range are ended by the first kernel.
+//  * Few tiles: the tiles' keys are cut into ranges of the same number of steps, about as many in all
+//    as workgroups are resident, a partial row (O, m, l) is written for each and map, and a second
+//    kernel merges and ends them. Tiles of one range are ended by the first kernel.
+//  * Sequences that bring one token, among prompts: the first workgroups' waves stream their K/V as
+//    the decode kernel does, beside the tiles that keep the matrix cores; a tile for one query would
+//    multiply 96 or 128 rows for it. The second kernel merges them too.
 // Tiles are numbered over the batch without gaps (their number per sequence is known on the device
 // only), each sequence's last ones first: they see the most keys.
-#include "decode_stream.h"
 #include "diff_common.h"
+#include "launch_rules.h"
 #include "lds_tiles.h"
 
 #include <algorithm>
@@ -38,8 +41,10 @@ namespace nkv {
 
 constexpr int kDiffStep = 64;        // keys per step
 constexpr float kDiffLazy = 8.f;     // log2 headroom before a running maximum is raised
-constexpr int kDiffMinSteps = 8;     // shortest range of a split tile
+constexpr int kDiffMinSteps = 4;     // shortest range of a cut tile
 constexpr int kDiffMergeWaves = 4;
+// Decode rows' share of the workgroups: CU time of a row's step against a tile's (see diff_plan).
+constexpr double kDiffRowShare = 0.6;
 
 // Waves of a workgroup, and 16-row groups of a wave. At head_dim 128 a step's tiles take 64 KiB, so
 // one workgroup is resident and brings both waves of each SIMD itself.
@@ -56,64 +61,156 @@ struct DiffPrefillArgs {
   const int32_t *cu_q, *cu_k, *block_tables;
   int64_t bt_row_stride;
   int32_t P, G, block_size, max_blocks, n_limit, n_seqs, total_q;
-  int32_t n_splits, min_steps;
+  // workgroups for a pair at a time (0: tiles stay whole), and the most ranges and tiles of a cut batch
+  int32_t target, range_cap, tile_cap;
+  float cus;
   float scale_log2, v_scale;
   DiffArgs diff;
   bf16_t* out;
   int64_t out_row_stride;
+  i32x4_t* tile_desc;  // of cut tiles: {ranges, the first one, first row of q, rows}; [tile_cap]: tiles
   float* part;
+  // decode rows apart from the tiles: the first row_groups workgroups stream them (0: they are tiles)
+  int32_t row_groups, ncg, min_chunks, max_tokens;
+  i32x4v_t* row_desc;
+  float* row_part;
 };
 
-// A tile of the batch: queries j0 .. of a sequence (row q0 of q), and its ranges of keys.
+// A range of a tile of the batch: queries j0 .. of a sequence (row q0 of q), the key steps of range sp
+// of `ranges`.
 struct DiffTile {
   int seq, q0, Lq, kb0, Lk, j0;
-  int n_steps, ranges;
+  int id, n_steps, ranges, sp;
 };
 
-// Tile `t` of the batch, QT queries each; false past the last one. By the whole wave.
-__device__ __forceinline__ bool diff_tile(const DiffPrefillArgs& a, int QT, int t, DiffTile& d) {
+__device__ __forceinline__ int diff_steps(int Lq, int Lk, int QT, int tile) {
+  const int last = min(Lk - 1, Lk - Lq + min(Lq, (tile + 1) * QT) - 1);
+  return last >= 0 ? last / kDiffStep + 1 : 0;
+}
+
+// Range x of a pair, by the whole wave; false past the last one. The tiles of a sequence have as many
+// places for ranges as its last one needs, so that a lane knows its sequence's number without a
+// loop; the others' last places stay empty. n_tiles: all tiles, 0 where none is cut.
+template <int D>
+__device__ __forceinline__ bool diff_range(const DiffPrefillArgs& a, int QT, int x, DiffTile& d,
+                                           int& n_tiles) {
+  // measured: a step of a workgroup alone on its CU and of one of two, two chunks' partial rows
+  // (101 and 266 KB a range) written and merged, and what the merge takes beside that
+  constexpr float kStepUs[2] = {D == 64 ? 1.6f : 2.2f, D == 64 ? 2.1f : 2.2f};
+  constexpr float kRangeUs = D == 64 ? 0.03f : 0.04f, kMergeUs = 6.f;
   const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int cb = 0; cb < a.n_seqs; cb += 64) {  // uniform
+  int q0 = 0, Lq = 0, kb0 = 0, Lk = 0, nt = 0, hi = 0, at = -1;
+  auto load = [&](int cb) {  // lane: sequence cb + lane
+    if (cb == at) return;
+    at = cb;
     const int s = cb + lane;
-    int q0 = 0, Lq = 0, kb0 = 0, Lk = 0;
+    Lq = 0;
     if (s < a.n_seqs) {
       q0 = a.cu_q[s];
       Lq = a.cu_q[s + 1] - q0;
       kb0 = a.cu_k[s];
       Lk = a.cu_k[s + 1] - kb0;
-      NKV_DBG(t == 0 && (Lq < 0 || Lk < 0 || Lq > Lk || q0 < 0 || q0 + Lq > a.total_q),
+      NKV_DBG(x == 0 && (Lq < 0 || Lk < 0 || Lq > Lk || q0 < 0 || q0 + Lq > a.total_q),
               NKV_DEBUG_LENGTH);
+      Lk = max(Lk, 0);
       if (q0 < 0 || q0 > a.total_q - Lq) Lq = 0;  // rows outside q
+      if (a.row_groups > 0 && Lq == 1) Lq = 0;    // not a tile
     }
-    const int nt = Lq > 0 ? (Lq - 1) / QT + 1 : 0;
-    const int incl = wave_incl_scan(nt);
+    nt = Lq > 0 ? (Lq - 1) / QT + 1 : 0;
+    hi = nt > 0 ? diff_steps(Lq, Lk, QT, nt - 1) : 0;
+  };
+  int R = INT32_MAX;  // steps of a range
+  n_tiles = 0;
+  if (a.target > 0) {
+    // Lane k tries ranges of 1 / (k + 1) of the longest tile and takes the time until all are through:
+    // steps, slower where two workgroups share a CU, and the partial rows, which all go through
+    // memory twice.
+    int longest = 0, tiles = 0;
+    for (int cb = 0; cb < a.n_seqs; cb += 64) {  // uniform
+      load(cb);
+      longest = max(longest, hi);
+      tiles += nt;
+    }
+    longest = (int)wave_max((float)longest);  // exact: below 2^24 steps of 64 keys, or near enough
+    tiles = __builtin_amdgcn_readlane(wave_incl_scan(tiles), 63);
+    const int mine = max(kDiffMinSteps, (longest + lane) / (lane + 1));
+    const float per = 1.f / (float)mine;
+    float T = 0.f, made = 0.f, places = 0.f;
+    for (int cb = 0; cb < a.n_seqs; cb += 64) {
+      load(cb);
+      const int lo = nt > 0 ? diff_steps(Lq, Lk, QT, 0) : 0;
+      for (uint64_t left = __ballot(nt > 0); left; left &= left - 1) {  // sequences with tiles
+        const int ln = __builtin_ctzll(left);
+        const float n = (float)__builtin_amdgcn_readlane(nt, ln);
+        const float last = (float)__builtin_amdgcn_readlane(hi, ln);
+        const float first = (float)__builtin_amdgcn_readlane(lo, ln);
+        const float most = fmaxf(1.f, ceilf(last * per));
+        T += n * 0.5f * (last + first);
+        made += n * 0.5f * (most + fmaxf(1.f, ceilf(first * per)));
+        places += n * most;
+      }
+    }
+    const float m = (float)a.target, range = (float)min(mine, longest);
+    const float groups = made * (float)a.P;
+    const float step = groups <= a.cus ? kStepUs[0] : kStepUs[1];
+    float cost = step * (made <= m ? range : T / m + 0.5f * range);
+    if (lane > 0) cost += kMergeUs + groups * kRangeUs;
+    if (lane > 0 && (places > (float)a.range_cap || (longest + lane - 1) / lane <= kDiffMinSteps))
+      cost = INFINITY;  // too many, or what the lane before tries
+    const float best = -wave_max(-cost);
+    const int k = __builtin_ctzll(__ballot(cost == best) | 1ull << 63);
+    // k = 0: whole tiles; as they are, too, for another batch than the plan was for
+    if (k > 0 && tiles <= a.tile_cap) {
+      R = __builtin_amdgcn_readlane(mine, k);
+      n_tiles = tiles;
+    }
+  }
+  int base = 0, tiles = 0;
+  for (int cb = 0; cb < a.n_seqs; cb += 64) {  // uniform
+    load(cb);
+    const int places = R == INT32_MAX ? 1 : max(1, (hi + R - 1) / R);
+    const int incl = wave_incl_scan(nt * places);
     const int total = __builtin_amdgcn_readlane(incl, 63);
-    if (t < base + total) {
+    const int tile_incl = wave_incl_scan(nt);
+    if (x < base + total) {
       const int ln =
-          __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(base + incl > t)));
+          __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(base + incl > x)));
       d.seq = cb + ln;
       d.q0 = __builtin_amdgcn_readlane(q0, ln);
       d.Lq = __builtin_amdgcn_readlane(Lq, ln);
       d.kb0 = __builtin_amdgcn_readlane(kb0, ln);
-      d.Lk = max(__builtin_amdgcn_readlane(Lk, ln), 0);
-      // the sequence's last tile first
-      d.j0 = (base + __builtin_amdgcn_readlane(incl, ln) - 1 - t) * QT;
-      const int last = min(d.Lk - 1, d.Lk - d.Lq + min(d.Lq, d.j0 + QT) - 1);
-      d.n_steps = last >= 0 ? last / kDiffStep + 1 : 0;
-      d.ranges = min(a.n_splits, max(1, d.n_steps / a.min_steps));
+      d.Lk = __builtin_amdgcn_readlane(Lk, ln);
+      const int tn = __builtin_amdgcn_readlane(nt, ln);
+      const int pl = __builtin_amdgcn_readlane(places, ln);
+      const int rest = x - (base + __builtin_amdgcn_readlane(incl, ln) - tn * pl);
+      const int k = __builtin_amdgcn_readfirstlane(rest / pl);  // the sequence's last tile first
+      d.sp = rest - k * pl;
+      d.id = tiles + __builtin_amdgcn_readlane(tile_incl, ln) - tn + k;
+      d.j0 = (tn - 1 - k) * QT;
+      d.n_steps = diff_steps(d.Lq, d.Lk, QT, tn - 1 - k);
+      d.ranges = pl == 1 ? 1
+                         : __builtin_amdgcn_readfirstlane(max(1, (d.n_steps + R - 1) / R));
       return true;
     }
     base += total;
+    tiles += __builtin_amdgcn_readlane(tile_incl, 63);
   }
   return false;
 }
 
-// The partial rows of range `sp` of (tile t, pair p), map 0's then map 1's.
+// The batch's decode rows that lie within q.
+struct OneDiffSeqs : OneRowSeqs {
+  int32_t total_q;
+  __device__ __forceinline__ int keys(int s) const {
+    const int r = cu_q[s];
+    return r >= 0 && r < total_q ? OneRowSeqs::keys(s) : 0;
+  }
+};
+
+// The partial rows of range x of pair p, map 0's then map 1's.
 template <int D>
-__device__ __forceinline__ float* diff_part(const DiffPrefillArgs& a, int t, int p, int sp) {
-  return a.part + (((int64_t)t * a.P + p) * a.n_splits + sp) *
-                      (2 * diff_rows(D) * diff_part_row(D));
+__device__ __forceinline__ float* diff_part(const DiffPrefillArgs& a, int x, int p) {
+  return a.part + ((int64_t)x * a.P + p) * (2 * diff_rows(D) * diff_part_row(D));
 }
 
 template <bool F8, int D, bool H16, bool PAGED>
@@ -139,7 +236,9 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   constexpr int kNl8 = kWR / kRpl8;             // F8: loads per wave per tile
   static_assert(kNl >= 1 && kNl8 >= 1, "a wave brings whole loads");
   static_assert(kWaves / 2 * kRG * kDb * 1024 <= kTiles * kTileB, "A_1 fits the ring");
-  __shared__ __attribute__((aligned(1024))) char ring[kTiles * kTileB];
+  constexpr int kRowLds = PAGED ? 2 * decode_lds_elems<F8, 1, kV>() : 0;  // bytes a wave
+  __shared__ __attribute__((aligned(1024))) char
+      ring[kWaves * kRowLds > kTiles * kTileB ? kWaves * kRowLds : kTiles * kTileB];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -151,15 +250,34 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   const int G = a.G, P = a.P;
   const int QT = diff_rows(D) / G;     // queries per tile
 
-  const int p = blockIdx.x % P;
-  const int sp = blockIdx.x / P % a.n_splits;
-  const int t = blockIdx.x / P / a.n_splits;
+  if constexpr (PAGED) {
+    if ((int)blockIdx.x < a.row_groups) {
+      decode_stream<F8, 1, kV, H16, true>(
+          OneDiffSeqs{{a.cu_q, a.cu_k, a.n_seqs, a.max_tokens}, a.total_q},
+          (int)blockIdx.x * kWaves + wave, a.row_groups * kWaves,
+          reinterpret_cast<bf16_t*>(ring + wave * kRowLds), a.q, a.q_row_stride, a.k, a.v,
+          a.block_tables, a.bt_row_stride, P, 2 * G, a.ncg, a.block_size, a.max_blocks, a.n_limit,
+          a.min_chunks, a.scale_log2, a.v_scale, a.row_part, a.row_desc);
+      return;
+    }
+  }
+  const int p = ((int)blockIdx.x - a.row_groups) % P;
+  const int x = ((int)blockIdx.x - a.row_groups) / P;
   DiffTile d;
-  if (!diff_tile(a, QT, t, d) || sp >= d.ranges) return;  // uniform
+  int n_tiles;
+  const bool some = diff_range<D>(a, QT, x, d, n_tiles);
+  if (a.target > 0 && p == 0 && tid == 0) {
+    if (x == 0) a.tile_desc[a.tile_cap] = i32x4_t{n_tiles, 0, 0, 0};
+    if (some && d.sp == 0 && d.id < a.tile_cap)
+      a.tile_desc[d.id] = i32x4_t{d.ranges, x, d.q0 + d.j0, min(QT, d.Lq - d.j0) * a.G};
+  }
+  if (!some || d.sp >= d.ranges) return;  // uniform
   const int j0 = d.j0, Lq = d.Lq, Lk = d.Lk;
   const int n_rows = min(QT, Lq - j0) * G;
-  const int s_lo = (int)((int64_t)d.n_steps * sp / d.ranges);
-  const int s_end = (int)((int64_t)d.n_steps * (sp + 1) / d.ranges);
+  // equal ranges but for one step; into scalar registers (the divisions are vector code)
+  const int each = d.n_steps / d.ranges, more = d.n_steps - each * d.ranges;
+  const int s_lo = __builtin_amdgcn_readfirstlane(d.sp * each + min(d.sp, more));
+  const int s_end = __builtin_amdgcn_readfirstlane(s_lo + each + (d.sp < more ? 1 : 0));
   const int diag = Lk - Lq;  // query j sees keys <= diag + j
 
   // ---- the wave's share of a step's K and V rows: kWR consecutive keys, which lie in one block
@@ -586,7 +704,7 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   for (int rr = 0; rr < kRG; ++rr) l[rr] = col_sum4(l_run[rr]);
   if (d.ranges > 1) {  // a part: O, m and l as they are
     if (!active) return;
-    float* rows = diff_part<D>(a, t, p, sp) + (int64_t)map * (diff_rows(D) * diff_part_row(D));
+    float* rows = diff_part<D>(a, x, p) + (int64_t)map * (diff_rows(D) * diff_part_row(D));
 #pragma unroll
     for (int rr = 0; rr < kRG; ++rr) {
       if (jrow[rr] >= Lq) continue;
@@ -641,108 +759,203 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   }
 }
 
-// Merges and ends the rows of tiles that have several ranges: one row a wave, lane l dims N*l ..,
-// both maps' partials of four ranges in flight.
+// Merges and ends the rows of tiles that have several ranges (workgroups below tile_groups); and the
+// decode rows, two waves for each (sequence, query pair). A wave has kMergeRows rows of a tile at once,
+// both maps of each: at head_dim 64 the halves of the wave have a map each, 4 dims a lane; at 128
+// every lane has 4 dims of both. kMergeFly ranges' loads are in flight. (One row a wave: 17 us over the
+// 50 MB of two prompts of 512 tokens, Hq 32, Hk 8, head_dim 64.)
+constexpr int kMergeRows = 4;
 template <int D, bool H16>
 __global__ __launch_bounds__(64 * kDiffMergeWaves) void diff_merge_kernel(
-    const DiffPrefillArgs a) {
-  constexpr int N = D / 32;
+    const DiffPrefillArgs a, const int32_t tile_groups) {
+  constexpr int kMaps = D / 64;  // of a lane
+  constexpr int kMergeFly = 4 / kMaps;
   constexpr int kV = 2 * D;
   constexpr int kRow = diff_part_row(D);
+  constexpr int kRowGroups = diff_rows(D) / (kDiffMergeWaves * kMergeRows);  // of a tile
+  static_assert(diff_rows(D) % (kDiffMergeWaves * kMergeRows) == 0, "whole workgroups");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int G = a.G, P = a.P;
-  const int QT = diff_rows(D) / G;
+  if ((int)blockIdx.x >= tile_groups) {
+    __shared__ DiffLds<kV, 1> lds[kDiffMergeWaves / 2];
+    const OneDiffSeqs seqs{{a.cu_q, a.cu_k, a.n_seqs, a.max_tokens}, a.total_q};
+    const int id = ((int)blockIdx.x - tile_groups) * (kDiffMergeWaves / 2) + wave / 2;
+    const int b = id / (P * G), r = b < a.n_seqs ? a.cu_q[b] : -1;
+    const bool live = r >= 0 && r < a.total_q && a.cu_q[b + 1] - r == 1;
+    diff_combine<kV, H16, 1>(seqs, b, id % (P * G), live, wave % 2, 2 * P * G, P, a.ncg,
+                             a.row_part, a.row_desc, a.diff, a.out, a.out_row_stride,
+                             lds[wave / 2]);
+    return;
+  }
   const int p = blockIdx.x % P;
-  const int t = blockIdx.x / P;
-  const int r = (int)blockIdx.y * kDiffMergeWaves + wave;
-  DiffTile d;
-  if (!diff_tile(a, QT, t, d) || d.ranges < 2 || r >= min(QT, d.Lq - d.j0) * G) return;
-  const float* part = diff_part<D>(a, t, p, 0) + (int64_t)r * kRow;
-  const int64_t map_f = (int64_t)diff_rows(D) * kRow;
-  float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f}, o[2][N] = {};
-  for (int s0 = 0; s0 < d.ranges; s0 += 4) {
-    float2 ml[4][2];
-    float v[4][2][N];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const float* row = part + (2 * (int64_t)min(s0 + u, d.ranges - 1) + m) * map_f;
-        ml[u][m] = *reinterpret_cast<const float2*>(row + kV);
-        load_dims<N>(row + N * lane, v[u][m]);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        if (s0 + u >= d.ranges || ml[u][m].x == -INFINITY) continue;  // uniform
-        const float top = fmaxf(M[m], ml[u][m].x);
-        const float alpha = fast_exp2(M[m] - top), w = fast_exp2(ml[u][m].x - top);
-        M[m] = top;
-        L[m] = fmaf(w, ml[u][m].y, L[m] * alpha);
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[m][e] = fmaf(w, v[u][m][e], o[m][e] * alpha);
-      }
-    }
-  }
+  const int t = blockIdx.x / P / kRowGroups;
+  const int r0 = ((int)(blockIdx.x / P % kRowGroups) * kDiffMergeWaves + wave) * kMergeRows;
+  const i32x4_t d = a.tile_desc[t];
+  const int ranges = d[0], rows = d[3];
+  if (t >= a.tile_desc[a.tile_cap][0] || ranges < 2 || r0 >= rows) return;
   const float lambda = diff_lambda<D>(a.diff);
-  float w[N], x[N], ss = 0.f;
-  const float i0 = L[0] > 0.f ? a.v_scale / L[0] : 0.f;
-  const float i1 = L[1] > 0.f ? a.v_scale / L[1] : 0.f;
+  const int dim = lane * 4 % kV;
+  float w[4];
+  diff_weight<4, H16>(a.diff.weight ? a.diff.weight + dim : nullptr, w);
+  const int64_t map_f = (int64_t)diff_rows(D) * kRow;
+  const int64_t range_f = 2 * map_f * P;
+  // the lane's map (the first of them) of row r0
+  const float* part = diff_part<D>(a, d[1], p) + (int64_t)r0 * kRow +
+                      (kMaps == 1 ? (lane >> 5) * map_f : 0);
+  float M[kMergeRows][kMaps], L[kMergeRows][kMaps];
+  f32x4_t o[kMergeRows][kMaps];
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    x[e] = fmaf(-lambda, o[1][e] * i1, o[0][e] * i0);
-    ss = fmaf(x[e], x[e], ss);
+  for (int i = 0; i < kMergeRows; ++i)
+#pragma unroll
+    for (int m = 0; m < kMaps; ++m) {
+      M[i][m] = -INFINITY;
+      L[i][m] = 0.f;
+      o[i][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+  for (int s0 = 0; s0 < ranges; s0 += kMergeFly) {
+    float2 ml[kMergeFly][kMergeRows][kMaps];
+    f32x4_t v[kMergeFly][kMergeRows][kMaps];
+#pragma unroll
+    for (int u = 0; u < kMergeFly; ++u) {
+      const float* range = part + min(s0 + u, ranges - 1) * range_f;
+#pragma unroll
+      for (int i = 0; i < kMergeRows; ++i)
+#pragma unroll
+        for (int m = 0; m < kMaps; ++m) {  // rows past the tile's: its last one again
+          const float* row = range + min(i, rows - 1 - r0) * kRow + m * map_f;
+          ml[u][i][m] = *reinterpret_cast<const float2*>(row + kV);
+          v[u][i][m] = *reinterpret_cast<const f32x4_t*>(row + dim);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kMergeFly; ++u) {
+      if (s0 + u >= ranges) continue;  // uniform
+#pragma unroll
+      for (int i = 0; i < kMergeRows; ++i)
+#pragma unroll
+        for (int m = 0; m < kMaps; ++m) {
+          // a range of no visible key has m = -inf, l = 0: weight 0 unless all have
+          const float top = fmaxf(M[i][m], ml[u][i][m].x);
+          const float mb = top == -INFINITY ? 0.f : top;
+          const float alpha = fast_exp2(M[i][m] - mb), wu = fast_exp2(ml[u][i][m].x - mb);
+          M[i][m] = top;
+          L[i][m] = fmaf(wu, ml[u][i][m].y, L[i][m] * alpha);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[i][m][e] = fmaf(wu, v[u][i][m][e], o[i][m][e] * alpha);
+        }
+    }
   }
-  const float norm = (1.f - a.diff.init) / sqrtf(wave_sum(ss) * (1.f / kV) + a.diff.eps);
-  diff_weight<N, H16>(a.diff.weight ? a.diff.weight + N * lane : nullptr, w);
 #pragma unroll
-  for (int e = 0; e < N; ++e) x[e] *= w[e];
-  store_dims<N, H16>(a.out + (int64_t)(d.q0 + d.j0 + r / G) * a.out_row_stride +
-                         (int64_t)(p * G + r % G) * kV + N * lane,
-                     x, norm);
+  for (int i = 0; i < kMergeRows; ++i) {
+    const int r = r0 + i;
+    if (r >= rows) break;  // uniform
+    float x[4], ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a0 = o[i][0][e] * (L[i][0] > 0.f ? a.v_scale / L[i][0] : 0.f);
+      float a1;
+      if constexpr (kMaps == 2) a1 = o[i][1][e] * (L[i][1] > 0.f ? a.v_scale / L[i][1] : 0.f);
+      else a1 = __shfl_xor(a0, 32, 64);  // map 1 for the lower half
+      x[e] = fmaf(-lambda, a1, a0);
+      ss = fmaf(x[e], x[e], ss);
+      x[e] *= w[e];
+    }
+#pragma unroll
+    for (int s = kMaps == 2 ? 32 : 16; s > 0; s >>= 1) ss += __shfl_xor(ss, s, 64);
+    const float norm = (1.f - a.diff.init) / sqrtf(ss * (1.f / kV) + a.diff.eps);
+    if (kMaps == 2 || lane < 32)
+      store_dims<4, H16>(a.out + (int64_t)(d[2] + r / G) * a.out_row_stride +
+                             (int64_t)(p * G + r % G) * kV + dim,
+                         x, norm);
+  }
 }
 
-// Tiles that a batch can have, and the ranges that a tile is cut into.
+// Tiles that a batch can have.
 static int64_t diff_max_tiles(int64_t total_q, int64_t n_seqs, int qt) {
   return total_q / qt + n_seqs;
 }
-static int diff_splits(int64_t total_q, int64_t n_seqs, int64_t max_seqlen_k, int pairs, int G,
-                       int D) {
-  const int64_t groups = diff_max_tiles(total_q, n_seqs, diff_rows(D) / G) * pairs;
+
+// What a launch with a workspace does: into how many ranges a tile's keys are cut, and how many
+// workgroups stream the decode rows.
+struct DiffPlan {
+  int64_t target, range_cap, tile_cap;
+  int row_groups, ncg;
+  size_t tile_bytes, part_bytes, desc_bytes, row_bytes;
+  size_t bytes() const { return tile_bytes + part_bytes + desc_bytes + row_bytes; }
+};
+static DiffPlan diff_plan(int64_t n_seqs, int64_t total_q, int64_t max_seqlen_q,
+                          int64_t max_seqlen_k, int P, int G, int D, bool f8, bool paged) {
+  const int qt = diff_rows(D) / G;
+  const BatchMix mix = batch_mix(n_seqs, total_q, std::max<int64_t>(max_seqlen_q, 1));
   const int64_t resident = (int64_t)device_cus() * (D == 128 ? 1 : 2);
-  const int64_t most = max_seqlen_k / (kDiffStep * kDiffMinSteps);
-  return (int)std::max<int64_t>(1, std::min(most, (2 * resident + groups - 1) / groups));
+  DiffPlan d{};
+  int64_t tiles = diff_max_tiles(total_q, n_seqs, qt);  // that the batch has, about
+  int64_t slots = resident;
+  // (max_seqlen_q = 1 with more rows than sequences: padding, or not known)
+  if (paged && mix.rows > 0 && (max_seqlen_q > 1 || (max_seqlen_q == 1 && total_q <= n_seqs))) {
+    // A row's step of 64 keys is bound by its K/V bytes, a tile's by the matrix cores; of a CU's
+    // time they take about as much at head_dim 128, a third more at 64, half of it with fp8.
+    tiles = mix.prompts > 0 ? diff_max_tiles(mix.prompt_rows, mix.prompts, qt) : 0;
+    const double rows = (double)mix.rows * kDiffRowShare * (f8 ? 0.5 : 1.0);
+    d.ncg = decode_ncg(2 * G);
+    const int np = P * d.ncg;  // groups of waves
+    const int64_t least = (np + diff_waves(D) - 1) / diff_waves(D);
+    d.row_groups = (int)std::max<int64_t>(
+        least, std::min<int64_t>((int64_t)(resident * rows / (rows + (double)tiles)),
+                                 mix.rows * P * std::max<int64_t>(1, max_seqlen_k / 64) /
+                                         diff_waves(D) + 1));
+    slots = std::max<int64_t>(resident - d.row_groups, 1);
+    const int64_t waves = (int64_t)d.row_groups * diff_waves(D) / np;  // of a group
+    d.desc_bytes = (size_t)n_seqs * P * d.ncg * sizeof(i32x4v_t);
+    d.row_bytes = (size_t)((waves + n_seqs) * 2 * G * P) * part_row(2 * D) * sizeof(float);
+  }
+  if (tiles > 0 && tiles * P < slots && max_seqlen_k >= 2 * kDiffStep * kDiffMinSteps) {
+    d.target = std::max<int64_t>(1, slots / P);
+    d.range_cap = d.target + d.target / 2 + tiles;
+    d.tile_cap = tiles;
+    d.tile_bytes = (size_t)(tiles + 1) * sizeof(i32x4_t);
+    d.part_bytes = (size_t)d.range_cap * P * 2 * diff_rows(D) * diff_part_row(D) * sizeof(float);
+  }
+  return d;
+}
+
+// Workgroups of a launch: the decode rows', and those of the ranges, or of the tiles where a batch
+// has more of them than its plan.
+static int64_t diff_groups_of(const DiffPrefillArgs& a, int64_t tiles) {
+  return a.row_groups + std::max<int64_t>(a.range_cap, tiles) * a.P;
 }
 
 template <bool F8, int D, bool H16, bool PAGED>
 static void diff_launch(const DiffPrefillArgs& a, int64_t tiles, hipStream_t s) {
   hipLaunchKernelGGL((diff_prefill_kernel<F8, D, H16, PAGED>),
-                     dim3((unsigned)(tiles * a.P * a.n_splits)), dim3(64 * diff_waves(D)), 0, s,
-                     a);
-  if (a.n_splits > 1)
-    hipLaunchKernelGGL((diff_merge_kernel<D, H16>),
-                       dim3((unsigned)(tiles * a.P), diff_rows(D) / kDiffMergeWaves),
-                       dim3(64 * kDiffMergeWaves), 0, s, a);
+                     dim3((unsigned)diff_groups_of(a, tiles)), dim3(64 * diff_waves(D)), 0, s, a);
+  const int64_t groups = (int64_t)a.tile_cap * a.P * (diff_rows(D) / (kDiffMergeWaves * kMergeRows));
+  const int64_t rows =
+      a.row_groups > 0 ? ((int64_t)a.n_seqs * a.P * a.G + kDiffMergeWaves / 2 - 1) /
+                             (kDiffMergeWaves / 2)
+                       : 0;
+  if (groups + rows > 0)
+    hipLaunchKernelGGL((diff_merge_kernel<D, H16>), dim3((unsigned)(groups + rows)),
+                       dim3(64 * kDiffMergeWaves), 0, s, a, (int32_t)groups);
 }
 
 }  // namespace nkv
 
-extern "C" size_t nkv_diff_prefill_workspace_bytes(int32_t n_seqs, int64_t total_q,
+extern "C" size_t nkv_diff_prefill_workspace_bytes(int32_t kv_type, int32_t n_seqs,
+                                                   int64_t total_q, int64_t max_seqlen_q,
                                                    int64_t max_seqlen_k, int32_t n_q_heads,
-                                                   int32_t n_kv_heads, int32_t head_dim) {
+                                                   int32_t n_kv_heads, int32_t head_dim,
+                                                   int32_t paged) {
   using namespace nkv;
   if (n_seqs <= 0 || total_q <= 0 || n_kv_heads <= 0 || n_kv_heads % 2 || n_q_heads <= 0 ||
       n_q_heads % n_kv_heads || n_q_heads / n_kv_heads > NKV_DIFF_MAX_GROUP ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  const int G = n_q_heads / n_kv_heads, P = n_kv_heads / 2;
-  const int splits = diff_splits(total_q, n_seqs, max_seqlen_k, P, G, head_dim);
-  if (splits < 2) return 0;
-  return (size_t)diff_max_tiles(total_q, n_seqs, diff_rows(head_dim) / G) * P * splits * 2 *
-         diff_rows(head_dim) * diff_part_row(head_dim) * sizeof(float);
+  return diff_plan(n_seqs, total_q, max_seqlen_q, max_seqlen_k, n_kv_heads / 2,
+                   n_q_heads / n_kv_heads, head_dim, kv_type == NKV_KV_FP8, paged != 0)
+      .bytes();
 }
 
 extern "C" int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_stride,
@@ -750,8 +963,8 @@ extern "C" int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_st
                                 int64_t k_row_stride, int64_t v_row_stride,
                                 const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
                                 const int32_t* block_tables, int64_t bt_row_stride,
-                                int32_t max_blocks_per_seq, int32_t n_seqs, int64_t max_seqlen_k,
-                                int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                int32_t max_blocks_per_seq, int32_t n_seqs, int64_t max_seqlen_q,
+                                int64_t max_seqlen_k, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
                                 int32_t block_size, int64_t n_rows, float scale, float k_scale,
                                 float v_scale, const float* lambdas, float lambda_init,
                                 const void* norm_weight, float eps, void* out,
@@ -798,18 +1011,37 @@ extern "C" int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_st
     NKV_REQUIRE(n_rows < (1ll << 31), NKV_EUNSUPPORTED, "diff_prefill: too many K/V rows");
   }
   DiffPrefillArgs a{};
-  a.n_splits = 1;
-  if (workspace) {
-    const size_t need = nkv_diff_prefill_workspace_bytes(n_seqs, total_q, max_seqlen_k, n_q_heads,
-                                                         n_kv_heads, head_dim);
-    NKV_REQUIRE(workspace_bytes >= need && aligned16(workspace), NKV_EWORKSPACE,
-                "diff_prefill: workspace needs %zu bytes, 16-byte aligned (got %zu)", need,
-                workspace_bytes);
-    a.n_splits = diff_splits(total_q, n_seqs, max_seqlen_k, P, G, head_dim);
-  }
   const int64_t tiles = diff_max_tiles(total_q, n_seqs, diff_rows(head_dim) / G);
-  NKV_REQUIRE(tiles * P * a.n_splits < (1ll << 31), NKV_EUNSUPPORTED,
-              "diff_prefill: too many tiles");
+  if (workspace) {
+    const DiffPlan d = diff_plan(n_seqs, total_q, max_seqlen_q, max_seqlen_k, P, G, head_dim, f8,
+                                 paged);
+    NKV_REQUIRE(workspace_bytes >= d.bytes() && aligned16(workspace), NKV_EWORKSPACE,
+                "diff_prefill: workspace needs %zu bytes, 16-byte aligned (got %zu)", d.bytes(),
+                workspace_bytes);
+    char* ws = static_cast<char*>(workspace);
+    a.target = (int32_t)d.target;
+    a.cus = (float)std::max(1, device_cus() - d.row_groups);
+    a.range_cap = (int32_t)d.range_cap;
+    a.tile_cap = (int32_t)d.tile_cap;
+    a.tile_desc = reinterpret_cast<i32x4_t*>(ws);
+    ws += d.tile_bytes;
+    a.part = reinterpret_cast<float*>(ws);
+    if (d.row_groups > 0) {
+      const int64_t max_chunks = decode_max_chunks(max_blocks_per_seq, block_size);
+      NKV_REQUIRE((int64_t)max_blocks_per_seq * block_size < (1ll << 30) &&
+                      max_chunks * n_seqs * P < (1ll << 31),
+                  NKV_EUNSUPPORTED, "diff_prefill: too many keys in one call");
+      a.row_groups = d.row_groups;
+      a.ncg = d.ncg;
+      a.min_chunks = decode_min_chunks(max_chunks, kMinChunks);
+      a.max_tokens = max_blocks_per_seq * block_size;
+      a.row_desc = reinterpret_cast<i32x4v_t*>(ws + d.part_bytes);
+      a.row_part = reinterpret_cast<float*>(ws + d.part_bytes + d.desc_bytes);
+    }
+  }
+  NKV_REQUIRE((tiles + (int64_t)a.range_cap) * P * diff_rows(head_dim) < (1ll << 30) &&
+                  (int64_t)n_seqs * n_q_heads < (1ll << 30),
+              NKV_EUNSUPPORTED, "diff_prefill: too many tiles");
   a.q = (const bf16_t*)q;
   a.q_row_stride = q_row_stride;
   a.k = k;
@@ -827,13 +1059,11 @@ extern "C" int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_st
   a.n_limit = (int32_t)(paged ? n_rows / block_size : n_rows);
   a.n_seqs = n_seqs;
   a.total_q = (int32_t)total_q;
-  a.min_steps = kDiffMinSteps;
   a.scale_log2 = scale * (f8 ? k_scale : 1.f) * kLog2e;
   a.v_scale = f8 ? v_scale : 1.f;
   a.diff = DiffArgs{lambdas, (const bf16_t*)norm_weight, lambda_init, eps};
   a.out = (bf16_t*)out;
   a.out_row_stride = out_row_stride;
-  a.part = static_cast<float*>(workspace);
   hipStream_t s = as_stream(stream);
 #define NKV_DIFF_LAUNCH(D)                                            \
   do {                                                                \

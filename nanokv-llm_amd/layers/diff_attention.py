@@ -122,13 +122,16 @@ def diff_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     return out
 
 
-def diff_prefill_workspace(q: torch.Tensor, k: torch.Tensor, n_seqs: int,
+def diff_prefill_workspace(q: torch.Tensor, k: torch.Tensor, n_seqs: int, max_seqlen_q: int,
                            max_seqlen_k: int) -> torch.Tensor | None:
     """The workspace for splitting diff_varlen_prefill's keys where that is of use (few query tiles
-    over long contexts), else None. Sized by the chip and the tiles, not by the lengths; None
-    too where the device has no such memory left, since nothing else needs any."""
-    nbytes = _lib.lib().nkv_diff_prefill_workspace_bytes(n_seqs, q.size(0), int(max_seqlen_k),
-                                                         q.size(1), k.size(-2), q.size(2))
+    over long contexts) and for streaming the sequences that bring one token, else None. Sized by
+    the chip and the tiles, not by the lengths; None too where the device has no such memory
+    left, since nothing else needs any."""
+    kv_type = _lib.NKV_KV_FP8 if k.dtype == _FP8 else _lib.NKV_KV_BF16
+    nbytes = _lib.lib().nkv_diff_prefill_workspace_bytes(
+        kv_type, n_seqs, q.size(0), int(max_seqlen_q), int(max_seqlen_k), q.size(1), k.size(-2),
+        q.size(2), 1 if k.dim() == 4 else 0)
     try:
         return torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     except torch.OutOfMemoryError:
@@ -148,9 +151,9 @@ def diff_varlen_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
     With ``block_tables`` k and v are the paged caches [NB, B, Hk, D] (q's dtype, or fp8 with bf16
     q); without, they are [sum Lk, Hk, D] rows, each with its own row stride. ``lambdas`` and
-    ``norm_weight`` are ``diff_paged_decode``'s, the rest ``varlen_prefill``'s (``max_seqlen_q`` is
-    not needed here: the rows of q say how many tiles there are). Given ``max_seqlen_k``, the keys
-    are split over the chip where few tiles would leave it idle, in ``workspace``
+    ``norm_weight`` are ``diff_paged_decode``'s, the rest ``varlen_prefill``'s. Given
+    ``max_seqlen_k``, the keys are split over the chip where few tiles would leave it idle and
+    sequences that bring one token are streamed apart from the tiles, in ``workspace``
     (diff_prefill_workspace) or in memory taken for the call; without, nothing but the output is
     allocated. A row that sees no key gives zeros.
     """
@@ -181,11 +184,11 @@ def diff_varlen_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
               f"{what}: workspace must be contiguous uint8")
     with _lib.device_of(q.get_device()):
         if workspace is None and max_seqlen_k is not None:
-            workspace = diff_prefill_workspace(q, k, n_seqs, max_seqlen_k)
+            workspace = diff_prefill_workspace(q, k, n_seqs, max_seqlen_q, max_seqlen_k)
         rc = _lib.lib().nkv_diff_prefill(
             kv_type, q.data_ptr(), q.stride(0), N, k.data_ptr(), v.data_ptr(), k_stride, v_stride,
             cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), bt, bt_stride, width, n_seqs,
-            0 if max_seqlen_k is None else int(max_seqlen_k), Hq, Hk, D, B, rows, scale, k_scale,
+            int(max_seqlen_q), 0 if max_seqlen_k is None else int(max_seqlen_k), Hq, Hk, D, B, rows, scale, k_scale,
             v_scale, lambdas.data_ptr(), lambda_init, _lib.ptr(norm_weight), eps, out.data_ptr(),
             out.stride(0), _lib.ptr(workspace), 0 if workspace is None else workspace.numel(),
             _lib.stream_of(q))

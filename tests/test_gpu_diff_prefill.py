@@ -109,7 +109,7 @@ def test_split_keys_against_whole_ones(dev, d, kv):
     """Few tiles over long contexts: the keys are split, and every range count gives the row."""
     c = make(dev, [40, 1, 7], [4500, 2100, 520], 8, 4, d, seed=d, kv=kv)
     q, k = c["q"].to(dev), c["k"].to(dev)
-    assert da.diff_prefill_workspace(q, k, 3, 4500) is not None
+    assert da.diff_prefill_workspace(q, k, 3, 40, 4500) is not None
     check(run(c), c)
     check(run(c, split=False), c)
 
