@@ -14,7 +14,11 @@
 // one walk over the counts for the free pages) and, where pages are copied or many table entries
 // change, a second launch of up to kCopyGroups workgroups that reads the plan from the workspace.
 // A copy is bound by HBM: rows are read once and written once, 16 bytes a lane, kCopyUnroll of them
-// in flight; the grid's y runs over the 2 * layers planes of the pool.
+// in flight; the grid's y runs over the 2 * layers planes of the pool. 50 pages of 1 MiB in each of 32
+// planes: 333 us, 5.0 TB/s read and written together (a copy of 2 GiB: 4.8); twice or half the loads in
+// flight or the workgroups within 3%, loads that bypass the caches 4% faster there and 15% slower where
+// the same rows are read several times (four beams of one sequence).
+// Kernel times: one token each for 64 rows 3.7 us; 33 rows rolled back 6.5 + 3.8.
 #include "nkv_common.h"
 
 #include <algorithm>
@@ -176,8 +180,7 @@ __device__ __forceinline__ void drop_ref(const PagesArgs& a, int id) {
 __global__ __launch_bounds__(kPlan) void pages_append_kernel(
     const PagesArgs a, const int32_t* __restrict__ rows, int n, const int32_t* __restrict__ cu,
     int64_t n_tokens, int32_t* __restrict__ slots, int32_t* __restrict__ status) {
-  extern __shared__ int lds[];  // marks, then the entries' prefix sums
-  __shared__ int granted;
+  extern __shared__ int lds[];
   int bad = 0;
   if (cu) {
     for (int i = threadIdx.x; i < n; i += kPlan)
@@ -186,7 +189,6 @@ __global__ __launch_bounds__(kPlan) void pages_append_kernel(
     bad = __syncthreads_or(bad);
   }
   mark_first(a, rows, n, lds);
-  if (threadIdx.x == 0) granted = 0;
   Needs needs;
   for (int base = 0; base < n; base += kPlan) {  // uniform
     const int i = base + (int)threadIdx.x;
@@ -217,11 +219,9 @@ __global__ __launch_bounds__(kPlan) void pages_append_kernel(
     const int need = it[0] < 0 ? 0 : pages_of(a, it[1] + it[2]) - have;
     const bool ok = it[0] >= 0 && (need == 0 || it[3] + need <= n_free);
     status[i] = ok;
-    lds[i] = it[3];
     if (ok) a.lens[it[0]] = it[1] + it[2];
-    if (cu) {
+    if (cu) {  // pages_slots_kernel gives the tokens their pages
       if (!ok) a.items[i] = i32x4w_t{-1, 0, 0, 0};
-      else if (need) atomicMax(&granted, it[3] + need);
     } else {  // one token: its page and its slot
       int slot = -1;
       if (ok) {
@@ -236,18 +236,10 @@ __global__ __launch_bounds__(kPlan) void pages_append_kernel(
       slots[i] = slot;
     }
   }
-  if (!cu) return;
-  __syncthreads();
-  for (int k = threadIdx.x; k < granted; k += kPlan) {
-    const int i = entry_of(lds, n, k);
-    const i32x4w_t it = a.items[i];
-    const int page = a.ids[k];
-    table_of(a, it[0])[pages_of(a, it[1]) + k - lds[i]] = page;
-    a.refs[page] = 1;
-  }
 }
 
-// The slots of the tokens that a call with cu appended, one a thread.
+// The slots of the tokens that a call with cu appended, one a thread; the first token of a new page
+// enters it in the table.
 __global__ __launch_bounds__(256) void pages_slots_kernel(const PagesArgs a, int n,
                                                           const int32_t* __restrict__ cu,
                                                           int64_t n_tokens,
@@ -257,11 +249,16 @@ __global__ __launch_bounds__(256) void pages_slots_kernel(const PagesArgs a, int
   int slot = -1;
   if (n > 0 && t >= cu[0] && t < cu[n]) {
     const int i = entry_of(cu, n, (int)t);
-    const i32x4w_t it = a.items[i];
+    const i32x4w_t it = a.items[i];  // {row, length before, tokens, pages before its own}
     const int j = (int)t - cu[i];
     if (it[0] >= 0 && j < it[2]) {
-      const int pos = it[1] + j;
-      const int page = table_of(a, it[0])[pos / a.B];
+      const int pos = it[1] + j, k = pos / a.B - pages_of(a, it[1]);
+      int32_t* entry = table_of(a, it[0]) + pos / a.B;
+      const int page = k >= 0 ? a.ids[it[3] + k] : *entry;
+      if (k >= 0 && pos % a.B == 0) {
+        *entry = page;
+        a.refs[page] = 1;
+      }
       if (page_ok(a, page)) slot = page * a.B + pos % a.B;
     }
   }
@@ -383,40 +380,61 @@ __global__ __launch_bounds__(kPlan) void pages_fork_kernel(
 __global__ __launch_bounds__(kPlan) void pages_compact_kernel(const PagesArgs a, int max_moves,
                                                               int32_t* __restrict__ info,
                                                               i32x2_t* __restrict__ moves) {
-  int n_live = 0;
-  for (int base = 0; base < a.n_pages; base += kPlan * kWalk) {  // uniform
-    int total;
-    plan_scan(__popc(count_bits<false>(a.refs, base + (int)threadIdx.x * kWalk, a.n_pages)),
-              total);
-    n_live += total;
-  }
-  const int n_holes = find_free(a.refs, n_live, n_live, a.ids);
-  const int n = min(n_holes, max_moves);
-  __syncthreads();
-  // the k-th lowest hole takes the k-th highest page in use; as many of those are at n_live and
-  // above as there are holes below
-  int rank = 0;
-  for (int base = n_live / kWalk * kWalk; base < a.n_pages; base += kPlan * kWalk) {  // uniform
-    const int i0 = base + (int)threadIdx.x * kWalk;
-    uint32_t bits = count_bits<false>(a.refs, i0, a.n_pages);
-    if (i0 < n_live) bits &= ~((1u << (n_live - i0)) - 1u);
-    int total;
-    int at = rank + plan_scan(__popc(bits), total);
-    for (int id = max(i0, n_live); id < min(i0 + kWalk, a.n_pages); ++id) {
-      const bool live = bits >> (id - i0) & 1u;
-      const int k = n_holes - 1 - at;
-      const bool moved = live && k >= 0 && k < n;
-      const int to = moved ? a.ids[k] : id;
-      a.map[id] = to;
-      if (moved) {
-        a.copies[k] = i32x4w_t{id, to, a.B, 0};
-        moves[k] = i32x2_t{id, to};
-        a.refs[to] = a.refs[id];
-        a.refs[id] = 0;
-      }
-      at += live;
+  // The k-th lowest hole takes the k-th highest page in use; as many of those are at n_live and
+  // above as there are holes below. `rank`: the page's, from below, among those.
+  int n_live = 0, n_holes = 0, n = 0;
+  auto place = [&](int id, bool live, int rank) {
+    const int k = n_holes - 1 - rank;
+    const bool moved = live && k >= 0 && k < n;
+    const int to = moved ? a.ids[k] : id;
+    a.map[id] = to;
+    if (moved) {
+      a.copies[k] = i32x4w_t{id, to, a.B, 0};
+      moves[k] = i32x2_t{id, to};
+      a.refs[to] = a.refs[id];
+      a.refs[id] = 0;
     }
-    rank += total;
+  };
+  if (a.n_pages <= kPlan * kWalk) {  // one step of a walk: the counts are read once
+    const int i0 = (int)threadIdx.x * kWalk;
+    const uint32_t live = count_bits<false>(a.refs, i0, a.n_pages);
+    int rank = plan_scan(__popc(live), n_live);
+    const int below = max(0, min(n_live - i0, kWalk));  // of the thread's pages, below n_live
+    uint32_t holes = ~live & ((1u << below) - 1u);
+    int at = plan_scan(__popc(holes), n_holes);
+    for (; holes; holes &= holes - 1) a.ids[at++] = i0 + __builtin_ctz(holes);
+    n = min(n_holes, max_moves);
+    __syncthreads();
+    rank += __popc(live & ((1u << below) - 1u)) - (n_live - n_holes);
+    for (int e = below; e < min(kWalk, a.n_pages - i0); ++e) {
+      const bool l = live >> e & 1u;
+      place(i0 + e, l, rank);
+      rank += l;
+    }
+  } else {
+    for (int base = 0; base < a.n_pages; base += kPlan * kWalk) {  // uniform
+      int total;
+      plan_scan(__popc(count_bits<false>(a.refs, base + (int)threadIdx.x * kWalk, a.n_pages)),
+                total);
+      n_live += total;
+    }
+    n_holes = find_free(a.refs, n_live, n_live, a.ids);
+    n = min(n_holes, max_moves);
+    __syncthreads();
+    int before = 0;
+    for (int base = n_live / kWalk * kWalk; base < a.n_pages; base += kPlan * kWalk) {  // uniform
+      const int i0 = base + (int)threadIdx.x * kWalk;
+      uint32_t bits = count_bits<false>(a.refs, i0, a.n_pages);
+      if (i0 < n_live) bits &= ~((1u << (n_live - i0)) - 1u);
+      int total;
+      int rank = before + plan_scan(__popc(bits), total);
+      for (int id = max(i0, n_live); id < min(i0 + kWalk, a.n_pages); ++id) {
+        const bool l = bits >> (id - i0) & 1u;
+        place(id, l, rank);
+        rank += l;
+      }
+      before += total;
+    }
   }
   for (int k = n + (int)threadIdx.x; k < max_moves; k += kPlan) moves[k] = i32x2_t{-1, -1};
   if (threadIdx.x == 0) {
@@ -505,7 +523,7 @@ __global__ __launch_bounds__(kCopyThreads) void pages_apply_kernel(
 #pragma unroll
     for (int e = 0; e < kCopyUnroll; ++e) {
       const int64_t o = at + e * (kCopyThreads * 16);
-      if (o < bytes) *reinterpret_cast<u32x4_t*>(dst + o) = v[e];
+      if (o < bytes) __builtin_nontemporal_store(v[e], reinterpret_cast<u32x4_t*>(dst + o));
     }
   }
 }
