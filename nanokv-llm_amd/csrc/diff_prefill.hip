@@ -46,11 +46,13 @@ constexpr int kDiffMergeWaves = 4;
 // Decode rows' share of the workgroups: CU time of a row's step against a tile's (see diff_plan).
 constexpr double kDiffRowShare = 0.6;
 
-// Waves of a workgroup, and 16-row groups of a wave. At head_dim 128 a step's tiles take 64 KiB, so
-// one workgroup is resident and brings both waves of each SIMD itself.
+// Waves of a workgroup, and 16-row groups of a wave at most. At head_dim 128 a step's tiles take
+// 64 KiB, so one workgroup is resident and brings both waves of each SIMD itself; with fp8 codes on
+// their way through registers two groups do not fit them (1006 us and spills, one 980: four chunks of
+// up to 2048 tokens over up to 6000, Hq 32, Hk 8).
 constexpr int diff_waves(int D) { return D == 128 ? 8 : 4; }
-constexpr int diff_groups(int D) { return D == 128 ? 2 : 3; }
-constexpr int diff_rows(int D) { return 8 * diff_waves(D) * diff_groups(D); }  // of a tile
+constexpr int diff_groups(int D, bool f8) { return D == 128 ? (f8 ? 1 : 2) : 3; }
+constexpr int diff_rows(int D, int rg) { return 8 * diff_waves(D) * rg; }  // of a tile
 constexpr int diff_part_row(int D) { return 2 * D + 4; }  // floats: O, m, l, 2 pad
 
 struct DiffPrefillArgs {
@@ -91,13 +93,14 @@ __device__ __forceinline__ int diff_steps(int Lq, int Lk, int QT, int tile) {
 // Range x of a pair, by the whole wave; false past the last one. The tiles of a sequence have as many
 // places for ranges as its last one needs, so that a lane knows its sequence's number without a
 // loop; the others' last places stay empty. n_tiles: all tiles, 0 where none is cut.
-template <int D>
+template <int D, int RG>
 __device__ __forceinline__ bool diff_range(const DiffPrefillArgs& a, int QT, int x, DiffTile& d,
                                            int& n_tiles) {
   // measured: a step of a workgroup alone on its CU and of one of two, two chunks' partial rows
   // (101 and 266 KB a range) written and merged, and what the merge takes beside that
-  constexpr float kStepUs[2] = {D == 64 ? 1.6f : 2.2f, D == 64 ? 2.1f : 2.2f};
-  constexpr float kRangeUs = D == 64 ? 0.03f : 0.04f, kMergeUs = 6.f;
+  constexpr float kStepUs[2] = {D == 64 ? (RG == 1 ? 0.8f : 1.6f) : (RG == 1 ? 1.4f : 2.2f),
+                                D == 64 ? (RG == 1 ? 1.1f : 2.1f) : (RG == 1 ? 1.4f : 2.2f)};
+  constexpr float kRangeUs = D == 64 ? 0.01f * RG : 0.02f * RG, kMergeUs = 6.f;
   const int lane = threadIdx.x & 63;
   int q0 = 0, Lq = 0, kb0 = 0, Lk = 0, nt = 0, hi = 0, at = -1;
   auto load = [&](int cb) {  // lane: sequence cb + lane
@@ -208,16 +211,16 @@ struct OneDiffSeqs : OneRowSeqs {
 };
 
 // The partial rows of range x of pair p, map 0's then map 1's.
-template <int D>
+template <int D, int RG>
 __device__ __forceinline__ float* diff_part(const DiffPrefillArgs& a, int x, int p) {
-  return a.part + ((int64_t)x * a.P + p) * (2 * diff_rows(D) * diff_part_row(D));
+  return a.part + ((int64_t)x * a.P + p) * (2 * diff_rows(D, RG) * diff_part_row(D));
 }
 
-template <bool F8, int D, bool H16, bool PAGED>
+template <bool F8, int D, bool H16, bool PAGED, int RG>
 __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
     const DiffPrefillArgs a) {
   static_assert(!(F8 && (H16 || !PAGED)), "fp8 caches are paged and read with bf16 queries");
-  constexpr int kWaves = diff_waves(D), kRG = diff_groups(D);
+  constexpr int kWaves = diff_waves(D), kRG = RG;
   constexpr bool kPing = kWaves == 8;
   constexpr int kV = 2 * D;                     // dims of a K or V row of the pair
   constexpr int kEl = F8 ? 1 : 2;               // bytes per cache element
@@ -248,7 +251,7 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   const int map = wave / (kWaves / 2);
   const int wi = wave % (kWaves / 2);  // which rows
   const int G = a.G, P = a.P;
-  const int QT = diff_rows(D) / G;     // queries per tile
+  const int QT = diff_rows(D, RG) / G;  // queries per tile
 
   if constexpr (PAGED) {
     if ((int)blockIdx.x < a.row_groups) {
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   const int x = ((int)blockIdx.x - a.row_groups) / P;
   DiffTile d;
   int n_tiles;
-  const bool some = diff_range<D>(a, QT, x, d, n_tiles);
+  const bool some = diff_range<D, RG>(a, QT, x, d, n_tiles);
   if (a.target > 0 && p == 0 && tid == 0) {
     if (x == 0) a.tile_desc[a.tile_cap] = i32x4_t{n_tiles, 0, 0, 0};
     if (some && d.sp == 0 && d.id < a.tile_cap)
@@ -704,7 +707,7 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   for (int rr = 0; rr < kRG; ++rr) l[rr] = col_sum4(l_run[rr]);
   if (d.ranges > 1) {  // a part: O, m and l as they are
     if (!active) return;
-    float* rows = diff_part<D>(a, x, p) + (int64_t)map * (diff_rows(D) * diff_part_row(D));
+    float* rows = diff_part<D, RG>(a, x, p) + (int64_t)map * (diff_rows(D, RG) * diff_part_row(D));
 #pragma unroll
     for (int rr = 0; rr < kRG; ++rr) {
       if (jrow[rr] >= Lq) continue;
@@ -765,15 +768,15 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
 // every lane has 4 dims of both. kMergeFly ranges' loads are in flight. (One row a wave: 17 us over the
 // 50 MB of two prompts of 512 tokens, Hq 32, Hk 8, head_dim 64.)
 constexpr int kMergeRows = 4;
-template <int D, bool H16>
+template <int D, bool H16, int RG>
 __global__ __launch_bounds__(64 * kDiffMergeWaves) void diff_merge_kernel(
     const DiffPrefillArgs a, const int32_t tile_groups) {
   constexpr int kMaps = D / 64;  // of a lane
   constexpr int kMergeFly = 4 / kMaps;
   constexpr int kV = 2 * D;
   constexpr int kRow = diff_part_row(D);
-  constexpr int kRowGroups = diff_rows(D) / (kDiffMergeWaves * kMergeRows);  // of a tile
-  static_assert(diff_rows(D) % (kDiffMergeWaves * kMergeRows) == 0, "whole workgroups");
+  constexpr int kRowGroups = diff_rows(D, RG) / (kDiffMergeWaves * kMergeRows);  // of a tile
+  static_assert(diff_rows(D, RG) % (kDiffMergeWaves * kMergeRows) == 0, "whole workgroups");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int G = a.G, P = a.P;
@@ -798,10 +801,10 @@ __global__ __launch_bounds__(64 * kDiffMergeWaves) void diff_merge_kernel(
   const int dim = lane * 4 % kV;
   float w[4];
   diff_weight<4, H16>(a.diff.weight ? a.diff.weight + dim : nullptr, w);
-  const int64_t map_f = (int64_t)diff_rows(D) * kRow;
+  const int64_t map_f = (int64_t)diff_rows(D, RG) * kRow;
   const int64_t range_f = 2 * map_f * P;
   // the lane's map (the first of them) of row r0
-  const float* part = diff_part<D>(a, d[1], p) + (int64_t)r0 * kRow +
+  const float* part = diff_part<D, RG>(a, d[1], p) + (int64_t)r0 * kRow +
                       (kMaps == 1 ? (lane >> 5) * map_f : 0);
   float M[kMergeRows][kMaps], L[kMergeRows][kMaps];
   f32x4_t o[kMergeRows][kMaps];
@@ -877,20 +880,38 @@ static int64_t diff_max_tiles(int64_t total_q, int64_t n_seqs, int qt) {
   return total_q / qt + n_seqs;
 }
 
+// 16-row groups of a wave: one where the tiles then are no more than the CUs, since fewer rows a step
+// are a shorter step, else as many as fit. One prompt of 300 / 900 tokens (Hq 16, Hk 8), us: head_dim
+// 128 37.5 -> 25.1 / 56.7 -> 41.5, 64 24.5 -> 16.6 / 38.5 -> 25.4. Not at head_dim 64 beside decode
+// rows, which leave no CU idle (two chunks of 512 beside 30, fp8: 57 -> 76; at 128 146 -> 131 for one of
+// 300 beside 100).
+static int diff_choose(int64_t n_seqs, int64_t total_q, int64_t max_seqlen_q, int P, int G, int D,
+                       bool f8) {
+  const int most = diff_groups(D, f8), rows = diff_rows(D, 1);
+  if (most == 1 || G > rows) return most;
+  const BatchMix mix = batch_mix(n_seqs, total_q, std::max<int64_t>(max_seqlen_q, 1));
+  const bool known = max_seqlen_q > 1;
+  const int64_t tiles = known ? diff_max_tiles(mix.prompt_rows, mix.prompts, rows / G)
+                              : diff_max_tiles(total_q, n_seqs, rows / G);
+  if (D == 64 && known && mix.rows > 0) return most;
+  return tiles * P <= device_cus() ? 1 : most;
+}
+
 // What a launch with a workspace does: into how many ranges a tile's keys are cut, and how many
 // workgroups stream the decode rows.
 struct DiffPlan {
   int64_t target, range_cap, tile_cap;
-  int row_groups, ncg;
+  int rg, row_groups, ncg;
   size_t tile_bytes, part_bytes, desc_bytes, row_bytes;
   size_t bytes() const { return tile_bytes + part_bytes + desc_bytes + row_bytes; }
 };
 static DiffPlan diff_plan(int64_t n_seqs, int64_t total_q, int64_t max_seqlen_q,
                           int64_t max_seqlen_k, int P, int G, int D, bool f8, bool paged) {
-  const int qt = diff_rows(D) / G;
+  DiffPlan d{};
+  d.rg = diff_choose(n_seqs, total_q, max_seqlen_q, P, G, D, f8);
+  const int rows_of = diff_rows(D, d.rg), qt = rows_of / G;
   const BatchMix mix = batch_mix(n_seqs, total_q, std::max<int64_t>(max_seqlen_q, 1));
   const int64_t resident = (int64_t)device_cus() * (D == 128 ? 1 : 2);
-  DiffPlan d{};
   int64_t tiles = diff_max_tiles(total_q, n_seqs, qt);  // that the batch has, about
   int64_t slots = resident;
   // (max_seqlen_q = 1 with more rows than sequences: padding, or not known)
@@ -916,7 +937,7 @@ static DiffPlan diff_plan(int64_t n_seqs, int64_t total_q, int64_t max_seqlen_q,
     d.range_cap = d.target + d.target / 2 + tiles;
     d.tile_cap = tiles;
     d.tile_bytes = (size_t)(tiles + 1) * sizeof(i32x4_t);
-    d.part_bytes = (size_t)d.range_cap * P * 2 * diff_rows(D) * diff_part_row(D) * sizeof(float);
+    d.part_bytes = (size_t)d.range_cap * P * 2 * rows_of * diff_part_row(D) * sizeof(float);
   }
   return d;
 }
@@ -927,18 +948,24 @@ static int64_t diff_groups_of(const DiffPrefillArgs& a, int64_t tiles) {
   return a.row_groups + std::max<int64_t>(a.range_cap, tiles) * a.P;
 }
 
-template <bool F8, int D, bool H16, bool PAGED>
+template <bool F8, int D, bool H16, bool PAGED, int RG>
 static void diff_launch(const DiffPrefillArgs& a, int64_t tiles, hipStream_t s) {
-  hipLaunchKernelGGL((diff_prefill_kernel<F8, D, H16, PAGED>),
+  hipLaunchKernelGGL((diff_prefill_kernel<F8, D, H16, PAGED, RG>),
                      dim3((unsigned)diff_groups_of(a, tiles)), dim3(64 * diff_waves(D)), 0, s, a);
-  const int64_t groups = (int64_t)a.tile_cap * a.P * (diff_rows(D) / (kDiffMergeWaves * kMergeRows));
+  const int64_t groups =
+      (int64_t)a.tile_cap * a.P * (diff_rows(D, RG) / (kDiffMergeWaves * kMergeRows));
   const int64_t rows =
       a.row_groups > 0 ? ((int64_t)a.n_seqs * a.P * a.G + kDiffMergeWaves / 2 - 1) /
                              (kDiffMergeWaves / 2)
                        : 0;
   if (groups + rows > 0)
-    hipLaunchKernelGGL((diff_merge_kernel<D, H16>), dim3((unsigned)(groups + rows)),
+    hipLaunchKernelGGL((diff_merge_kernel<D, H16, RG>), dim3((unsigned)(groups + rows)),
                        dim3(64 * kDiffMergeWaves), 0, s, a, (int32_t)groups);
+}
+template <bool F8, int D, bool H16, bool PAGED>
+static void diff_launch(const DiffPrefillArgs& a, int64_t tiles, int rg, hipStream_t s) {
+  if (rg == 1) diff_launch<F8, D, H16, PAGED, 1>(a, tiles, s);
+  else diff_launch<F8, D, H16, PAGED, diff_groups(D, F8)>(a, tiles, s);
 }
 
 }  // namespace nkv
@@ -1011,7 +1038,8 @@ extern "C" int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_st
     NKV_REQUIRE(n_rows < (1ll << 31), NKV_EUNSUPPORTED, "diff_prefill: too many K/V rows");
   }
   DiffPrefillArgs a{};
-  const int64_t tiles = diff_max_tiles(total_q, n_seqs, diff_rows(head_dim) / G);
+  const int rg = diff_choose(n_seqs, total_q, max_seqlen_q, P, G, head_dim, f8);
+  const int64_t tiles = diff_max_tiles(total_q, n_seqs, diff_rows(head_dim, rg) / G);
   if (workspace) {
     const DiffPlan d = diff_plan(n_seqs, total_q, max_seqlen_q, max_seqlen_k, P, G, head_dim, f8,
                                  paged);
@@ -1039,7 +1067,7 @@ extern "C" int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_st
       a.row_part = reinterpret_cast<float*>(ws + d.part_bytes + d.desc_bytes);
     }
   }
-  NKV_REQUIRE((tiles + (int64_t)a.range_cap) * P * diff_rows(head_dim) < (1ll << 30) &&
+  NKV_REQUIRE((tiles + (int64_t)a.range_cap) * P * diff_rows(head_dim, rg) < (1ll << 30) &&
                   (int64_t)n_seqs * n_q_heads < (1ll << 30),
               NKV_EUNSUPPORTED, "diff_prefill: too many tiles");
   a.q = (const bf16_t*)q;
@@ -1067,13 +1095,13 @@ extern "C" int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_st
   hipStream_t s = as_stream(stream);
 #define NKV_DIFF_LAUNCH(D)                                            \
   do {                                                                \
-    if (f8) diff_launch<true, D, false, true>(a, tiles, s);           \
+    if (f8) diff_launch<true, D, false, true>(a, tiles, rg, s);       \
     else if (kv_type == NKV_KV_F16)                                   \
-      paged ? diff_launch<false, D, true, true>(a, tiles, s)          \
-            : diff_launch<false, D, true, false>(a, tiles, s);        \
+      paged ? diff_launch<false, D, true, true>(a, tiles, rg, s)      \
+            : diff_launch<false, D, true, false>(a, tiles, rg, s);    \
     else                                                              \
-      paged ? diff_launch<false, D, false, true>(a, tiles, s)         \
-            : diff_launch<false, D, false, false>(a, tiles, s);       \
+      paged ? diff_launch<false, D, false, true>(a, tiles, rg, s)     \
+            : diff_launch<false, D, false, false>(a, tiles, rg, s);   \
   } while (0)
   if (head_dim == 64) NKV_DIFF_LAUNCH(64);
   else NKV_DIFF_LAUNCH(128);
