@@ -80,8 +80,9 @@ extern "C" int nkv_diff_decode(int32_t kv_type, const void* q, int64_t q_row_str
   int rc = diff_check("diff_decode", kv_type, n_q_heads, n_kv_heads, head_dim, scale, k_scale,
                       v_scale, lambdas, lambda_init, norm_weight, eps);
   if (rc) return rc;
+  if (batch == 0) return NKV_OK;
   // each lane stores its dims, 4 or 8 bytes
-  NKV_REQUIRE(batch <= 0 || (out && (reinterpret_cast<uintptr_t>(out) & 7u) == 0 &&
+  NKV_REQUIRE(batch < 0 || (out && (reinterpret_cast<uintptr_t>(out) & 7u) == 0 &&
                              out_row_stride >= (int64_t)n_q_heads * head_dim &&
                              out_row_stride % 4 == 0),
               NKV_EINVAL, "diff_decode: out must be 8-byte aligned with a row stride >= Hq*D that "
@@ -95,7 +96,7 @@ extern "C" int nkv_diff_decode(int32_t kv_type, const void* q, int64_t q_row_str
                           context_lens, batch, n_q_heads, n_kv_heads / 2, 2 * head_dim, block_size,
                           max_blocks_per_seq, n_blocks, scale, k_scale, v_scale, workspace,
                           workspace_bytes, stream, &p);
-  if (rc || batch == 0) return rc;
+  if (rc) return rc;
   const DiffArgs diff{lambdas, (const bf16_t*)norm_weight, lambda_init, eps};
   const dim3 grid((unsigned)(batch * (n_q_heads / 2)));
 #define NKV_DIFF_COMBINE(D, H16, W)                                                             \

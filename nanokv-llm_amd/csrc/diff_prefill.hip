@@ -162,10 +162,17 @@ __device__ __forceinline__ bool diff_range(const DiffPrefillArgs& a, int QT, int
       cost = INFINITY;  // too many, or what the lane before tries
     const float best = -wave_max(-cost);
     const int k = __builtin_ctzll(__ballot(cost == best) | 1ull << 63);
-    // k = 0: whole tiles; as they are, too, for another batch than the plan was for
+    // k = 0: whole tiles; as they are, too, for another batch than the plan was for (the places,
+    // counted exactly: the workgroups and the partial rows are for range_cap)
     if (k > 0 && tiles <= a.tile_cap) {
       R = __builtin_amdgcn_readlane(mine, k);
-      n_tiles = tiles;
+      int exact = 0;
+      for (int cb = 0; cb < a.n_seqs; cb += 64) {
+        load(cb);
+        exact += __builtin_amdgcn_readlane(wave_incl_scan(nt * max(1, (hi + R - 1) / R)), 63);
+      }
+      if (exact > a.range_cap) R = INT32_MAX;
+      else n_tiles = tiles;
     }
   }
   int base = 0, tiles = 0;

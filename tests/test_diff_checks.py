@@ -1,0 +1,147 @@
+"""Differential attention: the reference's own rules, and the refusals that need no GPU."""
+import importlib
+import math
+
+import pytest
+import torch
+
+from oracle.diff_attention_ref import diff_attention_ref, gather_rows
+
+da = importlib.import_module("nanokv-llm_amd.layers.diff_attention")
+L = importlib.import_module("nanokv-llm_amd._lib")
+BF, I32 = torch.bfloat16, torch.int32
+P = 0x10000
+
+
+def test_reference_against_two_softmaxes():
+    """One pair, written out: the difference of torch's softmaxes, the norm, the weight; lambda = 0
+    leaves the first map, and a row that sees nothing is zero."""
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(n, 2, 8, generator=g, dtype=torch.float64) for n in (3, 5, 5))
+    l, w = torch.randn(4, 8, generator=g) * 0.3, torch.randn(16, generator=g)
+    lam = math.exp(float(l[0].double() @ l[1].double())) \
+        - math.exp(float(l[2].double() @ l[3].double())) + 0.3
+    out = diff_attention_ref(q, k, v, 0.5, l, 0.3, w)
+    for j in range(3):
+        n = 3 + j
+        a = [torch.softmax(k[:n, m] @ q[j, m] * 0.5, 0) @ v[:n].flatten(1) for m in (0, 1)]
+        o = a[0] - lam * a[1]
+        want = 0.7 * o / (o.square().mean() + 1e-5).sqrt() * w.double()
+        assert torch.allclose(out[j, 0], want, rtol=1e-12, atol=1e-12)
+    zero = torch.zeros(4, 8)
+    first = diff_attention_ref(q, k, v, 0.5, zero, 0.0, eps=1e-9)  # lambda = 1 - 1 + 0
+    o = torch.softmax(k[:, 0] @ q[2, 0] * 0.5, 0) @ v.flatten(1)
+    assert torch.allclose(first[2, 0], o / o.square().mean().sqrt(), rtol=1e-6)
+    assert bool((diff_attention_ref(q, k[:2], v[:2], 0.5, l, 0.3, w)[0] == 0).all())
+
+
+def test_gathered_rows():
+    cache = torch.arange(3 * 2, dtype=torch.float32).view(3, 2, 1, 1)
+    table = torch.tensor([2, -1, 0])
+    assert gather_rows(cache, table, 5, 2).flatten().tolist() == [4, 5, 0]
+    assert gather_rows(cache, table, 7, 2, zeros=True).flatten().tolist() == [4, 5, 0, 0, 0, 1, 0]
+
+
+def test_lambda_init():
+    assert da.lambda_init_of(0) == pytest.approx(0.2)
+    assert da.lambda_init_of(1000) == pytest.approx(0.8)
+
+
+def test_layer_refuses_what_the_kernels_do_not_take():
+    D = importlib.import_module("nanokv-llm_amd").DifferentialAttention
+    D(8, 64, 0.125, 4, 0.2)
+    for args in ((8, 32, 0.1, 4, 0.2), (8, 256, 0.1, 4, 0.2), (7, 64, 0.1, 7, 0.2),
+                 (8, 64, 0.1, 3, 0.2), (12, 64, 0.1, 8, 0.2), (130, 64, 0.1, 2, 0.2),
+                 (8, 64, 0.0, 4, 0.2), (8, 64, 0.1, 4, 0.2, 0.0)):
+        with pytest.raises(ValueError, match="DifferentialAttention"):
+            D(*args)
+
+
+def test_layer_refuses_a_compression_step():
+    nkv = importlib.import_module("nanokv-llm_amd")
+    layer = nkv.DifferentialAttention(8, 64, 0.125, 4, 0.2)
+    nkv.set_context(True)
+    nkv.get_context().is_compress_step = True
+    try:
+        with pytest.raises(ValueError, match="compression"):
+            layer(None, None, None)
+    finally:
+        nkv.reset_context()
+
+
+def test_wrappers_refuse_host_tensors():
+    q, kc = torch.zeros(2, 8, 64, dtype=BF), torch.zeros(4, 16, 4, 64, dtype=BF)
+    lens, bt, l = torch.ones(2, dtype=I32), torch.zeros(2, 4, dtype=I32), torch.zeros(4, 64)
+    with pytest.raises(ValueError, match="expected GPU"):
+        da.diff_paged_decode(q, kc, kc, lens, bt, 0.1, l, 0.2)
+    with pytest.raises(ValueError, match="expected GPU"):
+        da.diff_varlen_prefill(q, kc, kc, lens, lens, 1, 0.1, l, 0.2, block_tables=bt)
+
+
+DECODE = dict(kv=0, q=P, qrs=512, k=P, v=P, bt=P, btrs=8, ctx=P, n=2, hq=8, hk=4, d=64, bs=16, mb=8,
+              nb=100, scale=0.1, ks=1.0, vs=1.0, l=P, init=0.2, w=P, eps=1e-5, out=P, ors=512, ws=P,
+              wsb=1 << 30)
+PREFILL = dict(kv=0, q=P, qrs=512, tq=10, k=P, v=P, krs=256, vrs=256, cq=P, ck=P, bt=P, btrs=8,
+               mb=8, n=2, mq=10, mk=100, hq=8, hk=4, d=64, bs=16, rows=1600, scale=0.1, ks=1.0,
+               vs=1.0, l=P, init=0.2, w=P, eps=1e-5, out=P, ors=512, ws=None, wsb=0)
+BOTH = [
+    (dict(kv=3), -1, b"kv_type"), (dict(hq=7), -1, b"pairs"), (dict(hk=3), -1, b"pairs"),
+    (dict(hq=12, hk=8), -1, b"pairs"), (dict(hq=0), -1, b"pairs"), (dict(d=96), -4, b"head_dim"),
+    (dict(d=256), -4, b"head_dim"), (dict(hq=260, hk=4), -4, b"above 64"),
+    (dict(scale=0.0), -1, b"scales"), (dict(scale=float("nan")), -1, b"scales"),
+    (dict(ks=0.0), -1, b"scales"), (dict(vs=float("inf")), -1, b"scales"),
+    (dict(init=float("inf")), -1, b"lambda_init"), (dict(eps=0.0), -1, b"eps"),
+    (dict(l=None), -1, b"lambdas"), (dict(w=P + 4), -1, b"norm_weight"),
+    (dict(out=P + 2), -1, b"8-byte"), (dict(ors=500), -1, b"stride"), (dict(ors=514), -1, b"stride"),
+    (dict(q=P + 8), -1, b"16-byte"), (dict(k=P + 8), -1, b"16-byte"),
+    (dict(qrs=511), -1, b"stride"), (dict(bs=8), -4, b"multiple of 16"),
+    (dict(btrs=4), -1, b"block table"),
+]
+
+
+@pytest.mark.parametrize("name,base", [("nkv_diff_decode", DECODE), ("nkv_diff_prefill", PREFILL)])
+@pytest.mark.parametrize("kw,code,msg", BOTH)
+def test_entry_points_refuse(name, base, kw, code, msg):
+    rc = getattr(L.lib(), name)(*dict(base, **kw).values(), None)
+    assert rc == code and msg in L.lib().nkv_last_error(), (rc, L.lib().nkv_last_error())
+
+
+@pytest.mark.parametrize("kw,code,msg", [
+    (dict(q=None), -1, b"null"), (dict(cq=None), -1, b"null"), (dict(out=None), -1, b"null"),
+    (dict(n=-1), -1, b"sizes"), (dict(tq=-1), -1, b"sizes"), (dict(tq=1 << 31), -1, b"sizes"),
+    (dict(krs=250), -1, b"row strides"), (dict(vrs=1 << 24), -1, b"row strides"),
+    (dict(krs=264), -1, b"paged rows"), (dict(kv=2, bt=None), -4, b"paged"),
+    (dict(bt=None, rows=1 << 31), -4, b"too many"), (dict(ws=P + 8, wsb=1 << 40), -3, b"workspace"),
+    (dict(ws=P, wsb=100, mq=10, mk=100000), -3, b"workspace"),
+    (dict(n=0), 0, b""), (dict(tq=0), 0, b""),
+])
+def test_prefill_refuses(kw, code, msg):
+    rc = L.lib().nkv_diff_prefill(*dict(PREFILL, **kw).values(), None)
+    assert rc == code and msg in L.lib().nkv_last_error(), (rc, L.lib().nkv_last_error())
+
+
+@pytest.mark.parametrize("kw,code,msg", [
+    (dict(q=None), -1, b"null"), (dict(ctx=None), -1, b"null"), (dict(out=None), -1, b"out must"),
+    (dict(n=-1), -1, b"sizes"), (dict(ws=None), -3, b"workspace"), (dict(wsb=100), -3, b"workspace"),
+    (dict(mb=1 << 27, btrs=1 << 27), -4, b"too large"), (dict(n=0, out=None), 0, b""),
+])
+def test_decode_refuses(kw, code, msg):
+    rc = L.lib().nkv_diff_decode(*dict(DECODE, **kw).values(), None)
+    assert rc == code and msg in L.lib().nkv_last_error(), (rc, L.lib().nkv_last_error())
+
+
+def test_workspace_sizes_follow_the_chip_not_the_lengths():
+    """(no device here: 256 CUs assumed)"""
+    f = L.lib().nkv_diff_prefill_workspace_bytes
+    assert f(0, 0, 10, 10, 10, 8, 4, 64, 1) == f(0, 2, 10, 10, 100, 7, 4, 64, 1) == 0
+    assert f(0, 2, 10, 10, 100, 8, 4, 32, 1) == 0
+    # one long chunk: cut; a batch that fills the chip: whole tiles, nothing needed
+    assert 0 < f(0, 1, 512, 512, 10 ** 4, 32, 8, 128, 1) == f(0, 1, 512, 512, 10 ** 6, 32, 8, 128, 1)
+    assert f(0, 8, 16384, 2048, 10 ** 5, 32, 8, 128, 1) == 0
+    for d in (64, 128):
+        for n, tq, mq in ((1, 512, 512), (500, 1010, 511), (2000, 2000, 1), (300, 600, 2),
+                          (1000, 1600, 100)):
+            assert f(0, n, tq, mq, 10 ** 6, 32, 8, d, 1) < 900e6
+    assert L.lib().nkv_diff_decode_workspace_bytes(4, 32, 96, 8, 256) == 0
+    assert L.lib().nkv_diff_decode_workspace_bytes(4, 32, 64, 8, 256) == \
+        L.lib().nkv_paged_decode_workspace_bytes(4, 32, 128, 8, 256)

@@ -114,6 +114,14 @@ def test_many_sequences(dev):
     check(run(c), c)
 
 
+@pytest.mark.parametrize("kv", [None, FP8])
+@pytest.mark.parametrize("hq,hk,d", [(8, 8, 64), (8, 8, 128), (16, 8, 64), (32, 8, 128), (12, 4, 64)])
+def test_several_pairs_a_wave(dev, hq, hk, d, kv):
+    """Wide tables, by which the launch is chosen: waves that read two or four pairs' rows at once."""
+    c = make(dev, [(11 * i) % 150 for i in range(128)], hq, hk, d, kv=kv, width=700, seed=hq + d)
+    check(run(c), c)
+
+
 def test_sharp_maps(dev):
     """Scores of tens: weights that underflow, one key that carries a row."""
     c = make(dev, [300, 40], 8, 4, 64, seed=6, spread=12.0)
@@ -123,6 +131,12 @@ def test_sharp_maps(dev):
 def test_without_a_norm_weight_and_other_eps(dev):
     c = make(dev, [50, 7], 4, 2, 64, seed=7)
     check(run(c, norm_weight=None, eps=0.5), c, weight=None, eps=0.5)
+
+
+def test_empty_batch(dev):
+    c = make(dev, [5], 4, 2, 64)
+    none = dict(c, q=c["q"][:0], lens=c["lens"][:0], bt=c["bt"][:0])
+    assert run(none).shape == (0, 2, 128)
 
 
 def test_empty_rows_are_zero(dev):

@@ -120,6 +120,14 @@ def test_more_sequences_than_lanes(dev):
     check(run(c), c)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_short_prompts_over_long_contexts(dev, d):
+    """More prompts than lanes, their tiles cut into ranges."""
+    new = [2 + i % 4 for i in range(75)]
+    c = make(dev, new, [n + (97 * i) % 1400 for i, n in enumerate(new)], 2, 2, d, seed=25)
+    check(run(c), c)
+
+
 def test_rows_that_see_no_key_are_zero(dev):
     """More queries than keys: the first ones see nothing; a sequence without keys."""
     c = make(dev, [20, 5, 3], [8, 0, 50], 4, 2, 64, seed=4)
@@ -304,3 +312,72 @@ def test_the_layer_over_shared_pages(dev, kv):
     step([2, 3, 1], [1, 25, 9], False)  # a mixed step
     for _ in range(3):
         step([1, 3, 2], [1, 1, 1], True)
+
+
+@pytest.mark.parametrize("d,hq,hk", [(64, 32, 4), (128, 32, 4), (128, 128, 2)])
+@pytest.mark.parametrize("prefix", [0, 700])
+def test_large_tiles(dev, d, hq, hk, prefix):
+    """More small tiles than CUs, so that the waves take as many row groups as they can: whole tiles,
+    and (over a prefix) tiles cut into ranges."""
+    n = {64: 600, 128: 1100}[d] if hq < 128 else 300
+    c = make(dev, [n, 33], [n + prefix, 33], hq, hk, d, seed=d + prefix)
+    check(run(c), c)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_length_bounds_that_are_not(dev, d):
+    """max_seqlen_q and max_seqlen_k only choose the launch: a plan for a few long prompts meets many
+    short ones, one for decode rows meets prompts, and bounds below the lengths."""
+    c = make(dev, [30] * 20, [90] * 20, 8, 4, d, seed=21)
+    want = reference(c)
+    dev_args = [c[x].to(dev) for x in ("q", "k", "v", "cu_q", "cu_k")]
+    for max_q, max_k in ((600, 9000), (581, 700), (2, 10 ** 6), (1, 5000), (30, 1), (0, 0)):
+        out = nkv.diff_varlen_prefill(*dev_args, max_q, c["scale"], c["lambdas"].to(dev), c["init"],
+                                      c["weight"].to(dev), block_tables=c["bt"].to(dev),
+                                      max_seqlen_k=max_k)
+        assert bool(((out.double().cpu() - want[0]).abs() <= want[1]).all()), (max_q, max_k)
+
+
+@pytest.mark.parametrize("kv", [None, FP8])
+@pytest.mark.parametrize("d", [64, 128])
+def test_decode_rows_among_prompts_in_any_place(dev, d, kv):
+    """Rows of one token (streamed apart) before, between and behind prompts, some without keys,
+    invalid blocks and keys past the table among their contexts."""
+    new = [1, 40, 1, 1, 0, 1, 70, 1]
+    ctx = [500, 700, 1, 0, 30, 90, 70, 2000]
+    c = make(dev, new, ctx, 20, 4, d, seed=22 + d, kv=kv)
+    c["bt"][0, 3], c["bt"][5, 0] = -1, 10 ** 7
+    check(run(c), c)
+    check(run(c, split=False), c)
+    c["bt"] = c["bt"][:, :100].contiguous()  # the last row's keys end past the table
+    check(run(c), c)
+
+
+def test_captured_prefill_and_decode(dev):
+    """Both operators in one graph, replayed over new inputs with eager calls between the replays."""
+    a = make(dev, [40, 1, 90], [900, 1500, 90], 8, 4, 64, seed=23)
+    b = make(dev, [40, 1, 90], [900, 1500, 90], 8, 4, 64, seed=24)
+    put = {x: a[x].to(dev) for x in ("q", "k", "v", "bt", "cu_q", "cu_k", "lambdas", "weight")}
+    lens = a["cu_k"].diff().to(dev)
+
+    def both():
+        p = nkv.diff_varlen_prefill(put["q"], put["k"], put["v"], put["cu_q"], put["cu_k"], 90,
+                                    a["scale"], put["lambdas"], a["init"], put["weight"],
+                                    block_tables=put["bt"], max_seqlen_k=1500)
+        d = nkv.diff_paged_decode(put["q"][:3], put["k"], put["v"], lens, put["bt"], a["scale"],
+                                  put["lambdas"], a["init"], put["weight"])
+        return p, d
+
+    both()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        p, d = both()
+    for c in (a, b, a, b):
+        for x in put:
+            put[x].copy_(c[x])
+        graph.replay()
+        torch.cuda.synchronize()
+        check(p, c)
+        eager = both()
+        assert torch.equal(eager[0], p) and torch.equal(eager[1], d)

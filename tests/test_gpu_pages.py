@@ -321,3 +321,73 @@ def test_a_decode_step_captured_in_a_graph(dev):
             p.truncate([0, 3], [5, 16])
         if i == 3:
             p.fork([1], [4]) if p.ref.lens[4] == 0 else p.truncate([4], [0])
+
+
+def test_compression_beside_shared_sequences(dev):
+    """A copy of a sequence is compressed in place: its freed blocks go back through truncate, the
+    shared pages of the others stay as they were, and new tokens take the freed pages."""
+    cu = importlib.import_module("nanokv-llm_amd.layers.compress_utils")
+    B, Hk, D, W, keep = 256, 2, 128, 4, 257
+    g = torch.Generator().manual_seed(9)
+    kv = torch.randn(2, 1, 24, B, Hk, D, generator=g).to(torch.bfloat16).to(dev)
+    seqs = nkv.PagedSequences(kv, 5, 8)
+    n = 5 * B + 20
+    seqs.append(ints([0], dev), ints([0, n], dev), n)
+    assert seqs.fork(ints([0], dev), ints([1], dev)).tolist() == [1]
+    assert seqs.fork(ints([0], dev), ints([2], dev), share_pages=False).tolist() == [1]
+    before = kv.clone()
+    base = seqs.context_lens.clone()
+    q = torch.randn(5, 4, D, generator=g).to(torch.bfloat16).to(dev)
+    events = torch.empty(1, 4 + 8, dtype=I32, device=dev)
+    cu.compress_step(q, kv[0, 0], kv[1, 0], seqs.block_tables, base, seqs.context_lens,
+                     ints([2], dev), W, keep, D ** -0.5, events=events)
+    empty = ints([], dev)
+    seqs.truncate(empty, empty, pages=events[0, 4:].contiguous())
+    held = seqs.block_tables.cpu()
+    assert seqs.context_lens.tolist() == [n, n, n - W * B + keep, 0, 0]
+    assert seqs.ref_counts.tolist() == [int((held == p).sum()) for p in range(24)]
+    for r in (0, 1):
+        pages = held[r][held[r] >= 0].long().to(dev)
+        assert torch.equal(kv[:, :, pages], before[:, :, pages])
+    free = int((seqs.ref_counts == 0).sum())
+    slots, status = seqs.append(ints([3], dev), ints([0, free * B], dev), free * B) \
+        if free <= 8 else seqs.append(ints([3], dev), ints([0, 8 * B], dev), 8 * B)
+    assert status.tolist() == [1] and bool((slots >= 0).all())
+
+
+def test_two_objects_at_once_on_two_streams(dev):
+    """Objects of their own share nothing: their calls may overlap."""
+    a, b = Pair(dev, seed=1), Pair(dev, seed=2)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for s, p in zip(streams, (a, b)):
+        with torch.cuda.stream(s):
+            out = [p.seqs.append(ints([0, 1, 2], dev), ints([0, 40, 77, 80], dev), 80)[1],
+                   p.seqs.fork(ints([0, 1], dev), ints([3, 4], dev)),
+                   p.seqs.truncate(ints([0, 3], dev), ints([20, 33], dev)),
+                   p.seqs.compact(20)[0]]
+            got.append(out)
+    torch.cuda.synchronize()
+    for p, out in zip((a, b), got):
+        want = [p.ref.append([0, 1, 2], cu=[0, 40, 77, 80], n_tokens=80)[1],
+                p.ref.fork([0, 1], [3, 4]), p.ref.truncate([0, 3], [20, 33]), p.ref.compact(20)[0]]
+        assert [x.tolist() for x in out] == want
+        p.check(out[3], want[3])
+
+
+def test_pages_past_4_gib(dev):
+    """Copies whose byte offsets pass 32 bits, in the last plane of a large pool."""
+    kv = torch.empty(2, 3, 1300, 256, 8, 128, dtype=torch.bfloat16, device=dev)  # 4.1 GB
+    kv.view(torch.int16).fill_(7)
+    seqs = nkv.PagedSequences(kv, 3, 1300)
+    n = 1296 * 256 + 100
+    assert seqs.append(ints([0], dev), ints([0, n], dev), n)[1].tolist() == [1]
+    kv[:, :, 1296].view(torch.int16).copy_(
+        torch.arange(256 * 8 * 128, device=dev).to(torch.int16).view(256, 8, 128))
+    assert seqs.fork(ints([0], dev), ints([1], dev)).tolist() == [1]
+    assert seqs.block_tables[1, 1296].item() == 1297
+    same = kv[:, :, 1297].view(torch.int16) == kv[:, :, 1296].view(torch.int16)
+    assert bool(same[:, :, :100].all())
+    assert bool((kv[:, :, 1297, 100:].view(torch.int16) == 7).all())
+    assert bool((kv[:, :, 1298:].view(torch.int16) == 7).all())
