@@ -219,7 +219,7 @@ _SAME_DEVICE = contextlib.nullcontext()
 def device_of(index: int):
     """A context in which device ``index`` is the current one: the library takes launch sizes from
     the current device, and a null stream belongs to it."""
-    return _SAME_DEVICE if index == torch.cuda.current_device() else torch.cuda.device(index)
+    return _SAME_DEVICE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def stream_of(t: torch.Tensor) -> int:

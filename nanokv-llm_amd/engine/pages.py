@@ -47,22 +47,23 @@ class PagedSequences:
     def __init__(self, kv_cache: torch.Tensor | KVCachePool, max_seqs: int,
                  max_blocks_per_seq: int, state: torch.Tensor | None = None):
         kv = kv_cache.kv_cache if isinstance(kv_cache, KVCachePool) else kv_cache
-        _lib.need(kv.dim() == 6 and kv.size(0) == 2 and kv.is_contiguous(),
-                  "PagedSequences: the pool must be contiguous [2, layers, pages, block_size, Hk, "
-                  f"D], got {tuple(kv.shape)}")
+        if kv.dim() != 6 or kv.size(0) != 2 or not kv.is_contiguous():
+            raise ValueError("PagedSequences: the pool must be contiguous [2, layers, pages, "
+                             f"block_size, Hk, D], got {tuple(kv.shape)}")
         _lib.require_device(kv.device, state=state)
-        _lib.need(max_seqs > 0 and max_blocks_per_seq > 0,
-                  "PagedSequences: max_seqs and max_blocks_per_seq must be > 0")
+        if max_seqs <= 0 or max_blocks_per_seq <= 0:
+            raise ValueError("PagedSequences: max_seqs and max_blocks_per_seq must be > 0")
         _, layers, pages, block, heads, dim = kv.shape
         n = pages + max_seqs + max_seqs * max_blocks_per_seq
         if state is None:
             state = torch.zeros(n, dtype=_I32, device=kv.device)
             state[pages + max_seqs:].fill_(-1)
-        _lib.need(state.dtype is _I32 and state.dim() == 1 and state.numel() == n
-                  and state.is_contiguous(),
-                  f"PagedSequences: state must be {n} contiguous int32")
+        if state.dtype is not _I32 or state.dim() != 1 or state.numel() != n \
+                or not state.is_contiguous():
+            raise ValueError(f"PagedSequences: state must be {n} contiguous int32")
         nbytes = _lib.lib().nkv_pages_workspace_bytes(pages)
-        _lib.need(nbytes > 0, f"PagedSequences: a pool of {pages} pages (1 to 2^20)")
+        if nbytes == 0:
+            raise ValueError(f"PagedSequences: a pool of {pages} pages (1 to 2^20)")
         self.kv_cache, self.state = kv, state
         self.max_seqs, self.max_blocks, self.block_size = max_seqs, max_blocks_per_seq, block
         self._pages, self._device = pages, kv.get_device()
@@ -106,16 +107,16 @@ class PagedSequences:
         order of the list, -1 for refused rows' and for those outside ``cu_seqlens_q``."""
         n = self._list("append: rows", rows)
         if cu_seqlens_q is None:
-            _lib.need(n_tokens is None or n_tokens == n,
-                      "append: without cu_seqlens_q there is one token a row")
+            if n_tokens is not None and n_tokens != n:
+                raise ValueError("append: without cu_seqlens_q there is one token a row")
             n_tokens, cu = n, None
         else:
             self._list("append: cu_seqlens_q", cu_seqlens_q, n + 1)
-            _lib.need(n_tokens is not None, "append: cu_seqlens_q needs n_tokens, the tokens' "
-                      "number on the host")
+            if n_tokens is None:
+                raise ValueError("append: cu_seqlens_q needs n_tokens, the tokens' number on the "
+                                 "host")
             cu = cu_seqlens_q.data_ptr()
-        out = rows.new_empty(n + n_tokens)
-        slots, status = out[n:], out[:n]
+        slots, status = rows.new_empty(n_tokens), rows.new_empty(n)
         self._call(_lib.lib().nkv_pages_append, "append", rows.data_ptr(), n, cu, n_tokens,
                    slots.data_ptr(), status.data_ptr())
         return slots, status
@@ -153,7 +154,8 @@ class PagedSequences:
         -1 padded)."""
         if max_moves is None:
             max_moves = self._pages
-        _lib.need(0 <= max_moves < 2 ** 31, f"compact: max_moves {max_moves} must be >= 0")
+        if not 0 <= max_moves < 2 ** 31:
+            raise ValueError(f"compact: max_moves {max_moves} must be >= 0")
         out = self.state.new_empty(2 + 2 * max_moves)
         self._call(_lib.lib().nkv_pages_compact, "compact", max_moves, out.data_ptr(),
                    out.data_ptr() + 8)

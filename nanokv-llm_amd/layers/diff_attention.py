@@ -35,44 +35,49 @@ def lambda_init_of(layer: int) -> float:
 
 
 def _check(what, q, k, v, lambdas, norm_weight, out, paged, **others):
-    """The checks that both operators share -> (rows, Hq, D, Hk, kv_type)."""
+    """The checks that both operators share -> (rows, Hq, D, Hk, kv_type). One pass over the
+    arguments where they are right (messages are made only for the others: building them all took
+    as long as a launch)."""
     _lib.require_device(q.device, k=k, v=v, lambdas=lambdas, norm_weight=norm_weight, out=out,
                         **others)
-    _lib.need(q.dim() == 3 and q.stride(2) == 1 and q.stride(1) == q.size(2),
-              f"{what}: q must be [rows, Hq, D], rows of contiguous heads")
-    N, Hq, D = q.shape
-    f16 = _lib.is_f16(q, f"{what}: q")
-    fp8 = paged and k.dtype == _FP8
-    _lib.need(k.dim() == (4 if paged else 3) and k.size(-1) == D and v.shape == k.shape
-              and v.dtype == k.dtype, f"{what}: k and v must share a shape and a dtype, with q's "
-              "head_dim")
-    _lib.need(k.dtype == q.dtype or (fp8 and not f16),
-              f"{what}: caches must have q's dtype (or fp8 with bf16 q)")
-    Hk = k.size(-2)
+    qs, ks, dt, ct = q.shape, k.shape, q.dtype, k.dtype
+    if len(qs) != 3 or q.stride(2) != 1 or q.stride(1) != qs[2]:
+        raise ValueError(f"{what}: q must be [rows, Hq, D], rows of contiguous heads")
+    N, Hq, D = qs
+    f16 = _lib.is_f16(q, what)
+    fp8 = paged and ct is _FP8
+    if len(ks) != (4 if paged else 3) or ks[-1] != D or v.shape != ks or v.dtype is not ct:
+        raise ValueError(f"{what}: k and v must share a shape and a dtype, with q's head_dim")
+    if ct is not dt and (not fp8 or f16):
+        raise ValueError(f"{what}: caches must have q's dtype (or fp8 with bf16 q)")
+    Hk = ks[-2]
     if paged:
-        _lib.need(k.is_contiguous() and v.is_contiguous(), f"{what}: caches must be contiguous")
-    else:
-        _lib.need(all(t.stride(1) == D and t.stride(2) == 1 for t in (k, v)),
-                  f"{what}: k and v must be rows of contiguous heads")
-    _lib.need(Hq > 0 and Hk > 0 and Hq % 2 == 0 and Hk % 2 == 0 and Hq % Hk == 0,
-              f"{what}: heads stand in pairs, whole groups of query pairs to a KV pair (got "
-              f"Hq={Hq}, Hk={Hk})")
-    _lib.need(lambdas.shape == (4, D) and lambdas.dtype == torch.float32
-              and lambdas.is_contiguous(), f"{what}: lambdas must be contiguous float32 [4, {D}]")
-    _lib.need(norm_weight is None or (norm_weight.shape == (2 * D,) and norm_weight.dtype == q.dtype
-                                      and norm_weight.is_contiguous()),
-              f"{what}: norm_weight must be contiguous [{2 * D}] in q's dtype")
-    _lib.need(out is None or (out.shape == (N, Hq // 2, 2 * D) and out.dtype == q.dtype
-                              and out.stride(2) == 1 and out.stride(1) == 2 * D),
-              f"{what}: out must be [rows, Hq/2, 2 D] in q's dtype, rows of contiguous heads")
+        if not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError(f"{what}: caches must be contiguous")
+    elif not all(t.stride(1) == D and t.stride(2) == 1 for t in (k, v)):
+        raise ValueError(f"{what}: k and v must be rows of contiguous heads")
+    if Hq <= 0 or Hk <= 0 or Hq % 2 or Hk % 2 or Hq % Hk:
+        raise ValueError(f"{what}: heads stand in pairs, whole groups of query pairs to a KV pair "
+                         f"(got Hq={Hq}, Hk={Hk})")
+    if lambdas.shape != (4, D) or lambdas.dtype is not torch.float32 \
+            or not lambdas.is_contiguous():
+        raise ValueError(f"{what}: lambdas must be contiguous float32 [4, {D}]")
+    if norm_weight is not None and (norm_weight.shape != (2 * D,) or norm_weight.dtype is not dt
+                                    or not norm_weight.is_contiguous()):
+        raise ValueError(f"{what}: norm_weight must be contiguous [{2 * D}] in q's dtype")
+    if out is not None and (out.shape != (N, Hq // 2, 2 * D) or out.dtype is not dt
+                            or out.stride(2) != 1 or out.stride(1) != 2 * D):
+        raise ValueError(f"{what}: out must be [rows, Hq/2, 2 D] in q's dtype, rows of contiguous "
+                         "heads")
     return N, Hq, D, Hk, (_lib.NKV_KV_FP8 if fp8 else _lib.NKV_KV_F16 if f16 else
                           _lib.NKV_KV_BF16)
 
 
 def _int32_rows(what, name, t, dims=1):
-    _lib.need(t.dtype is _I32 and t.dim() == dims and
-              (t.is_contiguous() if dims == 1 else t.stride(1) == 1),
-              f"{what}: {name} must be int32, {'contiguous' if dims == 1 else 'contiguous rows'}")
+    if t.dtype is not _I32 or t.dim() != dims or not (t.is_contiguous() if dims == 1
+                                                      else t.stride(1) == 1):
+        raise ValueError(f"{what}: {name} must be int32, "
+                         f"{'contiguous' if dims == 1 else 'contiguous rows'}")
 
 
 def diff_decode_workspace_bytes(bs: int, n_q_heads: int, max_blocks_per_seq: int, block_size: int,
@@ -100,16 +105,16 @@ def diff_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
                                     workspace=workspace)
     _int32_rows(what, "block_tables", block_tables, 2)
     _int32_rows(what, "context_lens", context_lens)
-    _lib.need(block_tables.size(0) >= bs and context_lens.numel() >= bs,
-              f"{what}: block_tables and context_lens need a row for each of q's {bs}")
+    if block_tables.size(0) < bs or context_lens.numel() < bs:
+        raise ValueError(f"{what}: block_tables and context_lens need a row for each of q's {bs}")
     NB, B, width = k_cache.size(0), k_cache.size(1), block_tables.size(1)
     if out is None:
         out = torch.empty(bs, Hq // 2, 2 * D, dtype=q.dtype, device=q.device)
     if workspace is None:
         workspace = torch.empty(max(diff_decode_workspace_bytes(bs, Hq, width, B, D), 4),
                                 dtype=torch.uint8, device=q.device)
-    _lib.need(workspace.dtype == torch.uint8 and workspace.is_contiguous(),
-              f"{what}: workspace must be contiguous uint8")
+    elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be contiguous uint8")
     with _lib.device_of(q.get_device()):
         rc = _lib.lib().nkv_diff_decode(
             kv_type, q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
@@ -165,12 +170,12 @@ def diff_varlen_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _int32_rows(what, "cu_seqlens_q", cu_seqlens_q)
     _int32_rows(what, "cu_seqlens_k", cu_seqlens_k)
     n_seqs = cu_seqlens_q.numel() - 1
-    _lib.need(n_seqs >= 0 and cu_seqlens_k.numel() == n_seqs + 1,
-              f"{what}: cu_seqlens_q and cu_seqlens_k need one entry per sequence + 1")
+    if n_seqs < 0 or cu_seqlens_k.numel() != n_seqs + 1:
+        raise ValueError(f"{what}: cu_seqlens_q and cu_seqlens_k need one entry per sequence + 1")
     if paged:
         _int32_rows(what, "block_tables", block_tables, 2)
-        _lib.need(block_tables.size(0) >= n_seqs,
-                  f"{what}: block_tables needs a row for each of the {n_seqs} sequences")
+        if block_tables.size(0) < n_seqs:
+            raise ValueError(f"{what}: block_tables needs a row for each of the {n_seqs} sequences")
         B, rows = k.size(1), k.size(0) * k.size(1)
         k_stride = v_stride = Hk * D
         bt, bt_stride, width = (block_tables.data_ptr(), block_tables.stride(0),
@@ -180,8 +185,9 @@ def diff_varlen_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         bt, bt_stride, width = None, 0, 0
     if out is None:
         out = torch.empty(N, Hq // 2, 2 * D, dtype=q.dtype, device=q.device)
-    _lib.need(workspace is None or (workspace.dtype == torch.uint8 and workspace.is_contiguous()),
-              f"{what}: workspace must be contiguous uint8")
+    if workspace is not None and (workspace.dtype is not torch.uint8
+                                  or not workspace.is_contiguous()):
+        raise ValueError(f"{what}: workspace must be contiguous uint8")
     with _lib.device_of(q.get_device()):
         if workspace is None and max_seqlen_k is not None:
             workspace = diff_prefill_workspace(q, k, n_seqs, max_seqlen_q, max_seqlen_k)
