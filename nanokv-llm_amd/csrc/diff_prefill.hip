@@ -96,8 +96,9 @@ __device__ __forceinline__ int diff_steps(int Lq, int Lk, int QT, int tile) {
 template <int D, int RG>
 __device__ __forceinline__ bool diff_range(const DiffPrefillArgs& a, int QT, int x, DiffTile& d,
                                            int& n_tiles) {
-  // measured: a step of a workgroup alone on its CU and of one of two, two chunks' partial rows
-  // (101 and 266 KB a range) written and merged, and what the merge takes beside that
+  // measured: a step of a workgroup alone on its CU, and of one of two on it; what a range's partial
+  // rows (101 KB at head_dim 64, 266 at 128) cost of the chip's time, written and read again; and what
+  // the merge takes beside that
   constexpr float kStepUs[2] = {D == 64 ? (RG == 1 ? 0.8f : 1.6f) : (RG == 1 ? 1.4f : 2.2f),
                                 D == 64 ? (RG == 1 ? 1.1f : 2.1f) : (RG == 1 ? 1.4f : 2.2f)};
   constexpr float kRangeUs = D == 64 ? 0.01f * RG : 0.02f * RG, kMergeUs = 6.f;
@@ -594,7 +595,7 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
     // i + 2 - kTiles on, and is fetched from then on until the end of half step i - 1: three half
     // steps with five places; fp8 codes, which wait in registers, two. Four chunks of up to 2048 tokens
     // over up to 6000 (Hq 32, Hk 8): whole steps with a barrier each 690 us, half steps and four
-    // places 685, five 665; without the fetches 600, and without the softmax too 555.
+    // places 685, five 660 to 678 in several runs; without the fetches 602, without the softmax too 554.
     constexpr int kAhead = F8 ? 2 : 3;
     auto next = [](uint32_t at) { return at + kTileB == kTiles * kTileB ? 0u : at + kTileB; };
     uint32_t rd = 0, wr = 2 * kTileB;  // places read and fetched next

@@ -14,11 +14,11 @@
 // one walk over the counts for the free pages) and, where pages are copied or many table entries
 // change, a second launch of up to kCopyGroups workgroups that reads the plan from the workspace.
 // A copy is bound by HBM: rows are read once and written once, 16 bytes a lane, kCopyUnroll of them
-// in flight; the grid's y runs over the 2 * layers planes of the pool. 50 pages of 1 MiB in each of 32
-// planes: 333 us, 5.0 TB/s read and written together (a copy of 2 GiB: 4.8); twice or half the loads in
-// flight or the workgroups within 3%, loads that bypass the caches 4% faster there and 15% slower where
-// the same rows are read several times (four beams of one sequence).
-// Kernel times: one token each for 64 rows 3.7 us; 33 rows rolled back 6.5 + 3.8.
+// in flight; the grid's y runs over the 2 * layers planes of the pool. 50 pages of 512 KiB in each
+// of 32 planes: 333 us, 5.0 TB/s read and written together (a copy of 2 GiB: 4.8); twice or half the
+// loads in flight or the workgroups within 1.5%; loads that bypass the caches 4% faster there, but
+// 32% slower where four beams of one sequence copy the same rows (24.4 -> 32.1 us).
+// Kernel times: one token each for 64 rows 3.5 us; 33 rows rolled back 6.0 + 3.7.
 #include "nkv_common.h"
 
 #include <algorithm>
