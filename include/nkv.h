@@ -826,7 +826,7 @@ int nkv_pages_fork(const nkv_pages* pages, const int32_t* parents, const int32_t
  * k-th lowest free page below n_live takes the k-th highest page in use, for
  * the first max_moves of them; all tables and counts follow. info[0] = n_live,
  * info[1] = the moves made; moves (int32 [max_moves, 2], 8-byte aligned) lists
- * them as (from, to), padded with -1. No counterpart in the reference.
+ * them as (from, to), padded with -1. max_moves: at most 2^20. No counterpart in the reference.
  */
 int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info, int32_t* moves,
                       void* stream);

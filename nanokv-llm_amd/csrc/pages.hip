@@ -674,8 +674,9 @@ extern "C" int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int3
   PagesArgs a;
   int rc = pages_check(pages, "pages_compact", a);
   if (rc) return rc;
-  NKV_REQUIRE(max_moves >= 0, NKV_EINVAL, "pages_compact: max_moves must be >= 0 (got %d)",
-              max_moves);
+  // the loop that pads the list counts in 32 bits
+  NKV_REQUIRE(max_moves >= 0 && max_moves <= kMaxPages, NKV_EINVAL,
+              "pages_compact: max_moves must be 0 to %d (got %d)", kMaxPages, max_moves);
   NKV_REQUIRE(info && (max_moves == 0 || moves) &&
                   (reinterpret_cast<uintptr_t>(moves) & 7u) == 0,
               NKV_EINVAL, "pages_compact: info and 8-byte aligned moves are needed");

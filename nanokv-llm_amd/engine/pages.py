@@ -33,8 +33,8 @@ class PagedSequences:
 
     Lists are int32 tensors on the pool's device. An entry of -1 is padding, and a row named twice
     counts where it is named first. Pages are taken lowest first and in the list's order: an entry
-    is carried out if the pages needed by all entries up to it are free before the call, else it is
-    refused and changes nothing. Each call returns a ``status`` (int32, 1: carried out, 0:
+    is carried out if it needs no page or the pages needed by all entries up to it are free before
+    the call, else it is refused and changes nothing. Each call returns a ``status`` (int32, 1: carried out, 0:
     refused or padding). A row's last page, where it is filled in part, belongs to that row alone;
     full pages may be shared, so code that writes rows in place (a compression step) needs a fork
     made with ``share_pages=False``.
@@ -154,8 +154,8 @@ class PagedSequences:
         -1 padded)."""
         if max_moves is None:
             max_moves = self._pages
-        if not 0 <= max_moves < 2 ** 31:
-            raise ValueError(f"compact: max_moves {max_moves} must be >= 0")
+        if not 0 <= max_moves <= 2 ** 20:
+            raise ValueError(f"compact: max_moves {max_moves} must be 0 to 2^20")
         out = self.state.new_empty(2 + 2 * max_moves)
         self._call(_lib.lib().nkv_pages_compact, "compact", max_moves, out.data_ptr(),
                    out.data_ptr() + 8)

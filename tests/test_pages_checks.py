@@ -129,3 +129,11 @@ def test_workspace_bytes():
     f = _lib.lib().nkv_pages_workspace_bytes
     assert f(0) == f(-1) == f((1 << 20) + 1) == 0
     assert f(1000) == 64 + 16 * 8192 + 24 * 1000
+
+
+@pytest.mark.parametrize("max_moves", [(1 << 20) + 1, (1 << 31) - 1024, (1 << 31) - 1])
+def test_compact_refuses_more_moves_than_a_pool_can_have(max_moves):
+    """The list's padding is counted in 32 bits, 1024 entries a step."""
+    lib = _lib.lib()
+    assert lib.nkv_pages_compact(_args(), max_moves, P, P, None) == -1
+    assert b"max_moves" in lib.nkv_last_error()
