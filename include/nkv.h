@@ -764,9 +764,9 @@ int nkv_build_step_metadata(const int32_t* packed, int32_t n_seqs, int32_t block
  *
  * Lists are taken as the state before the call has it. An entry of -1 is
  * padding; a row named twice counts where it is named first. Pages are taken
- * lowest first, in the list's order: an entry is granted if the pages of all
- * entries up to it are free before the call, else it is refused and changes
- * nothing. status[i] is 1 for an entry that was carried out, else 0. Calls on
+ * lowest first, in the list's order: an entry is granted if it needs no page or
+ * the pages of all entries up to it are free before the call, else it is refused
+ * and changes nothing. status[i] is 1 for an entry that was carried out, else 0. Calls on
  * the same pages must be ordered on a stream.
  *
  * Replaces: BlockManager's bookkeeping (nanokvllm/engine/block_manager.py:

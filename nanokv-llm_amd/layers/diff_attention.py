@@ -194,10 +194,10 @@ def diff_varlen_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         rc = _lib.lib().nkv_diff_prefill(
             kv_type, q.data_ptr(), q.stride(0), N, k.data_ptr(), v.data_ptr(), k_stride, v_stride,
             cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), bt, bt_stride, width, n_seqs,
-            int(max_seqlen_q), 0 if max_seqlen_k is None else int(max_seqlen_k), Hq, Hk, D, B, rows, scale, k_scale,
-            v_scale, lambdas.data_ptr(), lambda_init, _lib.ptr(norm_weight), eps, out.data_ptr(),
-            out.stride(0), _lib.ptr(workspace), 0 if workspace is None else workspace.numel(),
-            _lib.stream_of(q))
+            int(max_seqlen_q), 0 if max_seqlen_k is None else int(max_seqlen_k), Hq, Hk, D, B,
+            rows, scale, k_scale, v_scale, lambdas.data_ptr(), lambda_init,
+            _lib.ptr(norm_weight), eps, out.data_ptr(), out.stride(0), _lib.ptr(workspace),
+            0 if workspace is None else workspace.numel(), _lib.stream_of(q))
     if rc:
         _lib.check(rc, what)
     return out
