@@ -30,6 +30,7 @@ class PagedSequences:
     counts, the lengths (``context_lens``) and the tables (``block_tables``, -1 past a row's
     pages), each a view of it. A new object has all pages free and all rows empty; given a
     ``state`` (another object's, or a clone of one kept before a step) it goes on from there.
+    ``state.copy_(kept)`` takes an object back to one; ``state`` and ``kv_cache`` cannot be set.
 
     Lists are int32 tensors on the pool's device. An entry of -1 is padding, and a row named twice
     counts where it is named first. Pages are taken lowest first and in the list's order: an entry
@@ -64,7 +65,7 @@ class PagedSequences:
         nbytes = _lib.lib().nkv_pages_workspace_bytes(pages)
         if nbytes == 0:
             raise ValueError(f"PagedSequences: a pool of {pages} pages (1 to 2^20)")
-        self.kv_cache, self.state = kv, state
+        self._kv, self._state = kv, state
         self.max_seqs, self.max_blocks, self.block_size = max_seqs, max_blocks_per_seq, block
         self._pages, self._device = pages, kv.get_device()
         self._workspace = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
@@ -74,17 +75,27 @@ class PagedSequences:
                                  at + 4 * (pages + max_seqs), max_blocks_per_seq,
                                  max_blocks_per_seq, max_seqs, self._workspace.data_ptr(), nbytes)
 
+    # The kernels are given the addresses of these two once, so that an attribute set to another
+    # tensor would leave them writing to memory that nothing owns any more.
+    @property
+    def kv_cache(self) -> torch.Tensor:
+        return self._kv
+
+    @property
+    def state(self) -> torch.Tensor:
+        return self._state
+
     @property
     def ref_counts(self) -> torch.Tensor:
-        return self.state[:self._pages]
+        return self._state[:self._pages]
 
     @property
     def context_lens(self) -> torch.Tensor:
-        return self.state[self._pages:self._pages + self.max_seqs]
+        return self._state[self._pages:self._pages + self.max_seqs]
 
     @property
     def block_tables(self) -> torch.Tensor:
-        return self.state[self._pages + self.max_seqs:].view(self.max_seqs, self.max_blocks)
+        return self._state[self._pages + self.max_seqs:].view(self.max_seqs, self.max_blocks)
 
     def _list(self, what: str, t: torch.Tensor, n: int | None = None) -> int:
         """The list's length (``n`` entries, if given)."""
@@ -156,7 +167,7 @@ class PagedSequences:
             max_moves = self._pages
         if not 0 <= max_moves <= 2 ** 20:
             raise ValueError(f"compact: max_moves {max_moves} must be 0 to 2^20")
-        out = self.state.new_empty(2 + 2 * max_moves)
+        out = self._state.new_empty(2 + 2 * max_moves)
         self._call(_lib.lib().nkv_pages_compact, "compact", max_moves, out.data_ptr(),
                    out.data_ptr() + 8)
         return out[:2], out[2:].view(-1, 2)

@@ -2,6 +2,7 @@
 
 All outputs are whole numbers or copied rows, so every comparison is for equality.
 """
+import copy
 import importlib
 import random
 
@@ -391,3 +392,17 @@ def test_pages_past_4_gib(dev):
     assert bool(same[:, :, :100].all())
     assert bool((kv[:, :, 1297, 100:].view(torch.int16) == 7).all())
     assert bool((kv[:, :, 1298:].view(torch.int16) == 7).all())
+
+
+def test_a_kept_state_taken_back_in_place(dev):
+    """state.copy_(kept): views, calls and the next tokens' pages are those of the kept state."""
+    p = Pair(dev)
+    p.append([0, 1, 2], [20, 33, 5])
+    kept, oracle = p.seqs.state.clone(), copy.deepcopy(p.ref)
+    views = p.seqs.context_lens, p.seqs.block_tables
+    p.append([0, 3], [40, 16])
+    p.truncate([1], [0])
+    p.seqs.state.copy_(kept)
+    p.ref = oracle
+    assert p.append([1, 3, 0], [1, 50, 13]) == [1, 1, 1]
+    assert views[0].tolist() == p.ref.lens and views[1].tolist() == p.ref.tables

@@ -1,4 +1,5 @@
 """PagedSequences: the oracle's own rules, and the refusals that need no GPU."""
+import contextlib
 import importlib
 import random
 import struct
@@ -137,3 +138,40 @@ def test_compact_refuses_more_moves_than_a_pool_can_have(max_moves):
     lib = _lib.lib()
     assert lib.nkv_pages_compact(_args(), max_moves, P, P, None) == -1
     assert b"max_moves" in lib.nkv_last_error()
+
+
+@pytest.fixture
+def host_pool(monkeypatch):
+    """A PagedSequences over host tensors, whose calls are recorded: (entry point, arguments)."""
+    calls = []
+
+    class Lib:
+        nkv_pages_workspace_bytes = staticmethod(_lib.lib().nkv_pages_workspace_bytes)
+
+        def __getattr__(self, name):
+            return lambda *a: calls.append((name, a)) or 0
+
+    lib = Lib()
+    monkeypatch.setattr(_lib, "require_device", lambda *a, **kw: None)
+    monkeypatch.setattr(_lib, "lib", lambda: lib)
+    monkeypatch.setattr(_lib, "device_of", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 7, raising=False)
+    seqs = pages.PagedSequences(torch.zeros(2, 1, 4, 16, 2, 64, dtype=torch.bfloat16), 3, 2)
+    seqs.calls = calls
+    return seqs
+
+
+def test_state_and_pool_cannot_be_set(host_pool):
+    """The calls go on with the buffers that the object was made over, so that its views have to."""
+    kept = host_pool.state.clone()
+    for name in ("state", "kv_cache"):
+        with pytest.raises(AttributeError):
+            setattr(host_pool, name, getattr(host_pool, name).clone())
+    host_pool.state[4] = 9
+    assert host_pool.context_lens.tolist() == [9, 0, 0]
+    host_pool.state.copy_(kept)
+    host_pool.compact()
+    name, args = host_pool.calls[-1]
+    assert name == "nkv_pages_compact" and struct.unpack("13q", args[0])[5] == \
+        host_pool.state.data_ptr() == host_pool.ref_counts.data_ptr()
+    assert host_pool.context_lens.tolist() == [0, 0, 0]
