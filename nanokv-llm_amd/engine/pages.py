@@ -75,6 +75,9 @@ class PagedSequences:
                                  at + 4 * (pages + max_seqs), max_blocks_per_seq,
                                  max_blocks_per_seq, max_seqs, self._workspace.data_ptr(), nbytes)
 
+    def __reduce__(self):  # a copy's calls go to the copied buffers and a workspace of its own
+        return type(self), (self._kv, self.max_seqs, self.max_blocks, self._state)
+
     # The kernels are given the addresses of these two once, so that an attribute set to another
     # tensor would leave them writing to memory that nothing owns any more.
     @property

@@ -1,6 +1,8 @@
 """PagedSequences: the oracle's own rules, and the refusals that need no GPU."""
 import contextlib
+import copy
 import importlib
+import pickle
 import random
 import struct
 
@@ -175,3 +177,17 @@ def test_state_and_pool_cannot_be_set(host_pool):
     assert name == "nkv_pages_compact" and struct.unpack("13q", args[0])[5] == \
         host_pool.state.data_ptr() == host_pool.ref_counts.data_ptr()
     assert host_pool.context_lens.tolist() == [0, 0, 0]
+
+
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, lambda s: pickle.loads(pickle.dumps(s))])
+def test_a_copy_gives_the_kernels_its_own_buffers(host_pool, how):
+    calls = host_pool.__dict__.pop("calls")
+    host_pool.state[5] = 3
+    other = how(host_pool)
+    other.compact()
+    args = struct.unpack("13q", calls[-1][1][0])
+    assert args[0] == other.kv_cache.data_ptr() and args[5] == other.state.data_ptr()
+    assert args[11] != struct.unpack("13q", host_pool._args)[11]  # a workspace of its own
+    assert (args[5] == host_pool.state.data_ptr()) == (how is copy.copy)
+    assert other.context_lens.tolist() == [0, 3, 0]
+    assert (other.max_seqs, other.max_blocks, other.block_size) == (3, 2, 16)
