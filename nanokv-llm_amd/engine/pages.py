@@ -12,10 +12,12 @@ are (rows are then the batch) or indexed by the step's rows.
 from __future__ import annotations
 
 import struct
+import weakref
 
 import torch
 
 from .. import _lib
+from ..layers import attention
 from ..layers.kv_cache import KVCachePool
 
 _PAGES = struct.Struct("13q")  # nkv_pages
@@ -42,7 +44,9 @@ class PagedSequences:
 
     Calls run on the current stream of the pool's device and share the object's state and
     workspace: the caller orders calls of one object that it makes on several streams, captured
-    graphs' replays among them.
+    graphs' replays among them. A graph that captured a call needs the pool for as long as it is
+    replayed; state and workspace stay allocated after the object is dropped, until
+    ``release_retired_decode_workspaces()``.
     """
 
     def __init__(self, kv_cache: torch.Tensor | KVCachePool, max_seqs: int,
@@ -69,6 +73,7 @@ class PagedSequences:
         self.max_seqs, self.max_blocks, self.block_size = max_seqs, max_blocks_per_seq, block
         self._pages, self._device = pages, kv.get_device()
         self._workspace = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
+        self._captured = False
         at = state.data_ptr()
         self._args = _PAGES.pack(kv.data_ptr(), 2 * layers, pages, block,
                                  heads * dim * kv.element_size(), at, at + 4 * pages,
@@ -110,9 +115,20 @@ class PagedSequences:
 
     def _call(self, fn, what, *args):
         with _lib.device_of(self._device):
-            rc = fn(self._args, *args, torch._C._cuda_getCurrentRawStream(self._device))
+            stream = torch._C._cuda_getCurrentRawStream(self._device)
+            if torch.cuda.is_current_stream_capturing():
+                self._keep_for_graphs()
+            rc = fn(self._args, *args, stream)
         if rc:
             _lib.check(rc, what)
+
+    def _keep_for_graphs(self):
+        """A graph holds the buffers' addresses: dropping the object leaves them allocated until
+        release_retired_decode_workspaces()."""
+        if not self._captured:
+            self._captured = True
+            weakref.finalize(self, attention.retire_workspace, self._workspace,
+                             self._state).atexit = False
 
     def append(self, rows: torch.Tensor, cu_seqlens_q: torch.Tensor | None = None,
                n_tokens: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:

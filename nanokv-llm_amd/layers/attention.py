@@ -141,9 +141,15 @@ def shared_decode_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     return ws
 
 
+def retire_workspace(*buffers: torch.Tensor) -> None:
+    """Keep the buffers of an object that is gone, which a captured graph may still use."""
+    _RETIRED_WS.append(buffers)
+
+
 def release_retired_decode_workspaces() -> int:
-    """Free the replaced shared workspaces that graphs captured; call after dropping every
-    graph captured before the last regrowth. Returns how many were released."""
+    """Free the replaced shared workspaces that graphs captured, and the buffers of dropped
+    ``PagedSequences`` that they did; call after dropping every graph captured before the last
+    regrowth and with those objects. Returns how many were released."""
     n = len(_RETIRED_WS)
     _RETIRED_WS.clear()
     return n

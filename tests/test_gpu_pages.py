@@ -3,6 +3,7 @@
 All outputs are whole numbers or copied rows, so every comparison is for equality.
 """
 import copy
+import gc
 import importlib
 import random
 
@@ -406,3 +407,28 @@ def test_a_kept_state_taken_back_in_place(dev):
     p.ref = oracle
     assert p.append([1, 3, 0], [1, 50, 13]) == [1, 1, 1]
     assert views[0].tolist() == p.ref.lens and views[1].tolist() == p.ref.tables
+
+
+def test_a_graph_replayed_after_its_object_is_dropped(dev):
+    """The plan's workspace stays the graph's: what is allocated afterwards keeps its contents, and the
+    replays go on with the state and pool that the caller holds."""
+    p = Pair(dev, rows=5)
+    rows = ints([0, 2, 3], dev)
+    p.append([0, 1, 2, 3], [14, 33, 1, 15])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        slots, status = p.seqs.append(rows)
+    state, size = p.seqs.state, p.seqs._workspace.numel()
+    p.seqs = None
+    gc.collect()
+    torch.cuda.synchronize()
+    others = [torch.full((size,), 7, dtype=torch.uint8, device=dev) for _ in range(8)]
+    for _ in range(6):
+        graph.replay()
+        torch.cuda.synchronize()
+        want_slots, want = p.ref.append([0, 2, 3])
+        assert slots.cpu().tolist() == want_slots and status.cpu().tolist() == want
+        assert torch.equal(state.cpu(), p.ref.state())
+        assert all(bool((x == 7).all()) for x in others)
+    del graph
+    assert nkv.release_retired_decode_workspaces() >= 1

@@ -158,6 +158,7 @@ def host_pool(monkeypatch):
     monkeypatch.setattr(_lib, "lib", lambda: lib)
     monkeypatch.setattr(_lib, "device_of", lambda index: contextlib.nullcontext())
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 7, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     seqs = pages.PagedSequences(torch.zeros(2, 1, 4, 16, 2, 64, dtype=torch.bfloat16), 3, 2)
     seqs.calls = calls
     return seqs
@@ -191,3 +192,26 @@ def test_a_copy_gives_the_kernels_its_own_buffers(host_pool, how):
     assert (args[5] == host_pool.state.data_ptr()) == (how is copy.copy)
     assert other.context_lens.tolist() == [0, 3, 0]
     assert (other.max_seqs, other.max_blocks, other.block_size) == (3, 2, 16)
+
+
+def test_buffers_outlive_the_object_where_a_graph_captured_them(host_pool, monkeypatch):
+    """A replay writes the plan to the workspace's address, whoever still holds the object."""
+    attn = importlib.import_module("nanokv-llm_amd.layers.attention")
+    monkeypatch.setattr(attn, "_RETIRED_WS", [])
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    calls = host_pool.__dict__.pop("calls")
+    eager, graph = (copy.deepcopy(host_pool) for _ in range(2))
+    eager.compact()
+    graph.compact()
+    capturing[0] = True
+    graph.compact()
+    graph.compact()
+    capturing[0] = False
+    args = struct.unpack("13q", calls[-1][1][0])
+    del eager
+    assert attn._RETIRED_WS == []
+    del graph
+    (kept,) = attn._RETIRED_WS
+    assert [t.data_ptr() for t in kept] == [args[11], args[5]]
+    assert attn.release_retired_decode_workspaces() == 1 and attn._RETIRED_WS == []
