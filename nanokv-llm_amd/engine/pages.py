@@ -73,6 +73,7 @@ class PagedSequences:
         self.max_seqs, self.max_blocks, self.block_size = max_seqs, max_blocks_per_seq, block
         self._pages, self._device = pages, kv.get_device()
         self._workspace = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
+        self._streams = {torch._C._cuda_getCurrentRawStream(self._device)}  # the allocations' first
         self._captured = False
         at = state.data_ptr()
         self._args = _PAGES.pack(kv.data_ptr(), 2 * layers, pages, block,
@@ -118,9 +119,17 @@ class PagedSequences:
             stream = torch._C._cuda_getCurrentRawStream(self._device)
             if torch.cuda.is_current_stream_capturing():
                 self._keep_for_graphs()
+            elif stream not in self._streams:
+                self._use_on(stream)
             rc = fn(self._args, *args, stream)
         if rc:
             _lib.check(rc, what)
+
+    def _use_on(self, stream):
+        """The buffers' memory, once freed, waits for what still runs on another stream."""
+        for t in (self._workspace, self._state):
+            t.record_stream(torch.cuda.current_stream())
+        self._streams.add(stream)
 
     def _keep_for_graphs(self):
         """A graph holds the buffers' addresses: dropping the object leaves them allocated until

@@ -215,3 +215,24 @@ def test_buffers_outlive_the_object_where_a_graph_captured_them(host_pool, monke
     (kept,) = attn._RETIRED_WS
     assert [t.data_ptr() for t in kept] == [args[11], args[5]]
     assert attn.release_retired_decode_workspaces() == 1 and attn._RETIRED_WS == []
+
+
+def test_buffers_are_recorded_on_other_streams_than_their_own(host_pool, monkeypatch):
+    """Freed memory goes to its own stream's next allocation at once, so that what runs elsewhere has
+    to be known to the allocator: once a stream."""
+    recorded = []
+
+    class Seen(torch.Tensor):
+        def record_stream(self, stream):
+            recorded.append((self.data_ptr(), stream))
+
+    stream = [7]
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: stream[0],
+                        raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: f"stream {stream[0]}")
+    host_pool._workspace = host_pool._workspace.as_subclass(Seen)
+    host_pool._state = host_pool._state.as_subclass(Seen)
+    for stream[0] in (7, 8, 8, 7, 9):
+        host_pool.compact()
+    both = [host_pool._workspace.data_ptr(), host_pool._state.data_ptr()]
+    assert recorded == [(p, f"stream {s}") for s in (8, 9) for p in both]
