@@ -232,6 +232,21 @@ class DifferentialAttention(nn.Module):
         self.norm_weight = nn.Parameter(torch.ones(2 * head_dim), requires_grad=False)
         self.k_cache = self.v_cache = torch.tensor([])
         self.k_scale = self.v_scale = 1.0
+        self._cache_checked = None  # (k_cache data_ptr, shape) whose geometry was checked
+
+    def _check_cache(self):
+        """The bound cache's geometry, once per binding."""
+        kc = self.k_cache
+        key = (kc.data_ptr(), tuple(kc.shape))
+        if self._cache_checked == key:
+            return
+        _lib.need(kc.dim() == 4 and kc.size(2) == self.num_kv_heads and
+                  kc.size(3) == self.head_dim,
+                  f"DifferentialAttention: k_cache must be [blocks, block_size, "
+                  f"{self.num_kv_heads}, {self.head_dim}], got {tuple(kc.shape)}")
+        _lib.need(kc.size(1) % 16 == 0,
+                  f"DifferentialAttention: block_size {kc.size(1)} is not a multiple of 16")
+        self._cache_checked = key
 
     def forward(self, q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None, Layer=None,
                 kv_stored: bool = False):
@@ -240,7 +255,19 @@ class DifferentialAttention(nn.Module):
         ctx = get_context()
         _lib.need(not ctx.is_compress_step, "DifferentialAttention: its cache takes no part in "
                   "compression steps")
+        if q.dim() != 3 or q.size(1) != self.num_heads or q.size(2) != self.head_dim:
+            raise ValueError(f"DifferentialAttention: q must be [rows, {self.num_heads}, "
+                             f"{self.head_dim}], got {tuple(q.shape)}")
         kc, vc = self.k_cache, self.v_cache
+        paged = ctx.use_decode_kernel or ctx.block_tables is not None
+        if kc.numel():
+            self._check_cache()
+        elif paged:
+            raise ValueError("DifferentialAttention: no cache is bound")
+        if not paged and (k.dim() != 3 or k.size(1) != self.num_kv_heads
+                          or k.size(2) != self.head_dim):
+            raise ValueError(f"DifferentialAttention: k and v must be [rows, {self.num_kv_heads}, "
+                             f"{self.head_dim}], got {tuple(k.shape)}")
         if kc.numel() and not kv_stored:
             store_kvcache(k, v, kc, vc, ctx.slot_mapping, self.k_scale, self.v_scale)
         weights = (self.lambdas, self.lambda_init, self.norm_weight, self.norm_eps)

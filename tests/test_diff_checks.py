@@ -145,3 +145,45 @@ def test_workspace_sizes_follow_the_chip_not_the_lengths():
     assert L.lib().nkv_diff_decode_workspace_bytes(4, 32, 96, 8, 256) == 0
     assert L.lib().nkv_diff_decode_workspace_bytes(4, 32, 64, 8, 256) == \
         L.lib().nkv_paged_decode_workspace_bytes(4, 32, 128, 8, 256)
+
+
+def test_layer_refuses_another_geometry_than_its_own(monkeypatch):
+    """A cache or rows of other heads would be computed over the wrong pairs: before anything runs."""
+    nkv = importlib.import_module("nanokv-llm_amd")
+
+    def launched(*a, **kw):
+        raise AssertionError("launched")
+
+    for name in ("store_kvcache", "diff_paged_decode", "diff_varlen_prefill",
+                 "shared_decode_workspace"):
+        monkeypatch.setattr(da, name, launched)
+    layer = nkv.DifferentialAttention(8, 64, 0.125, 4, 0.2)
+
+    def rows(heads, d=64):
+        return torch.zeros(2, heads, d, dtype=BF)
+
+    def cache(hk=4, d=64, B=16):
+        return torch.zeros(3, B, hk, d, dtype=BF)
+
+    lens, bt = torch.ones(2, dtype=I32), torch.zeros(2, 3, dtype=I32)
+    cu = torch.tensor([0, 1, 2], dtype=I32)
+    try:
+        for decode, tables in ((True, bt), (False, bt), (False, None)):
+            nkv.set_context(decode, cu, cu, 1, 1, lens, lens, tables)
+            for stored in (False, True):
+                for kc in (cache(2), cache(8), cache(d=128), cache(B=24), cache()[0]):
+                    layer.k_cache = layer.v_cache = kc
+                    with pytest.raises(ValueError, match="k_cache must be|block_size"):
+                        layer(rows(8), rows(4), rows(4), kv_stored=stored)
+                layer.k_cache = layer.v_cache = cache()
+                for q in (rows(16), rows(4), rows(8, 128), rows(8)[0]):
+                    with pytest.raises(ValueError, match="q must be"):
+                        layer(q, rows(4), rows(4), kv_stored=stored)
+        layer.k_cache = layer.v_cache = torch.tensor([])  # a first prompt without a cache
+        with pytest.raises(ValueError, match="k and v must be"):
+            layer(rows(8), rows(2), rows(2))
+        nkv.set_context(True, cu, cu, 1, 1, lens, lens, bt)
+        with pytest.raises(ValueError, match="no cache"):
+            layer(rows(8), rows(4), rows(4))
+    finally:
+        nkv.reset_context()
