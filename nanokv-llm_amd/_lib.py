@@ -219,7 +219,9 @@ _SAME_DEVICE = contextlib.nullcontext()
 def device_of(index: int):
     """A context in which device ``index`` is the current one: the library takes launch sizes from
     the current device, and a null stream belongs to it."""
-    return _SAME_DEVICE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+    if index < 0 or index == torch._C._cuda_getDevice():  # < 0: a host tensor, refused later
+        return _SAME_DEVICE
+    return torch.cuda.device(index)
 
 
 def stream_of(t: torch.Tensor) -> int:

@@ -110,12 +110,13 @@ def diff_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     NB, B, width = k_cache.size(0), k_cache.size(1), block_tables.size(1)
     if out is None:
         out = torch.empty(bs, Hq // 2, 2 * D, dtype=q.dtype, device=q.device)
-    if workspace is None:
-        workspace = torch.empty(max(diff_decode_workspace_bytes(bs, Hq, width, B, D), 4),
-                                dtype=torch.uint8, device=q.device)
-    elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+    if workspace is not None and (workspace.dtype is not torch.uint8
+                                  or not workspace.is_contiguous()):
         raise ValueError(f"{what}: workspace must be contiguous uint8")
     with _lib.device_of(q.get_device()):
+        if workspace is None:
+            workspace = torch.empty(max(diff_decode_workspace_bytes(bs, Hq, width, B, D), 4),
+                                    dtype=torch.uint8, device=q.device)
         rc = _lib.lib().nkv_diff_decode(
             kv_type, q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
             block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(), bs, Hq, Hk,
@@ -268,6 +269,11 @@ class DifferentialAttention(nn.Module):
                           or k.size(2) != self.head_dim):
             raise ValueError(f"DifferentialAttention: k and v must be [rows, {self.num_kv_heads}, "
                              f"{self.head_dim}], got {tuple(k.shape)}")
+        with _lib.device_of(q.get_device()):
+            return self._step(q, k, v, ctx, kv_stored)
+
+    def _step(self, q, k, v, ctx, kv_stored):
+        kc, vc = self.k_cache, self.v_cache
         if kc.numel() and not kv_stored:
             store_kvcache(k, v, kc, vc, ctx.slot_mapping, self.k_scale, self.v_scale)
         weights = (self.lambdas, self.lambda_init, self.norm_weight, self.norm_eps)

@@ -187,3 +187,62 @@ def test_layer_refuses_another_geometry_than_its_own(monkeypatch):
             layer(rows(8), rows(4), rows(4))
     finally:
         nkv.reset_context()
+
+
+def test_another_device_than_the_current_one(monkeypatch):
+    """Every launch, the store's too, and every size that depends on the chip are made with q's device
+    as the current one: a null stream belongs to that."""
+    nkv = importlib.import_module("nanokv-llm_amd")
+    inside, seen = [], []
+
+    class Device:
+        def __enter__(self):
+            inside.append(1)
+
+        def __exit__(self, *a):
+            inside.pop()
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: seen.append((name, bool(inside))) or 0
+
+    attn = importlib.import_module("nanokv-llm_amd.layers.attention")
+    lib = Lib()
+    monkeypatch.setattr(L, "lib", lambda: lib)
+    monkeypatch.setattr(L, "require_device", lambda *a, **kw: None)
+    monkeypatch.setattr(L, "device_of", lambda index: Device())
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing",
+                        lambda: seen.append(("capturing", bool(inside))) or False)
+    monkeypatch.setattr(attn, "_SHARED_WS", {})
+    layer = nkv.DifferentialAttention(8, 64, 0.125, 4, 0.2)
+    layer.norm_weight.data = layer.norm_weight.data.to(BF)
+    layer.k_cache = layer.v_cache = torch.zeros(3, 16, 4, 64, dtype=BF)
+    q, k = torch.zeros(2, 8, 64, dtype=BF), torch.zeros(2, 4, 64, dtype=BF)
+    lens, bt = torch.ones(2, dtype=I32), torch.zeros(2, 3, dtype=I32)
+    cu = torch.tensor([0, 1, 2], dtype=I32)
+    try:
+        for decode, tables in ((True, bt), (False, bt), (False, None)):
+            nkv.set_context(decode, cu, cu, 1, 1, lens, lens, tables)
+            layer(q, k, k)
+    finally:
+        nkv.reset_context()
+    da.diff_paged_decode(q, layer.k_cache, layer.k_cache, lens, bt, 0.1, layer.lambdas, 0.2)
+    names = {n for n, _ in seen}
+    assert {"nkv_store_kvcache", "nkv_diff_decode", "nkv_diff_prefill", "capturing",
+            "nkv_diff_decode_workspace_bytes", "nkv_diff_prefill_workspace_bytes"} <= names
+    assert all(ok for _, ok in seen), [n for n, ok in seen if not ok]
+
+
+def test_layer_refuses_host_tensors():
+    nkv = importlib.import_module("nanokv-llm_amd")
+    layer = nkv.DifferentialAttention(8, 64, 0.125, 4, 0.2)
+    layer.k_cache = layer.v_cache = torch.zeros(3, 16, 4, 64, dtype=BF)
+    q, k = torch.zeros(2, 8, 64, dtype=BF), torch.zeros(2, 4, 64, dtype=BF)
+    nkv.set_context(True, None, None, 1, 1, torch.ones(2, dtype=I32), torch.ones(2, dtype=I32),
+                    torch.zeros(2, 3, dtype=I32))
+    try:
+        with pytest.raises(ValueError, match="expected GPU"):
+            layer(q, k, k)
+    finally:
+        nkv.reset_context()
