@@ -867,7 +867,9 @@ int nkv_diff_decode(int32_t kv_type, const void* q, int64_t q_row_stride, const 
  * sees keys 0 .. Lk-Lq+j, over the paged caches, or with block_tables NULL over
  * contiguous rows of k and v (bf16 or fp16; n_rows of them, each with its own row
  * stride). n_rows: the rows of k and v (paged: blocks * block_size). Keys of
- * invalid blocks and past the table are zeros, as there. Without a workspace a
+ * invalid blocks and past the table are zeros, as there. A value that is not
+ * finite reaches the rows of its query tile that do not see its key, too (zero
+ * times it), as there, but for rows that see no key. Without a workspace a
  * query tile's keys stay with one workgroup; with one of
  * nkv_diff_prefill_workspace_bytes (same arguments; 0: no use) they are split
  * where few tiles would leave the chip idle, and sequences that bring one token

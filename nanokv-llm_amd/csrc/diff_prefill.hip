@@ -712,7 +712,13 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   // ---- the end
   float l[kRG];
 #pragma unroll
-  for (int rr = 0; rr < kRG; ++rr) l[rr] = col_sum4(l_run[rr]);
+  for (int rr = 0; rr < kRG; ++rr) {
+    l[rr] = col_sum4(l_run[rr]);
+    if (l[rr] == 0.f) {  // no key seen: zero, also where other rows' values are not finite (0 * inf)
+#pragma unroll
+      for (int db = 0; db < kDb; ++db) acc[rr][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+  }
   if (d.ranges > 1) {  // a part: O, m and l as they are
     if (!active) return;
     float* rows = diff_part<D, RG>(a, x, p) + (int64_t)map * (diff_rows(D, RG) * diff_part_row(D));

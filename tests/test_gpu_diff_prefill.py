@@ -381,3 +381,21 @@ def test_captured_prefill_and_decode(dev):
         check(p, c)
         eager = both()
         assert torch.equal(eager[0], p) and torch.equal(eager[1], d)
+
+
+@pytest.mark.parametrize("kv", [None, FP8])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_rows_that_see_no_key_beside_values_that_are_not_finite(dev, bad, d, kv):
+    """More queries than keys, and a value that is not finite in a key that only the last one sees:
+    those that see none are zero all the same, in tiles of others that see some too."""
+    if kv is FP8 and bad == float("inf"):
+        bad = float("nan")  # e4m3fn has no infinity
+    c = make(dev, [40, 20], [13, 600], 4, 2, d, seed=30, kv=kv)
+    c["v"][c["bt"][0, 0], 12] = bad
+    for split in (False, True):
+        out = run(c, split=split)
+        assert bool((out[:27] == 0).all())
+        assert not bool(torch.isfinite(out[39].float()).any())
+        ref, tol = reference(c)
+        assert bool(((out[40:].double().cpu() - ref[40:]).abs() <= tol[40:]).all())
