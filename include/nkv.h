@@ -802,9 +802,9 @@ int nkv_pages_append(const nkv_pages* pages, const int32_t* rows, int32_t n,
  * more than it has, or fewer than 0: refused). Pages behind them lose a
  * reference and the table entries become -1. A page that stays in part while
  * other rows hold it too (its count before the call is above 1) is replaced by
- * a copy of its kept rows in a free page. Then every page of page_ids (int32
- * [n_page_ids], -1: none) loses a reference, as for the pages that a compression
- * step's events list. Counts do not go below 0.
+ * a copy of its kept rows in a free page. Every page of page_ids (int32
+ * [n_page_ids], -1: none) that was in use before the call loses a reference, as
+ * for the pages that a compression step's events list. Counts do not go below 0.
  * Replaces: BlockManager.deallocate / truncate_blocks (block_manager.py:82-92,
  *           117-138).
  */

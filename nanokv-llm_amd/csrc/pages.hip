@@ -447,6 +447,18 @@ __global__ __launch_bounds__(kPlan) void pages_compact_kernel(const PagesArgs a,
 // ---------------------------------------------------------------- the second launch
 enum { kTruncate, kFork, kCompact };
 
+// Whether page id is a copy's destination, and so free before the call: they ascend, as the plan
+// found them.
+__device__ __forceinline__ bool copied_to(const PagesArgs& a, int n_copies, int id) {
+  int lo = 0, hi = n_copies;  // the first destination from id on
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a.copies[mid][1] < id) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo < n_copies && a.copies[lo][1] == id;
+}
+
 // Workgroups x < books of plane 0 change counts and tables; the others copy rows.
 template <int OP>
 __global__ __launch_bounds__(kCopyThreads) void pages_apply_kernel(
@@ -472,7 +484,7 @@ __global__ __launch_bounds__(kCopyThreads) void pages_apply_kernel(
       }
       for (int k = t0; k < n_copies; k += threads) drop_ref(a, a.copies[k][0]);
       for (int k = t0; k < n_loose; k += threads)
-        if (loose[k] != -1) drop_ref(a, loose[k]);
+        if (loose[k] != -1 && !copied_to(a, n_copies, loose[k])) drop_ref(a, loose[k]);
     } else if constexpr (OP == kFork) {
       if (!share) return;
       for (int i = w0; i < n; i += waves) {

@@ -165,7 +165,7 @@ class PagedSequences:
         """Row ``rows[i]`` keeps its first ``lens[i]`` tokens (0: the sequence ends). Pages that no
         row holds any more are free; one that stays in part while others hold it is copied.
         ``pages``: ids that lose a reference besides, -1 for none (the freed blocks in the events
-        of a compression step). -> status [n]."""
+        of a compression step); those free before the call are passed over. -> status [n]."""
         n = self._list("truncate: rows", rows)
         self._list("truncate: lens", lens, n)
         m = 0 if pages is None else self._list("truncate: pages", pages)

@@ -76,7 +76,8 @@ class PagedSequencesRef:
             fit.append(ok)
             own.append(int(ok and k < self.lens[r] and k % self.B > 0
                            and self.refs[self.tables[r][k // self.B]] > 1))
-        got, drop = self._grant(fit, own), [p for p in pages if 0 <= p < self.NB]
+        got = self._grant(fit, own)
+        drop = [p for p in pages if 0 <= p < self.NB and self.refs[p] > 0]
         for r, k, new in zip(rows, keeps, got):
             if new is None:
                 continue

@@ -12,6 +12,7 @@ import torch
 
 from oracle.attention_ref import paged_decode_ref
 from oracle.pages_ref import PagedSequencesRef
+from test_pages_checks import free_page_listed
 
 pytestmark = pytest.mark.gpu
 
@@ -432,3 +433,17 @@ def test_a_graph_replayed_after_its_object_is_dropped(dev):
         assert all(bool((x == 7).all()) for x in others)
     del graph
     assert nkv.release_retired_decode_workspaces() >= 1
+
+
+def test_a_listed_page_that_was_free_keeps_its_new_row(dev):
+    free_page_listed(Pair(dev))
+
+
+def test_listed_pages_among_many_copies(dev):
+    """Every page of the pool listed beside 40 copies: those in use before lose a reference, the new
+    ones keep theirs."""
+    p = Pair(dev, pages=200, rows=90, width=4)
+    p.append(list(range(40)), [33 + r % 20 for r in range(40)])
+    p.fork(list(range(40)), list(range(40, 80)))
+    p.truncate(list(range(40, 80)), [17 + r % 15 for r in range(40)], pages=list(range(200)))
+    assert [p.ref.refs[p.ref.tables[r][1]] for r in range(40, 80)] == [1] * 40

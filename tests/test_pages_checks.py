@@ -236,3 +236,35 @@ def test_buffers_are_recorded_on_other_streams_than_their_own(host_pool, monkeyp
         host_pool.compact()
     both = [host_pool._workspace.data_ptr(), host_pool._state.data_ptr()]
     assert recorded == [(p, f"stream {s}") for s in (8, 9) for p in both]
+
+
+def free_page_listed(p):
+    """Two rows share pages; one is cut inside a shared page, so that it takes the lowest free page
+    for its copy, and the same call lists that page and the next free one."""
+    assert p.append([0], [40]) == [1] and p.fork([0], [1]) == [1]
+    free = [x for x, c in enumerate(p.ref.refs) if c == 0]
+    assert p.truncate([1], [20], pages=[free[0], free[1], free[0]]) == [1]
+    assert p.ref.tables[1][1] == free[0] and p.ref.refs[free[0]] == 1
+    held = [x for t in p.ref.tables for x in t if x >= 0]
+    assert p.ref.refs == [held.count(x) for x in range(len(p.ref.refs))]
+    assert p.append([2], [40]) == [1]  # takes other pages
+    assert not set(p.ref.tables[2]) & set(p.ref.tables[1]) - {-1}
+
+
+class OracleAlone:
+    def __init__(self):
+        self.ref = PagedSequencesRef(torch.zeros(2, 1, 40, 16, 1, 1, dtype=torch.int64), 8, 6)
+
+    def append(self, rows, counts):
+        return self.ref.append(rows, cu=[sum(counts[:i]) for i in range(len(counts) + 1)],
+                               n_tokens=sum(counts))[1]
+
+    def fork(self, parents, children):
+        return self.ref.fork(parents, children)
+
+    def truncate(self, rows, lens, pages):
+        return self.ref.truncate(rows, lens, pages)
+
+
+def test_a_listed_page_that_was_free_keeps_its_new_row():
+    free_page_listed(OracleAlone())
