@@ -246,3 +246,33 @@ def test_layer_refuses_host_tensors():
             layer(q, k, k)
     finally:
         nkv.reset_context()
+
+
+def test_a_device_without_memory_takes_the_launch_that_needs_none(monkeypatch):
+    """No workspace left: the prefill runs without one, as without max_seqlen_k."""
+    calls = []
+
+    class Lib:
+        def nkv_diff_prefill_workspace_bytes(self, *a):
+            return 1 << 40
+
+        def nkv_diff_prefill(self, *a):
+            calls.append(a)
+            return 0
+
+    lib, empty = Lib(), torch.empty
+
+    def no_memory(*size, **kw):
+        if size == (1 << 40,):
+            raise torch.OutOfMemoryError("no memory")
+        return empty(*size, **kw)
+
+    monkeypatch.setattr(L, "lib", lambda: lib)
+    monkeypatch.setattr(L, "require_device", lambda *a, **kw: None)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    monkeypatch.setattr(torch, "empty", no_memory)
+    q, kc = torch.zeros(2, 8, 64, dtype=BF), torch.zeros(4, 16, 4, 64, dtype=BF)
+    cu, bt, l = torch.tensor([0, 2], dtype=I32), torch.zeros(1, 4, dtype=I32), torch.zeros(4, 64)
+    assert da.diff_prefill_workspace(q, kc, 1, 2, 60) is None
+    da.diff_varlen_prefill(q, kc, kc, cu, cu, 2, 0.1, l, 0.2, block_tables=bt, max_seqlen_k=60)
+    assert calls[0][-3:] == (None, 0, 0)  # workspace, bytes, stream

@@ -399,3 +399,80 @@ def test_rows_that_see_no_key_beside_values_that_are_not_finite(dev, bad, d, kv)
         assert not bool(torch.isfinite(out[39].float()).any())
         ref, tol = reference(c)
         assert bool(((out[40:].double().cpu() - ref[40:]).abs() <= tol[40:]).all())
+
+
+def test_a_cache_past_4_gib(dev):
+    """Pages whose byte offset passes 32 bits: whole tiles, cut ones and a decode row."""
+    B, hk, d = 256, 8, 128
+    NB = (5 << 30) // (B * hk * d * 2)
+    g = torch.Generator().manual_seed(32)
+    k = torch.empty(NB, B, hk, d, dtype=BF, device=dev)
+    v = torch.empty(NB, B, hk, d, dtype=BF, device=dev)
+    bt = torch.tensor([[NB - 1, 0, NB - 2], [NB - 3, 1, -1]], dtype=I32)
+    at = [NB - 1, 0, NB - 2, NB - 3, 1]
+    rows = torch.randn(2, 5, B, hk, d, generator=g).to(BF)
+    k[at], v[at] = rows[0].to(dev), rows[1].to(dev)
+    q = torch.randn(91, 16, d, generator=g).to(BF)
+    lambdas = torch.randn(4, d, generator=g) * 0.1
+    cu_q, cu_k = torch.tensor([0, 90, 91], dtype=I32), torch.tensor([0, 700, 1000], dtype=I32)
+    for max_k in (700, None):
+        out = nkv.diff_varlen_prefill(q.to(dev), k, v, cu_q.to(dev), cu_k.to(dev), 90, d ** -0.5,
+                                      lambdas.to(dev), 0.2, block_tables=bt.to(dev),
+                                      max_seqlen_k=max_k)
+        for a, b, first, n in ((0, 90, 0, 700), (90, 91, 3, 300)):
+            kk, vv = (x[first:].flatten(0, 1)[:n] for x in rows)
+            ref = diff_attention_ref(q[a:b], kk, vv, d ** -0.5, lambdas, 0.2)
+            tol = tolerance(ref, 2 * float(vv.abs().max()), lambdas, 0.2, None, 1e-5, BF)
+            assert bool(((out[a:b].double().cpu() - ref).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("kv", [None, FP8])
+def test_the_layer_captured_over_a_reserved_workspace(dev, kv):
+    """Workspace reserved for heads of 2 head_dim, a decode step of the layer in one graph, replayed
+    over new inputs with eager steps and a regrowth of the shared workspace between the replays."""
+    hq, hk, d, B = 8, 4, 64, 16
+    g = torch.Generator().manual_seed(33)
+    c = make(dev, [1] * 5, [60, 1, 33, 700, 16], hq, hk, d, B=B, kv=kv, seed=33)
+    m = nkv.DifferentialAttention(hq, d, c["scale"], hk, c["init"]).to(dev)
+    m.lambdas.copy_(c["lambdas"])
+    m.norm_weight.data = c["weight"].to(dev)
+    m.k_cache, m.v_cache = c["k"].to(dev), c["v"].to(dev)
+    if kv is FP8:
+        m.k_scale, m.v_scale = KS, VS
+    bt, lens = c["bt"].to(dev), torch.tensor(c["ctx"], dtype=I32, device=dev)
+    slots = torch.tensor([int(c["bt"][i, (n - 1) // B]) * B + (n - 1) % B
+                          for i, n in enumerate(c["ctx"])], dtype=I32, device=dev)
+    q = torch.empty(5, hq, d, dtype=BF, device=dev)
+    k, v = (torch.empty(5, hk, d, dtype=BF, device=dev) for _ in range(2))
+    nkv.reserve_decode_workspace(dev, 5, hq, bt.size(1), B, head_dim=2 * d)
+
+    def fill():
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g).to(BF))
+
+    def expect(out):
+        now = dict(c, q=q.cpu(), k=m.k_cache.cpu(), v=m.v_cache.cpu())
+        check(out.squeeze(1), now, zeros=False)
+
+    nkv.set_context(True, slot_mapping=slots, context_lens=lens, block_tables=bt)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        fill()
+        m(q, k, v)  # warm-up
+        with torch.cuda.graph(graph):
+            out = m(q, k, v)
+        for i in range(5):
+            fill()
+            graph.replay()
+            torch.cuda.synchronize()
+            expect(out)
+            held = m.k_cache.view(torch.uint8).clone()
+            assert torch.equal(m(q, k, v), out)  # the same step again, eagerly
+            assert torch.equal(m.k_cache.view(torch.uint8), held)
+            if i == 2:
+                shared = importlib.import_module("nanokv-llm_amd.layers.attention")
+                ws = shared.shared_decode_workspace(q.device, 0)
+                nkv.reserve_decode_workspace(dev, 64, 64, 4096, B, head_dim=2 * d)
+                assert shared.shared_decode_workspace(q.device, 0).numel() >= ws.numel()
+    finally:
+        nkv.reset_context()
