@@ -765,9 +765,9 @@ int nkv_build_step_metadata(const int32_t* packed, int32_t n_seqs, int32_t block
  * Lists are taken as the state before the call has it. An entry of -1 is
  * padding; a row named twice counts where it is named first. Pages are taken
  * lowest first, in the list's order: an entry is granted if it needs no page or
- * the pages of all entries up to it are free before the call, else it is refused
- * and changes nothing. status[i] is 1 for an entry that was carried out, else 0. Calls on
- * the same pages must be ordered on a stream.
+ * the pages of all entries up to it are free before the call, else it is
+ * refused and changes nothing. status[i] is 1 for an entry that was carried
+ * out, else 0. Calls on the same pages must be ordered on a stream.
  *
  * Replaces: BlockManager's bookkeeping (nanokvllm/engine/block_manager.py:
  *           13-138) for callers that keep it on the device; forks, moves and
@@ -826,7 +826,8 @@ int nkv_pages_fork(const nkv_pages* pages, const int32_t* parents, const int32_t
  * k-th lowest free page below n_live takes the k-th highest page in use, for
  * the first max_moves of them; all tables and counts follow. info[0] = n_live,
  * info[1] = the moves made; moves (int32 [max_moves, 2], 8-byte aligned) lists
- * them as (from, to), padded with -1. max_moves: at most 2^20. No counterpart in the reference.
+ * them as (from, to), padded with -1. max_moves: at most 2^20. No counterpart
+ * in the reference.
  */
 int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info, int32_t* moves,
                       void* stream);

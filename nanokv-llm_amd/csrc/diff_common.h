@@ -59,8 +59,8 @@ __device__ __forceinline__ void diff_store(const DiffArgs& d, const float (&o)[D
 }
 
 // The end of one (sequence b, query pair h) of a decode stream over pairs (DIFF): the partials of
-// its two maps, merged by 2 x WAVES waves (`wave` of them) of a workgroup that all call it, those with
-// live = false for nothing but the barrier.
+// its two maps, merged by 2 x WAVES waves (`wave` of them) of a workgroup that all call it, those
+// with live = false for nothing but the barrier.
 template <int D, int WAVES>
 struct DiffLds {
   MergeLds<D, WAVES> merge[2];

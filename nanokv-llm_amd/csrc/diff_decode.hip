@@ -2,16 +2,19 @@
 // diff_common.h). No counterpart in the reference; it stands beside the decode of
 // nanokvllm/layers/attention.py:104-107 over the same cache.
 //
-// MI355X design (HBM-bound: every K/V byte is read once): two K heads beside each other in a token's
-// row are one head of twice the dims, and their V heads are the value that both maps share. So the
-// pair is streamed by the decode kernel's waves as one KV head of 128 or 256 dims with 2 G query
-// columns, of which the even ones are scored against the row's first half and the odd ones against
-// the second (decode_stream, DIFF): each V row is read once for both maps. Run as four ordinary
-// attentions (two maps, each over both halves of the value) K and V would be read twice.
+// MI355X design (HBM-bound: every K/V byte is read once): two K heads beside each other in a
+// token's row are one head of twice the dims, and their V heads are the value that both maps share.
+// So the pair is streamed by the decode kernel's waves as one KV head of 128 or 256 dims with 2 G
+// query columns, of which the even ones are scored against the row's first half and the odd ones
+// against the second (decode_stream, DIFF): each V row is read once for both maps. Run as four
+// ordinary attentions (two maps, each over both halves of the value) K and V would be read twice.
+// head_dim 256 would be a KV head of 512 dims, for which the stream has no instance (a wave's piece
+// of a row is at most 512 bytes), and 64 KiB a tile in the prefill, whose ring takes four: refused.
 // The combine merges the partials of a pair's two rows in the halves of one workgroup, and
 // subtracts, normalises and scales them in the wave that holds the first.
-// 64 sequences of 2048..8192 tokens (Hq 32, Hk 8, head_dim 128): 199 us and 7.5 for the combine; the
-// call 204 us, 6.2 TB/s, each byte of K and V read once.
+// 64 sequences of 2048..8192 tokens (Hq 32, Hk 8, head_dim 128): 199 us and 7.5 for the combine;
+// the call 204 us, 6.2 TB/s, each byte of K and V read once. An fp8 pool: 119 us, 5.3 TB/s;
+// head_dim 64: 110 us, 5.7 TB/s, fp8 69 us, 4.6 TB/s.
 #include "diff_common.h"
 
 #include <math.h>
@@ -46,8 +49,8 @@ int diff_check(const char* what, int32_t kv_type, int32_t n_q_heads, int32_t n_k
   NKV_REQUIRE(n_q_heads / n_kv_heads <= NKV_DIFF_MAX_GROUP, NKV_EUNSUPPORTED,
               "%s: %d query pairs to a KV pair, above %d", what, n_q_heads / n_kv_heads,
               NKV_DIFF_MAX_GROUP);
-  NKV_REQUIRE(scale > 0.f && isfinite(scale) && k_scale > 0.f && v_scale > 0.f && isfinite(k_scale) &&
-                  isfinite(v_scale),
+  NKV_REQUIRE(scale > 0.f && isfinite(scale) && k_scale > 0.f && v_scale > 0.f &&
+                  isfinite(k_scale) && isfinite(v_scale),
               NKV_EINVAL, "%s: scales must be finite and > 0", what);
   NKV_REQUIRE(isfinite(lambda_init) && eps > 0.f && isfinite(eps), NKV_EINVAL,
               "%s: lambda_init must be finite and eps > 0", what);

@@ -5,10 +5,11 @@
 //
 // MI355X design (MFMA-bound):
 //  * Workgroup = (sequence, tile of queries, KV pair, range of keys). A tile's R rows are its
-//    queries for all G query pairs of the KV pair, query-major, and each row is computed twice, once
-//    for each map: the first half of the waves takes map 0, the other half map 1 of the same rows.
-//    Both read the same V tile (the pair's value of 2 D dims), and each its own half of every K row, so
-//    that K and V are fetched once for both maps and no product is made with the other map's keys.
+//    queries for all G query pairs of the KV pair, query-major, and each row is computed twice,
+//    once for each map: the first half of the waves takes map 0, the other half map 1 of the same
+//    rows. Both read the same V tile (the pair's value of 2 D dims), and each its own half of
+//    every K row, so that K and V are fetched once for both maps and no product is made with the
+//    other map's keys.
 //  * Keys advance in steps of 64. A step's K and V rows (2 D dims each: the pair's two heads lie
 //    beside each other) go straight into LDS, one step ahead or more, with the chunk permutation
 //    of lds_tiles.h; fp8 codes pass through registers and are widened on the way.
@@ -18,16 +19,21 @@
 //  * S^T = K Q^T (A: 16 keys from LDS, B: the wave's Q^T, held in registers) leaves a lane with one
 //    row's scores of 4 keys in every 16; the weights, packed to 16 bits, are the B operand of
 //    O^T += V^T P^T, its A operand read transposed from LDS. A row's running maximum is raised only
-//    when it grows by more than kLazy (log2), its sum is over the rounded weights.
+//    when it grows by more than kDiffLazy (log2), its sum is over the rounded weights. Weights in
+//    16 bits are what the matrix cores take beside V as the cache holds it; summing them as rounded
+//    lets the roundings' common part cancel. Relative error against 64 bits 0.0020 to 0.0023, where
+//    32 bits throughout, with the output rounded, have 0.0017.
 //  * The end of a tile: map 1's waves leave A_1 in LDS (the tiles' ring, free by then), map 0's
-//    waves subtract, take the mean square over the row's 2 D dims (in the row's 4 lanes), normalise and
-//    store. Nothing but the output is written.
-//  * Few tiles: the tiles' keys are cut into ranges of the same number of steps, about as many in all
-//    as workgroups are resident, a partial row (O, m, l) is written for each and map, and a second
-//    kernel merges and ends them. Tiles of one range are ended by the first kernel.
+//    waves subtract, take the mean square over the row's 2 D dims (in the row's 4 lanes), normalise
+//    and store. Two row groups at head_dim 128 take all 256 VGPRs there and spill 28 to 34 more,
+//    behind the step loop: 31 KB a tile, as much as the call with four chunks below writes beyond
+//    its output (86 MB against 58). No other instance spills.
+//  * Few tiles: the tiles' keys are cut into ranges of the same number of steps, about as many in
+//    all as workgroups are resident, a partial row (O, m, l) is written for each and map, and a
+//    second kernel merges and ends them. Tiles of one range are ended by the first kernel.
 //  * Sequences that bring one token, among prompts: the first workgroups' waves stream their K/V as
-//    the decode kernel does, beside the tiles that keep the matrix cores; a tile for one query would
-//    multiply 96 or 128 rows for it. The second kernel merges them too.
+//    the decode kernel does, beside the tiles that keep the matrix cores; a tile for one query
+//    would multiply 96 or 128 rows for it. The second kernel merges them too.
 // Tiles are numbered over the batch without gaps (their number per sequence is known on the device
 // only), each sequence's last ones first: they see the most keys.
 #include "diff_common.h"
@@ -43,13 +49,23 @@ constexpr int kDiffStep = 64;        // keys per step
 constexpr float kDiffLazy = 8.f;     // log2 headroom before a running maximum is raised
 constexpr int kDiffMinSteps = 4;     // shortest range of a cut tile
 constexpr int kDiffMergeWaves = 4;
-// Decode rows' share of the workgroups: CU time of a row's step against a tile's (see diff_plan).
+// Weight of a decode row against a tile where workgroups are shared out between them (diff_plan);
+// half of it with fp8. An empirical choice, and it weighs a row by no length, since the host knows
+// none but the longest. Us with 0.3 / 0.6 / 1.33 (Hq 32, Hk 8, bf16, 40 rows
+// beside two chunks of 512; then fp8, 20 rows beside two of up to 2048), head_dim 128:
+//   rows of 50-300:    137 / 136 / 172    293 / 293 / 293
+//   rows of 300-4000:  158 / 166 / 175    808 / 427 / 304
+//   rows of 6000-8000: 388 / 297 / 233   2275 / 1156 / 512
+// and at head_dim 64: 98 / 95 / 74, 99 / 123 / 95, 187 / 158 / 150; 128 / 128 / 131, 265 / 148 /
+// 142, 702 / 368 / 188. Few rows of long contexts beside long chunks wait for their streams.
 constexpr double kDiffRowShare = 0.6;
 
 // Waves of a workgroup, and 16-row groups of a wave at most. At head_dim 128 a step's tiles take
-// 64 KiB, so one workgroup is resident and brings both waves of each SIMD itself; with fp8 codes on
-// their way through registers two groups do not fit them (1006 us and spills, one 980: four chunks of
-// up to 2048 tokens over up to 6000, Hq 32, Hk 8).
+// 64 KiB, so one workgroup is resident and brings both waves of each SIMD itself. With fp8 the
+// codes wait in 16 registers a lane until they are widened, and two groups then spilled
+// (1006 us, one 980: four chunks of up to 2048 tokens over up to 6000, Hq 32, Hk 8);
+// with one, each fragment read from LDS serves one product where 16-bit caches' serve two (675
+// us). Codes that wait in LDS would leave the registers free; not built.
 constexpr int diff_waves(int D) { return D == 128 ? 8 : 4; }
 constexpr int diff_groups(int D, bool f8) { return D == 128 ? (f8 ? 1 : 2) : 3; }
 constexpr int diff_rows(int D, int rg) { return 8 * diff_waves(D) * rg; }  // of a tile
@@ -63,23 +79,26 @@ struct DiffPrefillArgs {
   const int32_t *cu_q, *cu_k, *block_tables;
   int64_t bt_row_stride;
   int32_t P, G, block_size, max_blocks, n_limit, n_seqs, total_q;
-  // workgroups for a pair at a time (0: tiles stay whole), and the most ranges and tiles of a cut batch
+  // workgroups for a pair at a time (0: tiles stay whole), and the most ranges and tiles of a cut
+  // batch
   int32_t target, range_cap, tile_cap;
   float cus;
   float scale_log2, v_scale;
   DiffArgs diff;
   bf16_t* out;
   int64_t out_row_stride;
-  i32x4_t* tile_desc;  // of cut tiles: {ranges, the first one, first row of q, rows}; [tile_cap]: tiles
+  // of cut tiles: {ranges, the first one, first row of q, rows}; [tile_cap]: tiles
+  i32x4_t* tile_desc;
   float* part;
-  // decode rows apart from the tiles: the first row_groups workgroups stream them (0: they are tiles)
+  // decode rows apart from the tiles: the first row_groups workgroups stream them (0: they are
+  // tiles)
   int32_t row_groups, ncg, min_chunks, max_tokens;
   i32x4v_t* row_desc;
   float* row_part;
 };
 
-// A range of a tile of the batch: queries j0 .. of a sequence (row q0 of q), the key steps of range sp
-// of `ranges`.
+// A range of a tile of the batch: queries j0 .. of a sequence (row q0 of q), the key steps of range
+// sp of `ranges`.
 struct DiffTile {
   int seq, q0, Lq, kb0, Lk, j0;
   int id, n_steps, ranges, sp;
@@ -90,15 +109,19 @@ __device__ __forceinline__ int diff_steps(int Lq, int Lk, int QT, int tile) {
   return last >= 0 ? last / kDiffStep + 1 : 0;
 }
 
-// Range x of a pair, by the whole wave; false past the last one. The tiles of a sequence have as many
-// places for ranges as its last one needs, so that a lane knows its sequence's number without a
-// loop; the others' last places stay empty. n_tiles: all tiles, 0 where none is cut.
+// Range x of a pair, by the whole wave; false past the last one. The tiles of a sequence have as
+// many places for ranges as its last one needs, so that a lane knows its sequence's number without
+// a loop; the others' last places stay empty. n_tiles: all tiles, 0 where none is cut.
 template <int D, int RG>
 __device__ __forceinline__ bool diff_range(const DiffPrefillArgs& a, int QT, int x, DiffTile& d,
                                            int& n_tiles) {
-  // measured: a step of a workgroup alone on its CU, and of one of two on it; what a range's partial
-  // rows (101 KB at head_dim 64, 266 at 128) cost of the chip's time, written and read again; and what
-  // the merge takes beside that
+  // A step of a workgroup alone on its CU, and of one of two on it (at head_dim 128 one is
+  // resident). Measured with 256 and 512 workgroups, from 4096 keys to 12288, 16-bit caches
+  // (fp8): head_dim 64, one row group 0.70 and 1.01 us (0.92, 1.29), three 1.33 and 2.10 (1.67,
+  // 2.40); head_dim 128, one 1.56 (1.89), two 2.48. Only their ratio to what follows matters, and
+  // one table serves all types. Then what a range's partial rows (101 KB at head_dim 64 with
+  // three groups, 266 at 128 with two) cost of the chip's time, written and read again, and what
+  // the merge takes beside that: fitted to whole calls.
   constexpr float kStepUs[2] = {D == 64 ? (RG == 1 ? 0.8f : 1.6f) : (RG == 1 ? 1.4f : 2.2f),
                                 D == 64 ? (RG == 1 ? 1.1f : 2.1f) : (RG == 1 ? 1.4f : 2.2f)};
   constexpr float kRangeUs = D == 64 ? 0.01f * RG : 0.02f * RG, kMergeUs = 6.f;
@@ -126,9 +149,9 @@ __device__ __forceinline__ bool diff_range(const DiffPrefillArgs& a, int QT, int
   int R = INT32_MAX;  // steps of a range
   n_tiles = 0;
   if (a.target > 0) {
-    // Lane k tries ranges of 1 / (k + 1) of the longest tile and takes the time until all are through:
-    // steps, slower where two workgroups share a CU, and the partial rows, which all go through
-    // memory twice.
+    // Lane k tries ranges of 1 / (k + 1) of the longest tile and takes the time until all are
+    // through: steps, slower where two workgroups share a CU, and the partial rows, which all go
+    // through memory twice.
     int longest = 0, tiles = 0;
     for (int cb = 0; cb < a.n_seqs; cb += 64) {  // uniform
       load(cb);
@@ -394,8 +417,8 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
       }
     }
   };
-  // F8: codes in registers, widened into the wave's rows of an LDS tile. Lanes in the second half of
-  // a row write their pair's second chunk first, so that each 16-byte write instruction covers
+  // F8: codes in registers, widened into the wave's rows of an LDS tile. Lanes in the second half
+  // of a row write their pair's second chunk first, so that each 16-byte write instruction covers
   // distinct banks.
   const bool f8_swap = f8_c >= kLpr8 / 2;
   auto commit = [&](const u32x4_t (&codes)[kNl8], char* tile) {
@@ -441,7 +464,8 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   const uint32_t ko = (uint32_t)col * kRB +
                       (uint32_t)((map * (D / 8) + g4) ^ chunk_swz<kV>(col)) * 16u;
   // V^T by ds_read_b64_tr_b16: lane 16g + 4r + c reads row 4g + r (and +16), dims 16 db + 4c .. +3:
-  // chunk 2 db + c/2, half c%2. The low three bits of db likewise; the rows' permutation has no more.
+  // chunk 2 db + c/2, half c%2. The low three bits of db likewise; the rows' permutation has no
+  // more.
   const int vrow = 4 * g4 + (col >> 2);
   const uint32_t vo = (uint32_t)vrow * kRB + (uint32_t)chunk_swz<kV>(vrow) * 16u +
                       (uint32_t)(col & 3) * 8u;
@@ -593,9 +617,10 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
     // waves of map 0 work on tile h (scores of a K tile, products of a V tile), those of map 1 on
     // tile h - 1. Tile i lies in place i % kTiles of the ring, which is free from half step
     // i + 2 - kTiles on, and is fetched from then on until the end of half step i - 1: three half
-    // steps with five places; fp8 codes, which wait in registers, two. Four chunks of up to 2048 tokens
-    // over up to 6000 (Hq 32, Hk 8): whole steps with a barrier each 690 us, half steps and four
-    // places 685, five 660 to 678 in several runs; without the fetches 602, without the softmax too 554.
+    // steps with five places; fp8 codes, which wait in registers, two. Four chunks of up to 2048
+    // tokens over up to 6000 (Hq 32, Hk 8): whole steps with a barrier each 690 us, half steps and
+    // four places 685, five 660 to 678 in several runs; without the fetches 602, without the
+    // softmax too 554.
     constexpr int kAhead = F8 ? 2 : 3;
     auto next = [](uint32_t at) { return at + kTileB == kTiles * kTileB ? 0u : at + kTileB; };
     uint32_t rd = 0, wr = 2 * kTileB;  // places read and fetched next
@@ -714,7 +739,7 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
 #pragma unroll
   for (int rr = 0; rr < kRG; ++rr) {
     l[rr] = col_sum4(l_run[rr]);
-    if (l[rr] == 0.f) {  // no key seen: zero, also where other rows' values are not finite (0 * inf)
+    if (l[rr] == 0.f) {  // no key seen: zero, also beside values that are not finite (0 * inf)
 #pragma unroll
       for (int db = 0; db < kDb; ++db) acc[rr][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
@@ -776,11 +801,11 @@ __global__ __launch_bounds__(64 * diff_waves(D), 2) void diff_prefill_kernel(
   }
 }
 
-// Merges and ends the rows of tiles that have several ranges (workgroups below tile_groups); and the
-// decode rows, two waves for each (sequence, query pair). A wave has kMergeRows rows of a tile at once,
-// both maps of each: at head_dim 64 the halves of the wave have a map each, 4 dims a lane; at 128
-// every lane has 4 dims of both. kMergeFly ranges' loads are in flight. (One row a wave: 17 us over the
-// 50 MB of two prompts of 512 tokens, Hq 32, Hk 8, head_dim 64.)
+// Merges and ends the rows of tiles that have several ranges (workgroups below tile_groups); and
+// the decode rows, two waves for each (sequence, query pair). A wave has kMergeRows rows of a tile
+// at once, both maps of each: at head_dim 64 the halves of the wave have a map each, 4 dims a lane;
+// at 128 every lane has 4 dims of both. kMergeFly ranges' loads are in flight. (One row a wave:
+// 17 us over the 50 MB of two prompts of 512 tokens, Hq 32, Hk 8, head_dim 64.)
 constexpr int kMergeRows = 4;
 template <int D, bool H16, int RG>
 __global__ __launch_bounds__(64 * kDiffMergeWaves) void diff_merge_kernel(
@@ -894,11 +919,11 @@ static int64_t diff_max_tiles(int64_t total_q, int64_t n_seqs, int qt) {
   return total_q / qt + n_seqs;
 }
 
-// 16-row groups of a wave: one where the tiles then are no more than the CUs, since fewer rows a step
-// are a shorter step, else as many as fit. One prompt of 300 / 900 tokens (Hq 16, Hk 8), us: head_dim
-// 128 37.5 -> 25.1 / 56.7 -> 41.5, 64 24.5 -> 16.6 / 38.5 -> 25.4. Not at head_dim 64 beside decode
-// rows, which leave no CU idle (two chunks of 512 beside 30, fp8: 57 -> 76; at 128 146 -> 131 for one of
-// 300 beside 100).
+// 16-row groups of a wave: one where the tiles then are no more than the CUs, since fewer rows a
+// step are a shorter step, else as many as fit. One prompt of 300 / 900 tokens (Hq 16, Hk 8), us:
+// head_dim 128 37.5 -> 25.1 / 56.7 -> 41.5, 64 24.5 -> 16.6 / 38.5 -> 25.4. Not at head_dim 64
+// beside decode rows, which leave no CU idle (two chunks of 512 beside 30, fp8: 57 -> 76; at 128
+// 146 -> 131 for one of 300 beside 100).
 static int diff_choose(int64_t n_seqs, int64_t total_q, int64_t max_seqlen_q, int P, int G, int D,
                        bool f8) {
   const int most = diff_groups(D, f8), rows = diff_rows(D, 1);
@@ -930,8 +955,8 @@ static DiffPlan diff_plan(int64_t n_seqs, int64_t total_q, int64_t max_seqlen_q,
   int64_t slots = resident;
   // (max_seqlen_q = 1 with more rows than sequences: padding, or not known)
   if (paged && mix.rows > 0 && (max_seqlen_q > 1 || (max_seqlen_q == 1 && total_q <= n_seqs))) {
-    // A row's step of 64 keys is bound by its K/V bytes, a tile's by the matrix cores; of a CU's
-    // time they take about as much at head_dim 128, a third more at 64, half of it with fp8.
+    // A row's step of 64 keys is bound by its K/V bytes (half of them with fp8), a tile's by the
+    // matrix cores: each gets workgroups by kDiffRowShare, whatever its length and head_dim.
     tiles = mix.prompts > 0 ? diff_max_tiles(mix.prompt_rows, mix.prompts, qt) : 0;
     const double rows = (double)mix.rows * kDiffRowShare * (f8 ? 0.5 : 1.0);
     d.ncg = decode_ncg(2 * G);
@@ -1005,10 +1030,10 @@ extern "C" int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_st
                                 const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
                                 const int32_t* block_tables, int64_t bt_row_stride,
                                 int32_t max_blocks_per_seq, int32_t n_seqs, int64_t max_seqlen_q,
-                                int64_t max_seqlen_k, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
-                                int32_t block_size, int64_t n_rows, float scale, float k_scale,
-                                float v_scale, const float* lambdas, float lambda_init,
-                                const void* norm_weight, float eps, void* out,
+                                int64_t max_seqlen_k, int32_t n_q_heads, int32_t n_kv_heads,
+                                int32_t head_dim, int32_t block_size, int64_t n_rows, float scale,
+                                float k_scale, float v_scale, const float* lambdas,
+                                float lambda_init, const void* norm_weight, float eps, void* out,
                                 int64_t out_row_stride, void* workspace, size_t workspace_bytes,
                                 void* stream) {
   using namespace nkv;
@@ -1044,7 +1069,6 @@ extern "C" int nkv_diff_prefill(int32_t kv_type, const void* q, int64_t q_row_st
                 (long long)bt_row_stride);
     NKV_REQUIRE(k_row_stride == row && v_row_stride == row, NKV_EINVAL,
                 "diff_prefill: paged rows are Hk*D apart");
-    // fp8 rows are read 16 codes at a time
     NKV_REQUIRE(n_rows / block_size < (1ll << 31), NKV_EUNSUPPORTED,
                 "diff_prefill: too many blocks");
   } else {

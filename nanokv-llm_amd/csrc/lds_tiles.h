@@ -1,6 +1,6 @@
 // K/V tiles in LDS for the kernels that attend with many query rows (prefill.hip,
-// diff_prefill.hip): rows fetched straight into LDS, their 16-byte chunks permuted so that the K row
-// reads and the V transpose reads are free of bank conflicts.
+// diff_prefill.hip): rows fetched straight into LDS, their 16-byte chunks permuted so that the K
+// row reads and the V transpose reads are free of bank conflicts.
 #pragma once
 
 #include "nkv_common.h"

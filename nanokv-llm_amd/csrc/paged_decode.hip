@@ -277,8 +277,8 @@ static int decode_split(const void* q, int64_t q_row_stride, const void* k_cache
   const float scale_log2 = scale * k_scale * kLog2e;
   hipStream_t s = as_stream(stream);
 #define NKV_DECODE_LAUNCH(HP, D)                                                               \
-  hipLaunchKernelGGL((paged_decode_split_kernel<F8, HP, D, H16, DIFF>), dim3(p.grid), dim3(64), 0, s, \
-                     (const bf16_t*)q, q_row_stride, k_cache, v_cache, block_tables,           \
+  hipLaunchKernelGGL((paged_decode_split_kernel<F8, HP, D, H16, DIFF>), dim3(p.grid), dim3(64), \
+                     0, s, (const bf16_t*)q, q_row_stride, k_cache, v_cache, block_tables,     \
                      bt_row_stride, context_lens, batch, n_kv_heads, g, p.ncg, block_size,     \
                      max_blocks_per_seq, n_blocks, p.min_chunks, scale_log2, v_scale, part,    \
                      desc)

@@ -37,10 +37,10 @@ class PagedSequences:
     Lists are int32 tensors on the pool's device. An entry of -1 is padding, and a row named twice
     counts where it is named first. Pages are taken lowest first and in the list's order: an entry
     is carried out if it needs no page or the pages needed by all entries up to it are free before
-    the call, else it is refused and changes nothing. Each call returns a ``status`` (int32, 1: carried out, 0:
-    refused or padding). A row's last page, where it is filled in part, belongs to that row alone;
-    full pages may be shared, so code that writes rows in place (a compression step) needs a fork
-    made with ``share_pages=False``.
+    the call, else it is refused and changes nothing. Each call returns a ``status`` (int32, 1:
+    carried out, 0: refused or padding). A row's last page, where it is filled in part, belongs to
+    that row alone; full pages may be shared, so code that writes rows in place (a compression
+    step) needs a fork made with ``share_pages=False``.
 
     Calls run on the current stream of the pool's device and share the object's state and
     workspace: the caller orders calls of one object that it makes on several streams, captured

@@ -148,7 +148,7 @@ def test_workspace_sizes_follow_the_chip_not_the_lengths():
 
 
 def test_layer_refuses_another_geometry_than_its_own(monkeypatch):
-    """A cache or rows of other heads would be computed over the wrong pairs: before anything runs."""
+    """A cache or rows of other heads would be read over the wrong pairs: before anything runs."""
     nkv = importlib.import_module("nanokv-llm_amd")
 
     def launched(*a, **kw):
@@ -190,8 +190,8 @@ def test_layer_refuses_another_geometry_than_its_own(monkeypatch):
 
 
 def test_another_device_than_the_current_one(monkeypatch):
-    """Every launch, the store's too, and every size that depends on the chip are made with q's device
-    as the current one: a null stream belongs to that."""
+    """Every launch, the store's too, and every size that depends on the chip are made with q's
+    device as the current one: a null stream belongs to that."""
     nkv = importlib.import_module("nanokv-llm_amd")
     inside, seen = [], []
 

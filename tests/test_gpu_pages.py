@@ -411,8 +411,8 @@ def test_a_kept_state_taken_back_in_place(dev):
 
 
 def test_a_graph_replayed_after_its_object_is_dropped(dev):
-    """The plan's workspace stays the graph's: what is allocated afterwards keeps its contents, and the
-    replays go on with the state and pool that the caller holds."""
+    """The plan's workspace stays the graph's: what is allocated afterwards keeps its contents, and
+    the replays go on with the state and pool that the caller holds."""
     p = Pair(dev, rows=5)
     rows = ints([0, 2, 3], dev)
     p.append([0, 1, 2, 3], [14, 33, 1, 15])

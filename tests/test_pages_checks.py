@@ -218,8 +218,8 @@ def test_buffers_outlive_the_object_where_a_graph_captured_them(host_pool, monke
 
 
 def test_buffers_are_recorded_on_other_streams_than_their_own(host_pool, monkeypatch):
-    """Freed memory goes to its own stream's next allocation at once, so that what runs elsewhere has
-    to be known to the allocator: once a stream."""
+    """Freed memory goes to its own stream's next allocation at once, so that what runs elsewhere
+    has to be known to the allocator: once a stream."""
     recorded = []
 
     class Seen(torch.Tensor):
