@@ -833,6 +833,75 @@ int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info, 
                       void* stream);
 
 /*
+ * The block-scaled cache: 8-bit codes with a scale for every 32 tokens and head.
+ * It needs no calibration, and holds heads and tokens of any magnitude at E4M3's
+ * full precision. A cache is uint8 [n_blocks, block_size, n_kv_heads*head_dim +
+ * NKV_SCALED_ROW_PAD], block_size a multiple of 32; its rows stand in tiles of 32,
+ * a tile being the heads' codes (32*head_dim bytes each), then n_kv_heads scale
+ * bytes, the rest unused. A tile of a head holds code = E4M3(x * 2^-e) and the
+ * byte e + 127 (0: nothing written yet, which a new cache must be filled with).
+ * Within a head's codes:
+ *   K: byte ((t*(D/64) + i)*64 + r + 16*g)*16 + b is token 8*(r/4) + 4*t + r%4
+ *      (r < 16, t < 2), dim 64*i + 16*g + b
+ *   V: byte (j*64 + c + 16*g)*16 + 8*u + tt is token 8*g + tt, dim 32*j + 16*u + c
+ * head_dim D 64 or 128; q, k, v and outputs are bf16; caches 16-byte aligned.
+ * No counterpart in the reference (beside the pool of ModelRunner.
+ * allocate_kv_cache, nanokvllm/engine/model_runner.py:133-152).
+ */
+#define NKV_SCALED_ROW_PAD 16
+#define NKV_SCALED_MAX_HEADS 512
+
+/*
+ * New rows into a block-scaled cache: the slots, strides and skipped rows are
+ * nkv_store_kvcache's (rows and strides multiples of 8 elements, 16-byte aligned).
+ * Over the rows of a tile and head that the call writes, `need` is the smallest e
+ * in [-100, 119] with max |x| <= 448 * 2^e (the finite x's). If the tile's first
+ * row is among them the tile begins anew: e = need, and rows that the call does
+ * not write lose their values. Else e = max(e_old, need), and where that grows
+ * the other rows' codes become E4M3(code * 2^(e_old - e)). Rounding is to nearest
+ * even; larger values and infinities become +-448 * 2^e, NaN stays NaN.
+ * The tokens of a tile must stand next to each other in slot_mapping, in any
+ * order, as tokens listed sequence by sequence do (of two for one slot the later
+ * stays); what a tile holds whose tokens stand in two places is undefined.
+ */
+int nkv_scaled_store(const void* key, int64_t key_row_stride, const void* value,
+                     int64_t value_row_stride, void* k_cache, void* v_cache,
+                     const int32_t* slot_mapping, int64_t n_tokens, int32_t n_kv_heads,
+                     int32_t head_dim, int64_t n_slots, void* stream);
+
+/*
+ * Rows of a block-scaled cache as bf16 (exact: code * 2^e). Sequence i's tokens at
+ * positions starts[i] .. (NULL: 0 ..) become rows cu_seqlens[i] .. cu_seqlens[i+1]
+ * - 1 of k_out and v_out ([n_tokens, n_kv_heads, head_dim], contiguous, 16-byte
+ * aligned), nondecreasing from >= 0 to <= n_tokens; a sequence that reaches outside
+ * them is left out, and rows of no sequence stay as they were. Positions past the
+ * table or in an invalid block read as zeros. At most 2^20 sequences and 2^27
+ * tokens.
+ */
+int nkv_scaled_read(const void* k_cache, const void* v_cache, const int32_t* block_tables,
+                    int64_t bt_row_stride, int32_t max_blocks_per_seq, const int32_t* cu_seqlens,
+                    const int32_t* starts, int32_t n_seqs, int64_t n_tokens, int32_t n_kv_heads,
+                    int32_t head_dim, int32_t block_size, int64_t n_blocks, void* k_out,
+                    void* v_out, void* stream);
+
+/*
+ * Attention of one new token per sequence over block-scaled caches: the arguments
+ * and the workspace (nkv_paged_decode_workspace_bytes, 16-byte aligned) are
+ * nkv_paged_decode's; q rows are 16-byte aligned (stride a multiple of 8), out's
+ * stride is a multiple of 2. Any GQA group up to 256. A sequence of length 0, or
+ * none of whose blocks are valid, gives zeros; what a tile holds behind the
+ * sequence's end has no effect.
+ * No counterpart in the reference (beside nanokvllm/layers/attention.py:104-107).
+ */
+int nkv_scaled_decode(const void* q, int64_t q_row_stride, const void* k_cache,
+                      const void* v_cache, const int32_t* block_tables, int64_t bt_row_stride,
+                      const int32_t* context_lens, int32_t batch, int32_t n_q_heads,
+                      int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+                      int32_t max_blocks_per_seq, int64_t n_blocks, float scale, void* out,
+                      int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/*
  * Differential attention over the same caches. Heads stand in pairs: query
  * pair h (heads 2h, 2h+1 of q) reads KV pair p = h / (n_q_heads / n_kv_heads),
  * K heads 2p, 2p+1 and one value of 2*head_dim, V heads 2p and 2p+1 side by

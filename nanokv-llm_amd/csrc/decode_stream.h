@@ -55,6 +55,25 @@ static inline int32_t decode_min_chunks(int64_t max_chunks, int32_t floor) {
   return (int32_t)(c > floor ? c : floor);
 }
 
+// Waves per head group that full tables give ranges of kMinChunks (or more, see
+// decode_min_chunks).
+static inline int64_t decode_useful_waves(int32_t batch, int32_t max_blocks, int32_t block_size) {
+  const int64_t max_chunks = decode_max_chunks(max_blocks, block_size);
+  const int32_t min_chunks = decode_min_chunks(max_chunks, kMinChunks);
+  const int64_t waves = (batch * max_chunks + min_chunks - 1) / min_chunks;
+  return waves > 1 ? waves : 1;
+}
+// Bytes of the descriptors (one per sequence, KV head and column group; 16-byte aligned)
+// and of the partial rows a plan writes: each head group (waves + batch) x its columns,
+// i.e. (grid / head groups + batch) x Hq rows in all (grid * hp*g + batch * Hq for G <= 16;
+// at most grid * 16 + batch * Hq).
+static inline size_t decode_desc_bytes(int32_t batch, int32_t n_groups) {
+  return (size_t)batch * n_groups * sizeof(i32x4v_t);
+}
+static inline size_t decode_part_bytes(int64_t waves, int32_t batch, int32_t Hq, int32_t D) {
+  return (size_t)((waves + batch) * (int64_t)Hq) * part_row(D) * sizeof(float);
+}
+
 // Cursor over sequences in batches of 64 (one per lane): in the chunk stream
 // of one KV head, sequence s owns chunks [g_s, g_s + nc_s).
 struct SeqCursor {
@@ -92,16 +111,17 @@ struct OneRowSeqs {
   __device__ __forceinline__ int64_t row(int s) const { return cu_q[s]; }
 };
 
-// Chunks of a sequence of ctx keys.
+// Chunks (of CHUNK keys) of a sequence of ctx keys.
+template <int CHUNK = kChunk>
 __device__ __forceinline__ int seq_chunks(int ctx, int max_tokens) {
   NKV_DBG(ctx < 0 || ctx > max_tokens, NKV_DEBUG_LENGTH);
-  return ctx > 0 ? (min(ctx, max_tokens) + kChunk - 1) / kChunk : 0;
+  return ctx > 0 ? (min(ctx, max_tokens) + CHUNK - 1) / CHUNK : 0;
 }
-template <typename Seqs>
+template <int CHUNK = kChunk, typename Seqs>
 __device__ __forceinline__ void seq_load(SeqCursor& c, const Seqs& seqs, int max_tokens) {
   const int s = c.cb + (int)(threadIdx.x & 63);
   c.ctx = s < seqs.batch ? seqs.keys(s) : 0;
-  c.nc = seq_chunks(c.ctx, max_tokens);
+  c.nc = seq_chunks<CHUNK>(c.ctx, max_tokens);
   c.incl = wave_incl_scan(c.nc);
   c.tot = __builtin_amdgcn_readlane(c.incl, 63);
 }

@@ -169,14 +169,6 @@ struct DecodePlan {
   int32_t min_chunks;
 };
 
-// Waves per head group that full tables give ranges of kMinChunks (or more, see
-// decode_min_chunks).
-static int64_t decode_useful_waves(int32_t batch, int32_t max_blocks, int32_t block_size) {
-  const int64_t max_chunks = decode_max_chunks(max_blocks, block_size);
-  const int32_t min_chunks = decode_min_chunks(max_chunks, kMinChunks);
-  return std::max<int64_t>(1, (batch * max_chunks + min_chunks - 1) / min_chunks);
-}
-
 template <bool F8>
 static DecodePlan decode_plan(int32_t batch, int32_t Hq, int32_t Hk, int32_t max_blocks,
                               int32_t block_size, int32_t D) {
@@ -208,16 +200,6 @@ static DecodePlan decode_plan(int32_t batch, int32_t Hq, int32_t Hk, int32_t max
   return p;
 }
 
-// Bytes of the descriptors (one per sequence, KV head and column group; 16-byte aligned)
-// and of the partial rows a plan writes: each head group (waves + batch) x its columns,
-// i.e. (grid / head groups + batch) x Hq rows in all (grid * hp*g + batch * Hq for G <= 16;
-// at most grid * 16 + batch * Hq).
-static size_t decode_desc_bytes(int32_t batch, int32_t n_groups) {
-  return (size_t)batch * n_groups * sizeof(i32x4v_t);
-}
-static size_t decode_part_bytes(int64_t waves, int32_t batch, int32_t Hq, int32_t D) {
-  return (size_t)((waves + batch) * (int64_t)Hq) * part_row(D) * sizeof(float);
-}
 // Waves per head group of a plan.
 static int64_t decode_waves(const DecodePlan& p, int32_t Hk) {
   return (int64_t)p.grid / (Hk * p.ncg / p.hp);

@@ -1,0 +1,415 @@
+// The block-scaled K/V cache (scaled_cache.h): storing new rows into it and reading rows back.
+//
+// Reference: the store stands beside store_kvcache (nanokvllm/layers/attention.py:10-40), the cache
+// beside the pool of ModelRunner.allocate_kv_cache (nanokvllm/engine/model_runner.py:133-152), which
+// holds the model's dtype; reading back has no counterpart.
+//
+// A store takes a tile of a head at a time: over the rows that the call writes,
+//   need = scale of max |x|,    e = need               if the tile's first row is among them
+//                               e = max(e_old, need)   else, and where e grew the other rows' codes
+//                                                      become E4M3(code * 2^(e_old - e))
+//   code = E4M3(clamp(x * 2^-e, -448, 448)), to nearest even; NaN stays NaN.
+// MI355X design: one wave to a tile and 128 elements of its rows (a head of 128, two of 64), K and V
+// apart. Lane (x, y) holds dims 8x .. 8x+7 of tokens 8y .. 8y+7 in registers: one pass over the
+// memory for the maximum and the codes, and both orders of codes are packed from the block that the
+// lane holds (K's eight dims of a token, V's eight tokens of a dim), with no exchange. The tile's
+// owner is the wave whose token begins a run of tokens of that tile in slot_mapping.
+#include "scaled_cache.h"
+
+#include <algorithm>
+
+namespace nkv {
+
+constexpr int kScaledWaves = 4;  // of a workgroup: as many heads (or pairs), of K or V
+
+int scaled_check(const char* what, const void* k_cache, const void* v_cache, int32_t n_kv_heads,
+                 int32_t head_dim) {
+  NKV_REQUIRE(scaled_dim_ok(head_dim), NKV_EUNSUPPORTED, "%s: head_dim must be 64 or 128 (got %d)",
+              what, head_dim);
+  NKV_REQUIRE(n_kv_heads > 0 && n_kv_heads <= NKV_SCALED_MAX_HEADS, NKV_EUNSUPPORTED,
+              "%s: 1 to %d KV heads (got %d)", what, NKV_SCALED_MAX_HEADS, n_kv_heads);
+  NKV_REQUIRE(k_cache && v_cache && aligned16(k_cache) && aligned16(v_cache), NKV_EINVAL,
+              "%s: caches must be given, 16-byte aligned", what);
+  return NKV_OK;
+}
+
+// What a wave works on: 128 elements of a row of heads, of K or of V.
+template <int D>
+struct Unit {
+  static constexpr int kHeads = 128 / D;
+  static constexpr int kLanes = D / 8;  // of a head, eight dims each
+  int h0, head, hx, x, y;
+  bool is_v, live;
+  __device__ __forceinline__ Unit(int unit, int units, int Hk) {
+    const int lane = threadIdx.x & 63;
+    x = lane & 15;
+    y = lane >> 4;
+    is_v = unit >= units / 2;
+    h0 = (is_v ? unit - units / 2 : unit) * kHeads;
+    head = h0 + x / kLanes;
+    hx = x % kLanes;
+    live = head < Hk;
+  }
+};
+static int scaled_units(int Hk, int D) { return 2 * ((Hk * D + 127) / 128); }
+
+__device__ __forceinline__ uint32_t abs_max2(uint32_t m, uint32_t w) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                      __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+}
+__device__ __forceinline__ uint32_t drop_not_finite(uint32_t w) {
+  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+  return w;
+}
+
+// Two values to two codes in the low (or high) half of a word.
+template <bool HIGH, bool SPECIAL>
+__device__ __forceinline__ uint32_t put_codes(float a, float b, uint32_t old) {
+  if constexpr (SPECIAL) {
+    a = fp8_clamp(a);
+    b = fp8_clamp(b);
+  }
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, (int)old, HIGH);
+}
+
+// The codes of the lane's block into the head's tile. SPECIAL: there may be values past +-448 or
+// NaN among them. all: every row of the lane's eight is written.
+template <int D, bool SPECIAL>
+__device__ __forceinline__ void write_codes(const Unit<D>& un, const u32x4_t (&row)[8],
+                                            const int (&src)[8], bool all, float inv, char* tile) {
+  const auto value = [&](int k, int d) {
+    const uint32_t w = row[k][d >> 1];
+    return ((d & 1) ? bf16_hi(w) : bf16_lo(w)) * inv;
+  };
+  if (un.is_v) {
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      uint32_t c[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        c[h] = put_codes<false, SPECIAL>(value(4 * h, d), value(4 * h + 1, d), 0);
+        c[h] = put_codes<true, SPECIAL>(value(4 * h + 2, d), value(4 * h + 3, d), c[h]);
+      }
+      char* p = tile + v_piece(un.y, 8 * un.hx + d);
+      if (all) {
+        *reinterpret_cast<uint2*>(p) = uint2{c[0], c[1]};
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (src[k] >= 0) p[k] = (char)(c[k >> 2] >> (8 * (k & 3)));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint32_t c[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        c[h] = put_codes<false, SPECIAL>(value(k, 4 * h), value(k, 4 * h + 1), 0);
+        c[h] = put_codes<true, SPECIAL>(value(k, 4 * h + 2), value(k, 4 * h + 3), c[h]);
+      }
+      if (src[k] >= 0)
+        *reinterpret_cast<uint2*>(tile + k_piece<D>(8 * un.y + k, un.hx)) = uint2{c[0], c[1]};
+    }
+  }
+}
+
+// The codes of a tile's 128 elements (`heads` heads of them live) times 2^-(growth of their head).
+template <int D>
+__device__ __forceinline__ void rescale(char* codes, const int (&shrink)[2], int heads) {
+  constexpr int kPieces = kTileRows * D / 1024;  // of a head, 1 KiB each
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int h = 0; h < 128 / D; ++h) {
+    if (h >= heads || shrink[h] == 0) continue;  // uniform
+    const float f = __int_as_float((127 - min(shrink[h], 126)) << 23);
+    u32x4_t* p = reinterpret_cast<u32x4_t*>(codes + h * (kTileRows * D)) + lane;
+    u32x4_t w[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) w[i] = p[64 * i];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i][j], false);
+        const auto b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i][j], true);
+        uint32_t c = put_codes<false, false>(a[0] * f, a[1] * f, 0);
+        w[i][j] = put_codes<true, false>(b[0] * f, b[1] * f, c);
+      }
+      p[64 * i] = w[i];
+    }
+  }
+}
+
+// Workgroup (window, unit group): the runs that begin among tokens [w0, w0 + window).
+template <int D>
+__global__ __launch_bounds__(64 * kScaledWaves) void scaled_store_kernel(
+    const bf16_t* __restrict__ key, int64_t key_row_stride, const bf16_t* __restrict__ value,
+    int64_t value_row_stride, char* __restrict__ k_cache, char* __restrict__ v_cache,
+    const int32_t* __restrict__ slot_mapping, int64_t n_tokens, int32_t Hk, int64_t n_slots,
+    int32_t units, int32_t window) {
+  __shared__ int32_t rows[kScaledWaves][kTileRows];  // the token of each row of the tile, or -1
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int unit = blockIdx.y * kScaledWaves + wave;
+  if (unit >= units) return;
+  const Unit<D> un(unit, units, Hk);
+  const bf16_t* src = un.is_v ? value : key;
+  const int64_t stride = un.is_v ? value_row_stride : key_row_stride;
+  char* cache = un.is_v ? v_cache : k_cache;
+  const int64_t tile_bytes = (int64_t)kTileRows * (Hk * D + kRowPad);
+
+  const auto tile_of = [&](int64_t t) -> int {
+    if (t < 0 || t >= n_tokens) return -1;
+    const int64_t s = slot_mapping[t];
+    NKV_DBG(s < -1 || s >= n_slots, NKV_DEBUG_SLOT);
+    return s >= 0 && s < n_slots ? (int)(s / kTileRows) : -1;
+  };
+  const int64_t w0 = (int64_t)blockIdx.x * window;
+  const int mine = lane < window ? tile_of(w0 + lane) : -1;
+  int before = __shfl_up(mine, 1, 64);
+  if (lane == 0) before = tile_of(w0 - 1);
+  uint64_t begins = __ballot(mine >= 0 && mine != before);
+
+  for (; begins; begins &= begins - 1) {
+    const int ln = __builtin_ctzll(begins);
+    const int64_t t0 = w0 + ln;
+    const int tile = __builtin_amdgcn_readlane(mine, ln);
+    // the run's tokens by row; of two for a row the later one stays
+    if (lane < kTileRows) rows[wave][lane] = -1;
+    __builtin_amdgcn_wave_barrier();
+    for (int64_t at = t0;; at += 64) {
+      const bool in = tile_of(at + lane) == tile;
+      const uint64_t out = ~__ballot(in);
+      const int n = out ? __builtin_ctzll(out) : 64;
+      if (lane < n) atomicMax(&rows[wave][slot_mapping[at + lane] % kTileRows], (int)(at + lane));
+      if (n < 64) break;
+    }
+    __builtin_amdgcn_wave_barrier();
+    int from[8];
+    bool all = true;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      from[k] = rows[wave][8 * un.y + k];
+      all = all && from[k] >= 0;
+    }
+    const bool first = rows[wave][0] >= 0;
+    __builtin_amdgcn_wave_barrier();
+    char* base = cache + tile * tile_bytes;
+    char* scales = base + kTileRows * Hk * D;
+    const int old = un.live ? stored_scale((uint8_t)scales[un.head]) : kMinScale;
+    u32x4_t row[8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      row[k] = u32x4_t{0, 0, 0, 0};
+      if (from[k] >= 0 && un.live)
+        row[k] = *reinterpret_cast<const u32x4_t*>(src + from[k] * stride + un.h0 * D + 8 * un.x);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) m = abs_max2(m, row[k][w]);
+    uint32_t a = max(m & 0xffffu, m >> 16);
+    bool special = __ballot(a >= 0x7f80u) != 0;
+    if (special) {
+      m = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) m = abs_max2(m, drop_not_finite(row[k][w]));
+      a = max(m & 0xffffu, m >> 16);
+    }
+    // over the head's lanes and the four groups of tokens
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+      if (o < Unit<D>::kLanes || o >= 16) a = max(a, (uint32_t)__shfl_xor((int)a, o, 64));
+    const int need = scale_byte(__uint_as_float(a << 16));
+    const int e = first ? need : max(old, need);
+    special = special || __ballot(e == kMaxScale) != 0;
+    char* codes = base + un.h0 * (kTileRows * D);
+    if (!first) {
+      const int grown = e - old;
+      if (__ballot(un.live && grown > 0)) {
+        const int shrink[2] = {__builtin_amdgcn_readlane(grown, 0),
+                               __builtin_amdgcn_readlane(grown, Unit<D>::kLanes % 16)};
+        rescale<D>(codes, shrink, min(Unit<D>::kHeads, Hk - un.h0));
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // other lanes' bytes go into those words
+      }
+    }
+    if (un.live) {
+      char* to = base + un.head * (kTileRows * D);
+      if (special) write_codes<D, true>(un, row, from, all, inverse_scale(e), to);
+      else write_codes<D, false>(un, row, from, all, inverse_scale(e), to);
+      if (un.y == 0 && un.hx == 0) scales[un.head] = (char)e;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- reading back
+// Workgroup (tile, unit group): a tile of what sequence i holds at positions [start, start + n), n its
+// share of cu_seqlens. Every workgroup finds its sequence and tile itself.
+template <int D>
+__global__ __launch_bounds__(64 * kScaledWaves) void scaled_read_kernel(
+    const char* __restrict__ k_cache, const char* __restrict__ v_cache,
+    const int32_t* __restrict__ block_tables, int64_t bt_row_stride,
+    const int32_t* __restrict__ cu_seqlens, const int32_t* __restrict__ starts, int32_t n_seqs,
+    int64_t n_tokens, int32_t Hk, int32_t block_size, int32_t max_blocks, int64_t n_blocks,
+    int32_t units, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int unit = blockIdx.y * kScaledWaves + wave;
+  if (unit >= units) return;
+  const Unit<D> un(unit, units, Hk);
+
+  // the sequence that holds tile blockIdx.x of all of them
+  int cb = 0, base = 0, at = 0, n = 0, start = 0, tiles = 0, incl = 0;
+  for (;; cb += 64) {
+    if (cb >= n_seqs) return;
+    const int s = cb + lane;
+    n = start = tiles = 0;
+    if (s < n_seqs) {
+      at = cu_seqlens[s];
+      n = cu_seqlens[s + 1] - at;
+      start = starts ? starts[s] : 0;
+      // rows outside the outputs or of no position: none (the grid counts n_tokens rows)
+      const bool ok = at >= 0 && n > 0 && start >= 0 && (int64_t)at + n <= n_tokens &&
+                      (int64_t)start + n <= INT32_MAX;
+      NKV_DBG(!ok && n != 0, NKV_DEBUG_LENGTH);
+      if (!ok) n = 0;
+      if (n > 0) tiles = (start + n - 1) / kTileRows - start / kTileRows + 1;
+    }
+    incl = wave_incl_scan(tiles);
+    const int tot = __builtin_amdgcn_readlane(incl, 63);
+    if ((int)blockIdx.x < base + tot) break;
+    base += tot;
+  }
+  const int ln = __builtin_ctzll(__ballot(base + incl > (int)blockIdx.x));
+  at = __builtin_amdgcn_readlane(at, ln);
+  n = __builtin_amdgcn_readlane(n, ln);
+  start = __builtin_amdgcn_readlane(start, ln);
+  const int first = base + __builtin_amdgcn_readlane(incl - tiles, ln);
+  const int t0 = (start / kTileRows + (int)blockIdx.x - first) * kTileRows;  // the tile's position
+  const int bi = t0 / block_size;
+  const int id = bi < max_blocks ? block_tables[(int64_t)(cb + ln) * bt_row_stride + bi] : -1;
+  const bool valid = id >= 0 && id < n_blocks;
+  NKV_DBG(!valid, bi < max_blocks ? NKV_DEBUG_BLOCK : NKV_DEBUG_LENGTH);
+  if (!un.live) return;
+
+  u32x4_t row[8] = {};  // of token 8 y + k: dims 8 hx .. + 7
+  if (valid) {
+    const char* tile = (un.is_v ? v_cache : k_cache) +
+                       ((int64_t)id * (block_size / kTileRows) + t0 % block_size / kTileRows) *
+                           (kTileRows * (int64_t)(Hk * D + kRowPad));
+    const float scale = scale_of(stored_scale((uint8_t)tile[kTileRows * Hk * D + un.head]));
+    const char* codes = tile + un.head * (kTileRows * D);
+    uint2 c[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      c[k] = *reinterpret_cast<const uint2*>(
+          codes + (un.is_v ? v_piece(un.y, 8 * un.hx + k) : k_piece<D>(8 * un.y + k, un.hx)));
+    u32x4_t w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = codes_to_bf16(c[k].x, c[k].y, scale);
+    if (un.is_v) {  // w[d]: eight tokens of dim d
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int d = 0; d < 8; d += 2)
+          row[k][d / 2] = __builtin_amdgcn_perm(w[d + 1][k / 2], w[d][k / 2],
+                                                (k & 1) ? 0x07060302u : 0x05040100u);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) row[k] = w[k];
+    }
+  }
+  bf16_t* out = (un.is_v ? v_out : k_out) + un.h0 * D + 8 * un.x;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int j = t0 + 8 * un.y + k - start;
+    if (j >= 0 && j < n)
+      __builtin_nontemporal_store(
+          row[k], reinterpret_cast<u32x4_t*>(out + ((int64_t)at + j) * Hk * D));
+  }
+}
+
+}  // namespace nkv
+
+extern "C" int nkv_scaled_store(const void* key, int64_t key_row_stride, const void* value,
+                                int64_t value_row_stride, void* k_cache, void* v_cache,
+                                const int32_t* slot_mapping, int64_t n_tokens, int32_t n_kv_heads,
+                                int32_t head_dim, int64_t n_slots, void* stream) {
+  using namespace nkv;
+  clear_error();
+  NKV_REQUIRE(n_tokens >= 0 && n_tokens < (1ll << 31) && n_slots >= 0, NKV_EINVAL,
+              "scaled_store: bad sizes (%lld tokens, %lld slots)", (long long)n_tokens,
+              (long long)n_slots);
+  if (n_tokens == 0) return NKV_OK;
+  const int rc = scaled_check("scaled_store", k_cache, v_cache, n_kv_heads, head_dim);
+  if (rc) return rc;
+  const int64_t row = (int64_t)n_kv_heads * head_dim;
+  NKV_REQUIRE(n_slots % kTileRows == 0, NKV_EINVAL,
+              "scaled_store: the slots must be whole tiles of %d (got %lld)", kTileRows,
+              (long long)n_slots);
+  NKV_REQUIRE(key && value && slot_mapping && aligned16(key) && aligned16(value), NKV_EINVAL,
+              "scaled_store: null or misaligned pointer");
+  NKV_REQUIRE(key_row_stride >= row && value_row_stride >= row && key_row_stride % 8 == 0 &&
+                  value_row_stride % 8 == 0,
+              NKV_EINVAL, "scaled_store: row strides must be multiples of 8 covering the row");
+  const int units = scaled_units(n_kv_heads, head_dim);
+  const int window = n_tokens * units <= 8192 ? 1 : 8;
+  const dim3 grid((unsigned)((n_tokens + window - 1) / window),
+                  (unsigned)((units + kScaledWaves - 1) / kScaledWaves));
+#define NKV_SCALED_STORE(D)                                                                     \
+  hipLaunchKernelGGL((scaled_store_kernel<D>), grid, dim3(64 * kScaledWaves), 0,                \
+                     as_stream(stream), (const bf16_t*)key, key_row_stride,                     \
+                     (const bf16_t*)value, value_row_stride, (char*)k_cache, (char*)v_cache,    \
+                     slot_mapping, n_tokens, n_kv_heads, n_slots, units, window)
+  if (head_dim == 64) NKV_SCALED_STORE(64);
+  else NKV_SCALED_STORE(128);
+#undef NKV_SCALED_STORE
+  return check_launch("nkv_scaled_store");
+}
+
+extern "C" int nkv_scaled_read(const void* k_cache, const void* v_cache,
+                               const int32_t* block_tables, int64_t bt_row_stride,
+                               int32_t max_blocks_per_seq, const int32_t* cu_seqlens,
+                               const int32_t* starts, int32_t n_seqs, int64_t n_tokens,
+                               int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+                               int64_t n_blocks, void* k_out, void* v_out, void* stream) {
+  using namespace nkv;
+  clear_error();
+  NKV_REQUIRE(n_seqs >= 0 && n_tokens >= 0 && n_blocks >= 0, NKV_EINVAL,
+              "scaled_read: bad sizes (%d sequences, %lld tokens)", n_seqs, (long long)n_tokens);
+  // 64 sequences' tiles add up within 32 bits, whatever cu_seqlens holds
+  NKV_REQUIRE(n_seqs <= (1 << 20) && n_tokens <= (1 << 27), NKV_EUNSUPPORTED,
+              "scaled_read: at most 2^20 sequences and 2^27 tokens (got %d, %lld)", n_seqs,
+              (long long)n_tokens);
+  if (n_seqs == 0 || n_tokens == 0) return NKV_OK;
+  const int rc = scaled_check("scaled_read", k_cache, v_cache, n_kv_heads, head_dim);
+  if (rc) return rc;
+  NKV_REQUIRE(block_size > 0 && block_size % kTileRows == 0, NKV_EUNSUPPORTED,
+              "scaled_read: block_size must be a multiple of %d (got %d)", kTileRows, block_size);
+  NKV_REQUIRE(max_blocks_per_seq > 0 && bt_row_stride >= max_blocks_per_seq, NKV_EINVAL,
+              "scaled_read: bad block table width/stride (%d, %lld)", max_blocks_per_seq,
+              (long long)bt_row_stride);
+  NKV_REQUIRE(block_tables && cu_seqlens && k_out && v_out && aligned16(k_out) && aligned16(v_out),
+              NKV_EINVAL, "scaled_read: null or misaligned pointer");
+  const int units = scaled_units(n_kv_heads, head_dim);
+  // n rows reach into at most n / 32 + 2 tiles
+  const int64_t tiles = n_tokens / kTileRows + 2 * std::min<int64_t>(n_seqs, n_tokens);
+  const dim3 grid((unsigned)tiles, (unsigned)((units + kScaledWaves - 1) / kScaledWaves));
+#define NKV_SCALED_READ(D)                                                                      \
+  hipLaunchKernelGGL((scaled_read_kernel<D>), grid, dim3(64 * kScaledWaves), 0,                 \
+                     as_stream(stream), (const char*)k_cache, (const char*)v_cache,             \
+                     block_tables, bt_row_stride, cu_seqlens, starts, n_seqs, n_tokens,         \
+                     n_kv_heads, block_size, max_blocks_per_seq, n_blocks, units,               \
+                     (bf16_t*)k_out, (bf16_t*)v_out)
+  if (head_dim == 64) NKV_SCALED_READ(64);
+  else NKV_SCALED_READ(128);
+#undef NKV_SCALED_READ
+  return check_launch("nkv_scaled_read");
+}
