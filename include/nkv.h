@@ -902,6 +902,32 @@ int nkv_scaled_decode(const void* q, int64_t q_row_stride, const void* k_cache,
                       void* stream);
 
 /*
+ * Varlen causal (bottom-right) attention over block-scaled caches: the arguments
+ * are nkv_prefill_varlen's with block tables; total_q are q's rows, max_seqlen_k
+ * the longest sequence's keys. Given a workspace of
+ * nkv_scaled_prefill_workspace_bytes(...) (16-byte aligned; 0: none is of use),
+ * the keys are split over the chip where few query tiles would leave it idle. q
+ * rows are 16-byte aligned (stride a multiple of 8), out's 8-byte (of 4). Any GQA
+ * group up to NKV_SCALED_MAX_GROUP. A row that sees no key gives zeros, rows of no
+ * sequence stay as they were; keys past the table or in an invalid block are
+ * zeros, and keys that a row does not see have no effect on it, whatever they
+ * hold.
+ * No counterpart in the reference (beside nanokvllm/layers/attention.py:96-102).
+ */
+#define NKV_SCALED_MAX_GROUP 128
+size_t nkv_scaled_prefill_workspace_bytes(int32_t n_seqs, int64_t total_q, int64_t max_seqlen_q,
+                                          int64_t max_seqlen_k, int32_t n_q_heads,
+                                          int32_t n_kv_heads, int32_t head_dim);
+int nkv_scaled_prefill(const void* q, int64_t q_row_stride, int64_t total_q, const void* k_cache,
+                       const void* v_cache, const int32_t* cu_seqlens_q,
+                       const int32_t* cu_seqlens_k, const int32_t* block_tables,
+                       int64_t bt_row_stride, int32_t max_blocks_per_seq, int32_t n_seqs,
+                       int64_t max_seqlen_q, int64_t max_seqlen_k, int32_t n_q_heads,
+                       int32_t n_kv_heads, int32_t head_dim, int32_t block_size, int64_t n_blocks,
+                       float scale, void* out, int64_t out_row_stride, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/*
  * Differential attention over the same caches. Heads stand in pairs: query
  * pair h (heads 2h, 2h+1 of q) reads KV pair p = h / (n_q_heads / n_kv_heads),
  * K heads 2p, 2p+1 and one value of 2*head_dim, V heads 2p and 2p+1 side by

@@ -182,3 +182,61 @@ def scaled_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     if rc:
         _lib.check(rc, what)
     return out
+
+
+def scaled_prefill_workspace(q: torch.Tensor, k_cache: torch.Tensor, n_seqs: int,
+                             max_seqlen_q: int, max_seqlen_k: int) -> torch.Tensor | None:
+    """The workspace for splitting scaled_varlen_prefill's keys where few query tiles would leave the
+    chip idle, else None; None too where the device has no such memory left, since nothing else
+    needs any."""
+    D = q.size(2)
+    nbytes = _lib.lib().nkv_scaled_prefill_workspace_bytes(
+        n_seqs, q.size(0), int(max_seqlen_q), int(max_seqlen_k), q.size(1),
+        _kv_heads("scaled_varlen_prefill", k_cache, D), D)
+    try:
+        return torch.empty(nbytes, dtype=_U8, device=q.device) if nbytes else None
+    except torch.OutOfMemoryError:
+        return None
+
+
+def scaled_varlen_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                          cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor,
+                          max_seqlen_q: int, scale: float, block_tables: torch.Tensor,
+                          out: torch.Tensor | None = None, max_seqlen_k: int | None = None,
+                          workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Varlen causal (bottom-right) attention: q [sum Lq, Hq, D] -> [sum Lq, Hq, D] (bf16).
+
+    The arguments are ``varlen_prefill``'s with block tables. Given ``max_seqlen_k``, the keys are split
+    over the chip where few tiles would leave it idle, in ``workspace`` (scaled_prefill_workspace) or
+    in memory taken for the call; without, nothing but the output is allocated. A row that sees no
+    key gives zeros; what keys hold that a row does not see has no effect on it.
+    """
+    what = "scaled_varlen_prefill"
+    _lib.require_device(q.device, k_cache=k_cache, v_cache=v_cache, cu_seqlens_q=cu_seqlens_q,
+                        cu_seqlens_k=cu_seqlens_k, block_tables=block_tables, out=out,
+                        workspace=workspace)
+    _rows(what, "q", q)
+    N, Hq, D = q.shape
+    Hk = _kv_heads(what, k_cache, D)
+    NB, B = _caches(what, k_cache, v_cache, Hk * D)
+    n_seqs = cu_seqlens_q.numel() - 1
+    if n_seqs < 0 or cu_seqlens_k.numel() != n_seqs + 1:
+        raise ValueError(f"{what}: cu_seqlens_q and cu_seqlens_k need one entry per sequence + 1")
+    _int32(what, "cu_seqlens_q", cu_seqlens_q, n_seqs + 1)
+    _int32(what, "cu_seqlens_k", cu_seqlens_k, n_seqs + 1)
+    _int32(what, "block_tables", block_tables, n_seqs, 2)
+    _workspace_ok(what, workspace)
+    out = _out(what, q, out)
+    with _lib.device_of(q.get_device()):
+        if workspace is None and max_seqlen_k is not None:
+            workspace = scaled_prefill_workspace(q, k_cache, n_seqs, max_seqlen_q, max_seqlen_k)
+        rc = _lib.lib().nkv_scaled_prefill(
+            q.data_ptr(), q.stride(0), N, k_cache.data_ptr(), v_cache.data_ptr(),
+            cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), block_tables.data_ptr(),
+            block_tables.stride(0), block_tables.size(1), n_seqs, int(max_seqlen_q),
+            0 if max_seqlen_k is None else int(max_seqlen_k), Hq, Hk, D, B, NB, scale,
+            out.data_ptr(), out.stride(0), _lib.ptr(workspace),
+            0 if workspace is None else workspace.numel(), _lib.stream_of(q))
+    if rc:
+        _lib.check(rc, what)
+    return out
