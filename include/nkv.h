@@ -822,6 +822,18 @@ int nkv_pages_fork(const nkv_pages* pages, const int32_t* parents, const int32_t
                    int32_t n, int32_t share_pages, int32_t* status, void* stream);
 
 /*
+ * The same over a pool of block-scaled caches (nkv_scaled_store), whose pages are
+ * tiles of 32 rows: of the last tile that a copy reaches into, all is copied.
+ * row_bytes is n_kv_heads*head_dim + NKV_SCALED_ROW_PAD, block_size a multiple of
+ * 32. nkv_pages_append and nkv_pages_compact take such a pool as they are.
+ */
+int nkv_scaled_pages_truncate(const nkv_pages* pages, const int32_t* rows,
+                              const int32_t* keep_lens, int32_t n, const int32_t* page_ids,
+                              int64_t n_page_ids, int32_t* status, void* stream);
+int nkv_scaled_pages_fork(const nkv_pages* pages, const int32_t* parents, const int32_t* children,
+                          int32_t n, int32_t share_pages, int32_t* status, void* stream);
+
+/*
  * Moves pages in use to the pool's lower end: with n_live pages in use, the
  * k-th lowest free page below n_live takes the k-th highest page in use, for
  * the first max_moves of them; all tables and counts follow. info[0] = n_live,

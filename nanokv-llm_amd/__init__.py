@@ -13,8 +13,8 @@ from .layers.CompressMethod import SnapKV
 from .layers.diff_attention import (DifferentialAttention, diff_paged_decode,
                                     diff_varlen_prefill, lambda_init_of)
 from .layers.rotary_embedding import RotaryEmbedding, get_rope, qk_norm_rope_store
-from .layers.scaled_cache import (scaled_paged_decode, scaled_read_kvcache, scaled_store_kvcache,
-                                  scaled_varlen_prefill)
+from .layers.scaled_cache import (ScaledKVCachePool, scaled_paged_decode, scaled_read_kvcache,
+                                  scaled_store_kvcache, scaled_varlen_prefill)
 from .utils.context import Context, get_context, set_context, reset_context
 
 __all__ = [
@@ -23,7 +23,7 @@ __all__ = [
     "MyCompressCompact",
     "SnapKV", "Context", "get_context", "set_context", "reset_context", "RotaryEmbedding",
     "get_rope", "qk_norm_rope_store", "PagedSequences",
-    "scaled_store_kvcache", "scaled_read_kvcache", "scaled_paged_decode",
+    "ScaledKVCachePool", "scaled_store_kvcache", "scaled_read_kvcache", "scaled_paged_decode",
     "scaled_varlen_prefill",
     "DifferentialAttention", "diff_paged_decode", "diff_varlen_prefill", "lambda_init_of",
 ]

@@ -149,6 +149,8 @@ SIGNATURES = {
     "nkv_pages_append": (C.c_int, [C.c_char_p, _p, _i32, _p, _i64, _p, _p, _p]),
     "nkv_pages_truncate": (C.c_int, [C.c_char_p, _p, _p, _i32, _p, _i64, _p, _p]),
     "nkv_pages_fork": (C.c_int, [C.c_char_p, _p, _p, _i32, _i32, _p, _p]),
+    "nkv_scaled_pages_truncate": (C.c_int, [C.c_char_p, _p, _p, _i32, _p, _i64, _p, _p]),
+    "nkv_scaled_pages_fork": (C.c_int, [C.c_char_p, _p, _p, _i32, _i32, _p, _p]),
     "nkv_pages_compact": (C.c_int, [C.c_char_p, _i32, _p, _p, _p]),
 }
 

@@ -543,6 +543,25 @@ __global__ __launch_bounds__(kCopyThreads) void pages_apply_kernel(
   }
 }
 
+// A block-scaled pool's page is tiles of 32 rows' bytes, codes and scales not row by row: of a tile that
+// a copy's last row cuts, what the copies above left out (at most 31 rows' bytes, scales among them).
+constexpr int kScaledTile = 32;
+__global__ __launch_bounds__(kCopyThreads) void pages_tails_kernel(const PagesArgs a) {
+  const int n_copies = a.head->n_copies;
+  const int64_t page_bytes = (int64_t)a.B * a.row_bytes;
+  char* plane = a.kv + (int64_t)blockIdx.y * a.n_pages * page_bytes;
+  for (int k = blockIdx.x; k < n_copies; k += gridDim.x) {
+    const i32x4w_t c = a.copies[k];
+    if (c[2] % kScaledTile == 0 || !page_ok(a, c[0])) continue;
+    const int64_t from = (int64_t)c[2] * a.row_bytes;
+    const int64_t to = (int64_t)(c[2] / kScaledTile + 1) * kScaledTile * a.row_bytes;
+    const char* src = plane + c[0] * page_bytes;
+    char* dst = plane + c[1] * page_bytes;
+    for (int64_t o = from + (int)threadIdx.x * 16; o < to; o += kCopyThreads * 16)
+      *reinterpret_cast<u32x4_t*>(dst + o) = *reinterpret_cast<const u32x4_t*>(src + o);
+  }
+}
+
 static int pages_check(const nkv_pages* p, const char* what, PagesArgs& a) {
   NKV_REQUIRE(p, NKV_EINVAL, "%s: null arguments", what);
   NKV_REQUIRE(p->n_planes > 0 && p->n_pages > 0 && p->block_size > 0 && p->row_bytes > 0 &&
@@ -601,6 +620,23 @@ static int pages_apply(const PagesArgs& a, int32_t n, const int32_t* loose, int3
                      dim3((unsigned)(books + groups), (unsigned)a.n_planes), dim3(kCopyThreads),
                      0, as_stream(stream), a, n, loose, n_loose, share, books);
   return check_launch("nkv_pages");
+}
+
+// After a call that left a plan of at most `copies` copies in the workspace.
+static int pages_tails(const nkv_pages* pages, int64_t copies, void* stream) {
+  PagesArgs a;
+  const int rc = pages_check(pages, "scaled_pages", a);
+  if (rc) return rc;
+  const int64_t groups =
+      std::max<int64_t>(1, std::min<int64_t>(copies, std::max(1, kCopyGroups / a.n_planes)));
+  hipLaunchKernelGGL(pages_tails_kernel, dim3((unsigned)groups, (unsigned)a.n_planes),
+                     dim3(kCopyThreads), 0, as_stream(stream), a);
+  return check_launch("nkv_scaled_pages");
+}
+static int scaled_pages_check(const nkv_pages* p) {
+  NKV_REQUIRE(p && p->block_size % kScaledTile == 0, NKV_EUNSUPPORTED,
+              "scaled_pages: block_size must be a multiple of %d", kScaledTile);
+  return NKV_OK;
 }
 
 }  // namespace nkv
@@ -681,6 +717,28 @@ extern "C" int nkv_pages_fork(const nkv_pages* pages, const int32_t* parents,
                             share_pages ? n
                                         : std::min<int64_t>(a.n_pages, (int64_t)n * a.max_blocks),
                             stream);
+}
+
+extern "C" int nkv_scaled_pages_truncate(const nkv_pages* pages, const int32_t* rows,
+                                         const int32_t* keep_lens, int32_t n,
+                                         const int32_t* page_ids, int64_t n_page_ids,
+                                         int32_t* status, void* stream) {
+  nkv::clear_error();
+  int rc = nkv::scaled_pages_check(pages);
+  if (rc) return rc;
+  rc = nkv_pages_truncate(pages, rows, keep_lens, n, page_ids, n_page_ids, status, stream);
+  // without rows there is no copy, and without a launch no plan of this call's
+  return rc || n == 0 ? rc : nkv::pages_tails(pages, n, stream);
+}
+
+extern "C" int nkv_scaled_pages_fork(const nkv_pages* pages, const int32_t* parents,
+                                     const int32_t* children, int32_t n, int32_t share_pages,
+                                     int32_t* status, void* stream) {
+  nkv::clear_error();
+  int rc = nkv::scaled_pages_check(pages);
+  if (rc) return rc;
+  rc = nkv_pages_fork(pages, parents, children, n, share_pages, status, stream);
+  return rc || n == 0 ? rc : nkv::pages_tails(pages, n, stream);
 }
 
 extern "C" int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info,

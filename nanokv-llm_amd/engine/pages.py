@@ -19,6 +19,7 @@ import torch
 from .. import _lib
 from ..layers import attention
 from ..layers.kv_cache import KVCachePool
+from ..layers.scaled_cache import TILE, ScaledKVCachePool
 
 _PAGES = struct.Struct("13q")  # nkv_pages
 _I32 = torch.int32
@@ -26,7 +27,9 @@ _I32 = torch.int32
 
 class PagedSequences:
     """Up to ``max_seqs`` rows of at most ``max_blocks_per_seq`` pages each over ``kv_cache``, a
-    ``KVCachePool`` or its tensor [2, layers, pages, block_size, Hk, D].
+    ``KVCachePool`` or its tensor [2, layers, pages, block_size, Hk, D], or a ``ScaledKVCachePool`` or
+    its tensor (uint8 [2, layers, pages, block_size, row]; a copy of part of a page then brings whole
+    tiles, their scales among them).
 
     ``state`` is one int32 buffer [pages + max_seqs + max_seqs * max_blocks_per_seq]: the reference
     counts, the lengths (``context_lens``) and the tables (``block_tables``, -1 past a row's
@@ -49,16 +52,20 @@ class PagedSequences:
     ``release_retired_decode_workspaces()``.
     """
 
-    def __init__(self, kv_cache: torch.Tensor | KVCachePool, max_seqs: int,
+    def __init__(self, kv_cache: torch.Tensor | KVCachePool | ScaledKVCachePool, max_seqs: int,
                  max_blocks_per_seq: int, state: torch.Tensor | None = None):
-        kv = kv_cache.kv_cache if isinstance(kv_cache, KVCachePool) else kv_cache
-        if kv.dim() != 6 or kv.size(0) != 2 or not kv.is_contiguous():
+        kv = kv_cache.kv_cache if isinstance(kv_cache, (KVCachePool, ScaledKVCachePool)) else kv_cache
+        self._scaled = kv.dim() == 5 and kv.dtype is torch.uint8
+        if self._scaled and kv.size(3) % TILE:
+            raise ValueError(f"PagedSequences: block_size {kv.size(3)} of a block-scaled pool is not "
+                             f"a multiple of {TILE}")
+        if kv.dim() != (5 if self._scaled else 6) or kv.size(0) != 2 or not kv.is_contiguous():
             raise ValueError("PagedSequences: the pool must be contiguous [2, layers, pages, "
                              f"block_size, Hk, D], got {tuple(kv.shape)}")
         _lib.require_device(kv.device, state=state)
         if max_seqs <= 0 or max_blocks_per_seq <= 0:
             raise ValueError("PagedSequences: max_seqs and max_blocks_per_seq must be > 0")
-        _, layers, pages, block, heads, dim = kv.shape
+        _, layers, pages, block = kv.shape[:4]
         n = pages + max_seqs + max_seqs * max_blocks_per_seq
         if state is None:
             state = torch.zeros(n, dtype=_I32, device=kv.device)
@@ -77,7 +84,7 @@ class PagedSequences:
         self._captured = False
         at = state.data_ptr()
         self._args = _PAGES.pack(kv.data_ptr(), 2 * layers, pages, block,
-                                 heads * dim * kv.element_size(), at, at + 4 * pages,
+                                 kv.stride(3) * kv.element_size(), at, at + 4 * pages,
                                  at + 4 * (pages + max_seqs), max_blocks_per_seq,
                                  max_blocks_per_seq, max_seqs, self._workspace.data_ptr(), nbytes)
 
@@ -170,7 +177,8 @@ class PagedSequences:
         self._list("truncate: lens", lens, n)
         m = 0 if pages is None else self._list("truncate: pages", pages)
         status = rows.new_empty(n)
-        self._call(_lib.lib().nkv_pages_truncate, "truncate", rows.data_ptr(), lens.data_ptr(), n,
+        fn = _lib.lib().nkv_scaled_pages_truncate if self._scaled else _lib.lib().nkv_pages_truncate
+        self._call(fn, "truncate", rows.data_ptr(), lens.data_ptr(), n,
                    pages.data_ptr() if m else None, m, status.data_ptr())
         return status
 
@@ -182,7 +190,8 @@ class PagedSequences:
         n = self._list("fork: parents", parents)
         self._list("fork: children", children, n)
         status = parents.new_empty(n)
-        self._call(_lib.lib().nkv_pages_fork, "fork", parents.data_ptr(), children.data_ptr(), n,
+        fn = _lib.lib().nkv_scaled_pages_fork if self._scaled else _lib.lib().nkv_pages_fork
+        self._call(fn, "fork", parents.data_ptr(), children.data_ptr(), n,
                    1 if share_pages else 0, status.data_ptr())
         return status
 

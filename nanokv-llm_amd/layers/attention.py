@@ -16,11 +16,14 @@ from torch import nn
 from .. import _lib
 from ..utils.context import get_context
 from .compress_utils import MyCompressCompact
+from .scaled_cache import (ROW_PAD, TILE, scaled_paged_decode, scaled_store_kvcache,
+                           scaled_varlen_prefill)
 
 _BF16 = torch.bfloat16
 _F16 = torch.float16
 _FP8 = torch.float8_e4m3fn
 _I32 = torch.int32
+_U8 = torch.uint8  # block-scaled caches (scaled_cache.py)
 _ATTENTION_ARGS = struct.Struct("29q3d")  # nkv_attention_args
 
 
@@ -384,6 +387,10 @@ class Attention(nn.Module):
         key = (kc.data_ptr(), tuple(kc.shape))
         if self._cache_checked == key:
             return
+        if kc.dtype is _U8:
+            self._check_scaled_cache()
+            self._cache_checked = key
+            return
         _lib.need(kc.dim() == 4 and kc.size(2) == self.num_kv_heads and
                   kc.size(3) == self.head_dim,
                   f"Attention: k_cache must be [blocks, block_size, {self.num_kv_heads}, "
@@ -401,6 +408,34 @@ class Attention(nn.Module):
             # keep >= Lw is the reference's no-op (SnapKV returns False, CompressMethod.py:17-18)
             _lib.need(keep > 2, f"Attention: {keep} kept tokens (bos, selected, latest: > 2)")
         self._cache_checked = key
+
+    def _check_scaled_cache(self):
+        kc, row = self.k_cache, self.num_kv_heads * self.head_dim + ROW_PAD
+        _lib.need(self.head_dim in (64, 128), f"Attention: head_dim {self.head_dim} has no "
+                  "block-scaled cache (64 or 128)")
+        _lib.need(kc.dim() == 3 and kc.size(2) == row, "Attention: a block-scaled k_cache must be "
+                  f"[blocks, block_size, {row}], got {tuple(kc.shape)}")
+        _lib.need(kc.size(1) % TILE == 0, f"Attention: block_size {kc.size(1)} of a block-scaled "
+                  f"cache is not a multiple of {TILE}")
+        _lib.need(not self.kv_compress_enabled, "Attention: a block-scaled cache takes no part in "
+                  "compression steps (kv_compress_enabled)")
+
+    def _scaled_step(self, q, k, v, context, kv_stored):
+        """forward() over a block-scaled cache."""
+        kc, vc = self.k_cache, self.v_cache
+        if not kv_stored:
+            scaled_store_kvcache(k, v, kc, vc, context.slot_mapping)
+        if context.use_decode_kernel:
+            return scaled_paged_decode(q, kc, vc, context.context_lens, context.block_tables,
+                                       self.scale,
+                                       workspace=self._workspace(q, context.block_tables)
+                                       ).unsqueeze(1)
+        if context.block_tables is not None:
+            return scaled_varlen_prefill(q, kc, vc, context.cu_seqlens_q, context.cu_seqlens_k,
+                                         context.max_seqlen_q, self.scale, context.block_tables,
+                                         max_seqlen_k=context.max_seqlen_k)
+        return varlen_prefill(q, k, v, context.cu_seqlens_q, context.cu_seqlens_k,
+                              context.max_seqlen_q, self.scale)
 
     def _workspace(self, q, block_tables):
         """The device's decode workspace, shared with every other layer."""
@@ -491,6 +526,9 @@ class Attention(nn.Module):
         k_cache, v_cache = self.k_cache, self.v_cache
         if k_cache.numel():
             self._check_cache()
+            if k_cache.dtype is _U8:
+                with _lib.device_of(q.get_device()):
+                    return self._scaled_step(q, k, v, context, kv_stored)
             # the ordinary step (new rows, paged, no compression due) in one native call
             if not kv_stored and not (self.kv_compress_enabled and context.is_compress_step):
                 o = self._step(q, k, v, context, k_cache, v_cache)

@@ -51,6 +51,15 @@ def fp8_dequantize(codes: torch.Tensor, scale: float = 1.0, out: torch.Tensor | 
     return out
 
 
+def blocks_that_fit(block_bytes: int, gpu_memory_utilization: float, device) -> int:
+    """Blocks that the free device memory holds (model_runner.py:133-144)."""
+    free, total = torch.cuda.mem_get_info(device)
+    stats = torch.cuda.memory_stats(device)
+    peak = stats.get("allocated_bytes.all.peak", 0)
+    current = stats.get("allocated_bytes.all.current", 0)
+    return int(total * gpu_memory_utilization - (total - free) - peak + current) // block_bytes
+
+
 class KVCachePool:
     """One K/V tensor for every layer (model_runner.py:133-152): bf16 or fp16 (the model's
     dtype, as the reference allocates it) or fp8."""
@@ -65,13 +74,7 @@ class KVCachePool:
         itemsize = torch.tensor([], dtype=dtype).element_size()
         self.block_bytes = 2 * num_layers * block_size * num_kv_heads * head_dim * itemsize
         if num_blocks is None:
-            free, total = torch.cuda.mem_get_info(device)
-            stats = torch.cuda.memory_stats(device)
-            used = total - free
-            peak = stats.get("allocated_bytes.all.peak", 0)
-            current = stats.get("allocated_bytes.all.current", 0)
-            num_blocks = int(total * gpu_memory_utilization - used - peak + current) \
-                // self.block_bytes
+            num_blocks = blocks_that_fit(self.block_bytes, gpu_memory_utilization, device)
         if num_blocks <= 0:
             raise RuntimeError("no device memory left for the K/V pool")
         self.num_blocks = num_blocks

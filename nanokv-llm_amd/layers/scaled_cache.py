@@ -17,12 +17,47 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .attention import decode_workspace_bytes
+from .kv_cache import blocks_that_fit
 
 _BF16, _I32, _U8 = torch.bfloat16, torch.int32, torch.uint8
 TILE = 32      # tokens under one scale
 ROW_PAD = 16   # include/nkv.h, NKV_SCALED_ROW_PAD
 MAX_HEADS = 512
+
+
+class ScaledKVCachePool:
+    """One uint8 tensor of block-scaled K/V for every layer: ``kv_cache`` [2, layers, blocks,
+    block_size, Hk * D + 16], zeros (nothing written), sized from the free device memory as
+    ``KVCachePool`` is. ``PagedSequences`` takes it as it takes a ``KVCachePool``."""
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, block_size: int = 256,
+                 gpu_memory_utilization: float = 0.8, num_blocks: int | None = None,
+                 device="cuda"):
+        if head_dim not in (64, 128) or not 0 < num_kv_heads <= MAX_HEADS or num_layers <= 0:
+            raise ValueError(f"ScaledKVCachePool: {num_layers} layers of {num_kv_heads} KV heads of "
+                             f"{head_dim} (head_dim 64 or 128, 1 to {MAX_HEADS} heads)")
+        if block_size <= 0 or block_size % TILE:
+            raise ValueError(f"ScaledKVCachePool: block_size {block_size} is not a multiple of {TILE}")
+        row = num_kv_heads * head_dim + ROW_PAD
+        self.block_size, self.dtype = block_size, _U8
+        self.block_bytes = 2 * num_layers * block_size * row
+        if num_blocks is None:
+            num_blocks = blocks_that_fit(self.block_bytes, gpu_memory_utilization, device)
+        if num_blocks <= 0:
+            raise RuntimeError("no device memory left for the K/V pool")
+        self.num_blocks = num_blocks
+        self.kv_cache = torch.zeros(2, num_layers, num_blocks, block_size, row, dtype=_U8,
+                                    device=device)
+
+    def bind(self, modules) -> int:
+        """Assign layer i's views to the i-th module with k_cache/v_cache (model_runner.py
+        :148-152); returns the number of layers bound."""
+        layer = 0
+        for m in modules:
+            if hasattr(m, "k_cache") and hasattr(m, "v_cache"):
+                m.k_cache, m.v_cache = self.kv_cache[0, layer], self.kv_cache[1, layer]
+                layer += 1
+        return layer
 
 
 def _caches(what, k_cache, v_cache, row):
@@ -172,8 +207,8 @@ def scaled_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     with _lib.device_of(q.get_device()):
         width = block_tables.size(1)
         if workspace is None:
-            workspace = torch.empty(max(decode_workspace_bytes(bs, Hq, width, B, D), 4), dtype=_U8,
-                                    device=q.device)
+            nbytes = _lib.lib().nkv_paged_decode_workspace_bytes(bs, Hq, D, width, B)
+            workspace = torch.empty(max(nbytes, 4), dtype=_U8, device=q.device)
         rc = _lib.lib().nkv_scaled_decode(
             q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
             block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(), bs, Hq, Hk, D,
