@@ -266,21 +266,22 @@ __global__ __launch_bounds__(64 * kScaledWaves) void scaled_read_kernel(
   const Unit<D> un(unit, units, Hk);
 
   // the sequence that holds tile blockIdx.x of all of them
-  int cb = 0, base = 0, at = 0, n = 0, start = 0, tiles = 0, incl = 0;
+  int cb = 0, base = 0, at = 0, n = 0, tiles = 0, incl = 0;
+  uint32_t start = 0;  // positions may reach past 2^31: no table does
   for (;; cb += 64) {
     if (cb >= n_seqs) return;
     const int s = cb + lane;
-    n = start = tiles = 0;
+    n = tiles = 0;
     if (s < n_seqs) {
       at = cu_seqlens[s];
       n = cu_seqlens[s + 1] - at;
-      start = starts ? starts[s] : 0;
+      const int from = starts ? starts[s] : 0;
+      start = (uint32_t)from;
       // rows outside the outputs or of no position: none (the grid counts n_tokens rows)
-      const bool ok = at >= 0 && n > 0 && start >= 0 && (int64_t)at + n <= n_tokens &&
-                      (int64_t)start + n <= INT32_MAX;
+      const bool ok = at >= 0 && n > 0 && from >= 0 && (int64_t)at + n <= n_tokens;
       NKV_DBG(!ok && n != 0, NKV_DEBUG_LENGTH);
       if (!ok) n = 0;
-      if (n > 0) tiles = (start + n - 1) / kTileRows - start / kTileRows + 1;
+      if (n > 0) tiles = (int)((start + n - 1) / kTileRows - start / kTileRows) + 1;
     }
     incl = wave_incl_scan(tiles);
     const int tot = __builtin_amdgcn_readlane(incl, 63);
@@ -290,13 +291,13 @@ __global__ __launch_bounds__(64 * kScaledWaves) void scaled_read_kernel(
   const int ln = __builtin_ctzll(__ballot(base + incl > (int)blockIdx.x));
   at = __builtin_amdgcn_readlane(at, ln);
   n = __builtin_amdgcn_readlane(n, ln);
-  start = __builtin_amdgcn_readlane(start, ln);
+  start = (uint32_t)__builtin_amdgcn_readlane((int)start, ln);
   const int first = base + __builtin_amdgcn_readlane(incl - tiles, ln);
-  const int t0 = (start / kTileRows + (int)blockIdx.x - first) * kTileRows;  // the tile's position
-  const int bi = t0 / block_size;
-  const int id = bi < max_blocks ? block_tables[(int64_t)(cb + ln) * bt_row_stride + bi] : -1;
+  const uint32_t t0 = (start / kTileRows + (blockIdx.x - first)) * kTileRows;  // the tile's position
+  const uint32_t bi = t0 / (uint32_t)block_size;
+  const int id = bi < (uint32_t)max_blocks ? block_tables[(int64_t)(cb + ln) * bt_row_stride + bi] : -1;
   const bool valid = id >= 0 && id < n_blocks;
-  NKV_DBG(!valid, bi < max_blocks ? NKV_DEBUG_BLOCK : NKV_DEBUG_LENGTH);
+  NKV_DBG(!valid, bi < (uint32_t)max_blocks ? NKV_DEBUG_BLOCK : NKV_DEBUG_LENGTH);
   if (!un.live) return;
 
   u32x4_t row[8] = {};  // of token 8 y + k: dims 8 hx .. + 7
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(64 * kScaledWaves) void scaled_read_kernel(
   bf16_t* out = (un.is_v ? v_out : k_out) + un.h0 * D + 8 * un.x;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const int j = t0 + 8 * un.y + k - start;
+    const int j = (int)(t0 + 8 * un.y + k - start);
     if (j >= 0 && j < n)
       __builtin_nontemporal_store(
           row[k], reinterpret_cast<u32x4_t*>(out + ((int64_t)at + j) * Hk * D));

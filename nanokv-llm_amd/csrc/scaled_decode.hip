@@ -305,6 +305,7 @@ extern "C" int nkv_scaled_decode(const void* q, int64_t q_row_stride, const void
               "scaled_decode: max_blocks_per_seq * block_size too large");
   NKV_REQUIRE(scale > 0.f && isfinite(scale), NKV_EINVAL,
               "scaled_decode: scale must be finite and > 0");
+  if (batch == 0) return NKV_OK;
   const int64_t row = (int64_t)n_q_heads * head_dim;
   NKV_REQUIRE(q && block_tables && context_lens && out && aligned16(q) &&
                   (reinterpret_cast<uintptr_t>(out) & 3u) == 0,
@@ -313,7 +314,6 @@ extern "C" int nkv_scaled_decode(const void* q, int64_t q_row_stride, const void
                   out_row_stride % 2 == 0,
               NKV_EINVAL, "scaled_decode: row strides must cover Hq*D, q's in multiples of 8, "
               "out's of 2");
-  if (batch == 0) return NKV_OK;
   const int64_t max_tiles = (int64_t)max_blocks_per_seq * (block_size / kTileRows);
   const int ncg = decode_ncg(g), np = n_kv_heads * ncg;
   NKV_REQUIRE(max_tiles * batch < (1ll << 30), NKV_EUNSUPPORTED,

@@ -456,6 +456,7 @@ extern "C" int nkv_scaled_prefill(const void* q, int64_t q_row_stride, int64_t t
               NKV_EUNSUPPORTED, "scaled_prefill: blocks and lengths must fit 32 bits");
   NKV_REQUIRE(scale > 0.f && isfinite(scale), NKV_EINVAL,
               "scaled_prefill: scale must be finite and > 0");
+  if (n_seqs == 0 || total_q == 0 || max_seqlen_q == 0) return NKV_OK;
   const int64_t row = (int64_t)n_q_heads * head_dim;
   NKV_REQUIRE(q && cu_seqlens_q && cu_seqlens_k && block_tables && out && aligned16(q) &&
                   (reinterpret_cast<uintptr_t>(out) & 7u) == 0,
@@ -464,7 +465,6 @@ extern "C" int nkv_scaled_prefill(const void* q, int64_t q_row_stride, int64_t t
                   out_row_stride % 4 == 0,
               NKV_EINVAL, "scaled_prefill: row strides must cover Hq*D, q's in multiples of 8, "
               "out's of 4");
-  if (n_seqs == 0 || total_q == 0 || max_seqlen_q == 0) return NKV_OK;
   ScaledPrefillPlan p =
       scaled_prefill_plan(n_seqs, total_q, max_seqlen_q, workspace ? max_seqlen_k : 0, n_kv_heads, g);
   if (p.parts > 1) {
