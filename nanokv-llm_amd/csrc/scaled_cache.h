@@ -55,6 +55,12 @@ __device__ __forceinline__ float inverse_scale(int byte) {
   return __int_as_float((254 - byte) << 23);
 }
 
+// The word that holds a head's scale byte (its offset: scale_at & ~3): loaded whole and taken apart
+// where it is used, since the compiler widens a loaded byte at once, and waits for it.
+__device__ __forceinline__ int byte_of(uint32_t word, int scale_at) {
+  return (int)(word >> (8 * (scale_at & 3)) & 0xffu);
+}
+
 // Eight codes times a scale -> eight bf16 (exact).
 __device__ __forceinline__ u32x4_t codes_to_bf16(uint32_t lo, uint32_t hi, float scale) {
   return u32x4_t{

@@ -128,7 +128,7 @@ void scaled_decode_kernel(
       }
 
       u32x4_t kreg[kRing][kLoads], vreg[kRing][kLoads];
-      int kscale[kRing], vscale[kRing];
+      uint32_t kscale[kRing], vscale[kRing];  // words of the scale bytes
       int nv[kRing];  // keys of the tile in each ring slot (0: masked)
       auto issue = [&](int j, int s) {
         const int tile = wlo + j;
@@ -142,13 +142,13 @@ void scaled_decode_kernel(
             (void*)(k_cache + at * tile_bytes), (short)0, bytes, kBufferFlags);
         const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
             (void*)(v_cache + at * tile_bytes), (short)0, bytes, kBufferFlags);
-        kscale[s] = (int)__builtin_amdgcn_raw_buffer_load_b8(rk, scale_off, 0, 0);
+        kscale[s] = __builtin_amdgcn_raw_buffer_load_b32(rk, scale_off & ~3, 0, 0);
 #pragma unroll
         for (int p = 0; p < kLoads; ++p)
           kreg[s][p] = __builtin_bit_cast(
               u32x4_t,
               __builtin_amdgcn_raw_buffer_load_b128(rk, code_off + p * 1024, 0, kStreamPolicy));
-        vscale[s] = (int)__builtin_amdgcn_raw_buffer_load_b8(rv, scale_off, 0, 0);
+        vscale[s] = __builtin_amdgcn_raw_buffer_load_b32(rv, scale_off & ~3, 0, 0);
 #pragma unroll
         for (int p = 0; p < kLoads; ++p)
           vreg[s][p] = __builtin_bit_cast(
@@ -159,7 +159,7 @@ void scaled_decode_kernel(
       auto consume = [&](int s, auto refill, int nxt) {
         const int n = nv[s];  // the refill below overwrites the slot's count
         // S^T: lane -> column col, tokens 8 g4 + 4 t + 0..3
-        const float ks = scale_of(stored_scale(kscale[s]));
+        const float ks = scale_of(stored_scale(byte_of(kscale[s], scale_off)));
         f32x4_t st[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -210,7 +210,7 @@ void scaled_decode_kernel(
                             cvt_pk16<false>(p[4], p[5]), cvt_pk16<false>(p[6], p[7])};
 #pragma unroll
         for (int e = 0; e < 4; ++e) l_run = sum2_16<false>(pb[e], l_run);
-        const float vs = scale_of(stored_scale(vscale[s]));
+        const float vs = scale_of(stored_scale(byte_of(vscale[s], scale_off)));
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
           const u32x4_t c = vreg[s][j];

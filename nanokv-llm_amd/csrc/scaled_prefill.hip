@@ -18,6 +18,7 @@
 // Where the tiles are fewer than the chip's workgroups the keys of each are cut into `parts` equal
 // ranges, whose partial rows a second launch merges.
 #include "launch_rules.h"
+#include "lds_tiles.h"
 #include "scaled_cache.h"
 
 #include <math.h>
@@ -29,8 +30,7 @@ namespace nkv {
 
 constexpr int kStep = 64;      // keys a step
 constexpr float kLazy = 8.f;   // log2 headroom before the running maximum is raised
-constexpr int kMaxParts = 64;  // of a tile's keys
-constexpr int prefill_part_row(int D) { return D + 4; }  // floats of a partial row: O, m, l, 2 pad
+constexpr int part_floats(int D) { return D + 4; }  // of a partial row: O, m, l, 2 pad
 
 struct ScaledPrefillArgs {
   const bf16_t* q;
@@ -38,13 +38,113 @@ struct ScaledPrefillArgs {
   const char *k_cache, *v_cache;
   const int32_t *cu_q, *cu_k, *block_tables;
   int64_t bt_row_stride;
-  int32_t Hk, G, block_size, max_blocks, n_blocks, n_seqs, n_tiles, parts;
+  int32_t Hk, G, block_size, max_blocks, n_blocks, n_seqs, n_tiles;
   int64_t total_q;  // rows of q and out
   float scale_log2;
   bf16_t* out;
   int64_t out_row_stride;
-  float* part;  // [row of q][query head][parts] partial rows
+  // split launches: what a workgroup's range left unfinished
+  i32x4_t* desc;  // one per workgroup: {parts, first row of q, queries, KV head}
+  float* part;    // two tiles of partial rows per workgroup
 };
+
+// A sequence's queries and keys; none where its rows are not all rows of q.
+__device__ __forceinline__ void seq_lengths(const ScaledPrefillArgs& a, int s, int& q0, int& Lq,
+                                            int& Lk) {
+  q0 = a.cu_q[s];
+  Lq = a.cu_q[s + 1] - q0;
+  Lk = a.cu_k[s + 1] - a.cu_k[s];
+  NKV_DBG(Lq < 0 || Lk < 0 || Lq > Lk, NKV_DEBUG_LENGTH);
+  if (q0 < 0 || (int64_t)q0 + Lq > a.total_q) Lq = 0;
+}
+
+// The ranges of a split launch. The units of a KV head (sequence, tile) stand in one stream, a unit as
+// long as its steps cost; range w is [w C, (w+1) C), a cut near a unit's end moved to that end. Every
+// workgroup finds its own range from the lengths.
+struct Cursor {
+  int seq, tile, q0, Lq, Lk;  // the current unit
+  int u0;                     // its position in the stream
+  int C, T, x, x_end;         // range length, stream length, the range's begin and end
+};
+constexpr int kSnap = 2;      // steps
+constexpr int kLeastSteps = 4;  // shortest range
+template <int RG>
+__device__ __forceinline__ int step_cost(int rows) {
+  return kStepBase + (rows + 16 * RG - 1) / (16 * RG);
+}
+__device__ __forceinline__ int tile_steps(int Lq, int Lk, int qt, int t) {
+  const int last = Lk - Lq + min(Lq, (t + 1) * qt) - 1;
+  return last >= 0 ? min(last, Lk - 1) / kStep + 1 : 1;  // an empty one is masked whole
+}
+template <int RG>
+__device__ __forceinline__ int unit_cost(int Lq, int Lk, int qt, int t, int G) {
+  return tile_steps(Lq, Lk, qt, t) * step_cost<RG>(min(qt, Lq - t * qt) * G);
+}
+template <int RG>
+__device__ __forceinline__ bool split_begin(const ScaledPrefillArgs& a, int qt, Cursor& c) {
+  const int lane = threadIdx.x & 63;
+  int q0 = 0, Lq = 0, Lk = 0, cost = 0, incl = 0;
+  const auto load = [&](int cb) {  // lane: sequence cb + lane
+    Lq = Lk = cost = 0;
+    if (cb + lane < a.n_seqs) seq_lengths(a, cb + lane, q0, Lq, Lk);
+    for (int t = 0; t * qt < Lq; ++t) cost += unit_cost<RG>(Lq, Lk, qt, t, a.G);
+    incl = wave_incl_scan(cost);
+    return __builtin_amdgcn_readlane(incl, 63);
+  };
+  c.T = 0;
+  for (int cb = 0; cb < a.n_seqs; cb += 64) c.T += load(cb);
+  const int ranges = (int)gridDim.x / a.Hk;
+  c.C = max((c.T + ranges - 1) / ranges, kLeastSteps * kFullStep);
+  c.x = (int)blockIdx.x / a.Hk * c.C;
+  c.x_end = c.x + c.C;
+  if (c.x >= c.T) return false;
+  int base = 0, cb = 0;
+  if (a.n_seqs > 64) load(0);
+  for (int tot; c.x >= base + (tot = __builtin_amdgcn_readlane(incl, 63)); load(cb)) {
+    base += tot;
+    cb += 64;
+    if (cb >= a.n_seqs) return false;
+  }
+  const int ln = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(base + incl > c.x)));
+  c.seq = cb + ln;
+  c.q0 = __builtin_amdgcn_readlane(q0, ln);
+  c.Lq = __builtin_amdgcn_readlane(Lq, ln);
+  c.Lk = __builtin_amdgcn_readlane(Lk, ln);
+  c.u0 = base + __builtin_amdgcn_readlane(incl - cost, ln);
+  for (c.tile = 0; (c.tile + 1) * qt < c.Lq; ++c.tile) {
+    const int u = unit_cost<RG>(c.Lq, c.Lk, qt, c.tile, a.G);
+    if (c.x < c.u0 + u) break;
+    c.u0 += u;
+  }
+  return true;
+}
+// The unit after the current one, which ends at u1 (false at the end of the stream).
+__device__ __forceinline__ bool split_next(const ScaledPrefillArgs& a, int qt, int u1, Cursor& c) {
+  c.u0 = u1;
+  if (u1 >= c.T || u1 >= c.x_end) return false;
+  if (++c.tile * qt < c.Lq) return true;
+  c.tile = 0;
+  do {
+    if (++c.seq >= a.n_seqs) return false;
+    seq_lengths(a, c.seq, c.q0, c.Lq, c.Lk);
+  } while (c.Lq <= 0);
+  return true;
+}
+
+// 1 KiB (16 bytes a lane) or 256 bytes (4 a lane) from desc + voff to consecutive LDS bytes. Written
+// as asm so that the compiler adds no wait for it before a barrier; the ring's own s_waitcnt does.
+__device__ __forceinline__ void fetch16(i32x4_t desc, uint32_t lds_addr, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds_addr), "v"(voff), "s"(desc)
+               : "memory");
+}
+__device__ __forceinline__ void fetch4(i32x4_t desc, uint32_t lds_addr, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(lds_addr), "v"(voff), "s"(desc)
+               : "memory");
+}
 
 // Zeroes for NaN, and ones where there was one.
 __device__ __forceinline__ u32x4_t split_nan(u32x4_t v, u32x4_t& ones) {
@@ -59,16 +159,18 @@ __device__ __forceinline__ u32x4_t split_nan(u32x4_t v, u32x4_t& ones) {
   return clean;
 }
 
-template <int D, int RG>
+// A workgroup's tile, or (SPLIT) the units of its range.
+template <int D, int RG, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPrefillArgs a) {
   constexpr int kI = D / 64;
-  constexpr int kLoads = 2 * kI;          // 1 KiB loads of a cache tile's K, and of its V
-  constexpr int kKs = D / 32;             // k-steps of S^T
-  constexpr int kDb = D / 16;             // 16-dim blocks of O^T
-  constexpr int kHalfB = kTileRows * D * 2;  // bytes of a cache tile's K or V in LDS
-  constexpr int kStageB = 4 * kHalfB;     // K of two tiles, then V of two
-  __shared__ __attribute__((aligned(1024))) char ring[2 * kStageB];
-  __shared__ int nan_in[2][2];  // a stage's V tiles hold NaN (of steps that mask keys)
+  constexpr int kLoads = 2 * kI;           // 1 KiB loads of a cache tile's K, and of its V
+  constexpr int kKs = D / 32;              // k-steps of S^T
+  constexpr int kDb = D / 16;              // 16-dim blocks of O^T
+  constexpr int kTileB = kTileRows * D;    // bytes of a head's codes of a cache tile
+  constexpr int kCodesB = 4 * kTileB;      // of a step: K, V of the first cache tile, of the second
+  constexpr int kStageB = kCodesB + 1024;  // and a word (64 copies) with the scale of each
+  constexpr int kStages = 4;               // steps in LDS: one computed, three on their way
+  __shared__ __attribute__((aligned(1024))) char ring[kStages * kStageB];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -77,114 +179,63 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
   const int col = lane & 15;
   const int G = a.G, Hk = a.Hk;
   const int QT = 64 * RG / G;  // queries per tile
-
   const int kvh = blockIdx.x % Hk;
-  int rest = blockIdx.x / Hk;
-  const int z = rest % a.parts;
-  rest /= a.parts;
-  const int tile = a.n_tiles - 1 - rest % a.n_tiles;  // largest first
-  const int seq = rest / a.n_tiles;
-  const int q0 = a.cu_q[seq], Lq = a.cu_q[seq + 1] - q0;
-  const int Lk = a.cu_k[seq + 1] - a.cu_k[seq];
-  NKV_DBG(tid == 0 && tile == 0 && (Lq < 0 || Lk < 0 || Lq > Lk), NKV_DEBUG_LENGTH);
-  const int j0 = tile * QT;
-  if (j0 >= Lq || q0 < 0 || (int64_t)q0 + Lq > a.total_q) return;  // uniform
+  // loads: wave w brings the codes of cache tile 2 s + w / 2, K (even w) or V
+  const int half = wave >> 1;
+  const char* cache = (wave & 1) ? a.v_cache : a.k_cache;
+  const int tiles_per_block = a.block_size / kTileRows;
+  const int tile_bytes = kTileRows * (Hk * D + kRowPad);
+  const uint32_t code_off = (uint32_t)(kvh * kTileB + lane * 16);
+  const uint32_t scale_off = (uint32_t)(kTileRows * Hk * D + kvh);
+  const uint32_t ring_at =
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)ring + (uint32_t)wave * kTileB;
+
+  Cursor cur;
+  if constexpr (SPLIT) {
+    if (tid == 0) a.desc[blockIdx.x] = i32x4_t{0, 0, 0, 0};  // no unit cut at this range's end
+    if (!split_begin<RG>(a, QT, cur)) return;                // uniform
+  } else {
+    const int rest = blockIdx.x / Hk;
+    cur.tile = a.n_tiles - 1 - rest % a.n_tiles;  // largest first
+    cur.seq = rest / a.n_tiles;
+    seq_lengths(a, cur.seq, cur.q0, cur.Lq, cur.Lk);
+    if (cur.tile * QT >= cur.Lq) return;  // uniform
+  }
+  int u1 = 0;        // the unit's end in the stream
+  bool cut = false;  // the range ends inside the unit
+  do {
+  const auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  const int q0 = uni(cur.q0), Lq = uni(cur.Lq), Lk = uni(cur.Lk);
+  const int j0 = uni(cur.tile) * QT;
   const int diag = Lk - Lq;  // query j sees keys <= diag + j
   const int last_key = min(Lk - 1, diag + j0 + QT - 1);
-  const int n_steps = last_key >= 0 ? last_key / kStep + 1 : 0;
-  const int per = (n_steps + a.parts - 1) / a.parts;
-  const int s_lo = min(z * per, n_steps), s_end = min(s_lo + per, n_steps);
-
-  // ---- loads: wave w brings the codes of cache tile 2 s + w / 2, K (even w) or V
-  const bool is_v = wave & 1;
-  const int half = wave >> 1;
-  const char* cache = is_v ? a.v_cache : a.k_cache;
-  const int tiles_per_block = a.block_size / kTileRows;
-  const int64_t tile_bytes = (int64_t)kTileRows * (Hk * D + kRowPad);
-  const int code_off = kvh * (kTileRows * D) + lane * 16;
-  const int scale_off = kTileRows * Hk * D + kvh;
-  const int32_t* bt = a.block_tables + (int64_t)seq * a.bt_row_stride;
-  int bt_base = 0, bt_lane = -1;  // lane i: entry bt_base + i of the table row
-  auto load_window = [&]() {
-    const int e = bt_base + lane;
-    const int id = e < a.max_blocks ? bt[e] : -1;
-    NKV_DBG((int64_t)e * a.block_size < Lk && (e >= a.max_blocks || id < 0 || id >= a.n_blocks),
-            e >= a.max_blocks ? NKV_DEBUG_LENGTH : NKV_DEBUG_BLOCK);
-    bt_lane = (id >= 0 && id < a.n_blocks) ? id : -1;
-  };
-  int c_blk = (2 * s_lo + half) / tiles_per_block;  // block and tile in it of the step loaded next
-  int c_in = (2 * s_lo + half) % tiles_per_block;
-  bt_base = c_blk & ~63;
-  load_window();
-  u32x4_t code[kLoads];
-  int scale_in = 0;
-  auto issue = [&](int s) __attribute__((always_inline)) {
-    const int n = s < s_end ? min(Lk - (2 * s + half) * kTileRows, kTileRows) : 0;
-    const int pb = __builtin_amdgcn_readlane(bt_lane, c_blk - bt_base);
-    const bool ok = n > 0 && pb >= 0;  // else zeros
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)(cache + (ok ? (int64_t)pb * tiles_per_block + c_in : 0) * tile_bytes), (short)0,
-        ok ? (uint32_t)tile_bytes : 0u, kBufferFlags);
-    scale_in = (int)__builtin_amdgcn_raw_buffer_load_b8(r, scale_off, 0, 0);
-#pragma unroll
-    for (int p = 0; p < kLoads; ++p)
-      code[p] = __builtin_bit_cast(
-          u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, code_off + p * 1024, 0, 0));
-    c_in += 2;
-    while (c_in >= tiles_per_block) {  // at most twice: blocks of one tile
-      c_in -= tiles_per_block;
-      ++c_blk;
+  int s_lo = 0, s_end = last_key >= 0 ? last_key / kStep + 1 : 0;
+  int snap = 0;
+  if constexpr (SPLIT) {
+    const int sc = step_cost<RG>(min(QT, Lq - j0) * G);
+    const int n_steps = tile_steps(Lq, Lk, QT, cur.tile);
+    snap = kSnap * sc;
+    u1 = cur.u0 + n_steps * sc;
+    s_end = n_steps;
+    cut = false;
+    if (cur.x >= cur.u0 + snap) {     // the range's begin lies in its first unit
+      if (cur.x > u1 - snap) continue;  // which is the range's before (the condition steps on)
+      s_lo = (cur.x - cur.u0 + sc - 1) / sc;
     }
-    if (c_blk - bt_base >= 64) {  // uniform
-      bt_base = c_blk & ~63;
-      load_window();
+    if (cur.x_end < u1) {                     // the range ends within this unit
+      if (cur.x_end < cur.u0 + snap) return;  // which is the next range's
+      cut = cur.x_end <= u1 - snap;
     }
-  };
-  // a step masks keys of some row (uniform)
-  auto is_edge = [&](int s) { return s * kStep + kStep - 1 > diag + j0 || s * kStep + kStep > Lk; };
-  // the codes of the last issue(), step s's, widened into a stage
-  auto commit = [&](int s, int stage) __attribute__((always_inline)) {
-    char* at = ring + stage * kStageB + (is_v ? 2 * kHalfB : 0) + half * kHalfB + lane * 16;
-    const float scale = scale_of(stored_scale(scale_in));
-    if (is_v) {
-      const int n = Lk - (2 * s + half) * kTileRows;
-      if (n < kTileRows) {
-        // codes behind the end may be anything, NaN too: a zero weight would not hide them
-        const int m = min(max(n - 8 * g4, 0), 8);
-        const uint64_t keep = m >= 8 ? ~0ull : (1ull << (8 * m)) - 1;
-#pragma unroll
-        for (int p = 0; p < kLoads; ++p) {
-          code[p][0] &= (uint32_t)keep;
-          code[p][1] &= (uint32_t)(keep >> 32);
-          code[p][2] &= (uint32_t)keep;
-          code[p][3] &= (uint32_t)(keep >> 32);
-        }
-      }
-      if (is_edge(s)) {
-        uint32_t found = 0;  // bytes x111 1111
-#pragma unroll
-        for (int p = 0; p < kLoads; ++p)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) found |= ((code[p][w] & 0x7f7f7f7fu) + 0x01010101u);
-        const bool any = __ballot((found & 0x80808080u) != 0) != 0;
-        if (lane == 0) nan_in[stage][half] = any;
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < kLoads; ++p) {
-      *reinterpret_cast<u32x4_t*>(at + p * 2048) = codes_to_bf16(code[p][0], code[p][1], scale);
-      *reinterpret_cast<u32x4_t*>(at + p * 2048 + 1024) =
-          codes_to_bf16(code[p][2], code[p][3], scale);
-    }
-  };
+    if (cut) s_end = (cur.x_end - cur.u0 + sc - 1) / sc;
+    s_lo = uni(s_lo);
+    s_end = uni(s_end);
+  }
 
   // ---- this wave's row groups: head and query of this lane's row (rows past the tile's queries
   // take query Lq: attended like the others, never stored)
   const bool idle = wave * (16 * RG) >= min(QT, Lq - j0) * G;  // only brings its share of the codes
   int head[RG], jrow[RG];
   u32x4_t qreg[RG][kKs];
-  f32x4_t acc[RG][kDb];  // O^T: lane l -> row l%16, dims 16*db + 4*(l/16) .. +3
-  float m_run[RG], l_run[RG], mb[RG];  // mb: m_run, or 0 while the row has seen no key
 #pragma unroll
   for (int rr = 0; rr < RG; ++rr) {
     const int r = (wave * RG + rr) * 16 + col;
@@ -199,24 +250,81 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
       qreg[rr][2 * i] = qp[8 * i];
       qreg[rr][2 * i + 1] = qp[8 * i + 1];
     }
+  }
+
+  // ---- the ring
+  const int32_t* bt = a.block_tables + (int64_t)uni(cur.seq) * a.bt_row_stride;
+  int c_blk = (2 * s_lo + half) / tiles_per_block;  // block and tile in it of the step loaded next
+  int c_in = (2 * s_lo + half) - c_blk * tiles_per_block;
+  int c_left = min(Lk, s_end * kStep) - (2 * s_lo + half) * kTileRows;  // keys from there on
+  int c_stage = 0;
+  int bt_base = c_blk & ~63, bt_lane = -1;  // lane i: entry bt_base + i of the table row
+  auto load_window = [&]() {
+    const int e = bt_base + lane;
+    const int id = e < a.max_blocks ? bt[e] : -1;
+    NKV_DBG((int64_t)e * a.block_size < Lk && (e >= a.max_blocks || id < 0 || id >= a.n_blocks),
+            e >= a.max_blocks ? NKV_DEBUG_LENGTH : NKV_DEBUG_BLOCK);
+    bt_lane = (id >= 0 && id < a.n_blocks) ? id : -1;
+  };
+  load_window();
+  auto issue = [&]() __attribute__((always_inline)) {
+    const int pb = __builtin_amdgcn_readlane(bt_lane, c_blk - bt_base);
+    const bool ok = c_left > 0 && pb >= 0;  // else zeros
+    const int64_t at = ((int64_t)(ok ? pb : 0) * tiles_per_block + c_in) * tile_bytes;
+    const i32x4_t desc = buffer_desc(cache + at, ok ? (uint32_t)tile_bytes : 0u);
+    const uint32_t to = ring_at + (uint32_t)c_stage * kStageB;
+#pragma unroll
+    for (int p = 0; p < kLoads; ++p) fetch16(desc, to + p * 1024, code_off + p * 1024);
+    fetch4(desc, to - (uint32_t)wave * kTileB + kCodesB + wave * 256, scale_off & ~3u);
+    c_stage = c_stage + 1 == kStages ? 0 : c_stage + 1;
+    c_left -= kStep;
+    c_in += 2;  // at most two blocks on
+    const int n = (c_in >= tiles_per_block) + (c_in >= 2 * tiles_per_block);
+    c_in -= n * tiles_per_block;
+    c_blk = uni(c_blk + n);
+    if (c_blk - bt_base >= 64) {  // uniform; once per 64 blocks
+      bt_base = c_blk & ~63;
+      load_window();
+    }
+  };
+  f32x4_t acc[RG][kDb];  // O^T: lane l -> row l%16, dims 16*db + 4*(l/16) .. +3
+  float m_run[RG], l_run[RG], mb[RG];  // mb: m_run, or 0 while the row has seen no key
+#pragma unroll
+  for (int rr = 0; rr < RG; ++rr) {
 #pragma unroll
     for (int db = 0; db < kDb; ++db) acc[rr][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     m_run[rr] = -INFINITY;
     l_run[rr] = 0.f;
     mb[rr] = 0.f;
+    // q is in registers before the ring's first loads: a wait for it later would wait for them too
+#pragma unroll
+    for (int ks = 0; ks < kKs; ++ks) asm volatile("" ::"v"(qreg[rr][ks]));
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last unit's stores
+#pragma unroll
+  for (int st = 0; st < kStages - 1; ++st) issue();
 
-  auto compute = [&](int s, int stage) __attribute__((always_inline)) {
+  auto compute = [&](int s, int stage, auto edge_c) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge_c)::value;
     const char* kt = ring + stage * kStageB + lane * 16;
-    const char* vt = kt + 2 * kHalfB;
+    const char* st = ring + stage * kStageB + kCodesB + lane * 4;
+    float scale[4];  // K, V of the first cache tile, of the second
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      scale[w] = scale_of(stored_scale(
+          byte_of(*reinterpret_cast<const uint32_t*>(st + w * 256), (int)scale_off)));
     // S^T of quarter h: tokens 32 (h / 2) + 8 g4 + 4 (h % 2) + 0..3 of the step
     float sv[RG][16];
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
       u32x4_t ka[kKs];
 #pragma unroll
-      for (int ks = 0; ks < kKs; ++ks)
-        ka[ks] = *reinterpret_cast<const u32x4_t*>(kt + (h * kKs + ks) * 1024);
+      for (int i = 0; i < kI; ++i) {
+        const u32x4_t c = *reinterpret_cast<const u32x4_t*>(
+            kt + (h >> 1) * (2 * kTileB) + ((h & 1) * kI + i) * 1024);
+        ka[2 * i] = codes_to_bf16(c[0], c[1], scale[h & 2]);
+        ka[2 * i + 1] = codes_to_bf16(c[2], c[3], scale[h & 2]);
+      }
 #pragma unroll
       for (int rr = 0; rr < RG; ++rr) {
         f32x4_t x = {0.f, 0.f, 0.f, 0.f};
@@ -226,16 +334,15 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
         for (int r = 0; r < 4; ++r) sv[rr][4 * h + r] = x[r];
       }
     }
-    const bool edge = is_edge(s);
-    int lim[RG];  // last key that the row sees, from the lane's first of the step on
+    [[maybe_unused]] int lim[RG];  // last key that the row sees, from the lane's first of the step on
+    if constexpr (EDGE) {
 #pragma unroll
-    for (int rr = 0; rr < RG; ++rr) lim[rr] = min(diag + jrow[rr], Lk - 1) - s * kStep - 8 * g4;
-    if (edge) {
-#pragma unroll
-      for (int rr = 0; rr < RG; ++rr)
+      for (int rr = 0; rr < RG; ++rr) {
+        lim[rr] = min(diag + jrow[rr], Lk - 1) - s * kStep - 8 * g4;
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if ((e >> 3) * kTileRows + (e & 7) > lim[rr]) sv[rr][e] = -INFINITY;
+      }
     }
     // the maxima are only raised where a row's exceeds its running one by kLazy
     float top[RG];
@@ -276,134 +383,186 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
 #pragma unroll
         for (int e = 0; e < 4; ++e) l_run[rr] = sum2_16<false>(pb[rr][e], l_run[rr]);
       }
-      if (edge && nan_in[stage][c]) {  // uniform, rare
-        // rows that do not see a key must not see its NaN: count those that each row sees
+      const char* vt = kt + kTileB + c * (2 * kTileB);
+      if constexpr (EDGE) {
+        // codes behind the end may be anything, NaN too, which a zero weight would not hide; and
+        // rows that do not see a key must not see its NaN: those that each row sees are counted
+        const int m = min(max(Lk - s * kStep - c * kTileRows - 8 * g4, 0), 8);
+        const uint32_t keep0 = m >= 4 ? ~0u : (1u << (8 * m)) - 1;
+        const uint32_t keep1 = m >= 8 ? ~0u : m > 4 ? (1u << (8 * (m - 4))) - 1 : 0u;
 #pragma unroll
-        for (int db = 0; db < kDb; ++db) {
-          u32x4_t ones;
-          const u32x4_t va = split_nan(
-              *reinterpret_cast<const u32x4_t*>(vt + (c * kDb + db) * 1024), ones);
+        for (int j = 0; j < kLoads; ++j) {
+          u32x4_t code = *reinterpret_cast<const u32x4_t*>(vt + j * 1024);
+          code &= u32x4_t{keep0, keep1, keep0, keep1};
+          uint32_t found = 0;  // bytes x111 1111
 #pragma unroll
-          for (int rr = 0; rr < RG; ++rr) {
-            u32x4_t seen;
+          for (int w = 0; w < 4; ++w) found |= (code[w] & 0x7f7f7f7fu) + 0x01010101u;
+          const bool nan = __ballot((found & 0x80808080u) != 0) != 0;
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-              seen[w] = (c * kTileRows + 2 * w <= lim[rr] ? 0x3f80u : 0u) |
-                        (c * kTileRows + 2 * w + 1 <= lim[rr] ? 0x3f800000u : 0u);
-            const f32x4_t n = mfma_16x16x32<false>(ones, seen, f32x4_t{0.f, 0.f, 0.f, 0.f});
-            acc[rr][db] = mfma_16x16x32<false>(va, pb[rr], acc[rr][db]);
+          for (int u = 0; u < 2; ++u) {
+            const int db = 2 * j + u;
+            u32x4_t va = codes_to_bf16(code[2 * u], code[2 * u + 1], scale[2 * c + 1]);
+            if (nan) {  // uniform, rare
+              u32x4_t ones;
+              va = split_nan(va, ones);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[rr][db][r] = n[r] > 0.f ? NAN : acc[rr][db][r];
+              for (int rr = 0; rr < RG; ++rr) {
+                u32x4_t seen;
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                  seen[w] = (c * kTileRows + 2 * w <= lim[rr] ? 0x3f80u : 0u) |
+                            (c * kTileRows + 2 * w + 1 <= lim[rr] ? 0x3f800000u : 0u);
+                const f32x4_t n = mfma_16x16x32<false>(ones, seen, f32x4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[rr][db][r] = n[r] > 0.f ? NAN : acc[rr][db][r];
+              }
+            }
+#pragma unroll
+            for (int rr = 0; rr < RG; ++rr)
+              acc[rr][db] = mfma_16x16x32<false>(va, pb[rr], acc[rr][db]);
           }
         }
-        continue;
-      }
+      } else {
 #pragma unroll
-      for (int db = 0; db < kDb; ++db) {
-        const u32x4_t va = *reinterpret_cast<const u32x4_t*>(vt + (c * kDb + db) * 1024);
+        for (int j = 0; j < kLoads; ++j) {
+          const u32x4_t code = *reinterpret_cast<const u32x4_t*>(vt + j * 1024);
 #pragma unroll
-        for (int rr = 0; rr < RG; ++rr)
-          acc[rr][db] = mfma_16x16x32<false>(va, pb[rr], acc[rr][db]);
+          for (int u = 0; u < 2; ++u) {
+            const u32x4_t va = codes_to_bf16(code[2 * u], code[2 * u + 1], scale[2 * c + 1]);
+#pragma unroll
+            for (int rr = 0; rr < RG; ++rr)
+              acc[rr][2 * j + u] = mfma_16x16x32<false>(va, pb[rr], acc[rr][2 * j + u]);
+          }
+        }
       }
     }
   };
 
-  if (s_lo < s_end) {
-    issue(s_lo);
-    commit(s_lo, 0);
+  // steps from s_edge on mask keys of some row
+  const int s_edge = max(0, min(diag + j0 + 1, Lk)) / kStep;
+  int stage = 0;
+  auto step = [&](int s, auto edge_c) __attribute__((always_inline)) {
+    // this wave's loads of step s have landed, then everyone's have, and everyone is done with step
+    // s - 1, whose stage takes the step kStages - 1 ahead
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 2) * (kLoads + 1)) : "memory");
     __syncthreads();
-    auto step = [&](int s, auto st) {
-      constexpr int kStage = decltype(st)::value;
-      issue(s + 1);
-      if (!idle) compute(s, kStage);
-      if (s + 1 < s_end) commit(s + 1, 1 - kStage);
-      __syncthreads();
-    };
-    for (int s = s_lo;;) {
-      step(s, std::integral_constant<int, 0>{});
-      if (++s >= s_end) break;
-      step(s, std::integral_constant<int, 1>{});
-      if (++s >= s_end) break;
-    }
-  }
-  if (idle) return;
+    issue();
+    if (!idle) compute(s, stage, edge_c);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  };
+  int s = s_lo;
+  for (; s < min(s_edge, s_end); ++s) step(s, std::integral_constant<bool, false>{});
+  for (; s < s_end; ++s) step(s, std::integral_constant<bool, true>{});
+  // no load into LDS outlives the workgroup, or meets the next unit's
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if constexpr (SPLIT) __syncthreads();
+  if (idle) continue;
 
+  const bool part = SPLIT && (cut || s_lo > 0);
 #pragma unroll
   for (int rr = 0; rr < RG; ++rr) {
     const float l = col_sum4(l_run[rr]);
     if (jrow[rr] >= Lq) continue;
-    const int64_t row = q0 + jrow[rr];
-    const int h = kvh * G + head[rr];
-    if (a.parts > 1) {
-      float* pr = a.part + ((row * (Hk * G) + h) * a.parts + z) * prefill_part_row(D);
+    if constexpr (SPLIT) {
+      if (part) {  // to one of two slots: the end of a unit begun before, or a unit's begin
+        float* pr = a.part + (((int64_t)blockIdx.x * 2 + (s_lo == 0)) * (64 * RG) +
+                              (wave * RG + rr) * 16 + col) * part_floats(D);
 #pragma unroll
-      for (int db = 0; db < kDb; ++db)
-        *reinterpret_cast<f32x4_t*>(pr + db * 16 + g4 * 4) = acc[rr][db];
-      if (g4 == 0) *reinterpret_cast<float2*>(pr + D) = float2{m_run[rr], l};
-      continue;
+        for (int db = 0; db < kDb; ++db)
+          *reinterpret_cast<f32x4_t*>(pr + db * 16 + g4 * 4) = acc[rr][db];
+        if (g4 == 0) *reinterpret_cast<float2*>(pr + D) = float2{m_run[rr], l};
+        continue;
+      }
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;
-    bf16_t* op = a.out + row * a.out_row_stride + (int64_t)h * D + g4 * 4;
+    bf16_t* op = a.out + (int64_t)(q0 + jrow[rr]) * a.out_row_stride +
+                 (int64_t)(kvh * G + head[rr]) * D + g4 * 4;
 #pragma unroll
     for (int db = 0; db < kDb; ++db)
       *reinterpret_cast<uint2*>(op + db * 16) =
           uint2{cvt_pk16<false>(acc[rr][db][0] * inv, acc[rr][db][1] * inv),
                 cvt_pk16<false>(acc[rr][db][2] * inv, acc[rr][db][3] * inv)};
   }
+  if constexpr (SPLIT) {
+    if (part && s_lo == 0 && tid == 0) {  // the unit's first part: describe it to the merge
+      const int w0 = (cur.u0 + snap + cur.C - 1) / cur.C;  // the unit's first cut
+      a.desc[blockIdx.x] =
+          i32x4_t{(u1 - snap) / cur.C - w0 + 2, q0 + j0, min(QT, Lq - j0), kvh};
+    }
+  }
+  } while (SPLIT && !cut && split_next(a, QT, u1, cur));
 }
 
-// One wave per (row of q, query head): its partials merged.
+// Merges the parts of the units that ranges cut: descriptor x (of the workgroup that holds a unit's
+// first part; part p > 0 is in the first slot of the workgroup p * Hk after it), a row of its tile a
+// wave. Lane l owns output dims N l .. N l + N - 1, eight parts in flight.
 template <int D>
 __global__ __launch_bounds__(256) void scaled_merge_kernel(const ScaledPrefillArgs a,
-                                                           int32_t max_rows) {
+                                                           int32_t tile_rows) {
   constexpr int N = D / 64;
+  constexpr int kInFlight = 8;
   const int lane = threadIdx.x & 63;
-  const int Hq = a.Hk * a.G;
-  const int64_t unit =
-      (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int64_t row = unit / Hq;
-  if (row >= a.total_q) return;
-  const int h = (int)(unit - row * Hq);
-  // rows of no sequence, and those past the tiles that were launched, are left as they are
-  bool mine = false;
-  for (int s = lane; s < a.n_seqs; s += 64) {
-    const int b = a.cu_q[s], e = a.cu_q[s + 1];
-    mine = mine || (b >= 0 && row >= b && row < e && e <= a.total_q && row - b < max_rows);
-  }
-  if (__ballot(mine) == 0) return;
-  const float* p = a.part + (row * Hq + h) * a.parts * prefill_part_row(D);
-  float2 ml = {-INFINITY, 0.f};
-  if (lane < a.parts) ml = *reinterpret_cast<const float2*>(p + lane * prefill_part_row(D) + D);
-  const float M = wave_max(ml.x);
-  const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : fast_exp2(ml.x - M);
-  const float L = wave_sum(w * ml.y);
-  float o[N] = {};
-  for (int z = 0; z < a.parts; ++z) {
-    const float wz = __shfl(w, z, 64);
-    float v[N];
-    load_dims<N>(p + z * prefill_part_row(D) + N * lane, v);
+  const i32x4_t d = a.desc[blockIdx.x];
+  const int r = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  if (d[0] < 2 || r >= d[2] * a.G) return;
+  const int64_t tile = (int64_t)tile_rows * part_floats(D);
+  const float* first = a.part + ((int64_t)blockIdx.x * 2 + 1) * tile + r * part_floats(D);
+  const float* next = first - tile;  // + p * 2 * Hk tiles
+  float M = -INFINITY, L = 0.f, o[N] = {};
+  for (int p0 = 0; p0 < d[0]; p0 += kInFlight) {
+    float2 ml[kInFlight];
+    float v[kInFlight][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = fmaf(wz, v[i], o[i]);
+    for (int u = 0; u < kInFlight; ++u) {
+      const int p = min(p0 + u, d[0] - 1);
+      const float* row = p == 0 ? first : next + (int64_t)p * 2 * a.Hk * tile;
+      ml[u] = *reinterpret_cast<const float2*>(row + D);
+      load_dims<N>(row + N * lane, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const float m = ml[u].x, l = ml[u].y;
+      // (no key of the part that the row sees: m = -inf, l = 0)
+      if (p0 + u >= d[0] || (m == -INFINITY && l == 0.f)) continue;
+      const float top = fmaxf(M, m);
+      const float mb = top == -INFINITY ? 0.f : top;  // scores that are all NaN leave no maximum
+      const float alpha = fast_exp2(M - mb), w = m == -INFINITY ? 1.f : fast_exp2(m - mb);
+      M = top;
+      L = fmaf(w, l, L * alpha);
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] = fmaf(w, v[u][e], o[e] * alpha);
+    }
   }
-  store_dims<N, false>(a.out + row * a.out_row_stride + (int64_t)h * D + N * lane, o,
-                       L != 0.f ? 1.f / L : 0.f);
+  store_dims<N, false>(a.out + (int64_t)(d[1] + r / a.G) * a.out_row_stride +
+                           (int64_t)(d[3] * a.G + r % a.G) * D + N * lane,
+                       o, L != 0.f ? 1.f / L : 0.f);
 }
 
 struct ScaledPrefillPlan {
-  int groups, parts;
+  int groups;      // row groups a wave
+  bool split;
+  int64_t grid;    // workgroups
+  int64_t tiles;   // plain: tiles a sequence
+  size_t bytes(int D) const {  // of the workspace
+    return split ? grid * (sizeof(i32x4_t) + 2 * 64 * groups * part_floats(D) * sizeof(float)) : 0;
+  }
 };
 static ScaledPrefillPlan scaled_prefill_plan(int64_t n_seqs, int64_t total_q, int64_t max_q,
-                                             int64_t max_k, int32_t Hk, int g) {
+                                             int64_t max_k, int32_t Hk, int g, int D) {
   ScaledPrefillPlan p;
   const int cus = device_cus();
   p.groups = plain_groups(n_seqs, total_q, max_q, Hk, g, 2, cus);
   const BatchMix m = batch_mix(n_seqs, total_q, max_q);
   const int64_t qt = 64 * p.groups / g;
-  const int64_t tiles =
-      std::min(m.prompts * ((max_q + qt - 1) / qt), m.prompt_rows / qt + m.prompts) + m.rows;
-  const int64_t steps = (max_k + kStep - 1) / kStep;
-  p.parts = (int)std::max<int64_t>(
-      1, std::min<int64_t>({2 * cus / std::max<int64_t>(1, tiles * Hk), steps / 4, kMaxParts}));
+  const int64_t each = (max_q + qt - 1) / qt;
+  const int64_t tiles = std::min(m.prompts * each, m.prompt_rows / qt + m.prompts) + m.rows;
+  const int64_t most = std::min(n_seqs * each, total_q / qt + n_seqs);
+  p.tiles = plain_tiles(n_seqs, max_q, qt);
+  // workgroups that are resident at once: by the ring's LDS (69 KiB, 36 at head_dim 64), or registers
+  const int resident = cus * (D == 128 ? 2 : p.groups == 1 ? 4 : 3);
+  p.split = max_k >= 8 * kStep && each <= 96 && tiles * Hk <= 2 * resident && resident >= Hk &&
+            split_fits(n_seqs, most, max_k);
+  p.grid = p.split ? resident / Hk * Hk : n_seqs * p.tiles * Hk;
   return p;
 }
 
@@ -419,9 +578,8 @@ extern "C" size_t nkv_scaled_prefill_workspace_bytes(int32_t n_seqs, int64_t tot
       n_q_heads / n_kv_heads > NKV_SCALED_MAX_GROUP || !scaled_dim_ok(head_dim))
     return 0;
   const ScaledPrefillPlan p = scaled_prefill_plan(n_seqs, total_q, max_seqlen_q, max_seqlen_k,
-                                                  n_kv_heads, n_q_heads / n_kv_heads);
-  if (p.parts == 1) return 0;
-  return (size_t)total_q * n_q_heads * p.parts * prefill_part_row(head_dim) * sizeof(float);
+                                                  n_kv_heads, n_q_heads / n_kv_heads, head_dim);
+  return p.bytes(head_dim);
 }
 
 extern "C" int nkv_scaled_prefill(const void* q, int64_t q_row_stride, int64_t total_q,
@@ -435,7 +593,7 @@ extern "C" int nkv_scaled_prefill(const void* q, int64_t q_row_stride, int64_t t
                                   size_t workspace_bytes, void* stream) {
   using namespace nkv;
   clear_error();
-  NKV_REQUIRE(n_seqs >= 0 && total_q >= 0 && total_q < (1ll << 31) && max_seqlen_q >= 0 &&
+  NKV_REQUIRE(n_seqs >= 0 && total_q >= 0 && total_q <= (1 << 30) && max_seqlen_q >= 0 &&
                   n_q_heads > 0 && n_kv_heads > 0 && n_blocks >= 0,
               NKV_EINVAL, "scaled_prefill: bad sizes (%d sequences, %lld rows, Hq=%d, Hk=%d)",
               n_seqs, (long long)total_q, n_q_heads, n_kv_heads);
@@ -465,29 +623,29 @@ extern "C" int nkv_scaled_prefill(const void* q, int64_t q_row_stride, int64_t t
                   out_row_stride % 4 == 0,
               NKV_EINVAL, "scaled_prefill: row strides must cover Hq*D, q's in multiples of 8, "
               "out's of 4");
-  ScaledPrefillPlan p =
-      scaled_prefill_plan(n_seqs, total_q, max_seqlen_q, workspace ? max_seqlen_k : 0, n_kv_heads, g);
-  if (p.parts > 1) {
-    const size_t need =
-        (size_t)total_q * n_q_heads * p.parts * prefill_part_row(head_dim) * sizeof(float);
-    NKV_REQUIRE(aligned16(workspace) && workspace_bytes >= need, NKV_EWORKSPACE,
-                "scaled_prefill: workspace needs %zu bytes, 16-byte aligned (got %zu)", need,
-                workspace_bytes);
-  }
-  const int64_t qt = 64 * p.groups / g;
-  const int64_t tiles = plain_tiles(n_seqs, max_seqlen_q, qt);
-  const int64_t grid = n_seqs * tiles * n_kv_heads * p.parts;
-  NKV_REQUIRE(tiles < (1ll << 31) && grid < (1ll << 31), NKV_EUNSUPPORTED,
+  const ScaledPrefillPlan p = scaled_prefill_plan(n_seqs, total_q, max_seqlen_q,
+                                                  workspace ? max_seqlen_k : 0, n_kv_heads, g,
+                                                  head_dim);
+  NKV_REQUIRE(!p.split || (aligned16(workspace) && workspace_bytes >= p.bytes(head_dim)),
+              NKV_EWORKSPACE, "scaled_prefill: workspace needs %zu bytes, 16-byte aligned (got %zu)",
+              p.bytes(head_dim), workspace_bytes);
+  NKV_REQUIRE(p.tiles < (1ll << 31) && p.grid < (1ll << 31), NKV_EUNSUPPORTED,
               "scaled_prefill: too many tiles in one call");
+  i32x4_t* desc = static_cast<i32x4_t*>(workspace);
   const ScaledPrefillArgs a{(const bf16_t*)q, q_row_stride, (const char*)k_cache,
                             (const char*)v_cache, cu_seqlens_q, cu_seqlens_k, block_tables,
                             bt_row_stride, n_kv_heads, g, block_size, max_blocks_per_seq,
-                            (int32_t)n_blocks, n_seqs, (int32_t)tiles, p.parts, total_q,
-                            scale * kLog2e,
-                            (bf16_t*)out, out_row_stride, (float*)workspace};
-#define NKV_SCALED_PREFILL(D, RG)                                                          \
-  hipLaunchKernelGGL((scaled_prefill_kernel<D, RG>), dim3((unsigned)grid), dim3(256), 0, \
-                     as_stream(stream), a)
+                            (int32_t)n_blocks, n_seqs, (int32_t)p.tiles, total_q, scale * kLog2e,
+                            (bf16_t*)out, out_row_stride, desc,
+                            p.split ? reinterpret_cast<float*>(desc + p.grid) : nullptr};
+  const dim3 grid((unsigned)p.grid);
+#define NKV_SCALED_PREFILL_S(D, RG, SPLIT)                                                       \
+  hipLaunchKernelGGL((scaled_prefill_kernel<D, RG, SPLIT>), grid, dim3(256), 0, as_stream(stream), a)
+#define NKV_SCALED_PREFILL(D, RG)                       \
+  do {                                                  \
+    if (p.split) NKV_SCALED_PREFILL_S(D, RG, true);     \
+    else NKV_SCALED_PREFILL_S(D, RG, false);            \
+  } while (0)
   if (head_dim == 64) {
     if (p.groups == 1) NKV_SCALED_PREFILL(64, 1);
     else NKV_SCALED_PREFILL(64, 2);
@@ -496,15 +654,16 @@ extern "C" int nkv_scaled_prefill(const void* q, int64_t q_row_stride, int64_t t
     else NKV_SCALED_PREFILL(128, 2);
   }
 #undef NKV_SCALED_PREFILL
+#undef NKV_SCALED_PREFILL_S
   rc = check_launch("nkv_scaled_prefill");
-  if (rc || p.parts == 1) return rc;
-  const dim3 merge((unsigned)((total_q * n_q_heads + 3) / 4));
-  const int32_t max_rows = (int32_t)std::min<int64_t>(tiles * qt, INT32_MAX);
+  if (rc || !p.split) return rc;
+  const int32_t tile_rows = 64 * p.groups;
+  const dim3 merge((unsigned)p.grid, (unsigned)(tile_rows / 4));
   if (head_dim == 64)
     hipLaunchKernelGGL((scaled_merge_kernel<64>), merge, dim3(256), 0, as_stream(stream), a,
-                       max_rows);
+                       tile_rows);
   else
     hipLaunchKernelGGL((scaled_merge_kernel<128>), merge, dim3(256), 0, as_stream(stream), a,
-                       max_rows);
+                       tile_rows);
   return check_launch("nkv_scaled_prefill");
 }

@@ -60,8 +60,11 @@ class ScaledKVCachePool:
         return layer
 
 
+# ---------------------------------------------------------------- checks
+# Each operator passes its arguments by one expression where they are right; only for others does its
+# _refuse_* function look for what is wrong (with messages made and checks by name, they kept the host
+# busy for 8 to 20 us a call, longer than a small call runs).
 def _caches(what, k_cache, v_cache, row):
-    """Blocks and block size of caches whose rows hold ``row`` codes."""
     if not (k_cache.dtype is _U8 and v_cache.dtype is _U8 and k_cache.dim() == 3
             and v_cache.shape == k_cache.shape and k_cache.size(2) == row + ROW_PAD
             and k_cache.is_contiguous() and v_cache.is_contiguous()):
@@ -70,19 +73,17 @@ def _caches(what, k_cache, v_cache, row):
                          f"{v_cache.dtype} {tuple(v_cache.shape)}")
     if k_cache.size(1) % TILE or k_cache.size(1) == 0:
         raise ValueError(f"{what}: block_size {k_cache.size(1)} is not a multiple of {TILE}")
-    return k_cache.size(0), k_cache.size(1)
 
 
-def _kv_heads(what, k_cache, D):
-    """The KV heads of a cache of head_dim D."""
+def _heads_of(what, k_cache, D):
     row = k_cache.size(-1) - ROW_PAD
-    if row <= 0 or row % D:
+    if row <= 0 or D <= 0 or row % D:
         raise ValueError(f"{what}: the cache's rows of {row} codes are not heads of {D}")
-    return row // D
+    return row
 
 
-def _rows(what, name, t, dtype=_BF16):
-    if t.dim() != 3 or t.dtype is not dtype or t.stride(2) != 1 or t.stride(1) != t.size(2):
+def _rows(what, name, t):
+    if t.dim() != 3 or t.dtype is not _BF16 or t.stride(2) != 1 or t.stride(1) != t.size(2):
         raise ValueError(f"{what}: {name} must be bf16 [rows, heads, head_dim], rows of contiguous "
                          f"heads, got {t.dtype} {tuple(t.shape)}")
 
@@ -96,6 +97,96 @@ def _int32(what, name, t, n, dims=1):
                          f"{tuple(t.shape)}")
 
 
+def _out_rows(what, q, out):
+    if out is not None and (out.shape != q.shape or out.dtype is not _BF16 or out.stride(2) != 1
+                            or out.stride(1) != q.size(2)):
+        raise ValueError(f"{what}: out must be bf16 and shaped like q, rows of contiguous heads")
+
+
+def _workspace_ok(what, workspace):
+    if workspace is not None and (workspace.dtype is not _U8 or not workspace.is_contiguous()):
+        raise ValueError(f"{what}: workspace must be contiguous uint8")
+
+
+def _refuse_store(what, key, value, k_cache, v_cache, slot_mapping):
+    _lib.require_device(key.device, value=value, k_cache=k_cache, v_cache=v_cache,
+                        slot_mapping=slot_mapping)
+    _rows(what, "key", key)
+    _rows(what, "value", value)
+    N, Hk, D = key.shape
+    if value.shape != key.shape:
+        raise ValueError(f"{what}: value shape differs from key")
+    _caches(what, k_cache, v_cache, Hk * D)
+    _int32(what, "slot_mapping", slot_mapping, N)
+    if slot_mapping.numel() != N:
+        raise ValueError(f"{what}: {slot_mapping.numel()} slots for {N} rows")
+
+
+def _refuse_read(what, k_cache, v_cache, block_tables, cu_seqlens, n_tokens, Hk, starts, out):
+    _lib.require_device(k_cache.device, v_cache=v_cache, block_tables=block_tables,
+                        cu_seqlens=cu_seqlens, starts=starts)
+    row = k_cache.size(-1) - ROW_PAD
+    if Hk <= 0 or row <= 0 or row % Hk:
+        raise ValueError(f"{what}: the cache's rows of {row} codes are not {Hk} heads")
+    _caches(what, k_cache, v_cache, row)
+    n_seqs = cu_seqlens.numel() - 1
+    if n_seqs < 0 or n_tokens < 0:
+        raise ValueError(f"{what}: cu_seqlens needs one entry per sequence + 1, n_tokens >= 0")
+    _int32(what, "cu_seqlens", cu_seqlens, n_seqs + 1)
+    _int32(what, "block_tables", block_tables, n_seqs, 2)
+    if starts is not None:
+        _int32(what, "starts", starts, n_seqs)
+    if out is not None:
+        k, v = out
+        _lib.require_device(k_cache.device, k=k, v=v)
+        shape = (n_tokens, Hk, row // Hk)
+        for t in (k, v):
+            if t.shape != shape or t.dtype is not _BF16 or not t.is_contiguous():
+                raise ValueError(f"{what}: out must be two contiguous bf16 {shape}")
+
+
+def _refuse_decode(what, q, k_cache, v_cache, context_lens, block_tables, out, workspace):
+    _lib.require_device(q.device, k_cache=k_cache, v_cache=v_cache, context_lens=context_lens,
+                        block_tables=block_tables, out=out, workspace=workspace)
+    _rows(what, "q", q)
+    _caches(what, k_cache, v_cache, _heads_of(what, k_cache, q.size(2)))
+    _int32(what, "context_lens", context_lens, q.size(0))
+    _int32(what, "block_tables", block_tables, q.size(0), 2)
+    _workspace_ok(what, workspace)
+    _out_rows(what, q, out)
+
+
+def _refuse_prefill(what, q, k_cache, v_cache, cu_q, cu_k, block_tables, out, workspace):
+    _lib.require_device(q.device, k_cache=k_cache, v_cache=v_cache, cu_seqlens_q=cu_q,
+                        cu_seqlens_k=cu_k, block_tables=block_tables, out=out, workspace=workspace)
+    _rows(what, "q", q)
+    _caches(what, k_cache, v_cache, _heads_of(what, k_cache, q.size(2)))
+    n_seqs = cu_q.numel() - 1
+    if n_seqs < 0 or cu_k.numel() != n_seqs + 1:
+        raise ValueError(f"{what}: cu_seqlens_q and cu_seqlens_k need one entry per sequence + 1")
+    _int32(what, "cu_seqlens_q", cu_q, n_seqs + 1)
+    _int32(what, "cu_seqlens_k", cu_k, n_seqs + 1)
+    _int32(what, "block_tables", block_tables, n_seqs, 2)
+    _workspace_ok(what, workspace)
+    _out_rows(what, q, out)
+
+
+def _caches_right(k_cache, v_cache, cs, di):
+    return (len(cs) == 3 and v_cache.shape == cs and k_cache.dtype is _U8 and v_cache.dtype is _U8
+            and k_cache.get_device() == di and v_cache.get_device() == di and cs[1] > 0
+            and cs[1] % TILE == 0 and k_cache.is_contiguous() and v_cache.is_contiguous())
+
+
+def _entries_right(t, di):
+    return t.dtype is _I32 and t.get_device() == di and t.dim() == 1 and t.is_contiguous()
+
+
+def _tables_right(t, shape, di, n):
+    return (len(shape) == 2 and shape[0] >= n and shape[1] > 0 and t.dtype is _I32
+            and t.get_device() == di and t.stride(1) == 1)
+
+
+# ---------------------------------------------------------------- the operators
 def scaled_store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
                          v_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
     """Rows key[i] and value[i] ([N, Hk, D]) into row slot_mapping[i]; -1 slots are skipped.
@@ -106,22 +197,19 @@ def scaled_store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.
     sequence do.
     """
     what = "scaled_store_kvcache"
-    _lib.require_device(key.device, value=value, k_cache=k_cache, v_cache=v_cache,
-                        slot_mapping=slot_mapping)
-    _rows(what, "key", key)
-    _rows(what, "value", value)
-    N, Hk, D = key.shape
-    if value.shape != key.shape:
-        raise ValueError(f"{what}: value shape differs from key")
-    NB, B = _caches(what, k_cache, v_cache, Hk * D)
-    _int32(what, "slot_mapping", slot_mapping, N)
-    if slot_mapping.numel() != N:
-        raise ValueError(f"{what}: {slot_mapping.numel()} slots for {N} rows")
-    with _lib.device_of(key.get_device()):
-        rc = _lib.lib().nkv_scaled_store(key.data_ptr(), key.stride(0), value.data_ptr(),
-                                         value.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
-                                         slot_mapping.data_ptr(), N, Hk, D, NB * B,
-                                         _lib.stream_of(key))
+    ks, cs, di = key.shape, k_cache.shape, key.get_device()
+    k_st, v_st = key.stride(), value.stride()
+    if not (di >= 0 and len(ks) == 3 and value.shape == ks and value.get_device() == di
+            and key.dtype is _BF16 and value.dtype is _BF16 and k_st[2] == 1 and v_st[2] == 1
+            and k_st[1] == ks[2] and v_st[1] == ks[2] and _caches_right(k_cache, v_cache, cs, di)
+            and cs[2] == ks[1] * ks[2] + ROW_PAD and _entries_right(slot_mapping, di)
+            and slot_mapping.size(0) == ks[0]):
+        _refuse_store(what, key, value, k_cache, v_cache, slot_mapping)
+    with _lib.device_of(di):
+        rc = _lib.lib().nkv_scaled_store(key.data_ptr(), k_st[0], value.data_ptr(), v_st[0],
+                                         k_cache.data_ptr(), v_cache.data_ptr(),
+                                         slot_mapping.data_ptr(), ks[0], ks[1], ks[2],
+                                         cs[0] * cs[1], torch._C._cuda_getCurrentRawStream(di))
     if rc:
         _lib.check(rc, what)
 
@@ -137,51 +225,29 @@ def scaled_read_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tabl
     of the outputs [n_tokens, Hk, D] (``out``, or new ones; rows of no sequence are left as they
     are). Positions that its table has no valid block for read as zeros.
     """
-    what = "scaled_read_kvcache"
-    _lib.require_device(k_cache.device, v_cache=v_cache, block_tables=block_tables,
-                        cu_seqlens=cu_seqlens, starts=starts)
-    Hk, row = num_kv_heads, k_cache.size(-1) - ROW_PAD
-    if Hk <= 0 or row <= 0 or row % Hk:
-        raise ValueError(f"{what}: the cache's rows of {row} codes are not {Hk} heads")
+    what, Hk = "scaled_read_kvcache", num_kv_heads
+    cs, bs, di = k_cache.shape, block_tables.shape, k_cache.get_device()
+    row, n = cs[-1] - ROW_PAD, cu_seqlens.numel() - 1
+    if not (di >= 0 and _caches_right(k_cache, v_cache, cs, di) and Hk > 0 and row > 0
+            and row % Hk == 0 and n >= 0 and n_tokens >= 0 and _entries_right(cu_seqlens, di)
+            and _tables_right(block_tables, bs, di, n)
+            and (starts is None or _entries_right(starts, di) and starts.size(0) >= n)
+            and out is None):
+        _refuse_read(what, k_cache, v_cache, block_tables, cu_seqlens, n_tokens, Hk, starts, out)
     D = row // Hk
-    NB, B = _caches(what, k_cache, v_cache, row)
-    n_seqs = cu_seqlens.numel() - 1
-    if n_seqs < 0 or n_tokens < 0:
-        raise ValueError(f"{what}: cu_seqlens needs one entry per sequence + 1, n_tokens >= 0")
-    _int32(what, "cu_seqlens", cu_seqlens, n_seqs + 1)
-    _int32(what, "block_tables", block_tables, n_seqs, 2)
-    if starts is not None:
-        _int32(what, "starts", starts, n_seqs)
-    shape = (n_tokens, Hk, D)
-    if out is None:
-        out = tuple(torch.empty(shape, dtype=_BF16, device=k_cache.device) for _ in range(2))
-    k, v = out
-    _lib.require_device(k_cache.device, k=k, v=v)
-    for t in out:
-        if t.shape != shape or t.dtype is not _BF16 or not t.is_contiguous():
-            raise ValueError(f"{what}: out must be two contiguous bf16 {shape}")
-    with _lib.device_of(k_cache.get_device()):
+    with _lib.device_of(di):
+        if out is None:
+            device = k_cache.device
+            out = (torch.empty((n_tokens, Hk, D), dtype=_BF16, device=device),
+                   torch.empty((n_tokens, Hk, D), dtype=_BF16, device=device))
         rc = _lib.lib().nkv_scaled_read(
             k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
-            block_tables.size(1), cu_seqlens.data_ptr(), _lib.ptr(starts), n_seqs, n_tokens, Hk, D,
-            B, NB, k.data_ptr(), v.data_ptr(), _lib.stream_of(k_cache))
+            bs[1], cu_seqlens.data_ptr(), None if starts is None else starts.data_ptr(), n, n_tokens,
+            Hk, D, cs[1], cs[0], out[0].data_ptr(), out[1].data_ptr(),
+            torch._C._cuda_getCurrentRawStream(di))
     if rc:
         _lib.check(rc, what)
     return out
-
-
-def _out(what, q, out):
-    if out is None:
-        return q.new_empty(q.shape)
-    if out.shape != q.shape or out.dtype is not _BF16 or out.stride(2) != 1 \
-            or out.stride(1) != q.size(2):
-        raise ValueError(f"{what}: out must be bf16 and shaped like q, rows of contiguous heads")
-    return out
-
-
-def _workspace_ok(what, workspace):
-    if workspace is not None and (workspace.dtype is not _U8 or not workspace.is_contiguous()):
-        raise ValueError(f"{what}: workspace must be contiguous uint8")
 
 
 def scaled_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -194,29 +260,34 @@ def scaled_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     of length 0 gives zeros.
     """
     what = "scaled_paged_decode"
-    _lib.require_device(q.device, k_cache=k_cache, v_cache=v_cache, context_lens=context_lens,
-                        block_tables=block_tables, out=out, workspace=workspace)
-    _rows(what, "q", q)
-    bs, Hq, D = q.shape
-    Hk = _kv_heads(what, k_cache, D)
-    NB, B = _caches(what, k_cache, v_cache, Hk * D)
-    _int32(what, "context_lens", context_lens, bs)
-    _int32(what, "block_tables", block_tables, bs, 2)
-    _workspace_ok(what, workspace)
-    out = _out(what, q, out)
-    with _lib.device_of(q.get_device()):
-        width = block_tables.size(1)
+    qs, cs, bs, di = q.shape, k_cache.shape, block_tables.shape, q.get_device()
+    q_st = q.stride()
+    if not (di >= 0 and len(qs) == 3 and q.dtype is _BF16 and q_st[2] == 1 and q_st[1] == qs[2] > 0
+            and _caches_right(k_cache, v_cache, cs, di) and cs[2] > ROW_PAD
+            and (cs[2] - ROW_PAD) % qs[2] == 0 and _entries_right(context_lens, di)
+            and context_lens.size(0) >= qs[0] and _tables_right(block_tables, bs, di, qs[0])
+            and out is None and workspace is None):
+        _refuse_decode(what, q, k_cache, v_cache, context_lens, block_tables, out, workspace)
+    n, Hq, D = qs
+    lib = _lib.lib()
+    with _lib.device_of(di):
+        if out is None:
+            out = torch.empty(qs, dtype=_BF16, device=q.device)
         if workspace is None:
-            nbytes = _lib.lib().nkv_paged_decode_workspace_bytes(bs, Hq, D, width, B)
+            nbytes = lib.nkv_paged_decode_workspace_bytes(n, Hq, D, bs[1], cs[1])
             workspace = torch.empty(max(nbytes, 4), dtype=_U8, device=q.device)
-        rc = _lib.lib().nkv_scaled_decode(
-            q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
-            block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(), bs, Hq, Hk, D,
-            B, width, NB, scale, out.data_ptr(), out.stride(0), workspace.data_ptr(),
-            workspace.numel(), _lib.stream_of(q))
+        rc = lib.nkv_scaled_decode(
+            q.data_ptr(), q_st[0], k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
+            block_tables.stride(0), context_lens.data_ptr(), n, Hq, (cs[2] - ROW_PAD) // D, D, cs[1],
+            bs[1], cs[0], scale, out.data_ptr(), out.stride(0), workspace.data_ptr(),
+            workspace.numel(), torch._C._cuda_getCurrentRawStream(di))
     if rc:
         _lib.check(rc, what)
     return out
+
+
+# Steps of fewer keys are not split: the plan need not be asked.
+_SPLIT_MIN_KEYS = 512
 
 
 def scaled_prefill_workspace(q: torch.Tensor, k_cache: torch.Tensor, n_seqs: int,
@@ -224,10 +295,12 @@ def scaled_prefill_workspace(q: torch.Tensor, k_cache: torch.Tensor, n_seqs: int
     """The workspace for splitting scaled_varlen_prefill's keys where few query tiles would leave the
     chip idle, else None; None too where the device has no such memory left, since nothing else
     needs any."""
+    if max_seqlen_k < _SPLIT_MIN_KEYS:
+        return None
     D = q.size(2)
     nbytes = _lib.lib().nkv_scaled_prefill_workspace_bytes(
         n_seqs, q.size(0), int(max_seqlen_q), int(max_seqlen_k), q.size(1),
-        _kv_heads("scaled_varlen_prefill", k_cache, D), D)
+        (k_cache.size(2) - ROW_PAD) // D, D)
     try:
         return torch.empty(nbytes, dtype=_U8, device=q.device) if nbytes else None
     except torch.OutOfMemoryError:
@@ -247,31 +320,29 @@ def scaled_varlen_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     key gives zeros; what keys hold that a row does not see has no effect on it.
     """
     what = "scaled_varlen_prefill"
-    _lib.require_device(q.device, k_cache=k_cache, v_cache=v_cache, cu_seqlens_q=cu_seqlens_q,
-                        cu_seqlens_k=cu_seqlens_k, block_tables=block_tables, out=out,
-                        workspace=workspace)
-    _rows(what, "q", q)
-    N, Hq, D = q.shape
-    Hk = _kv_heads(what, k_cache, D)
-    NB, B = _caches(what, k_cache, v_cache, Hk * D)
-    n_seqs = cu_seqlens_q.numel() - 1
-    if n_seqs < 0 or cu_seqlens_k.numel() != n_seqs + 1:
-        raise ValueError(f"{what}: cu_seqlens_q and cu_seqlens_k need one entry per sequence + 1")
-    _int32(what, "cu_seqlens_q", cu_seqlens_q, n_seqs + 1)
-    _int32(what, "cu_seqlens_k", cu_seqlens_k, n_seqs + 1)
-    _int32(what, "block_tables", block_tables, n_seqs, 2)
-    _workspace_ok(what, workspace)
-    out = _out(what, q, out)
-    with _lib.device_of(q.get_device()):
+    qs, cs, bs, di = q.shape, k_cache.shape, block_tables.shape, q.get_device()
+    q_st, n = q.stride(), cu_seqlens_q.numel() - 1
+    if not (di >= 0 and len(qs) == 3 and q.dtype is _BF16 and q_st[2] == 1 and q_st[1] == qs[2] > 0
+            and _caches_right(k_cache, v_cache, cs, di) and cs[2] > ROW_PAD
+            and (cs[2] - ROW_PAD) % qs[2] == 0 and n >= 0 and _entries_right(cu_seqlens_q, di)
+            and _entries_right(cu_seqlens_k, di) and cu_seqlens_k.size(0) == n + 1
+            and _tables_right(block_tables, bs, di, n) and out is None and workspace is None):
+        _refuse_prefill(what, q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_tables, out,
+                        workspace)
+    D = qs[2]
+    with _lib.device_of(di):
+        if out is None:
+            out = torch.empty(qs, dtype=_BF16, device=q.device)
         if workspace is None and max_seqlen_k is not None:
-            workspace = scaled_prefill_workspace(q, k_cache, n_seqs, max_seqlen_q, max_seqlen_k)
+            workspace = scaled_prefill_workspace(q, k_cache, n, max_seqlen_q, max_seqlen_k)
         rc = _lib.lib().nkv_scaled_prefill(
-            q.data_ptr(), q.stride(0), N, k_cache.data_ptr(), v_cache.data_ptr(),
+            q.data_ptr(), q_st[0], qs[0], k_cache.data_ptr(), v_cache.data_ptr(),
             cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), block_tables.data_ptr(),
-            block_tables.stride(0), block_tables.size(1), n_seqs, int(max_seqlen_q),
-            0 if max_seqlen_k is None else int(max_seqlen_k), Hq, Hk, D, B, NB, scale,
-            out.data_ptr(), out.stride(0), _lib.ptr(workspace),
-            0 if workspace is None else workspace.numel(), _lib.stream_of(q))
+            block_tables.stride(0), bs[1], n, int(max_seqlen_q),
+            0 if max_seqlen_k is None else int(max_seqlen_k), qs[1], (cs[2] - ROW_PAD) // D, D, cs[1],
+            cs[0], scale, out.data_ptr(), out.stride(0),
+            None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel(), torch._C._cuda_getCurrentRawStream(di))
     if rc:
         _lib.check(rc, what)
     return out
