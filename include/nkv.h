@@ -856,7 +856,8 @@ int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info, 
  *   K: byte ((t*(D/64) + i)*64 + r + 16*g)*16 + b is token 8*(r/4) + 4*t + r%4
  *      (r < 16, t < 2), dim 64*i + 16*g + b
  *   V: byte (j*64 + c + 16*g)*16 + 8*u + tt is token 8*g + tt, dim 32*j + 16*u + c
- * head_dim D 64 or 128; q, k, v and outputs are bf16; caches 16-byte aligned.
+ * head_dim D 64 or 128; q, k, v and outputs are bf16; caches 16-byte aligned. The
+ * calls take their arguments as one block of 8-byte fields.
  * No counterpart in the reference (beside the pool of ModelRunner.
  * allocate_kv_cache, nanokvllm/engine/model_runner.py:133-152).
  */
@@ -876,10 +877,17 @@ int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info, 
  * order, as tokens listed sequence by sequence do (of two for one slot the later
  * stays); what a tile holds whose tokens stand in two places is undefined.
  */
-int nkv_scaled_store(const void* key, int64_t key_row_stride, const void* value,
-                     int64_t value_row_stride, void* k_cache, void* v_cache,
-                     const int32_t* slot_mapping, int64_t n_tokens, int32_t n_kv_heads,
-                     int32_t head_dim, int64_t n_slots, void* stream);
+typedef struct nkv_scaled_store_args {
+  const void* key;
+  int64_t key_row_stride;
+  const void* value;
+  int64_t value_row_stride;
+  void *k_cache, *v_cache;
+  const int32_t* slot_mapping;
+  int64_t n_tokens, n_kv_heads, head_dim, n_slots;
+  void* stream;
+} nkv_scaled_store_args;
+int nkv_scaled_store(const nkv_scaled_store_args* args);
 
 /*
  * Rows of a block-scaled cache as bf16 (exact: code * 2^e). Sequence i's tokens at
@@ -890,11 +898,16 @@ int nkv_scaled_store(const void* key, int64_t key_row_stride, const void* value,
  * table or in an invalid block read as zeros. At most 2^20 sequences and 2^27
  * tokens.
  */
-int nkv_scaled_read(const void* k_cache, const void* v_cache, const int32_t* block_tables,
-                    int64_t bt_row_stride, int32_t max_blocks_per_seq, const int32_t* cu_seqlens,
-                    const int32_t* starts, int32_t n_seqs, int64_t n_tokens, int32_t n_kv_heads,
-                    int32_t head_dim, int32_t block_size, int64_t n_blocks, void* k_out,
-                    void* v_out, void* stream);
+typedef struct nkv_scaled_read_args {
+  const void *k_cache, *v_cache;
+  const int32_t* block_tables;
+  int64_t bt_row_stride, max_blocks_per_seq;
+  const int32_t *cu_seqlens, *starts;
+  int64_t n_seqs, n_tokens, n_kv_heads, head_dim, block_size, n_blocks;
+  void *k_out, *v_out;
+  void* stream;
+} nkv_scaled_read_args;
+int nkv_scaled_read(const nkv_scaled_read_args* args);
 
 /*
  * Attention of one new token per sequence over block-scaled caches: the arguments
@@ -905,13 +918,22 @@ int nkv_scaled_read(const void* k_cache, const void* v_cache, const int32_t* blo
  * sequence's end has no effect.
  * No counterpart in the reference (beside nanokvllm/layers/attention.py:104-107).
  */
-int nkv_scaled_decode(const void* q, int64_t q_row_stride, const void* k_cache,
-                      const void* v_cache, const int32_t* block_tables, int64_t bt_row_stride,
-                      const int32_t* context_lens, int32_t batch, int32_t n_q_heads,
-                      int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
-                      int32_t max_blocks_per_seq, int64_t n_blocks, float scale, void* out,
-                      int64_t out_row_stride, void* workspace, size_t workspace_bytes,
-                      void* stream);
+typedef struct nkv_scaled_decode_args {
+  const void* q;
+  int64_t q_row_stride;
+  const void *k_cache, *v_cache;
+  const int32_t* block_tables;
+  int64_t bt_row_stride;
+  const int32_t* context_lens;
+  int64_t batch, n_q_heads, n_kv_heads, head_dim, block_size, max_blocks_per_seq, n_blocks;
+  void* out;
+  int64_t out_row_stride;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+  double scale;
+} nkv_scaled_decode_args;
+int nkv_scaled_decode(const nkv_scaled_decode_args* args);
 
 /*
  * Varlen causal (bottom-right) attention over block-scaled caches: the arguments
@@ -927,17 +949,24 @@ int nkv_scaled_decode(const void* q, int64_t q_row_stride, const void* k_cache,
  * No counterpart in the reference (beside nanokvllm/layers/attention.py:96-102).
  */
 #define NKV_SCALED_MAX_GROUP 128
+typedef struct nkv_scaled_prefill_args {
+  const void* q;
+  int64_t q_row_stride, total_q;
+  const void *k_cache, *v_cache;
+  const int32_t *cu_seqlens_q, *cu_seqlens_k, *block_tables;
+  int64_t bt_row_stride, max_blocks_per_seq, n_seqs, max_seqlen_q, max_seqlen_k, n_q_heads,
+      n_kv_heads, head_dim, block_size, n_blocks;
+  void* out;
+  int64_t out_row_stride;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+  double scale;
+} nkv_scaled_prefill_args;
 size_t nkv_scaled_prefill_workspace_bytes(int32_t n_seqs, int64_t total_q, int64_t max_seqlen_q,
                                           int64_t max_seqlen_k, int32_t n_q_heads,
                                           int32_t n_kv_heads, int32_t head_dim);
-int nkv_scaled_prefill(const void* q, int64_t q_row_stride, int64_t total_q, const void* k_cache,
-                       const void* v_cache, const int32_t* cu_seqlens_q,
-                       const int32_t* cu_seqlens_k, const int32_t* block_tables,
-                       int64_t bt_row_stride, int32_t max_blocks_per_seq, int32_t n_seqs,
-                       int64_t max_seqlen_q, int64_t max_seqlen_k, int32_t n_q_heads,
-                       int32_t n_kv_heads, int32_t head_dim, int32_t block_size, int64_t n_blocks,
-                       float scale, void* out, int64_t out_row_stride, void* workspace,
-                       size_t workspace_bytes, void* stream);
+int nkv_scaled_prefill(const nkv_scaled_prefill_args* args);
 
 /*
  * Differential attention over the same caches. Heads stand in pairs: query

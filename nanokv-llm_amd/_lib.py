@@ -135,15 +135,11 @@ SIGNATURES = {
     "nkv_diff_prefill": (C.c_int, [_i32, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p, _i64,
                                    _i32, _i32, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _f32,
                                    _f32, _f32, _p, _f32, _p, _f32, _p, _i64, _p, _sz, _p]),
-    "nkv_scaled_store": (C.c_int, [_p, _i64, _p, _i64, _p, _p, _p, _i64, _i32, _i32, _i64, _p]),
-    "nkv_scaled_read": (C.c_int, [_p, _p, _p, _i64, _i32, _p, _p, _i32, _i64, _i32, _i32, _i32, _i64,
-                                  _p, _p, _p]),
-    "nkv_scaled_decode": (C.c_int, [_p, _i64, _p, _p, _p, _i64, _p, _i32, _i32, _i32, _i32, _i32,
-                                    _i32, _i64, _f32, _p, _i64, _p, _sz, _p]),
+    "nkv_scaled_store": (C.c_int, [C.c_char_p]),  # each its packed block of arguments
+    "nkv_scaled_read": (C.c_int, [C.c_char_p]),
+    "nkv_scaled_decode": (C.c_int, [C.c_char_p]),
+    "nkv_scaled_prefill": (C.c_int, [C.c_char_p]),
     "nkv_scaled_prefill_workspace_bytes": (_sz, [_i32, _i64, _i64, _i64, _i32, _i32, _i32]),
-    "nkv_scaled_prefill": (C.c_int, [_p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i64,
-                                     _i64, _i32, _i32, _i32, _i32, _i64, _f32, _p, _i64, _p, _sz,
-                                     _p]),
     # the first argument: a packed nkv_pages
     "nkv_pages_workspace_bytes": (_sz, [_i64]),
     "nkv_pages_append": (C.c_int, [C.c_char_p, _p, _i32, _p, _i64, _p, _p, _p]),

@@ -28,7 +28,7 @@ namespace nkv {
 constexpr int kTileRows = 32;
 constexpr int kRowPad = 16;  // bytes of a row beside its codes (NKV_SCALED_ROW_PAD)
 constexpr int kMinScale = 127 - 100, kMaxScale = 127 + 119;  // bytes
-constexpr bool scaled_dim_ok(int D) { return D == 64 || D == 128; }
+constexpr bool scaled_dim_ok(int64_t D) { return D == 64 || D == 128; }
 
 // Offset of the eight codes of dims 8 hx .. 8 hx + 7 of a token in a head's K tile.
 template <int D>
@@ -71,7 +71,12 @@ __device__ __forceinline__ u32x4_t codes_to_bf16(uint32_t lo, uint32_t hi, float
 }
 
 // What every operator over such caches checks (0: fine).
-int scaled_check(const char* what, const void* k_cache, const void* v_cache, int32_t n_kv_heads,
-                 int32_t head_dim);
+int scaled_check(const char* what, const void* k_cache, const void* v_cache, int64_t n_kv_heads,
+                 int64_t head_dim);
+int scaled_check_tables(const char* what, const int32_t* block_tables, int64_t bt_row_stride,
+                        int64_t max_blocks, int64_t block_size, int64_t n_blocks);
+// ... and attention's: the query heads and the scale.
+int scaled_check_heads(const char* what, int64_t n_q_heads, int64_t n_kv_heads, int64_t most,
+                       double scale);
 
 }  // namespace nkv

@@ -22,14 +22,28 @@ namespace nkv {
 
 constexpr int kScaledWaves = 4;  // of a workgroup: as many heads (or pairs), of K or V
 
-int scaled_check(const char* what, const void* k_cache, const void* v_cache, int32_t n_kv_heads,
-                 int32_t head_dim) {
-  NKV_REQUIRE(scaled_dim_ok(head_dim), NKV_EUNSUPPORTED, "%s: head_dim must be 64 or 128 (got %d)",
-              what, head_dim);
+int scaled_check(const char* what, const void* k_cache, const void* v_cache, int64_t n_kv_heads,
+                 int64_t head_dim) {
+  NKV_REQUIRE(scaled_dim_ok(head_dim), NKV_EUNSUPPORTED, "%s: head_dim must be 64 or 128 (got %lld)",
+              what, (long long)head_dim);
   NKV_REQUIRE(n_kv_heads > 0 && n_kv_heads <= NKV_SCALED_MAX_HEADS, NKV_EUNSUPPORTED,
-              "%s: 1 to %d KV heads (got %d)", what, NKV_SCALED_MAX_HEADS, n_kv_heads);
+              "%s: 1 to %d KV heads (got %lld)", what, NKV_SCALED_MAX_HEADS, (long long)n_kv_heads);
   NKV_REQUIRE(k_cache && v_cache && aligned16(k_cache) && aligned16(v_cache), NKV_EINVAL,
               "%s: caches must be given, 16-byte aligned", what);
+  return NKV_OK;
+}
+int scaled_check_tables(const char* what, const int32_t* block_tables, int64_t bt_row_stride,
+                        int64_t max_blocks, int64_t block_size, int64_t n_blocks) {
+  NKV_REQUIRE(block_size > 0 && block_size % kTileRows == 0, NKV_EUNSUPPORTED,
+              "%s: block_size must be a multiple of %d (got %lld)", what, kTileRows,
+              (long long)block_size);
+  NKV_REQUIRE(max_blocks > 0 && bt_row_stride >= max_blocks, NKV_EINVAL,
+              "%s: bad block table width/stride (%lld, %lld)", what, (long long)max_blocks,
+              (long long)bt_row_stride);
+  NKV_REQUIRE(n_blocks <= INT32_MAX && block_size < (1ll << 30) &&
+                  max_blocks < (1ll << 30) / block_size,
+              NKV_EUNSUPPORTED, "%s: max_blocks_per_seq * block_size too large", what);
+  NKV_REQUIRE(block_tables, NKV_EINVAL, "%s: null block_tables", what);
   return NKV_OK;
 }
 
@@ -339,77 +353,72 @@ __global__ __launch_bounds__(64 * kScaledWaves) void scaled_read_kernel(
 
 }  // namespace nkv
 
-extern "C" int nkv_scaled_store(const void* key, int64_t key_row_stride, const void* value,
-                                int64_t value_row_stride, void* k_cache, void* v_cache,
-                                const int32_t* slot_mapping, int64_t n_tokens, int32_t n_kv_heads,
-                                int32_t head_dim, int64_t n_slots, void* stream) {
+extern "C" int nkv_scaled_store(const nkv_scaled_store_args* args) {
   using namespace nkv;
   clear_error();
-  NKV_REQUIRE(n_tokens >= 0 && n_tokens < (1ll << 31) && n_slots >= 0, NKV_EINVAL,
-              "scaled_store: bad sizes (%lld tokens, %lld slots)", (long long)n_tokens,
-              (long long)n_slots);
-  if (n_tokens == 0) return NKV_OK;
-  const int rc = scaled_check("scaled_store", k_cache, v_cache, n_kv_heads, head_dim);
+  NKV_REQUIRE(args, NKV_EINVAL, "scaled_store: null arguments");
+  const nkv_scaled_store_args& g = *args;
+  NKV_REQUIRE(g.n_tokens >= 0 && g.n_tokens < (1ll << 31) && g.n_slots >= 0, NKV_EINVAL,
+              "scaled_store: bad sizes (%lld tokens, %lld slots)", (long long)g.n_tokens,
+              (long long)g.n_slots);
+  if (g.n_tokens == 0) return NKV_OK;
+  const int rc = scaled_check("scaled_store", g.k_cache, g.v_cache, g.n_kv_heads, g.head_dim);
   if (rc) return rc;
-  const int64_t row = (int64_t)n_kv_heads * head_dim;
-  NKV_REQUIRE(n_slots % kTileRows == 0, NKV_EINVAL,
+  const int64_t row = g.n_kv_heads * g.head_dim;
+  NKV_REQUIRE(g.n_slots % kTileRows == 0, NKV_EINVAL,
               "scaled_store: the slots must be whole tiles of %d (got %lld)", kTileRows,
-              (long long)n_slots);
-  NKV_REQUIRE(key && value && slot_mapping && aligned16(key) && aligned16(value), NKV_EINVAL,
-              "scaled_store: null or misaligned pointer");
-  NKV_REQUIRE(key_row_stride >= row && value_row_stride >= row && key_row_stride % 8 == 0 &&
-                  value_row_stride % 8 == 0,
+              (long long)g.n_slots);
+  NKV_REQUIRE(g.key && g.value && g.slot_mapping && aligned16(g.key) && aligned16(g.value),
+              NKV_EINVAL, "scaled_store: null or misaligned pointer");
+  NKV_REQUIRE(g.key_row_stride >= row && g.value_row_stride >= row && g.key_row_stride % 8 == 0 &&
+                  g.value_row_stride % 8 == 0,
               NKV_EINVAL, "scaled_store: row strides must be multiples of 8 covering the row");
-  const int units = scaled_units(n_kv_heads, head_dim);
-  const int window = n_tokens * units <= 8192 ? 1 : 8;
-  const dim3 grid((unsigned)((n_tokens + window - 1) / window),
+  const int Hk = (int)g.n_kv_heads, units = scaled_units(Hk, (int)g.head_dim);
+  const int window = g.n_tokens * units <= 8192 ? 1 : 8;
+  const dim3 grid((unsigned)((g.n_tokens + window - 1) / window),
                   (unsigned)((units + kScaledWaves - 1) / kScaledWaves));
-#define NKV_SCALED_STORE(D)                                                                     \
-  hipLaunchKernelGGL((scaled_store_kernel<D>), grid, dim3(64 * kScaledWaves), 0,                \
-                     as_stream(stream), (const bf16_t*)key, key_row_stride,                     \
-                     (const bf16_t*)value, value_row_stride, (char*)k_cache, (char*)v_cache,    \
-                     slot_mapping, n_tokens, n_kv_heads, n_slots, units, window)
-  if (head_dim == 64) NKV_SCALED_STORE(64);
+#define NKV_SCALED_STORE(D)                                                                      \
+  hipLaunchKernelGGL((scaled_store_kernel<D>), grid, dim3(64 * kScaledWaves), 0,                 \
+                     as_stream(g.stream), (const bf16_t*)g.key, g.key_row_stride,                \
+                     (const bf16_t*)g.value, g.value_row_stride, (char*)g.k_cache,               \
+                     (char*)g.v_cache, g.slot_mapping, g.n_tokens, Hk, g.n_slots, units, window)
+  if (g.head_dim == 64) NKV_SCALED_STORE(64);
   else NKV_SCALED_STORE(128);
 #undef NKV_SCALED_STORE
   return check_launch("nkv_scaled_store");
 }
 
-extern "C" int nkv_scaled_read(const void* k_cache, const void* v_cache,
-                               const int32_t* block_tables, int64_t bt_row_stride,
-                               int32_t max_blocks_per_seq, const int32_t* cu_seqlens,
-                               const int32_t* starts, int32_t n_seqs, int64_t n_tokens,
-                               int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
-                               int64_t n_blocks, void* k_out, void* v_out, void* stream) {
+extern "C" int nkv_scaled_read(const nkv_scaled_read_args* args) {
   using namespace nkv;
   clear_error();
-  NKV_REQUIRE(n_seqs >= 0 && n_tokens >= 0 && n_blocks >= 0, NKV_EINVAL,
-              "scaled_read: bad sizes (%d sequences, %lld tokens)", n_seqs, (long long)n_tokens);
+  NKV_REQUIRE(args, NKV_EINVAL, "scaled_read: null arguments");
+  const nkv_scaled_read_args& g = *args;
+  NKV_REQUIRE(g.n_seqs >= 0 && g.n_tokens >= 0 && g.n_blocks >= 0, NKV_EINVAL,
+              "scaled_read: bad sizes (%lld sequences, %lld tokens)", (long long)g.n_seqs,
+              (long long)g.n_tokens);
   // 64 sequences' tiles add up within 32 bits, whatever cu_seqlens holds
-  NKV_REQUIRE(n_seqs <= (1 << 20) && n_tokens <= (1 << 27), NKV_EUNSUPPORTED,
-              "scaled_read: at most 2^20 sequences and 2^27 tokens (got %d, %lld)", n_seqs,
-              (long long)n_tokens);
-  if (n_seqs == 0 || n_tokens == 0) return NKV_OK;
-  const int rc = scaled_check("scaled_read", k_cache, v_cache, n_kv_heads, head_dim);
+  NKV_REQUIRE(g.n_seqs <= (1 << 20) && g.n_tokens <= (1 << 27), NKV_EUNSUPPORTED,
+              "scaled_read: at most 2^20 sequences and 2^27 tokens (got %lld, %lld)",
+              (long long)g.n_seqs, (long long)g.n_tokens);
+  if (g.n_seqs == 0 || g.n_tokens == 0) return NKV_OK;
+  int rc = scaled_check("scaled_read", g.k_cache, g.v_cache, g.n_kv_heads, g.head_dim);
   if (rc) return rc;
-  NKV_REQUIRE(block_size > 0 && block_size % kTileRows == 0, NKV_EUNSUPPORTED,
-              "scaled_read: block_size must be a multiple of %d (got %d)", kTileRows, block_size);
-  NKV_REQUIRE(max_blocks_per_seq > 0 && bt_row_stride >= max_blocks_per_seq, NKV_EINVAL,
-              "scaled_read: bad block table width/stride (%d, %lld)", max_blocks_per_seq,
-              (long long)bt_row_stride);
-  NKV_REQUIRE(block_tables && cu_seqlens && k_out && v_out && aligned16(k_out) && aligned16(v_out),
+  rc = scaled_check_tables("scaled_read", g.block_tables, g.bt_row_stride, g.max_blocks_per_seq,
+                           g.block_size, g.n_blocks);
+  if (rc) return rc;
+  NKV_REQUIRE(g.cu_seqlens && g.k_out && g.v_out && aligned16(g.k_out) && aligned16(g.v_out),
               NKV_EINVAL, "scaled_read: null or misaligned pointer");
-  const int units = scaled_units(n_kv_heads, head_dim);
+  const int Hk = (int)g.n_kv_heads, units = scaled_units(Hk, (int)g.head_dim);
   // n rows reach into at most n / 32 + 2 tiles
-  const int64_t tiles = n_tokens / kTileRows + 2 * std::min<int64_t>(n_seqs, n_tokens);
+  const int64_t tiles = g.n_tokens / kTileRows + 2 * std::min<int64_t>(g.n_seqs, g.n_tokens);
   const dim3 grid((unsigned)tiles, (unsigned)((units + kScaledWaves - 1) / kScaledWaves));
-#define NKV_SCALED_READ(D)                                                                      \
-  hipLaunchKernelGGL((scaled_read_kernel<D>), grid, dim3(64 * kScaledWaves), 0,                 \
-                     as_stream(stream), (const char*)k_cache, (const char*)v_cache,             \
-                     block_tables, bt_row_stride, cu_seqlens, starts, n_seqs, n_tokens,         \
-                     n_kv_heads, block_size, max_blocks_per_seq, n_blocks, units,               \
-                     (bf16_t*)k_out, (bf16_t*)v_out)
-  if (head_dim == 64) NKV_SCALED_READ(64);
+#define NKV_SCALED_READ(D)                                                                        \
+  hipLaunchKernelGGL((scaled_read_kernel<D>), grid, dim3(64 * kScaledWaves), 0,                   \
+                     as_stream(g.stream), (const char*)g.k_cache, (const char*)g.v_cache,         \
+                     g.block_tables, g.bt_row_stride, g.cu_seqlens, g.starts, (int32_t)g.n_seqs,  \
+                     g.n_tokens, Hk, (int32_t)g.block_size, (int32_t)g.max_blocks_per_seq,        \
+                     g.n_blocks, units, (bf16_t*)g.k_out, (bf16_t*)g.v_out)
+  if (g.head_dim == 64) NKV_SCALED_READ(64);
   else NKV_SCALED_READ(128);
 #undef NKV_SCALED_READ
   return check_launch("nkv_scaled_read");

@@ -275,77 +275,76 @@ static int scaled_decode_grid() {
   return n;
 }
 
+int scaled_check_heads(const char* what, int64_t n_q_heads, int64_t n_kv_heads, int64_t most,
+                       double scale) {
+  NKV_REQUIRE(n_kv_heads > 0 && n_q_heads > 0 && n_q_heads % n_kv_heads == 0, NKV_EINVAL,
+              "%s: n_q_heads must be a multiple of n_kv_heads (got %lld, %lld)", what,
+              (long long)n_q_heads, (long long)n_kv_heads);
+  NKV_REQUIRE(n_q_heads / n_kv_heads <= most, NKV_EUNSUPPORTED, "%s: GQA group %lld above %lld",
+              what, (long long)(n_q_heads / n_kv_heads), (long long)most);
+  NKV_REQUIRE(scale > 0 && isfinite((float)scale), NKV_EINVAL, "%s: scale must be finite and > 0",
+              what);
+  return NKV_OK;
+}
+
 }  // namespace nkv
 
-extern "C" int nkv_scaled_decode(const void* q, int64_t q_row_stride, const void* k_cache,
-                                 const void* v_cache, const int32_t* block_tables,
-                                 int64_t bt_row_stride, const int32_t* context_lens, int32_t batch,
-                                 int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
-                                 int32_t block_size, int32_t max_blocks_per_seq, int64_t n_blocks,
-                                 float scale, void* out, int64_t out_row_stride, void* workspace,
-                                 size_t workspace_bytes, void* stream) {
+extern "C" int nkv_scaled_decode(const nkv_scaled_decode_args* args) {
   using namespace nkv;
   clear_error();
-  NKV_REQUIRE(batch >= 0 && n_q_heads > 0 && n_kv_heads > 0 && n_blocks >= 0, NKV_EINVAL,
-              "scaled_decode: bad sizes (batch=%d, Hq=%d, Hk=%d)", batch, n_q_heads, n_kv_heads);
-  NKV_REQUIRE(n_q_heads % n_kv_heads == 0, NKV_EINVAL,
-              "scaled_decode: n_q_heads %% n_kv_heads != 0 (%d, %d)", n_q_heads, n_kv_heads);
-  const int g = n_q_heads / n_kv_heads;
-  NKV_REQUIRE(g <= kMaxGroup, NKV_EUNSUPPORTED, "scaled_decode: GQA group %d above %d", g,
-              kMaxGroup);
-  int rc = scaled_check("scaled_decode", k_cache, v_cache, n_kv_heads, head_dim);
+  NKV_REQUIRE(args, NKV_EINVAL, "scaled_decode: null arguments");
+  const nkv_scaled_decode_args& g = *args;
+  NKV_REQUIRE(g.batch >= 0 && g.n_blocks >= 0, NKV_EINVAL, "scaled_decode: bad sizes (batch=%lld)",
+              (long long)g.batch);
+  int rc = scaled_check("scaled_decode", g.k_cache, g.v_cache, g.n_kv_heads, g.head_dim);
   if (rc) return rc;
-  NKV_REQUIRE(block_size > 0 && block_size % kTileRows == 0, NKV_EUNSUPPORTED,
-              "scaled_decode: block_size must be a multiple of %d (got %d)", kTileRows,
-              block_size);
-  NKV_REQUIRE(max_blocks_per_seq > 0 && bt_row_stride >= max_blocks_per_seq, NKV_EINVAL,
-              "scaled_decode: bad block table width/stride (%d, %lld)", max_blocks_per_seq,
-              (long long)bt_row_stride);
-  NKV_REQUIRE((int64_t)max_blocks_per_seq * block_size < (1ll << 30), NKV_EUNSUPPORTED,
-              "scaled_decode: max_blocks_per_seq * block_size too large");
-  NKV_REQUIRE(scale > 0.f && isfinite(scale), NKV_EINVAL,
-              "scaled_decode: scale must be finite and > 0");
-  if (batch == 0) return NKV_OK;
-  const int64_t row = (int64_t)n_q_heads * head_dim;
-  NKV_REQUIRE(q && block_tables && context_lens && out && aligned16(q) &&
-                  (reinterpret_cast<uintptr_t>(out) & 3u) == 0,
+  rc = scaled_check_heads("scaled_decode", g.n_q_heads, g.n_kv_heads, kMaxGroup, g.scale);
+  if (rc) return rc;
+  if (g.batch == 0) return NKV_OK;
+  rc = scaled_check_tables("scaled_decode", g.block_tables, g.bt_row_stride, g.max_blocks_per_seq,
+                           g.block_size, g.n_blocks);
+  if (rc) return rc;
+  const int64_t row = g.n_q_heads * g.head_dim;
+  NKV_REQUIRE(g.q && g.context_lens && g.out && aligned16(g.q) &&
+                  (reinterpret_cast<uintptr_t>(g.out) & 3u) == 0,
               NKV_EINVAL, "scaled_decode: null or misaligned pointer");
-  NKV_REQUIRE(q_row_stride >= row && q_row_stride % 8 == 0 && out_row_stride >= row &&
-                  out_row_stride % 2 == 0,
+  NKV_REQUIRE(g.q_row_stride >= row && g.q_row_stride % 8 == 0 && g.out_row_stride >= row &&
+                  g.out_row_stride % 2 == 0,
               NKV_EINVAL, "scaled_decode: row strides must cover Hq*D, q's in multiples of 8, "
               "out's of 2");
-  const int64_t max_tiles = (int64_t)max_blocks_per_seq * (block_size / kTileRows);
-  const int ncg = decode_ncg(g), np = n_kv_heads * ncg;
-  NKV_REQUIRE(max_tiles * batch < (1ll << 30), NKV_EUNSUPPORTED,
+  const int64_t max_tiles = g.max_blocks_per_seq * (g.block_size / kTileRows);
+  NKV_REQUIRE(g.batch < (1ll << 30) / max_tiles, NKV_EUNSUPPORTED,
               "scaled_decode: too many tiles in one call");
-  // ranges of at least kMinTiles, and no more partials a row than the combine holds
+  const int32_t batch = (int32_t)g.batch, Hq = (int32_t)g.n_q_heads, Hk = (int32_t)g.n_kv_heads,
+                D = (int32_t)g.head_dim, B = (int32_t)g.block_size,
+                width = (int32_t)g.max_blocks_per_seq;
+  const int group = Hq / Hk, ncg = decode_ncg(group), np = Hk * ncg;
+  // ranges of at least two tiles, and no more partials a row than the combine holds
   const int32_t min_tiles = decode_min_chunks(max_tiles, 2);
-  const int resident =
-      head_dim == 64 ? scaled_decode_grid<64>() : scaled_decode_grid<128>();
-  const int64_t waves =
-      std::min<int64_t>(std::max(1, resident / np),
-                        decode_useful_waves(batch, max_blocks_per_seq, block_size));
+  const int resident = D == 64 ? scaled_decode_grid<64>() : scaled_decode_grid<128>();
+  const int64_t waves = std::min<int64_t>(std::max(1, resident / np),
+                                          decode_useful_waves(batch, width, B));
   const size_t desc_b = decode_desc_bytes(batch, np);
-  const size_t need = desc_b + decode_part_bytes(waves, batch, n_q_heads, head_dim);
-  NKV_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, NKV_EWORKSPACE,
-              "scaled_decode: workspace needs %zu bytes, 16-byte aligned (got %zu)", need,
-              workspace_bytes);
-  NKV_REQUIRE((waves + batch) * n_q_heads < (1ll << 31) && waves * np < (1ll << 31),
-              NKV_EUNSUPPORTED, "scaled_decode: too many partial rows");
-  i32x4v_t* desc = static_cast<i32x4v_t*>(workspace);
-  float* part = reinterpret_cast<float*>(static_cast<char*>(workspace) + desc_b);
-#define NKV_SCALED_DECODE(D)                                                                    \
-  hipLaunchKernelGGL((scaled_decode_kernel<D>), dim3((unsigned)(waves * np)), dim3(64), 0,      \
-                     as_stream(stream), (const bf16_t*)q, q_row_stride, (const char*)k_cache,   \
-                     (const char*)v_cache, block_tables, bt_row_stride, context_lens, batch,    \
-                     n_kv_heads, g, ncg, block_size, max_blocks_per_seq, n_blocks, min_tiles,   \
-                     scale * kLog2e, part, desc)
-  if (head_dim == 64) NKV_SCALED_DECODE(64);
+  const size_t need = desc_b + decode_part_bytes(waves, batch, Hq, D);
+  NKV_REQUIRE(g.workspace && aligned16(g.workspace) && g.workspace_bytes >= (int64_t)need,
+              NKV_EWORKSPACE, "scaled_decode: workspace needs %zu bytes, 16-byte aligned (got %lld)",
+              need, (long long)g.workspace_bytes);
+  NKV_REQUIRE((waves + batch) * Hq < (1ll << 31) && waves * np < (1ll << 31), NKV_EUNSUPPORTED,
+              "scaled_decode: too many partial rows");
+  i32x4v_t* desc = static_cast<i32x4v_t*>(g.workspace);
+  float* part = reinterpret_cast<float*>(static_cast<char*>(g.workspace) + desc_b);
+#define NKV_SCALED_DECODE(D)                                                                      \
+  hipLaunchKernelGGL((scaled_decode_kernel<D>), dim3((unsigned)(waves * np)), dim3(64), 0,        \
+                     as_stream(g.stream), (const bf16_t*)g.q, g.q_row_stride,                     \
+                     (const char*)g.k_cache, (const char*)g.v_cache, g.block_tables,              \
+                     g.bt_row_stride, g.context_lens, batch, Hk, group, ncg, B, width,            \
+                     g.n_blocks, min_tiles, (float)g.scale * kLog2e, part, desc)
+  if (D == 64) NKV_SCALED_DECODE(64);
   else NKV_SCALED_DECODE(128);
 #undef NKV_SCALED_DECODE
   rc = check_launch("nkv_scaled_decode");
   if (rc) return rc;
-  return nkv_paged_decode_combine(context_lens, batch, n_q_heads, n_kv_heads, head_dim, block_size,
-                                  max_blocks_per_seq, out, out_row_stride, workspace,
-                                  workspace_bytes, stream);
+  return nkv_paged_decode_combine(g.context_lens, batch, Hq, Hk, D, B, width, g.out,
+                                  g.out_row_stride, g.workspace, (size_t)g.workspace_bytes,
+                                  g.stream);
 }

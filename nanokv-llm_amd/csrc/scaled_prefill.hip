@@ -582,71 +582,59 @@ extern "C" size_t nkv_scaled_prefill_workspace_bytes(int32_t n_seqs, int64_t tot
   return p.bytes(head_dim);
 }
 
-extern "C" int nkv_scaled_prefill(const void* q, int64_t q_row_stride, int64_t total_q,
-                                  const void* k_cache, const void* v_cache,
-                                  const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
-                                  const int32_t* block_tables, int64_t bt_row_stride,
-                                  int32_t max_blocks_per_seq, int32_t n_seqs, int64_t max_seqlen_q,
-                                  int64_t max_seqlen_k, int32_t n_q_heads, int32_t n_kv_heads,
-                                  int32_t head_dim, int32_t block_size, int64_t n_blocks,
-                                  float scale, void* out, int64_t out_row_stride, void* workspace,
-                                  size_t workspace_bytes, void* stream) {
+extern "C" int nkv_scaled_prefill(const nkv_scaled_prefill_args* args) {
   using namespace nkv;
   clear_error();
-  NKV_REQUIRE(n_seqs >= 0 && total_q >= 0 && total_q <= (1 << 30) && max_seqlen_q >= 0 &&
-                  n_q_heads > 0 && n_kv_heads > 0 && n_blocks >= 0,
-              NKV_EINVAL, "scaled_prefill: bad sizes (%d sequences, %lld rows, Hq=%d, Hk=%d)",
-              n_seqs, (long long)total_q, n_q_heads, n_kv_heads);
-  NKV_REQUIRE(n_q_heads % n_kv_heads == 0, NKV_EINVAL,
-              "scaled_prefill: n_q_heads %% n_kv_heads != 0 (%d, %d)", n_q_heads, n_kv_heads);
-  const int g = n_q_heads / n_kv_heads;
-  NKV_REQUIRE(g <= NKV_SCALED_MAX_GROUP, NKV_EUNSUPPORTED, "scaled_prefill: GQA group %d above %d",
-              g, NKV_SCALED_MAX_GROUP);
-  int rc = scaled_check("scaled_prefill", k_cache, v_cache, n_kv_heads, head_dim);
+  NKV_REQUIRE(args, NKV_EINVAL, "scaled_prefill: null arguments");
+  const nkv_scaled_prefill_args& g = *args;
+  NKV_REQUIRE(g.n_seqs >= 0 && g.n_seqs < (1ll << 31) && g.total_q >= 0 && g.total_q <= (1 << 30) &&
+                  g.max_seqlen_q >= 0 && g.n_blocks >= 0,
+              NKV_EINVAL, "scaled_prefill: bad sizes (%lld sequences, %lld rows)",
+              (long long)g.n_seqs, (long long)g.total_q);
+  int rc = scaled_check("scaled_prefill", g.k_cache, g.v_cache, g.n_kv_heads, g.head_dim);
   if (rc) return rc;
-  NKV_REQUIRE(block_size > 0 && block_size % kTileRows == 0, NKV_EUNSUPPORTED,
-              "scaled_prefill: block_size must be a multiple of %d (got %d)", kTileRows,
-              block_size);
-  NKV_REQUIRE(max_blocks_per_seq > 0 && bt_row_stride >= max_blocks_per_seq, NKV_EINVAL,
-              "scaled_prefill: bad block table width/stride (%d, %lld)", max_blocks_per_seq,
-              (long long)bt_row_stride);
-  NKV_REQUIRE(n_blocks < (1ll << 31) && max_blocks_per_seq <= INT32_MAX / block_size,
-              NKV_EUNSUPPORTED, "scaled_prefill: blocks and lengths must fit 32 bits");
-  NKV_REQUIRE(scale > 0.f && isfinite(scale), NKV_EINVAL,
-              "scaled_prefill: scale must be finite and > 0");
-  if (n_seqs == 0 || total_q == 0 || max_seqlen_q == 0) return NKV_OK;
-  const int64_t row = (int64_t)n_q_heads * head_dim;
-  NKV_REQUIRE(q && cu_seqlens_q && cu_seqlens_k && block_tables && out && aligned16(q) &&
-                  (reinterpret_cast<uintptr_t>(out) & 7u) == 0,
+  rc = scaled_check_heads("scaled_prefill", g.n_q_heads, g.n_kv_heads, NKV_SCALED_MAX_GROUP, g.scale);
+  if (rc) return rc;
+  if (g.n_seqs == 0 || g.total_q == 0 || g.max_seqlen_q == 0) return NKV_OK;
+  rc = scaled_check_tables("scaled_prefill", g.block_tables, g.bt_row_stride, g.max_blocks_per_seq,
+                           g.block_size, g.n_blocks);
+  if (rc) return rc;
+  const int64_t row = g.n_q_heads * g.head_dim;
+  NKV_REQUIRE(g.q && g.cu_seqlens_q && g.cu_seqlens_k && g.out && aligned16(g.q) &&
+                  (reinterpret_cast<uintptr_t>(g.out) & 7u) == 0,
               NKV_EINVAL, "scaled_prefill: null or misaligned pointer");
-  NKV_REQUIRE(q_row_stride >= row && q_row_stride % 8 == 0 && out_row_stride >= row &&
-                  out_row_stride % 4 == 0,
+  NKV_REQUIRE(g.q_row_stride >= row && g.q_row_stride % 8 == 0 && g.out_row_stride >= row &&
+                  g.out_row_stride % 4 == 0,
               NKV_EINVAL, "scaled_prefill: row strides must cover Hq*D, q's in multiples of 8, "
               "out's of 4");
-  const ScaledPrefillPlan p = scaled_prefill_plan(n_seqs, total_q, max_seqlen_q,
-                                                  workspace ? max_seqlen_k : 0, n_kv_heads, g,
-                                                  head_dim);
-  NKV_REQUIRE(!p.split || (aligned16(workspace) && workspace_bytes >= p.bytes(head_dim)),
-              NKV_EWORKSPACE, "scaled_prefill: workspace needs %zu bytes, 16-byte aligned (got %zu)",
-              p.bytes(head_dim), workspace_bytes);
+  const int32_t Hk = (int32_t)g.n_kv_heads, group = (int32_t)(g.n_q_heads / g.n_kv_heads);
+  const ScaledPrefillPlan p = scaled_prefill_plan(g.n_seqs, g.total_q, g.max_seqlen_q,
+                                                  g.workspace ? g.max_seqlen_k : 0, Hk, group,
+                                                  (int)g.head_dim);
+  const size_t need = p.bytes((int)g.head_dim);
+  NKV_REQUIRE(!p.split || (aligned16(g.workspace) && g.workspace_bytes >= (int64_t)need),
+              NKV_EWORKSPACE, "scaled_prefill: workspace needs %zu bytes, 16-byte aligned (got %lld)",
+              need, (long long)g.workspace_bytes);
   NKV_REQUIRE(p.tiles < (1ll << 31) && p.grid < (1ll << 31), NKV_EUNSUPPORTED,
               "scaled_prefill: too many tiles in one call");
-  i32x4_t* desc = static_cast<i32x4_t*>(workspace);
-  const ScaledPrefillArgs a{(const bf16_t*)q, q_row_stride, (const char*)k_cache,
-                            (const char*)v_cache, cu_seqlens_q, cu_seqlens_k, block_tables,
-                            bt_row_stride, n_kv_heads, g, block_size, max_blocks_per_seq,
-                            (int32_t)n_blocks, n_seqs, (int32_t)p.tiles, total_q, scale * kLog2e,
-                            (bf16_t*)out, out_row_stride, desc,
+  i32x4_t* desc = static_cast<i32x4_t*>(g.workspace);
+  const ScaledPrefillArgs a{(const bf16_t*)g.q, g.q_row_stride, (const char*)g.k_cache,
+                            (const char*)g.v_cache, g.cu_seqlens_q, g.cu_seqlens_k, g.block_tables,
+                            g.bt_row_stride, Hk, group, (int32_t)g.block_size,
+                            (int32_t)g.max_blocks_per_seq, (int32_t)g.n_blocks, (int32_t)g.n_seqs,
+                            (int32_t)p.tiles, g.total_q, (float)g.scale * kLog2e, (bf16_t*)g.out,
+                            g.out_row_stride, desc,
                             p.split ? reinterpret_cast<float*>(desc + p.grid) : nullptr};
   const dim3 grid((unsigned)p.grid);
 #define NKV_SCALED_PREFILL_S(D, RG, SPLIT)                                                       \
-  hipLaunchKernelGGL((scaled_prefill_kernel<D, RG, SPLIT>), grid, dim3(256), 0, as_stream(stream), a)
+  hipLaunchKernelGGL((scaled_prefill_kernel<D, RG, SPLIT>), grid, dim3(256), 0,       \
+                     as_stream(g.stream), a)
 #define NKV_SCALED_PREFILL(D, RG)                       \
   do {                                                  \
     if (p.split) NKV_SCALED_PREFILL_S(D, RG, true);     \
     else NKV_SCALED_PREFILL_S(D, RG, false);            \
   } while (0)
-  if (head_dim == 64) {
+  if (g.head_dim == 64) {
     if (p.groups == 1) NKV_SCALED_PREFILL(64, 1);
     else NKV_SCALED_PREFILL(64, 2);
   } else {
@@ -659,11 +647,11 @@ extern "C" int nkv_scaled_prefill(const void* q, int64_t q_row_stride, int64_t t
   if (rc || !p.split) return rc;
   const int32_t tile_rows = 64 * p.groups;
   const dim3 merge((unsigned)p.grid, (unsigned)(tile_rows / 4));
-  if (head_dim == 64)
-    hipLaunchKernelGGL((scaled_merge_kernel<64>), merge, dim3(256), 0, as_stream(stream), a,
+  if (g.head_dim == 64)
+    hipLaunchKernelGGL((scaled_merge_kernel<64>), merge, dim3(256), 0, as_stream(g.stream), a,
                        tile_rows);
   else
-    hipLaunchKernelGGL((scaled_merge_kernel<128>), merge, dim3(256), 0, as_stream(stream), a,
+    hipLaunchKernelGGL((scaled_merge_kernel<128>), merge, dim3(256), 0, as_stream(g.stream), a,
                        tile_rows);
   return check_launch("nkv_scaled_prefill");
 }

@@ -14,6 +14,9 @@ pool of nanokvllm/engine/model_runner.py:133-152 and the calls of layers/attenti
 """
 from __future__ import annotations
 
+import functools
+import struct
+
 import torch
 
 from .. import _lib
@@ -23,6 +26,8 @@ _BF16, _I32, _U8 = torch.bfloat16, torch.int32, torch.uint8
 TILE = 32      # tokens under one scale
 ROW_PAD = 16   # include/nkv.h, NKV_SCALED_ROW_PAD
 MAX_HEADS = 512
+_STORE_ARGS, _READ_ARGS = struct.Struct("12q"), struct.Struct("16q")  # include/nkv.h
+_DECODE_ARGS, _PREFILL_ARGS = struct.Struct("19qd"), struct.Struct("23qd")
 
 
 class ScaledKVCachePool:
@@ -206,10 +211,10 @@ def scaled_store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.
             and slot_mapping.size(0) == ks[0]):
         _refuse_store(what, key, value, k_cache, v_cache, slot_mapping)
     with _lib.device_of(di):
-        rc = _lib.lib().nkv_scaled_store(key.data_ptr(), k_st[0], value.data_ptr(), v_st[0],
-                                         k_cache.data_ptr(), v_cache.data_ptr(),
-                                         slot_mapping.data_ptr(), ks[0], ks[1], ks[2],
-                                         cs[0] * cs[1], torch._C._cuda_getCurrentRawStream(di))
+        rc = _lib.lib().nkv_scaled_store(_STORE_ARGS.pack(
+            key.data_ptr(), k_st[0], value.data_ptr(), v_st[0], k_cache.data_ptr(),
+            v_cache.data_ptr(), slot_mapping.data_ptr(), *ks, cs[0] * cs[1],
+            torch._C._cuda_getCurrentRawStream(di)))
     if rc:
         _lib.check(rc, what)
 
@@ -240,14 +245,20 @@ def scaled_read_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tabl
             device = k_cache.device
             out = (torch.empty((n_tokens, Hk, D), dtype=_BF16, device=device),
                    torch.empty((n_tokens, Hk, D), dtype=_BF16, device=device))
-        rc = _lib.lib().nkv_scaled_read(
+        rc = _lib.lib().nkv_scaled_read(_READ_ARGS.pack(
             k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
-            bs[1], cu_seqlens.data_ptr(), None if starts is None else starts.data_ptr(), n, n_tokens,
+            bs[1], cu_seqlens.data_ptr(), 0 if starts is None else starts.data_ptr(), n, n_tokens,
             Hk, D, cs[1], cs[0], out[0].data_ptr(), out[1].data_ptr(),
-            torch._C._cuda_getCurrentRawStream(di))
+            torch._C._cuda_getCurrentRawStream(di)))
     if rc:
         _lib.check(rc, what)
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_bytes(device: int, *sizes: int) -> int:
+    """Workspace bytes on a device (current), a call into the library each where they are new."""
+    return max(_lib.lib().nkv_paged_decode_workspace_bytes(*sizes), 4)
 
 
 def scaled_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -274,13 +285,13 @@ def scaled_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         if out is None:
             out = torch.empty(qs, dtype=_BF16, device=q.device)
         if workspace is None:
-            nbytes = lib.nkv_paged_decode_workspace_bytes(n, Hq, D, bs[1], cs[1])
-            workspace = torch.empty(max(nbytes, 4), dtype=_U8, device=q.device)
-        rc = lib.nkv_scaled_decode(
+            workspace = torch.empty(_decode_bytes(di, n, Hq, D, bs[1], cs[1]), dtype=_U8,
+                                    device=q.device)
+        rc = lib.nkv_scaled_decode(_DECODE_ARGS.pack(
             q.data_ptr(), q_st[0], k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
             block_tables.stride(0), context_lens.data_ptr(), n, Hq, (cs[2] - ROW_PAD) // D, D, cs[1],
-            bs[1], cs[0], scale, out.data_ptr(), out.stride(0), workspace.data_ptr(),
-            workspace.numel(), torch._C._cuda_getCurrentRawStream(di))
+            bs[1], cs[0], out.data_ptr(), out.stride(0), workspace.data_ptr(), workspace.numel(),
+            torch._C._cuda_getCurrentRawStream(di), scale))
     if rc:
         _lib.check(rc, what)
     return out
@@ -335,14 +346,15 @@ def scaled_varlen_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
             out = torch.empty(qs, dtype=_BF16, device=q.device)
         if workspace is None and max_seqlen_k is not None:
             workspace = scaled_prefill_workspace(q, k_cache, n, max_seqlen_q, max_seqlen_k)
-        rc = _lib.lib().nkv_scaled_prefill(
+        rc = _lib.lib().nkv_scaled_prefill(_PREFILL_ARGS.pack(
             q.data_ptr(), q_st[0], qs[0], k_cache.data_ptr(), v_cache.data_ptr(),
             cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), block_tables.data_ptr(),
             block_tables.stride(0), bs[1], n, int(max_seqlen_q),
             0 if max_seqlen_k is None else int(max_seqlen_k), qs[1], (cs[2] - ROW_PAD) // D, D, cs[1],
-            cs[0], scale, out.data_ptr(), out.stride(0),
-            None if workspace is None else workspace.data_ptr(),
-            0 if workspace is None else workspace.numel(), torch._C._cuda_getCurrentRawStream(di))
+            cs[0], out.data_ptr(), out.stride(0),
+            0 if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel(),
+            torch._C._cuda_getCurrentRawStream(di), scale))
     if rc:
         _lib.check(rc, what)
     return out

@@ -105,7 +105,7 @@ TABLES = ALL + [(dict(bs=16), -4, b"multiple of 32"), (dict(bs=0), -4, b"multipl
                 (dict(bs=48), -4, b"multiple of 32"), (dict(btrs=4), -1, b"block table"),
                 (dict(mb=0), -1, b"block table"), (dict(bt=None), -1, b"null"),
                 (dict(nb=-1), -1, b"sizes"), (dict(n=-1), -1, b"sizes")]
-BOTH = TABLES + [(dict(hk=3), -1, b"n_q_heads"), (dict(hq=0), -1, b"sizes"),
+BOTH = TABLES + [(dict(hk=3), -1, b"n_q_heads"), (dict(hq=0), -1, b"n_q_heads"),
                  (dict(scale=0.0), -1, b"scale"), (dict(scale=float("nan")), -1, b"scale"),
                  (dict(scale=float("inf")), -1, b"scale"), (dict(q=P + 8), -1, b"misaligned"),
                  (dict(q=None), -1, b"null"), (dict(out=None), -1, b"null"),
@@ -124,16 +124,16 @@ CASES = (
         (dict(cu=None), -1, b"null"), (dict(ko=P + 2), -1, b"misaligned"), (dict(vo=None), -1, b"null"),
         (dict(n=0, cu=None), 0, b""), (dict(nt=0), 0, b"")]]
     + [("nkv_scaled_decode", DECODE, *c) for c in BOTH + [
-        (dict(hk=0), -1, b"sizes"), (dict(hq=257 * 4), -4, b"above 256"), (dict(ctx=None), -1, b"null"),
+        (dict(hk=0), -4, b"KV heads"), (dict(hq=257 * 4), -4, b"above 256"), (dict(ctx=None), -1, b"null"),
         (dict(ws=None), -3, b"workspace"), (dict(ws=P + 4), -3, b"workspace"),
         (dict(wsb=100), -3, b"workspace"), (dict(mb=1 << 26, btrs=1 << 26), -4, b"too large"),
         (dict(n=1 << 24, mb=1 << 10, btrs=1 << 10), -4, b"too many"), (dict(n=0, ws=None), 0, b"")]]
     + [("nkv_scaled_prefill", PREFILL, *c) for c in BOTH + [
-        (dict(hk=0), -1, b"sizes"), (dict(hq=129 * 4), -4, b"above 128"), (dict(cq=None), -1, b"null"),
+        (dict(hk=0), -4, b"KV heads"), (dict(hq=129 * 4), -4, b"above 128"), (dict(cq=None), -1, b"null"),
         (dict(ck=None), -1, b"null"), (dict(tq=-1), -1, b"sizes"), (dict(tq=1 << 31), -1, b"sizes"),
         (dict(mq=-1), -1, b"sizes"), (dict(out=P + 4), -1, b"misaligned"),
-        (dict(ors=514), -1, b"strides"), (dict(nb=1 << 31), -4, b"32 bits"),
-        (dict(mb=1 << 27, btrs=1 << 27), -4, b"32 bits"), (dict(n=1 << 30, mq=1 << 20), -4, b"too many"),
+        (dict(ors=514), -1, b"strides"), (dict(nb=1 << 31), -4, b"too large"),
+        (dict(mb=1 << 27, btrs=1 << 27), -4, b"too large"), (dict(n=1 << 30, mq=1 << 20), -4, b"too many"),
         (dict(ws=P, wsb=100, mk=100000), -3, b"workspace"),
         (dict(ws=P + 8, wsb=1 << 40, mk=100000), -3, b"workspace"),
         (dict(n=0), 0, b""), (dict(tq=0), 0, b""), (dict(mq=0), 0, b"")]]
@@ -142,8 +142,17 @@ CASES = (
 
 @pytest.mark.parametrize("name,base,kw,code,msg", CASES)
 def test_entry_points_refuse(name, base, kw, code, msg):
-    rc = getattr(L.lib(), name)(*dict(base, **kw).values(), None)
+    a = dict(base, **kw)
+    scale = [a.pop("scale")] if "scale" in a else []
+    args = [0 if x is None else x for x in (*a.values(), None)] + scale  # the stream: NULL
+    rc = getattr(L.lib(), name)(struct.pack(f"{len(args) - len(scale)}q{len(scale)}d", *args))
     assert rc == code and msg in L.lib().nkv_last_error(), (rc, L.lib().nkv_last_error())
+
+
+def test_entry_points_refuse_null_arguments():
+    for name in ("store", "read", "decode", "prefill"):
+        assert getattr(L.lib(), "nkv_scaled_" + name)(None) == -1
+        assert b"null arguments" in L.lib().nkv_last_error()
 
 
 def test_page_calls_refuse():
