@@ -6,21 +6,30 @@
 // queries and Lk keys sees keys 0 .. Lk-Lq+j).
 //   out_j = softmax(scale * q_j . K) V    over the keys that it sees, K and V = code * 2^e
 //
-// MI355X design (MFMA-bound). Workgroup = (sequence, tile of queries, KV head, part of the keys) x 4
-// waves; a tile's rows are its queries for all G heads of the KV head (row r: query r / G, head r % G),
-// 16 * RG of them a wave. Keys advance 64 a step, two tiles of the cache: each wave brings one tile's K
-// or V codes into registers while the step before computes, widens them to bf16 with the tile's scale
-// (exactly, v_cvt_scalef32_pk_bf16_fp8) and writes them to one of two LDS stages. Codes come in the
-// lanes' order for the matrix instructions, so that the loads, the LDS writes and the LDS reads are all
-// 1 KiB of consecutive bytes a wave: no swizzle, no transposing read, no bank conflict.
+// MI355X design (MFMA- and issue-bound). Workgroup = (sequence, tile of queries, KV head) x 4 waves; a
+// tile's rows are its queries for all G heads of the KV head (row r: query r / G, head r % G), 16 * RG of
+// them a wave. Keys advance 64 a step, two tiles of the cache. Each wave brings one tile's K or V codes
+// straight into a ring of four steps in LDS (buffer_load ... lds, three steps ahead, one barrier a step)
+// and every wave widens them to bf16 with the tile's scale as it reads them (exactly,
+// v_cvt_scalef32_pk_bf16_fp8). Codes stand in memory in the lanes' order for the matrix instructions, so
+// that the loads and the LDS reads are 1 KiB of consecutive bytes a wave: no swizzle, no transposing
+// read, no bank conflict; and the ring holds a byte a value, half of what widened tiles would take.
 //   S^T = K q^T      v_mfma_f32_16x16x32_bf16, A = 16 keys from LDS, B = q in registers
 //   O^T += V^T P^T   the same, A = 16 dims x 32 keys from LDS, B = the lane's own eight weights
-// Where the tiles are fewer than the chip's workgroups the keys of each are cut into `parts` equal
-// ranges, whose partial rows a second launch merges.
+// Each wave widens for itself, so the more rows it has the less that counts: of 392 us (4 chunks of
+// 1500 - 2048 behind up to 6000 keys, Hq 32, Hk 8, D 128, RG 2, q's products 104 us) K's widening took
+// 35, V's 29 and the exponentials 34. RG 3 with the longest sequences first: 342 us, 1.01 PFLOP/s.
+// Products of K's codes as they are (v_mfma_scale_f32_16x16x128_f8f6f4, q as the sum of two E4M3 codes)
+// take as long in the matrix cores, and save only the widening: 341 us against 346, and 7.9 us against
+// 7.1 for one prompt of 77, which q's taking apart costs; not taken.
+//
+// SPLIT: where few tiles would leave the chip idle, the workgroups that fit it at once take equal ranges
+// of all the key steps, and a second launch merges the rows whose keys were cut.
 #include "launch_rules.h"
 #include "lds_tiles.h"
 #include "scaled_cache.h"
 
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -38,7 +47,7 @@ struct ScaledPrefillArgs {
   const char *k_cache, *v_cache;
   const int32_t *cu_q, *cu_k, *block_tables;
   int64_t bt_row_stride;
-  int32_t Hk, G, block_size, max_blocks, n_blocks, n_seqs, n_tiles;
+  int32_t Hk, G, block_size, max_blocks, n_blocks, n_seqs, n_tiles, sort;
   int64_t total_q;  // rows of q and out
   float scale_log2;
   bf16_t* out;
@@ -59,26 +68,30 @@ __device__ __forceinline__ void seq_lengths(const ScaledPrefillArgs& a, int s, i
 }
 
 // The ranges of a split launch. The units of a KV head (sequence, tile) stand in one stream, a unit as
-// long as its steps cost; range w is [w C, (w+1) C), a cut near a unit's end moved to that end. Every
-// workgroup finds its own range from the lengths.
+// long as its keys cost; range w is [w C, (w+1) C), a cut near a unit's end moved to that end. Every
+// workgroup finds its own range from the lengths: the units' costs are series that sum in closed form.
 struct Cursor {
   int seq, tile, q0, Lq, Lk;  // the current unit
   int u0;                     // its position in the stream
   int C, T, x, x_end;         // range length, stream length, the range's begin and end
 };
-constexpr int kSnap = 2;      // steps
+constexpr int kSnap = 2;        // steps
 constexpr int kLeastSteps = 4;  // shortest range
 template <int RG>
-__device__ __forceinline__ int step_cost(int rows) {
+__device__ __forceinline__ int key_cost(int rows) {
   return kStepBase + (rows + 16 * RG - 1) / (16 * RG);
 }
 __device__ __forceinline__ int tile_steps(int Lq, int Lk, int qt, int t) {
   const int last = Lk - Lq + min(Lq, (t + 1) * qt) - 1;
   return last >= 0 ? min(last, Lk - 1) / kStep + 1 : 1;  // an empty one is masked whole
 }
+// Keys of tile t as the stream counts them, and the cost of the tiles before tile t, all full.
+__device__ __forceinline__ int tile_keys(int Lq, int Lk, int qt, int t) {
+  return max(Lk - Lq, 0) + min(Lq, (t + 1) * qt);
+}
 template <int RG>
-__device__ __forceinline__ int unit_cost(int Lq, int Lk, int qt, int t, int G) {
-  return tile_steps(Lq, Lk, qt, t) * step_cost<RG>(min(qt, Lq - t * qt) * G);
+__device__ __forceinline__ int cost_before(int Lq, int Lk, int qt, int t, int G) {
+  return key_cost<RG>(qt * G) * (t * max(Lk - Lq, 0) + qt * (t * (t + 1) / 2));
 }
 template <int RG>
 __device__ __forceinline__ bool split_begin(const ScaledPrefillArgs& a, int qt, Cursor& c) {
@@ -87,14 +100,18 @@ __device__ __forceinline__ bool split_begin(const ScaledPrefillArgs& a, int qt, 
   const auto load = [&](int cb) {  // lane: sequence cb + lane
     Lq = Lk = cost = 0;
     if (cb + lane < a.n_seqs) seq_lengths(a, cb + lane, q0, Lq, Lk);
-    for (int t = 0; t * qt < Lq; ++t) cost += unit_cost<RG>(Lq, Lk, qt, t, a.G);
+    if (Lq > 0) {
+      const int t = (Lq - 1) / qt;
+      cost = cost_before<RG>(Lq, Lk, qt, t, a.G) +
+             tile_keys(Lq, Lk, qt, t) * key_cost<RG>((Lq - t * qt) * a.G);
+    }
     incl = wave_incl_scan(cost);
     return __builtin_amdgcn_readlane(incl, 63);
   };
   c.T = 0;
   for (int cb = 0; cb < a.n_seqs; cb += 64) c.T += load(cb);
   const int ranges = (int)gridDim.x / a.Hk;
-  c.C = max((c.T + ranges - 1) / ranges, kLeastSteps * kFullStep);
+  c.C = max((c.T + ranges - 1) / ranges, kLeastSteps * kStep * kFullStep);
   c.x = (int)blockIdx.x / a.Hk * c.C;
   c.x_end = c.x + c.C;
   if (c.x >= c.T) return false;
@@ -111,11 +128,14 @@ __device__ __forceinline__ bool split_begin(const ScaledPrefillArgs& a, int qt, 
   c.Lq = __builtin_amdgcn_readlane(Lq, ln);
   c.Lk = __builtin_amdgcn_readlane(Lk, ln);
   c.u0 = base + __builtin_amdgcn_readlane(incl - cost, ln);
-  for (c.tile = 0; (c.tile + 1) * qt < c.Lq; ++c.tile) {
-    const int u = unit_cost<RG>(c.Lq, c.Lk, qt, c.tile, a.G);
-    if (c.x < c.u0 + u) break;
-    c.u0 += u;
+  c.tile = -1;  // the last that begins at x or before
+  for (int t0 = 0; t0 * qt < c.Lq; t0 += 64) {
+    const int t = t0 + lane;
+    c.tile += __builtin_popcountll(__ballot(
+        t * qt < c.Lq && c.u0 + cost_before<RG>(c.Lq, c.Lk, qt, t, a.G) <= c.x));
   }
+  c.tile = max(c.tile, 0);
+  c.u0 += cost_before<RG>(c.Lq, c.Lk, qt, c.tile, a.G);
   return true;
 }
 // The unit after the current one, which ends at u1 (false at the end of the stream).
@@ -131,13 +151,28 @@ __device__ __forceinline__ bool split_next(const ScaledPrefillArgs& a, int qt, i
   return true;
 }
 
-// 1 KiB (16 bytes a lane) or 256 bytes (4 a lane) from desc + voff to consecutive LDS bytes. Written
-// as asm so that the compiler adds no wait for it before a barrier; the ring's own s_waitcnt does.
+// N KiB (16 bytes a lane each) or 256 bytes (4 a lane) from desc + voff to consecutive LDS bytes (an
+// instruction's offset moves both addresses). Written as asm so that the compiler adds no wait for it
+// before a barrier; the ring's own s_waitcnt does.
+template <int N>
 __device__ __forceinline__ void fetch16(i32x4_t desc, uint32_t lds_addr, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(lds_addr), "v"(voff), "s"(desc)
-               : "memory");
+  static_assert(N == 2 || N == 4, "a tile of codes");
+  if constexpr (N == 2)
+    asm volatile("s_mov_b32 m0, %0\n\t"
+                 "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
+                 "buffer_load_dwordx4 %1, %2, 0 offen offset:0x400 lds"
+                 :
+                 : "s"(lds_addr), "v"(voff), "s"(desc)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\t"
+                 "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
+                 "buffer_load_dwordx4 %1, %2, 0 offen offset:0x400 lds\n\t"
+                 "buffer_load_dwordx4 %1, %2, 0 offen offset:0x800 lds\n\t"
+                 "buffer_load_dwordx4 %1, %2, 0 offen offset:0xc00 lds"
+                 :
+                 : "s"(lds_addr), "v"(voff), "s"(desc)
+                 : "memory");
 }
 __device__ __forceinline__ void fetch4(i32x4_t desc, uint32_t lds_addr, uint32_t voff) {
   asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
@@ -159,7 +194,8 @@ __device__ __forceinline__ u32x4_t split_nan(u32x4_t v, u32x4_t& ones) {
   return clean;
 }
 
-// A workgroup's tile, or (SPLIT) the units of its range.
+// A workgroup's tile, or (SPLIT) the units of its range. (RG 3 at head_dim 128 takes all 256 registers
+// and spills four.)
 template <int D, int RG, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPrefillArgs a) {
   constexpr int kI = D / 64;
@@ -198,6 +234,16 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
     const int rest = blockIdx.x / Hk;
     cur.tile = a.n_tiles - 1 - rest % a.n_tiles;  // largest first
     cur.seq = rest / a.n_tiles;
+    if (a.sort) {  // the longest sequences first (as many as a wave has lanes)
+      const int n = a.n_seqs;
+      const int len = lane < n ? a.cu_k[lane + 1] - a.cu_k[lane] : -1;
+      int rank = 0;
+      for (int i = 0; i < n; ++i) {
+        const int other = __builtin_amdgcn_readlane(len, i);
+        rank += other > len || (other == len && i < lane);
+      }
+      cur.seq = __builtin_ctzll(__ballot(lane < n && rank == cur.seq));
+    }
     seq_lengths(a, cur.seq, cur.q0, cur.Lq, cur.Lk);
     if (cur.tile * QT >= cur.Lq) return;  // uniform
   }
@@ -212,11 +258,10 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
   int s_lo = 0, s_end = last_key >= 0 ? last_key / kStep + 1 : 0;
   int snap = 0;
   if constexpr (SPLIT) {
-    const int sc = step_cost<RG>(min(QT, Lq - j0) * G);
-    const int n_steps = tile_steps(Lq, Lk, QT, cur.tile);
+    const int kc = key_cost<RG>(min(QT, Lq - j0) * G), sc = kStep * kc;
     snap = kSnap * sc;
-    u1 = cur.u0 + n_steps * sc;
-    s_end = n_steps;
+    u1 = cur.u0 + tile_keys(Lq, Lk, QT, cur.tile) * kc;
+    s_end = tile_steps(Lq, Lk, QT, cur.tile);
     cut = false;
     if (cur.x >= cur.u0 + snap) {     // the range's begin lies in its first unit
       if (cur.x > u1 - snap) continue;  // which is the range's before (the condition steps on)
@@ -226,25 +271,26 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
       if (cur.x_end < cur.u0 + snap) return;  // which is the next range's
       cut = cur.x_end <= u1 - snap;
     }
-    if (cut) s_end = (cur.x_end - cur.u0 + sc - 1) / sc;
-    s_lo = uni(s_lo);
+    if (cut) s_end = min(s_end, (cur.x_end - cur.u0 + sc - 1) / sc);
+    // (within the tile also where lengths beyond the call's maxima have overflown the stream)
     s_end = uni(s_end);
+    s_lo = max(min(uni(s_lo), s_end), 0);
   }
 
   // ---- this wave's row groups: head and query of this lane's row (rows past the tile's queries
   // take query Lq: attended like the others, never stored)
   const bool idle = wave * (16 * RG) >= min(QT, Lq - j0) * G;  // only brings its share of the codes
-  int head[RG], jrow[RG];
+  int jrow[RG];
   u32x4_t qreg[RG][kKs];
 #pragma unroll
   for (int rr = 0; rr < RG; ++rr) {
     const int r = (wave * RG + rr) * 16 + col;
     const bool real = r < QT * G;
-    head[rr] = real ? r % G : 0;
+    const int head = real ? r % G : 0;
     jrow[rr] = real ? j0 + r / G : Lq;
     const int jc = jrow[rr] < Lq ? jrow[rr] : j0;
     const u32x4_t* qp = reinterpret_cast<const u32x4_t*>(
-        a.q + (int64_t)(q0 + jc) * a.q_row_stride + (int64_t)(kvh * G + head[rr]) * D + g4 * 16);
+        a.q + (int64_t)(q0 + jc) * a.q_row_stride + (int64_t)(kvh * G + head) * D + g4 * 16);
 #pragma unroll
     for (int i = 0; i < kI; ++i) {
       qreg[rr][2 * i] = qp[8 * i];
@@ -273,8 +319,7 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
     const int64_t at = ((int64_t)(ok ? pb : 0) * tiles_per_block + c_in) * tile_bytes;
     const i32x4_t desc = buffer_desc(cache + at, ok ? (uint32_t)tile_bytes : 0u);
     const uint32_t to = ring_at + (uint32_t)c_stage * kStageB;
-#pragma unroll
-    for (int p = 0; p < kLoads; ++p) fetch16(desc, to + p * 1024, code_off + p * 1024);
+    fetch16<kLoads>(desc, to, code_off);
     fetch4(desc, to - (uint32_t)wave * kTileB + kCodesB + wave * 256, scale_off & ~3u);
     c_stage = c_stage + 1 == kStages ? 0 : c_stage + 1;
     c_left -= kStep;
@@ -288,14 +333,13 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
     }
   };
   f32x4_t acc[RG][kDb];  // O^T: lane l -> row l%16, dims 16*db + 4*(l/16) .. +3
-  float m_run[RG], l_run[RG], mb[RG];  // mb: m_run, or 0 while the row has seen no key
+  float m_run[RG], l_run[RG];
 #pragma unroll
   for (int rr = 0; rr < RG; ++rr) {
 #pragma unroll
     for (int db = 0; db < kDb; ++db) acc[rr][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    m_run[rr] = -INFINITY;
+    m_run[rr] = -FLT_MAX;  // finite: a masked key's weight is exp2(-inf - m), 0, from the first on
     l_run[rr] = 0.f;
-    mb[rr] = 0.f;
     // q is in registers before the ring's first loads: a wait for it later would wait for them too
 #pragma unroll
     for (int ks = 0; ks < kKs; ++ks) asm volatile("" ::"v"(qreg[rr][ks]));
@@ -311,8 +355,8 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
     float scale[4];  // K, V of the first cache tile, of the second
 #pragma unroll
     for (int w = 0; w < 4; ++w)
-      scale[w] = scale_of(stored_scale(
-          byte_of(*reinterpret_cast<const uint32_t*>(st + w * 256), (int)scale_off)));
+      scale[w] = scale_of(stored_scale(byte_of(
+          uni((int)*reinterpret_cast<const uint32_t*>(st + w * 256)), (int)scale_off)));
     // S^T of quarter h: tokens 32 (h / 2) + 8 g4 + 4 (h % 2) + 0..3 of the step
     float sv[RG][16];
 #pragma unroll
@@ -360,9 +404,8 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
       for (int rr = 0; rr < RG; ++rr) {
         const float cm = col_max4(top[rr]) * a.scale_log2;
         const bool raise = cm > m_run[rr] + kLazy;
-        const float alpha = raise ? fast_exp2(m_run[rr] - cm) : 1.f;  // exp2(-inf) = 0
+        const float alpha = raise ? fast_exp2(m_run[rr] - cm) : 1.f;
         m_run[rr] = raise ? cm : m_run[rr];
-        mb[rr] = m_run[rr] == -INFINITY ? 0.f : m_run[rr];
         l_run[rr] *= alpha;
 #pragma unroll
         for (int db = 0; db < kDb; ++db) acc[rr][db] *= alpha;
@@ -376,7 +419,7 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          p[e] = fast_exp2(fmaf(sv[rr][8 * c + e], a.scale_log2, -mb[rr]));
+          p[e] = fast_exp2(fmaf(sv[rr][8 * c + e], a.scale_log2, -m_run[rr]));
         pb[rr] = u32x4_t{cvt_pk16<false>(p[0], p[1]), cvt_pk16<false>(p[2], p[3]),
                          cvt_pk16<false>(p[4], p[5]), cvt_pk16<false>(p[6], p[7])};
         // the sum is that of the rounded weights, which multiply V
@@ -475,8 +518,9 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
       }
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;
+    const int head = (wave * RG + rr) * 16 + col - (jrow[rr] - j0) * G;
     bf16_t* op = a.out + (int64_t)(q0 + jrow[rr]) * a.out_row_stride +
-                 (int64_t)(kvh * G + head[rr]) * D + g4 * 4;
+                 (int64_t)(kvh * G + head) * D + g4 * 4;
 #pragma unroll
     for (int db = 0; db < kDb; ++db)
       *reinterpret_cast<uint2*>(op + db * 16) =
@@ -493,76 +537,133 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
   } while (SPLIT && !cut && split_next(a, QT, u1, cur));
 }
 
-// Merges the parts of the units that ranges cut: descriptor x (of the workgroup that holds a unit's
-// first part; part p > 0 is in the first slot of the workgroup p * Hk after it), a row of its tile a
-// wave. Lane l owns output dims N l .. N l + N - 1, eight parts in flight.
+// // Merges the parts of the units that ranges cut: descriptor x (of the workgroup that holds a unit's
+// first part; part p > 0 is in the first slot of the workgroup p * Hk after it), four rows of its tile a
+// wave, 16 lanes each. Lane c of a row owns dims 4 c + 64 i .. + 3, eight parts in flight. (A row a wave: 11
+// us where this takes 6, for the four times as many workgroups to hand out.)
 template <int D>
 __global__ __launch_bounds__(256) void scaled_merge_kernel(const ScaledPrefillArgs a,
                                                            int32_t tile_rows) {
-  constexpr int N = D / 64;
+  constexpr int kI = D / 64;
   constexpr int kInFlight = 8;
-  const int lane = threadIdx.x & 63;
   const i32x4_t d = a.desc[blockIdx.x];
-  const int r = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int r = blockIdx.y * 16 + (int)threadIdx.x / 16, c4 = (int)threadIdx.x % 16 * 4;
   if (d[0] < 2 || r >= d[2] * a.G) return;
   const int64_t tile = (int64_t)tile_rows * part_floats(D);
   const float* first = a.part + ((int64_t)blockIdx.x * 2 + 1) * tile + r * part_floats(D);
   const float* next = first - tile;  // + p * 2 * Hk tiles
-  float M = -INFINITY, L = 0.f, o[N] = {};
-  for (int p0 = 0; p0 < d[0]; p0 += kInFlight) {
+  const int parts = min(d[0], (int)(gridDim.x - 1 - blockIdx.x) / a.Hk + 1);
+  float M = -FLT_MAX, L = 0.f;
+  f32x4_t o[kI] = {};
+  for (int p0 = 0; p0 < parts; p0 += kInFlight) {
     float2 ml[kInFlight];
-    float v[kInFlight][N];
+    f32x4_t v[kInFlight][kI];
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
-      const int p = min(p0 + u, d[0] - 1);
+      const int p = min(p0 + u, parts - 1);
       const float* row = p == 0 ? first : next + (int64_t)p * 2 * a.Hk * tile;
       ml[u] = *reinterpret_cast<const float2*>(row + D);
-      load_dims<N>(row + N * lane, v[u]);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) v[u][i] = *reinterpret_cast<const f32x4_t*>(row + c4 + 64 * i);
     }
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       const float m = ml[u].x, l = ml[u].y;
-      // (no key of the part that the row sees: m = -inf, l = 0)
-      if (p0 + u >= d[0] || (m == -INFINITY && l == 0.f)) continue;
-      const float top = fmaxf(M, m);
-      const float mb = top == -INFINITY ? 0.f : top;  // scores that are all NaN leave no maximum
-      const float alpha = fast_exp2(M - mb), w = m == -INFINITY ? 1.f : fast_exp2(m - mb);
+      if (p0 + u >= parts) break;
+      const float top = fmaxf(M, m);  // (finite, as each m is from the start)
+      const float alpha = fast_exp2(M - top), w = fast_exp2(m - top);
       M = top;
       L = fmaf(w, l, L * alpha);
 #pragma unroll
-      for (int e = 0; e < N; ++e) o[e] = fmaf(w, v[u][e], o[e] * alpha);
+      for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = fmaf(w, v[u][i][e], o[i][e] * alpha);
     }
   }
-  store_dims<N, false>(a.out + (int64_t)(d[1] + r / a.G) * a.out_row_stride +
-                           (int64_t)(d[3] * a.G + r % a.G) * D + N * lane,
-                       o, L != 0.f ? 1.f / L : 0.f);
+  const float inv = L != 0.f ? 1.f / L : 0.f;
+  bf16_t* op = a.out + (int64_t)(d[1] + r / a.G) * a.out_row_stride +
+               (int64_t)(d[3] * a.G + r % a.G) * D + c4;
+#pragma unroll
+  for (int i = 0; i < kI; ++i)
+    *reinterpret_cast<uint2*>(op + 64 * i) =
+        uint2{cvt_pk16<false>(o[i][0] * inv, o[i][1] * inv),
+              cvt_pk16<false>(o[i][2] * inv, o[i][3] * inv)};
 }
 
 struct ScaledPrefillPlan {
   int groups;      // row groups a wave
   bool split;
+  bool sort;       // plain: sequences by length
   int64_t grid;    // workgroups
   int64_t tiles;   // plain: tiles a sequence
   size_t bytes(int D) const {  // of the workspace
     return split ? grid * (sizeof(i32x4_t) + 2 * 64 * groups * part_floats(D) * sizeof(float)) : 0;
   }
 };
+// How a call is launched, from its sizes alone.
+//
+// Split or whole. Whole, the longest tile sets the time, about 0.65 us a step of its own; split, the
+// steps are spread evenly, for about 8 us of ranges, partial rows and their merge (12 steps) and as much
+// again in proportion (a quarter). In graphs, whole / split, us (Hq 32, Hk 8, D 128 but where noted):
+//   1 draft of 8 behind 500 - 1000 / 2000 - 4000 / 8000 - 16000   16.7 / 15.8, 46.8 / 16.3, 169 / 25.8
+//   8 drafts behind up to 1000 / 2000 / 4000                     21.2 / 17.9, 35.7 / 23.7, 63 / 32.5
+//   32 behind up to 2000, 64 and 128 up to 4000                  37.2 / 40.0, 97 / 99, 181 / 182
+//   1 chunk of 512 behind up to 4000 / 16000                     56.5 / 53.3, 181 / 127
+//   4 chunks of 128 / of 256 behind up to 4000                   90 / 62, 97 / 103
+//   a prompt of 512 / 2048 / 4096                                13.7 / 13.7, 55 / 80, 143 / 194
+//   2 chunks of 400 behind up to 1000, 30 tokens (16, 4, 64)     29.2 / 27.7
+//
+// Row groups a wave. More of them read, widen and wait for the keys less often; fewer fill the chip
+// sooner. Whole, 1 / 2 / 3 groups, us (Hk 8; workgroups of one group):
+//   512 (256)       13.8 / 18.4 / 24.9        4096 (2048)               172 / 143 / 145
+//   1024 (512)      23.9 / 29.7 / 39.1        2 of 2048 + 4000 (2048)   371 / 284 / 315
+//   2048 (1024)     56.9 / 55.7 / 70.7        8 of 1024 + 1000 (3600)   252 / 205 / 203
+//     + 6000        254 / 207 / 262           8192 (4096)               623 / 483 / 456
+// At head_dim 64 (four workgroups of one group to a CU, three of two, two of three) 1 / 2 / 3 / 4:
+//   1024 (512)      17.1 / 21.6 / 27.1 / 32.1     4096 (2048)   97 / 92 / 99 / 111
+//   2048 (1024)     35.9 / 39.2 / 48.6 / 56.8     8192 (4096)   357 / 297 / 304 / 300
+// Split, two groups cost less where the tiles are many: 4 chunks of 128 70.6 / 62.3, 1 of 512 behind
+// 16000 155 / 127, but 2 of 64 29.1 / 33.4 and 4 drafts 53.5 / 59.7.
+//
+// Order. Workgroups are handed out in turn, the last of them ends alone: longest sequences first, tiles
+// from the last, 342 us for the chunks above and 430 as they come. (Tiles of all sequences in turn: 620,
+// since their keys do not fit the L2 together.)
 static ScaledPrefillPlan scaled_prefill_plan(int64_t n_seqs, int64_t total_q, int64_t max_q,
                                              int64_t max_k, int32_t Hk, int g, int D) {
-  ScaledPrefillPlan p;
   const int cus = device_cus();
-  p.groups = plain_groups(n_seqs, total_q, max_q, Hk, g, 2, cus);
   const BatchMix m = batch_mix(n_seqs, total_q, max_q);
-  const int64_t qt = 64 * p.groups / g;
-  const int64_t each = (max_q + qt - 1) / qt;
-  const int64_t tiles = std::min(m.prompts * each, m.prompt_rows / qt + m.prompts) + m.rows;
-  const int64_t most = std::min(n_seqs * each, total_q / qt + n_seqs);
-  p.tiles = plain_tiles(n_seqs, max_q, qt);
+  const auto queries = [&](int groups) -> int64_t { return 64 * groups / g; };  // of a tile
+  const auto tiles = [&](int groups) -> int64_t {  // that hold queries
+    const int64_t qt = queries(groups);
+    return std::min(m.prompts * ((max_q + qt - 1) / qt), m.prompt_rows / qt + m.prompts) + m.rows;
+  };
+  const auto launched = [&](int groups) -> int64_t {  // of a plain launch
+    return n_seqs * plain_tiles(n_seqs, max_q, queries(groups)) * Hk;
+  };
   // workgroups that are resident at once: by the ring's LDS (69 KiB, 36 at head_dim 64), or registers
-  const int resident = cus * (D == 128 ? 2 : p.groups == 1 ? 4 : 3);
-  p.split = max_k >= 8 * kStep && each <= 96 && tiles * Hk <= 2 * resident && resident >= Hk &&
-            split_fits(n_seqs, most, max_k);
-  p.grid = p.split ? resident / Hk * Hk : n_seqs * p.tiles * Hk;
+  const auto resident = [&](int groups) { return cus * (D == 128 ? 2 : groups == 1 ? 4 : 3); };
+  const int least = g > 64 ? 2 : 1;
+  ScaledPrefillPlan p;
+  p.groups = least;
+  int64_t size = tiles(least) * Hk;
+  const int64_t steps = (max_k + kStep - 1) / kStep;
+  p.split = (steps - 12) * resident(least) > 5 * size * steps / 4;
+  if (p.split) {
+    if (size >= cus / 2 && max_q * g > 64) p.groups = 2;
+  } else {
+    if (2 * size > 3 * resident(1) || launched(least) > 24576) p.groups = 2;
+    if (D == 128 && p.groups == 2 && 7 * queries(2) <= 5 * queries(3) &&
+        (2 * tiles(2) * Hk > 5 * resident(2) || launched(2) > 49152))
+      p.groups = 3;
+  }
+  const int64_t qt = queries(p.groups);
+  if (p.split)
+    p.split = resident(p.groups) >= Hk &&
+              split_fits(n_seqs, std::min(n_seqs * ((max_q + qt - 1) / qt), total_q / qt + n_seqs),
+                         max_k * kStep);
+  p.tiles = plain_tiles(n_seqs, max_q, qt);
+  p.grid = p.split ? resident(p.groups) / Hk * Hk : n_seqs * p.tiles * Hk;
+  p.sort = !p.split && n_seqs > 1 && n_seqs <= 64 && p.grid > resident(p.groups);
   return p;
 }
 
@@ -622,7 +723,7 @@ extern "C" int nkv_scaled_prefill(const nkv_scaled_prefill_args* args) {
                             (const char*)g.v_cache, g.cu_seqlens_q, g.cu_seqlens_k, g.block_tables,
                             g.bt_row_stride, Hk, group, (int32_t)g.block_size,
                             (int32_t)g.max_blocks_per_seq, (int32_t)g.n_blocks, (int32_t)g.n_seqs,
-                            (int32_t)p.tiles, g.total_q, (float)g.scale * kLog2e, (bf16_t*)g.out,
+                            (int32_t)p.tiles, (int32_t)p.sort, g.total_q, (float)g.scale * kLog2e, (bf16_t*)g.out,
                             g.out_row_stride, desc,
                             p.split ? reinterpret_cast<float*>(desc + p.grid) : nullptr};
   const dim3 grid((unsigned)p.grid);
@@ -639,14 +740,15 @@ extern "C" int nkv_scaled_prefill(const nkv_scaled_prefill_args* args) {
     else NKV_SCALED_PREFILL(64, 2);
   } else {
     if (p.groups == 1) NKV_SCALED_PREFILL(128, 1);
-    else NKV_SCALED_PREFILL(128, 2);
+    else if (p.groups == 2) NKV_SCALED_PREFILL(128, 2);
+    else NKV_SCALED_PREFILL_S(128, 3, false);
   }
 #undef NKV_SCALED_PREFILL
 #undef NKV_SCALED_PREFILL_S
   rc = check_launch("nkv_scaled_prefill");
   if (rc || !p.split) return rc;
   const int32_t tile_rows = 64 * p.groups;
-  const dim3 merge((unsigned)p.grid, (unsigned)(tile_rows / 4));
+  const dim3 merge((unsigned)p.grid, (unsigned)(tile_rows / 16));
   if (g.head_dim == 64)
     hipLaunchKernelGGL((scaled_merge_kernel<64>), merge, dim3(256), 0, as_stream(g.stream), a,
                        tile_rows);

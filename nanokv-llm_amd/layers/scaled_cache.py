@@ -297,8 +297,8 @@ def scaled_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     return out
 
 
-# Steps of fewer keys are not split: the plan need not be asked.
-_SPLIT_MIN_KEYS = 512
+# Up to so many keys a step is never split: the plan need not be asked.
+_WHOLE_KEYS = 768
 
 
 def scaled_prefill_workspace(q: torch.Tensor, k_cache: torch.Tensor, n_seqs: int,
@@ -306,7 +306,7 @@ def scaled_prefill_workspace(q: torch.Tensor, k_cache: torch.Tensor, n_seqs: int
     """The workspace for splitting scaled_varlen_prefill's keys where few query tiles would leave the
     chip idle, else None; None too where the device has no such memory left, since nothing else
     needs any."""
-    if max_seqlen_k < _SPLIT_MIN_KEYS:
+    if max_seqlen_k <= _WHOLE_KEYS:
         return None
     D = q.size(2)
     nbytes = _lib.lib().nkv_scaled_prefill_workspace_bytes(

@@ -224,6 +224,27 @@ def test_prefill_row_groups(dev):
         check_prefill(dev, make(dev, [37] * 40, 8, D, 64, seed=D, garbage=False), [37] * 40, 16)
 
 
+@pytest.mark.parametrize("new,lens,Hq,Hk,D", [
+    ([50, 200, 90], [400, 230, 90], 512, 8, 128),  # three row groups a wave, longest first
+    ([200, 5, 210], [200, 300, 211], 256, 8, 64),  # two
+    ([3] * 70, [3 + 5 * i for i in range(70)], 32, 2, 128),  # more sequences than are sorted
+])
+def test_prefill_more_tiles_than_the_chip_holds(dev, new, lens, Hq, Hk, D):
+    check_prefill(dev, make(dev, lens, Hk, D, 64, seed=D + len(new), garbage=False), new, Hq)
+
+
+@pytest.mark.parametrize("new,lens,Hq,Hk,D", [
+    ([100, 130], [2000, 1500], 64, 8, 128), ([100, 130], [2000, 1500], 64, 8, 64),
+    ([1] * 70 + [9], [7 * i + 1 for i in range(70)] + [1000], 4, 1, 64),
+    ([65, 1, 0, 4, 66], [65, 1200, 0, 4, 900], 4, 2, 128),
+])
+def test_prefill_ranges_of_many_units(dev, new, lens, Hq, Hk, D):
+    """Ranges that hold whole units and parts of others, of sequences past a wave's lanes too."""
+    assert L.lib().nkv_scaled_prefill_workspace_bytes(len(new), sum(new) + 3, max(new), max(lens), Hq,
+                                                      Hk, D) > 0
+    check_prefill(dev, make(dev, lens, Hk, D, 64, seed=D + len(new)), new, Hq)
+
+
 @pytest.mark.parametrize("split", [True, False])
 def test_prefill_rows_that_see_nothing(dev, split):
     """More queries than keys: the first rows see no key and are zeros."""
