@@ -24,7 +24,10 @@
 // 7.1 for one prompt of 77, which q's taking apart costs; not taken.
 //
 // SPLIT: where few tiles would leave the chip idle, the workgroups that fit it at once take equal ranges
-// of all the key steps, and a second launch merges the rows whose keys were cut.
+// of all the key steps, and a second launch merges the rows whose keys were cut. Units of few rows (single
+// tokens, drafts) give a wave's rows to two waves, one for each cache tile of a step, joined in LDS at
+// the unit's end: 2 chunks of 400 with 30 tokens behind up to 8000 keys (Hq 16, Hk 4, D 128) 91 us against
+// 109, 4 drafts behind 9000 - 30000 (Hq 32, Hk 8) 50 against 53, of which the codes alone take 25.
 #include "launch_rules.h"
 #include "lds_tiles.h"
 #include "scaled_cache.h"
@@ -279,12 +282,16 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
 
   // ---- this wave's row groups: head and query of this lane's row (rows past the tile's queries
   // take query Lq: attended like the others, never stored)
-  const bool idle = wave * (16 * RG) >= min(QT, Lq - j0) * G;  // only brings its share of the codes
+  const int rows = min(QT, Lq - j0) * G;
+  // few rows: waves 0 and 1 attend to them in the even cache tiles, 2 and 3 in the odd ones
+  const bool by_keys = SPLIT && rows <= 2 * (16 * RG);
+  const int rwave = by_keys ? wave & 1 : wave;
+  const bool idle = rwave * (16 * RG) >= rows;  // only brings its share of the codes
   int jrow[RG];
   u32x4_t qreg[RG][kKs];
 #pragma unroll
   for (int rr = 0; rr < RG; ++rr) {
-    const int r = (wave * RG + rr) * 16 + col;
+    const int r = (rwave * RG + rr) * 16 + col;
     const bool real = r < QT * G;
     const int head = real ? r % G : 0;
     jrow[rr] = real ? j0 + r / G : Lq;
@@ -348,19 +355,23 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
 #pragma unroll
   for (int st = 0; st < kStages - 1; ++st) issue();
 
-  auto compute = [&](int s, int stage, auto edge_c) __attribute__((always_inline)) {
+  // NC cache tiles of step s, from tile t0 on
+  auto compute = [&](int s, int stage, int t0, auto nc_c, auto edge_c)
+                     __attribute__((always_inline)) {
+    constexpr int NC = decltype(nc_c)::value;
     constexpr bool EDGE = decltype(edge_c)::value;
-    const char* kt = ring + stage * kStageB + lane * 16;
-    const char* st = ring + stage * kStageB + kCodesB + lane * 4;
-    float scale[4];  // K, V of the first cache tile, of the second
+    const char* kt = ring + stage * kStageB + t0 * (2 * kTileB) + lane * 16;
+    const char* st = ring + stage * kStageB + kCodesB + t0 * 512 + lane * 4;
+    const int at = s * kStep + t0 * kTileRows + 8 * g4;  // the lane's first key
+    float scale[2 * NC];  // K, V of each cache tile
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
+    for (int w = 0; w < 2 * NC; ++w)
       scale[w] = scale_of(stored_scale(byte_of(
           uni((int)*reinterpret_cast<const uint32_t*>(st + w * 256)), (int)scale_off)));
-    // S^T of quarter h: tokens 32 (h / 2) + 8 g4 + 4 (h % 2) + 0..3 of the step
-    float sv[RG][16];
+    // S^T of half h of a tile: tokens 32 (h / 2) + 8 g4 + 4 (h % 2) + 0..3 from the first tile's on
+    float sv[RG][8 * NC];
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
+    for (int h = 0; h < 2 * NC; ++h) {
       u32x4_t ka[kKs];
 #pragma unroll
       for (int i = 0; i < kI; ++i) {
@@ -378,13 +389,13 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
         for (int r = 0; r < 4; ++r) sv[rr][4 * h + r] = x[r];
       }
     }
-    [[maybe_unused]] int lim[RG];  // last key that the row sees, from the lane's first of the step on
+    [[maybe_unused]] int lim[RG];  // last key that the row sees, from the lane's first on
     if constexpr (EDGE) {
 #pragma unroll
       for (int rr = 0; rr < RG; ++rr) {
-        lim[rr] = min(diag + jrow[rr], Lk - 1) - s * kStep - 8 * g4;
+        lim[rr] = min(diag + jrow[rr], Lk - 1) - at;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
+        for (int e = 0; e < 8 * NC; ++e)
           if ((e >> 3) * kTileRows + (e & 7) > lim[rr]) sv[rr][e] = -INFINITY;
       }
     }
@@ -394,9 +405,13 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
 #pragma unroll
     for (int rr = 0; rr < RG; ++rr) {
       const float* v = sv[rr];
-      top[rr] = fmax3(fmax3(fmax3(v[0], v[1], v[2]), fmax3(v[3], v[4], v[5]),
-                            fmax3(v[6], v[7], v[8])),
-                      fmax3(v[9], v[10], v[11]), fmax3(fmax3(v[12], v[13], v[14]), v[15], -INFINITY));
+      if constexpr (NC == 1)
+        top[rr] = fmax3(fmax3(v[0], v[1], v[2]), fmax3(v[3], v[4], v[5]), fmaxf(v[6], v[7]));
+      else
+        top[rr] = fmax3(fmax3(fmax3(v[0], v[1], v[2]), fmax3(v[3], v[4], v[5]),
+                              fmax3(v[6], v[7], v[8])),
+                        fmax3(v[9], v[10], v[11]),
+                        fmax3(fmax3(v[12], v[13], v[14]), v[15], -INFINITY));
       raise_any = raise_any || top[rr] * a.scale_log2 > m_run[rr] + kLazy;
     }
     if (__builtin_amdgcn_ballot_w64(raise_any) != 0) {
@@ -412,7 +427,7 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
       }
     }
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < NC; ++c) {
       u32x4_t pb[RG];
 #pragma unroll
       for (int rr = 0; rr < RG; ++rr) {
@@ -430,7 +445,7 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
       if constexpr (EDGE) {
         // codes behind the end may be anything, NaN too, which a zero weight would not hide; and
         // rows that do not see a key must not see its NaN: those that each row sees are counted
-        const int m = min(max(Lk - s * kStep - c * kTileRows - 8 * g4, 0), 8);
+        const int m = min(max(Lk - at - c * kTileRows, 0), 8);
         const uint32_t keep0 = m >= 4 ? ~0u : (1u << (8 * m)) - 1;
         const uint32_t keep1 = m >= 8 ? ~0u : m > 4 ? (1u << (8 * (m - 4))) - 1 : 0u;
 #pragma unroll
@@ -484,21 +499,59 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
   // steps from s_edge on mask keys of some row
   const int s_edge = max(0, min(diag + j0 + 1, Lk)) / kStep;
   int stage = 0;
-  auto step = [&](int s, auto edge_c) __attribute__((always_inline)) {
-    // this wave's loads of step s have landed, then everyone's have, and everyone is done with step
-    // s - 1, whose stage takes the step kStages - 1 ahead
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 2) * (kLoads + 1)) : "memory");
-    __syncthreads();
-    issue();
-    if (!idle) compute(s, stage, edge_c);
-    stage = stage + 1 == kStages ? 0 : stage + 1;
+  auto steps = [&](int t0, auto nc_c) __attribute__((always_inline)) {
+    auto step = [&](int s, auto edge_c) __attribute__((always_inline)) {
+      // this wave's loads of step s have landed, then everyone's have, and everyone is done with step
+      // s - 1, whose stage takes the step kStages - 1 ahead
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 2) * (kLoads + 1)) : "memory");
+      __syncthreads();
+      issue();
+      if (!idle) compute(s, stage, t0, nc_c, edge_c);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    };
+    int s = s_lo;
+    for (; s < min(s_edge, s_end); ++s) step(s, std::integral_constant<bool, false>{});
+    for (; s < s_end; ++s) step(s, std::integral_constant<bool, true>{});
   };
-  int s = s_lo;
-  for (; s < min(s_edge, s_end); ++s) step(s, std::integral_constant<bool, false>{});
-  for (; s < s_end; ++s) step(s, std::integral_constant<bool, true>{});
+  if (by_keys) steps(wave >> 1, std::integral_constant<int, 1>{});
+  else steps(0, std::integral_constant<int, 2>{});
   // no load into LDS outlives the workgroup, or meets the next unit's
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  if constexpr (SPLIT) __syncthreads();
+  if constexpr (SPLIT) {
+    __syncthreads();
+    if (by_keys) {  // the odd tiles' sums join the even ones'
+      float* mine = reinterpret_cast<float*>(ring) + rwave * (RG * (kDb + 1) * 4 * 64) + lane * 4;
+      if (wave >= 2 && !idle) {
+#pragma unroll
+        for (int rr = 0; rr < RG; ++rr) {
+          float* x = mine + rr * ((kDb + 1) * 4 * 64);
+#pragma unroll
+          for (int db = 0; db < kDb; ++db) *reinterpret_cast<f32x4_t*>(x + db * 256) = acc[rr][db];
+          *reinterpret_cast<float2*>(x + kDb * 256) = float2{m_run[rr], l_run[rr]};
+        }
+      }
+      __syncthreads();
+      if (wave < 2 && !idle) {
+#pragma unroll
+        for (int rr = 0; rr < RG; ++rr) {
+          const float* x = mine + rr * ((kDb + 1) * 4 * 64);
+          const float2 ml = *reinterpret_cast<const float2*>(x + kDb * 256);
+          const float m = fmaxf(m_run[rr], ml.x);
+          const float w0 = fast_exp2(m_run[rr] - m), w1 = fast_exp2(ml.x - m);
+          m_run[rr] = m;
+          l_run[rr] = l_run[rr] * w0 + ml.y * w1;
+#pragma unroll
+          for (int db = 0; db < kDb; ++db) {
+            const f32x4_t o = *reinterpret_cast<const f32x4_t*>(x + db * 256);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[rr][db][e] = fmaf(o[e], w1, acc[rr][db][e] * w0);
+          }
+        }
+      }
+      __syncthreads();
+      if (wave >= 2) continue;
+    }
+  }
   if (idle) continue;
 
   const bool part = SPLIT && (cut || s_lo > 0);
@@ -509,7 +562,7 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
     if constexpr (SPLIT) {
       if (part) {  // to one of two slots: the end of a unit begun before, or a unit's begin
         float* pr = a.part + (((int64_t)blockIdx.x * 2 + (s_lo == 0)) * (64 * RG) +
-                              (wave * RG + rr) * 16 + col) * part_floats(D);
+                              (rwave * RG + rr) * 16 + col) * part_floats(D);
 #pragma unroll
         for (int db = 0; db < kDb; ++db)
           *reinterpret_cast<f32x4_t*>(pr + db * 16 + g4 * 4) = acc[rr][db];
@@ -518,7 +571,7 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
       }
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;
-    const int head = (wave * RG + rr) * 16 + col - (jrow[rr] - j0) * G;
+    const int head = (rwave * RG + rr) * 16 + col - (jrow[rr] - j0) * G;
     bf16_t* op = a.out + (int64_t)(q0 + jrow[rr]) * a.out_row_stride +
                  (int64_t)(kvh * G + head) * D + g4 * 4;
 #pragma unroll
