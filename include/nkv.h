@@ -874,8 +874,9 @@ int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info, 
  * the other rows' codes become E4M3(code * 2^(e_old - e)). Rounding is to nearest
  * even; larger values and infinities become +-448 * 2^e, NaN stays NaN.
  * The tokens of a tile must stand next to each other in slot_mapping, in any
- * order, as tokens listed sequence by sequence do (of two for one slot the later
- * stays); what a tile holds whose tokens stand in two places is undefined.
+ * order, as tokens listed sequence by sequence do, with fewer than 32 skipped ones
+ * between any two (of two for one slot the later stays); what a tile holds whose
+ * tokens stand in two places is undefined.
  */
 typedef struct nkv_scaled_store_args {
   const void* key;
@@ -945,7 +946,7 @@ int nkv_scaled_decode(const nkv_scaled_decode_args* args);
  * group up to NKV_SCALED_MAX_GROUP. A row that sees no key gives zeros, rows of no
  * sequence stay as they were; keys past the table or in an invalid block are
  * zeros, and keys that a row does not see have no effect on it, whatever they
- * hold.
+ * hold. At most 2^20 sequences and 2^30 rows.
  * No counterpart in the reference (beside nanokvllm/layers/attention.py:96-102).
  */
 #define NKV_SCALED_MAX_GROUP 128

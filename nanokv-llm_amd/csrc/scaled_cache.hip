@@ -13,13 +13,15 @@
 // apart. Lane (x, y) holds dims 8x .. 8x+7 of tokens 8y .. 8y+7 in registers: one pass over the
 // memory for the maximum and the codes, and both orders of codes are packed from the block that the
 // lane holds (K's eight dims of a token, V's eight tokens of a dim), with no exchange. The tile's
-// owner is the wave whose token begins a run of tokens of that tile in slot_mapping.
+// owner is the wave whose token begins a run of tokens of that tile in slot_mapping, which skipped
+// tokens between them do not end.
 #include "scaled_cache.h"
 
 #include <algorithm>
 
 namespace nkv {
 
+constexpr int kGap = 32;         // so many skipped tokens end a run
 constexpr int kScaledWaves = 4;  // of a workgroup: as many heads (or pairs), of K or V
 
 int scaled_check(const char* what, const void* k_cache, const void* v_cache, int64_t n_kv_heads,
@@ -176,17 +178,20 @@ __global__ __launch_bounds__(64 * kScaledWaves) void scaled_store_kernel(
   char* cache = un.is_v ? v_cache : k_cache;
   const int64_t tile_bytes = (int64_t)kTileRows * (Hk * D + kRowPad);
 
-  const auto tile_of = [&](int64_t t) -> int {
-    if (t < 0 || t >= n_tokens) return -1;
+  const auto tile_of = [&](int64_t t) -> int {  // -1: skipped, -2: no token
+    if (t < 0 || t >= n_tokens) return -2;
     const int64_t s = slot_mapping[t];
     NKV_DBG(s < -1 || s >= n_slots, NKV_DEBUG_SLOT);
     return s >= 0 && s < n_slots ? (int)(s / kTileRows) : -1;
   };
-  const int64_t w0 = (int64_t)blockIdx.x * window;
-  const int mine = lane < window ? tile_of(w0 + lane) : -1;
-  int before = __shfl_up(mine, 1, 64);
-  if (lane == 0) before = tile_of(w0 - 1);
-  uint64_t begins = __ballot(mine >= 0 && mine != before);
+  // lanes kGap ..: the window; a run goes on over fewer than kGap skipped tokens
+  const int64_t w0 = (int64_t)blockIdx.x * window - kGap;
+  const int mine = lane < kGap + window ? tile_of(w0 + lane) : -2;
+  const uint64_t before = __ballot(mine >= 0) & ((1ull << lane) - 1);
+  const int last = before ? 63 - __builtin_clzll(before) : 0;
+  const int last_tile = __shfl(mine, last, 64);
+  uint64_t begins = __ballot(lane >= kGap && mine >= 0 &&
+                             (!before || last < lane - kGap || last_tile != mine));
 
   for (; begins; begins &= begins - 1) {
     const int ln = __builtin_ctzll(begins);
@@ -195,12 +200,20 @@ __global__ __launch_bounds__(64 * kScaledWaves) void scaled_store_kernel(
     // the run's tokens by row; of two for a row the later one stays
     if (lane < kTileRows) rows[wave][lane] = -1;
     __builtin_amdgcn_wave_barrier();
-    for (int64_t at = t0;; at += 64) {
-      const bool in = tile_of(at + lane) == tile;
-      const uint64_t out = ~__ballot(in);
+    int skipped = 0;  // tokens since the run's last
+    for (int64_t at = t0;;) {
+      const int tl = tile_of(at + lane);
+      const uint64_t out = ~__ballot(tl == tile);
       const int n = out ? __builtin_ctzll(out) : 64;
       if (lane < n) atomicMax(&rows[wave][slot_mapping[at + lane] % kTileRows], (int)(at + lane));
-      if (n < 64) break;
+      if (n > 0) skipped = 0;
+      at += n;
+      if (n == 64) continue;
+      const uint64_t next = ~__ballot(tl == -1) >> n;
+      const int k = next ? __builtin_ctzll(next) : 64 - n;
+      skipped += k;
+      at += k;
+      if (k == 0 || skipped >= kGap) break;
     }
     __builtin_amdgcn_wave_barrier();
     int from[8];

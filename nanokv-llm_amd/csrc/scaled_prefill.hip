@@ -42,6 +42,7 @@ namespace nkv {
 
 constexpr int kStep = 64;      // keys a step
 constexpr float kLazy = 8.f;   // log2 headroom before the running maximum is raised
+constexpr int64_t kMostSeqs = 1 << 20, kMostRows = 1 << 30;  // the plan's products stay in 64 bits
 constexpr int part_floats(int D) { return D + 4; }  // of a partial row: O, m, l, 2 pad
 
 struct ScaledPrefillArgs {
@@ -684,6 +685,8 @@ struct ScaledPrefillPlan {
 static ScaledPrefillPlan scaled_prefill_plan(int64_t n_seqs, int64_t total_q, int64_t max_q,
                                              int64_t max_k, int32_t Hk, int g, int D) {
   const int cus = device_cus();
+  max_q = std::min(max_q, total_q);  // no sequence has more
+  max_k = std::min<int64_t>(std::max<int64_t>(max_k, 0), INT32_MAX);
   const BatchMix m = batch_mix(n_seqs, total_q, max_q);
   const auto queries = [&](int groups) -> int64_t { return 64 * groups / g; };  // of a tile
   const auto tiles = [&](int groups) -> int64_t {  // that hold queries
@@ -698,7 +701,7 @@ static ScaledPrefillPlan scaled_prefill_plan(int64_t n_seqs, int64_t total_q, in
   const int least = g > 64 ? 2 : 1;
   ScaledPrefillPlan p;
   p.groups = least;
-  int64_t size = tiles(least) * Hk;
+  const int64_t size = std::min<int64_t>(tiles(least) * Hk, INT32_MAX);
   const int64_t steps = (max_k + kStep - 1) / kStep;
   p.split = (steps - 12) * resident(least) > 5 * size * steps / 4;
   if (p.split) {
@@ -727,7 +730,8 @@ extern "C" size_t nkv_scaled_prefill_workspace_bytes(int32_t n_seqs, int64_t tot
                                                      int32_t n_q_heads, int32_t n_kv_heads,
                                                      int32_t head_dim) {
   using namespace nkv;
-  if (n_seqs <= 0 || total_q <= 0 || max_seqlen_q <= 0 || n_kv_heads <= 0 ||
+  if (n_seqs <= 0 || n_seqs > kMostSeqs || total_q <= 0 || total_q > kMostRows ||
+      max_seqlen_q <= 0 || n_kv_heads <= 0 || n_kv_heads > NKV_SCALED_MAX_HEADS ||
       n_q_heads % n_kv_heads != 0 || n_q_heads / n_kv_heads <= 0 ||
       n_q_heads / n_kv_heads > NKV_SCALED_MAX_GROUP || !scaled_dim_ok(head_dim))
     return 0;
@@ -741,7 +745,9 @@ extern "C" int nkv_scaled_prefill(const nkv_scaled_prefill_args* args) {
   clear_error();
   NKV_REQUIRE(args, NKV_EINVAL, "scaled_prefill: null arguments");
   const nkv_scaled_prefill_args& g = *args;
-  NKV_REQUIRE(g.n_seqs >= 0 && g.n_seqs < (1ll << 31) && g.total_q >= 0 && g.total_q <= (1 << 30) &&
+  NKV_REQUIRE(g.n_seqs <= kMostSeqs, NKV_EUNSUPPORTED, "scaled_prefill: too many sequences (%lld)",
+              (long long)g.n_seqs);
+  NKV_REQUIRE(g.n_seqs >= 0 && g.total_q >= 0 && g.total_q <= kMostRows &&
                   g.max_seqlen_q >= 0 && g.n_blocks >= 0,
               NKV_EINVAL, "scaled_prefill: bad sizes (%lld sequences, %lld rows)",
               (long long)g.n_seqs, (long long)g.total_q);

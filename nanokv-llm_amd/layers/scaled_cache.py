@@ -199,7 +199,7 @@ def scaled_store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.
     A call that writes a tile's first row begins the tile anew, with the scale of the rows that it
     writes there; otherwise the scale only grows, and the rows held so far are rounded to it where it
     does. The tokens of one tile must stand next to each other in ``slot_mapping``, as those of a
-    sequence do.
+    sequence do, fewer than 32 skipped ones between any two.
     """
     what = "scaled_store_kvcache"
     ks, cs, di = key.shape, k_cache.shape, key.get_device()

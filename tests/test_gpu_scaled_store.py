@@ -123,6 +123,23 @@ def test_slots_that_are_skipped(dev, D):
     c.check()
 
 
+@pytest.mark.parametrize("Hk,D,n", [(2, 64, 6), (2, 128, 6), (8, 64, 200), (8, 128, 200)])
+def test_slots_that_are_skipped_inside_a_tile(dev, Hk, D, n):
+    """Skipped slots between a tile's tokens, up to 31 at once and over the borders of what a wave
+    looks at: one scale all the same, also where it grows and the rows held are rounded again."""
+    rng, g = random.Random(n), torch.Generator().manual_seed(n)
+    c = Caches(dev, n, 32, Hk, D)
+    c.store(values(n, Hk, D, g) * 2.0 ** -6, values(n, Hk, D, g) * 2.0 ** -6,
+            [32 * i + 3 for i in range(n)])
+    slots = []
+    for i in range(n):
+        for r in sorted(rng.sample(range(1, 32), rng.choice([1, 2, 5, 31]))):
+            slots += [32 * i + r] + [-1] * rng.choice([0, 0, 0, 1, 2, 7, 31])
+        slots += [-1] * rng.choice([0, 40])
+    c.store(values(len(slots), Hk, D, g), values(len(slots), Hk, D, g), slots)
+    c.check()
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_special_values(dev, D):
     """NaN, infinities, zeros of both signs, subnormals and the largest values."""

@@ -184,6 +184,20 @@ def test_workspace_follows_the_chip():
             assert f(n, tq, mq, 10 ** 6, 32, 8, d) < 600e6
 
 
+def test_prefill_maxima_of_any_size():
+    """max_seqlen_q and max_seqlen_k far past what there is: as if they were q's rows and 2^31 keys; more
+    tiles than a launch holds are refused, not counted wrongly."""
+    f = L.lib().nkv_scaled_prefill_workspace_bytes
+    for n, tq in ((1, 8), (4, 36), (16, 64)):
+        assert f(n, tq, 1 << 62, 10 ** 6, 32, 8, 128) == f(n, tq, tq, 10 ** 6, 32, 8, 128) > 0
+    assert f(1, 8, 8, 1 << 62, 32, 8, 128) == f(1, 8, 8, (1 << 31) - 1, 32, 8, 128)
+    assert f(1, 8, 8, -(1 << 62), 32, 8, 128) == 0 == f((1 << 20) + 1, 8, 8, 9000, 32, 8, 128)
+    for kw in (dict(n=1 << 20, tq=1 << 30, mq=1 << 62), dict(n=1 << 20, tq=1 << 30, mq=1 << 30, hk=512,
+                                                              hq=512, qrs=1 << 15, ors=1 << 15),
+               dict(n=(1 << 20) + 1), dict(n=1 << 62)):
+        test_entry_points_refuse("nkv_scaled_prefill", PREFILL, kw, -4, b"too many")
+
+
 # ---------------------------------------------------------------- the wrappers' refusals
 def _gpu_free(monkeypatch):
     """The checks of the wrappers, with host tensors taken for the GPU's."""
