@@ -12,7 +12,9 @@
 // MI355X design: one wave to a tile and 128 elements of its rows (a head of 128, two of 64), K and V
 // apart. Lane (x, y) holds dims 8x .. 8x+7 of tokens 8y .. 8y+7 in registers: one pass over the
 // memory for the maximum and the codes, and both orders of codes are packed from the block that the
-// lane holds (K's eight dims of a token, V's eight tokens of a dim), with no exchange. The tile's
+// lane holds (K's eight dims of a token, V's eight tokens of a dim), with no exchange. A tile that is
+// written whole goes through LDS, which makes 1 KiB of consecutive bytes of each store instead of 32
+// pieces of 16 (15800 rows of Hk 8, D 128: 25 us instead of 28, 3.9 TB/s). The tile's
 // owner is the wave whose token begins a run of tokens of that tile in slot_mapping, which skipped
 // tokens between them do not end.
 #include "scaled_cache.h"
@@ -22,6 +24,10 @@
 namespace nkv {
 
 constexpr int kGap = 32;         // so many skipped tokens end a run
+// Neighbouring workgroups take windows a 37th of the list apart: with a tile's run in every fourth window
+// those with work would else go to two of the eight XCDs (8 prompts of 512, Hk 8, D 128: 16.6 us, now
+// 9.4; 16 of 2000: 52.7, now 37.4).
+constexpr unsigned kScatter = 37;
 constexpr int kScaledWaves = 4;  // of a workgroup: as many heads (or pairs), of K or V
 
 int scaled_check(const char* what, const void* k_cache, const void* v_cache, int64_t n_kv_heads,
@@ -91,7 +97,7 @@ __device__ __forceinline__ uint32_t put_codes(float a, float b, uint32_t old) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, (int)old, HIGH);
 }
 
-// The codes of the lane's block into the head's tile. SPECIAL: there may be values past +-448 or
+// The codes of the lane's block into the head's tile (or its copy in LDS). SPECIAL: there may be values past +-448 or
 // NaN among them. all: every row of the lane's eight is written.
 template <int D, bool SPECIAL>
 __device__ __forceinline__ void write_codes(const Unit<D>& un, const u32x4_t (&row)[8],
@@ -168,6 +174,7 @@ __global__ __launch_bounds__(64 * kScaledWaves) void scaled_store_kernel(
     const int32_t* __restrict__ slot_mapping, int64_t n_tokens, int32_t Hk, int64_t n_slots,
     int32_t units, int32_t window) {
   __shared__ int32_t rows[kScaledWaves][kTileRows];  // the token of each row of the tile, or -1
+  __shared__ __attribute__((aligned(16))) char staged[kScaledWaves][kTileRows * 128];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int unit = blockIdx.y * kScaledWaves + wave;
@@ -185,7 +192,10 @@ __global__ __launch_bounds__(64 * kScaledWaves) void scaled_store_kernel(
     return s >= 0 && s < n_slots ? (int)(s / kTileRows) : -1;
   };
   // lanes kGap ..: the window; a run goes on over fewer than kGap skipped tokens
-  const int64_t w0 = (int64_t)blockIdx.x * window - kGap;
+  const uint32_t wi = window == 1 ? blockIdx.x
+                                  : blockIdx.x % kScatter * (gridDim.x / kScatter) +
+                                        blockIdx.x / kScatter;
+  const int64_t w0 = (int64_t)wi * window - kGap;
   const int mine = lane < kGap + window ? tile_of(w0 + lane) : -2;
   const uint64_t before = __ballot(mine >= 0) & ((1ull << lane) - 1);
   const int last = before ? 63 - __builtin_clzll(before) : 0;
@@ -258,6 +268,22 @@ __global__ __launch_bounds__(64 * kScaledWaves) void scaled_store_kernel(
     const int e = first ? need : max(old, need);
     special = special || __ballot(e == kMaxScale) != 0;
     char* codes = base + un.h0 * (kTileRows * D);
+    if (__ballot(all) == ~0ull) {
+      // a whole tile: put together in LDS, written as 1 KiB of consecutive bytes at a time
+      char* mine_at = staged[wave] + (un.head - un.h0) * (kTileRows * D);
+      if (special) write_codes<D, true>(un, row, from, true, inverse_scale(e), mine_at);
+      else write_codes<D, false>(un, row, from, true, inverse_scale(e), mine_at);
+      __builtin_amdgcn_wave_barrier();
+      const int pieces = min(Unit<D>::kHeads, Hk - un.h0) * (kTileRows * D / 1024);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < pieces)
+          *reinterpret_cast<u32x4_t*>(codes + i * 1024 + lane * 16) =
+              *reinterpret_cast<const u32x4_t*>(staged[wave] + i * 1024 + lane * 16);
+      if (un.live && un.y == 0 && un.hx == 0) scales[un.head] = (char)e;
+      __builtin_amdgcn_wave_barrier();
+      continue;
+    }
     if (!first) {
       const int grown = e - old;
       if (__ballot(un.live && grown > 0)) {
@@ -387,9 +413,19 @@ extern "C" int nkv_scaled_store(const nkv_scaled_store_args* args) {
                   g.value_row_stride % 8 == 0,
               NKV_EINVAL, "scaled_store: row strides must be multiples of 8 covering the row");
   const int Hk = (int)g.n_kv_heads, units = scaled_units(Hk, (int)g.head_dim);
-  const int window = g.n_tokens * units <= 8192 ? 1 : 8;
-  const dim3 grid((unsigned)((g.n_tokens + window - 1) / window),
-                  (unsigned)((units + kScaledWaves - 1) / kScaledWaves));
+  // Tokens a wave looks at. Runs in one window follow each other (2.5 us each), and a wave without one
+  // costs its dispatch (about 0.9 ns of the chip). 1 / 4 / 8 / 16 tokens (Hk 8, D 128), us:
+  //   256 tokens of as many sequences (4096 of these products)   7.5 / 16.0 / 27.5 / 51
+  //   1024, 2048 (16384, 32768)      19.1 / 24.5 / 31.6, 34.2 / 37.8 / 44.3
+  //   8 prompts of 512 (65536)       73.8 / 10.4 / 9.4 / 7.9
+  //   16 of 500 (128000)             46.3 / 15.8 / 14.0 / 13.4
+  //   16 of 2000 (512000)            480 / 43.2 / 37.3 / 34.2
+  // A list of prompts may hold single tokens too, whose windows should not outlast the rest.
+  const int64_t waves = g.n_tokens * units;
+  const int window = waves <= 8192 ? 1 : waves <= 131072 ? 4 : 8;
+  int64_t windows = (g.n_tokens + window - 1) / window;
+  if (window > 1) windows = (windows + kScatter - 1) / kScatter * kScatter;
+  const dim3 grid((unsigned)windows, (unsigned)((units + kScaledWaves - 1) / kScaledWaves));
 #define NKV_SCALED_STORE(D)                                                                      \
   hipLaunchKernelGGL((scaled_store_kernel<D>), grid, dim3(64 * kScaledWaves), 0,                 \
                      as_stream(g.stream), (const bf16_t*)g.key, g.key_row_stride,                \
