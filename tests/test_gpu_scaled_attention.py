@@ -280,6 +280,71 @@ def test_prefill_blocks_that_are_not_there(dev, split):
     check_prefill(dev, c, [50, 96, 6], 4, split=split, lens=[150, 96, 720])
 
 
+def splits(new, lens, Hq, Hk, D):
+    return L.lib().nkv_scaled_prefill_workspace_bytes(len(new), sum(new) + 3, max(new), max(lens), Hq,
+                                                      Hk, D) > 0
+
+
+def test_prefill_ranges_of_rows_that_see_nothing(dev):
+    new, lens = [7, 2, 41, 1301, 5], [3, 0, 40, 1300, 1000]
+    assert splits(new, lens, 4, 2, 64)
+    got = check_prefill(dev, make(dev, lens, 2, 64, 32, seed=18), new, 4)
+    assert not bool(got[:4].any()) and not bool(got[7:9].any()) and not bool(got[9].any())
+    assert not bool(got[50].any()) and bool(got[51].any())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_prefill_ranges_of_keys_that_rows_do_not_see(dev, D):
+    """NaN in later keys, of units that one wave takes a row group of and of those that two share."""
+    from oracle.scaled_ref import places
+    Hk, lens, new = 2, [1100, 900, 1000], [20, 70, 5]
+    assert splits(new, lens, 4, Hk, D)
+    c = make(dev, lens, Hk, D, 32, seed=19)
+    mem = {x: c[x].view(c[x].size(0), -1) for x in "kv"}
+    for i, p, h, dim, x in ((0, 1091, 0, 3, "v"), (0, 1095, 1, D - 1, "v"), (0, 1097, 1, 5, "k"),
+                            (1, 860, 0, 0, "v"), (1, 897, 1, 17, "k"), (2, 999, 1, 1, "v")):
+        at = h * TILE * D + int(places(D)[int(x == "v")][p % TILE, dim])
+        mem[x][int(c["bt"][i, p // 32]), at] = 0x7f
+    got = check_prefill(dev, c, new, 4)
+    assert not bool(got[:11].isnan().any()) and bool(got[19].isnan().any())
+    assert not bool(got[20:50].isnan().any()) and bool(got[89].isnan().any())
+    assert not bool(got[90:94].isnan().any()) and bool(got[94].isnan().any())
+
+
+def test_prefill_ranges_over_blocks_that_are_not_there(dev):
+    new, lens = [50, 96, 6], [150, 96, 1320]
+    assert splits(new, lens, 4, 2, 64)
+    c = make(dev, [150, 96, 1300], 2, 64, 32, width=41, seed=20)
+    c["bt"][0, 1] = -1
+    c["bt"][1, :] = 10 ** 6
+    c["bt"][2, 20:23] = -5
+    check_prefill(dev, c, new, 4, lens=lens)
+
+
+def test_two_streams_at_once(dev):
+    """Calls that overlap, each with what it allocates: as one after the other."""
+    new, lens = [9, 70, 1, 5], [1500, 1300, 900, 1100]
+    c = make(dev, lens, 2, 64, 32, seed=21, garbage=False)
+    k, v, bt = gpu(dev, c)
+    i32 = dict(dtype=I32, device=dev)
+    q = values(sum(new), 8, 64, c["g"], outliers=False).to(dev)
+    cu_q, cu_k = ([sum(x[:i]) for i in range(len(x) + 1)] for x in (new, lens))
+    args = (torch.tensor(cu_q, **i32), torch.tensor(cu_k, **i32), max(new), 0.1, bt)
+    ctx = torch.tensor(lens, **i32)
+    want = (nkv.scaled_varlen_prefill(q, k, v, *args, max_seqlen_k=max(lens)),
+            nkv.scaled_paged_decode(q[:4], k, v, ctx, bt, 0.1))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, nkv.scaled_varlen_prefill(q, k, v, *args, max_seqlen_k=max(lens))
+                            if i < 2 else nkv.scaled_paged_decode(q[:4], k, v, ctx, bt, 0.1)))
+    torch.cuda.synchronize()
+    for i, x in got:
+        assert torch.equal(x, want[i == 2])
+
+
 def test_prefill_sequences_outside_the_rows(dev):
     """cu_seqlens_q that names rows which q does not have: left out, nothing else touched."""
     c = make(dev, [40, 40, 40], 2, 64, 32, seed=11)
