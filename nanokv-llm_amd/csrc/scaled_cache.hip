@@ -303,6 +303,8 @@ __global__ __launch_bounds__(64 * kScaledWaves) void scaled_store_kernel(
 }
 
 // ---------------------------------------------------------------- reading back
+// HBM-bound: 414 MB read and written (12 sequences, Hk 8, D 128) in 82 us, 5.04 TB/s, a copy's rate. The
+// wave's place in a tile is the store's, so that V's codes turn back into rows within the lane.
 // Workgroup (tile, unit group): a tile of what sequence i holds at positions [start, start + n), n its
 // share of cu_seqlens. Every workgroup finds its sequence and tile itself.
 template <int D>
