@@ -27,7 +27,7 @@
 // of all the key steps, and a second launch merges the rows whose keys were cut. Units of few rows (single
 // tokens, drafts) give a wave's rows to two waves, one for each cache tile of a step, joined in LDS at
 // the unit's end: 2 chunks of 400 with 30 tokens behind up to 8000 keys (Hq 16, Hk 4, D 128) 91 us against
-// 109, 4 drafts behind 9000 - 30000 (Hq 32, Hk 8) 50 against 53, of which the codes alone take 25.
+// 109, 4 drafts behind 9000 - 30000 (Hq 32, Hk 8) 50 against 53 (48 now), of which the codes alone take 25.
 #include "launch_rules.h"
 #include "lds_tiles.h"
 #include "scaled_cache.h"
@@ -80,6 +80,10 @@ struct Cursor {
   int C, T, x, x_end;         // range length, stream length, the range's begin and end
 };
 constexpr int kSnap = 2;        // steps
+// What a unit's start and end cost, counted before its first step. 0 / 2 / 3 / 4 / 6, us: drafts 50.5 / 48.3 /
+// 47.9 / 47.5 / 47.7, 30 tokens and two chunks 36.8 / 34.8 / 34.5 / 34.4 / 36.0, 8 drafts behind up to 4000
+// 29.3 / 27.0 / 27.0 / 26.3 / 26.1, 4 chunks of 128 63.6 / 59.4 / 60.1 / 59.8 / 62.1.
+constexpr int kUnitSteps = 3;
 constexpr int kLeastSteps = 4;  // shortest range
 template <int RG>
 __device__ __forceinline__ int key_cost(int rows) {
@@ -91,11 +95,11 @@ __device__ __forceinline__ int tile_steps(int Lq, int Lk, int qt, int t) {
 }
 // Keys of tile t as the stream counts them, and the cost of the tiles before tile t, all full.
 __device__ __forceinline__ int tile_keys(int Lq, int Lk, int qt, int t) {
-  return max(Lk - Lq, 0) + min(Lq, (t + 1) * qt);
+  return max(Lk - Lq, 0) + min(Lq, (t + 1) * qt) + kUnitSteps * kStep;
 }
 template <int RG>
 __device__ __forceinline__ int cost_before(int Lq, int Lk, int qt, int t, int G) {
-  return key_cost<RG>(qt * G) * (t * max(Lk - Lq, 0) + qt * (t * (t + 1) / 2));
+  return key_cost<RG>(qt * G) * (t * (max(Lk - Lq, 0) + kUnitSteps * kStep) + qt * (t * (t + 1) / 2));
 }
 template <int RG>
 __device__ __forceinline__ bool split_begin(const ScaledPrefillArgs& a, int qt, Cursor& c) {
@@ -260,22 +264,23 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
   const int diag = Lk - Lq;  // query j sees keys <= diag + j
   const int last_key = min(Lk - 1, diag + j0 + QT - 1);
   int s_lo = 0, s_end = last_key >= 0 ? last_key / kStep + 1 : 0;
-  int snap = 0;
+  [[maybe_unused]] int lead = 0, snap = 0;
   if constexpr (SPLIT) {
     const int kc = key_cost<RG>(min(QT, Lq - j0) * G), sc = kStep * kc;
+    lead = kUnitSteps * sc;
     snap = kSnap * sc;
     u1 = cur.u0 + tile_keys(Lq, Lk, QT, cur.tile) * kc;
     s_end = tile_steps(Lq, Lk, QT, cur.tile);
     cut = false;
-    if (cur.x >= cur.u0 + snap) {     // the range's begin lies in its first unit
+    if (cur.x >= cur.u0 + lead + snap) {  // the range's begin lies in its first unit
       if (cur.x > u1 - snap) continue;  // which is the range's before (the condition steps on)
-      s_lo = (cur.x - cur.u0 + sc - 1) / sc;
+      s_lo = (cur.x - cur.u0 - lead + sc - 1) / sc;
     }
     if (cur.x_end < u1) {                     // the range ends within this unit
-      if (cur.x_end < cur.u0 + snap) return;  // which is the next range's
+      if (cur.x_end < cur.u0 + lead + snap) return;  // which is the next range's
       cut = cur.x_end <= u1 - snap;
     }
-    if (cut) s_end = min(s_end, (cur.x_end - cur.u0 + sc - 1) / sc);
+    if (cut) s_end = min(s_end, (cur.x_end - cur.u0 - lead + sc - 1) / sc);
     // (within the tile also where lengths beyond the call's maxima have overflown the stream)
     s_end = uni(s_end);
     s_lo = max(min(uni(s_lo), s_end), 0);
@@ -583,7 +588,7 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
   }
   if constexpr (SPLIT) {
     if (part && s_lo == 0 && tid == 0) {  // the unit's first part: describe it to the merge
-      const int w0 = (cur.u0 + snap + cur.C - 1) / cur.C;  // the unit's first cut
+      const int w0 = (cur.u0 + lead + snap + cur.C - 1) / cur.C;  // the unit's first cut
       a.desc[blockIdx.x] =
           i32x4_t{(u1 - snap) / cur.C - w0 + 2, q0 + j0, min(QT, Lq - j0), kvh};
     }
@@ -716,7 +721,7 @@ static ScaledPrefillPlan scaled_prefill_plan(int64_t n_seqs, int64_t total_q, in
   if (p.split)
     p.split = resident(p.groups) >= Hk &&
               split_fits(n_seqs, std::min(n_seqs * ((max_q + qt - 1) / qt), total_q / qt + n_seqs),
-                         max_k * kStep);
+                         (max_k + kUnitSteps * kStep) * kStep);
   p.tiles = plain_tiles(n_seqs, max_q, qt);
   p.grid = p.split ? resident(p.groups) / Hk * Hk : n_seqs * p.tiles * Hk;
   p.sort = !p.split && n_seqs > 1 && n_seqs <= 64 && p.grid > resident(p.groups);
