@@ -146,6 +146,56 @@ __device__ __forceinline__ bool split_begin(const ScaledPrefillArgs& a, int qt, 
   c.u0 += cost_before<RG>(c.Lq, c.Lk, qt, c.tile, a.G);
   return true;
 }
+// A whole launch's tile. Either every sequence has n_tiles places (few of them empty), or the tiles stand
+// in line, a sequence's from its last (the longest) on: up to 64 sequences as they come or, if `sort`,
+// the longest first; more at place cu_q[s] / qt + s, which leaves each room for its tiles and is found
+// by trying 64 sequences at a time. A workgroup without a tile keeps its LDS from another for a few
+// us: with as many places for each sequence as the longest needs, a chunk of 512 among 40 single tokens took 79
+// us where this takes 38, and four prompts of 512 among 60 95 and 41 (Hq 32, Hk 8, D 128).
+__device__ __forceinline__ bool whole_begin(const ScaledPrefillArgs& a, int qt, Cursor& c) {
+  const int lane = threadIdx.x & 63;
+  int b = (int)blockIdx.x / a.Hk;
+  if (a.n_tiles > 0) {
+    c.seq = b / a.n_tiles;
+    c.tile = a.n_tiles - 1 - b % a.n_tiles;
+    seq_lengths(a, c.seq, c.q0, c.Lq, c.Lk);
+    return c.tile * qt < c.Lq;
+  }
+  if (a.n_seqs > 64) {
+    int lo = 0, step = 1;  // a sequence that stands at b or before; the last one is within 64 steps
+    while ((int64_t)step * 64 < a.n_seqs) step *= 64;
+    for (;; step /= 64) {
+      const int s = (int)min((int64_t)lo + (int64_t)lane * step, (int64_t)a.n_seqs);
+      const bool before = s < a.n_seqs && max(a.cu_q[s], 0) / qt + s <= b;
+      lo += (__builtin_popcountll(__ballot(before) | 1) - 1) * step;
+      if (step == 1) break;
+    }
+    c.seq = __builtin_amdgcn_readfirstlane(min(lo, a.n_seqs - 1));
+    seq_lengths(a, c.seq, c.q0, c.Lq, c.Lk);
+    c.tile = (c.Lq + qt - 1) / qt - 1 - (b - (c.q0 / qt + c.seq));
+    return c.Lq > 0 && c.tile >= 0 && c.tile * qt < c.Lq;
+  }
+  int q0 = 0, Lq = 0, Lk = 0, before = 0;
+  if (lane < a.n_seqs) seq_lengths(a, lane, q0, Lq, Lk);
+  const int n = Lq > 0 ? (Lq + qt - 1) / qt : 0;
+  if (a.sort) {
+    for (int i = 0; i < a.n_seqs; ++i) {
+      const int other = __builtin_amdgcn_readlane(Lk, i), tiles = __builtin_amdgcn_readlane(n, i);
+      before += other > Lk || (other == Lk && i < lane) ? tiles : 0;
+    }
+  } else {
+    before = wave_incl_scan(n) - n;
+  }
+  const uint64_t at = __ballot((uint32_t)(b - before) < (uint32_t)n);
+  if (at == 0) return false;
+  const int ln = __builtin_ctzll(at);
+  c.seq = ln;
+  c.q0 = __builtin_amdgcn_readlane(q0, ln);
+  c.Lq = __builtin_amdgcn_readlane(Lq, ln);
+  c.Lk = __builtin_amdgcn_readlane(Lk, ln);
+  c.tile = __builtin_amdgcn_readlane(n - 1 + before, ln) - b;
+  return true;
+}
 // The unit after the current one, which ends at u1 (false at the end of the stream).
 __device__ __forceinline__ bool split_next(const ScaledPrefillArgs& a, int qt, int u1, Cursor& c) {
   c.u0 = u1;
@@ -239,21 +289,7 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
     if (tid == 0) a.desc[blockIdx.x] = i32x4_t{0, 0, 0, 0};  // no unit cut at this range's end
     if (!split_begin<RG>(a, QT, cur)) return;                // uniform
   } else {
-    const int rest = blockIdx.x / Hk;
-    cur.tile = a.n_tiles - 1 - rest % a.n_tiles;  // largest first
-    cur.seq = rest / a.n_tiles;
-    if (a.sort) {  // the longest sequences first (as many as a wave has lanes)
-      const int n = a.n_seqs;
-      const int len = lane < n ? a.cu_k[lane + 1] - a.cu_k[lane] : -1;
-      int rank = 0;
-      for (int i = 0; i < n; ++i) {
-        const int other = __builtin_amdgcn_readlane(len, i);
-        rank += other > len || (other == len && i < lane);
-      }
-      cur.seq = __builtin_ctzll(__ballot(lane < n && rank == cur.seq));
-    }
-    seq_lengths(a, cur.seq, cur.q0, cur.Lq, cur.Lk);
-    if (cur.tile * QT >= cur.Lq) return;  // uniform
+    if (!whole_begin(a, QT, cur)) return;  // uniform
   }
   int u1 = 0;        // the unit's end in the stream
   bool cut = false;  // the range ends inside the unit
@@ -652,25 +688,30 @@ __global__ __launch_bounds__(256) void scaled_merge_kernel(const ScaledPrefillAr
 struct ScaledPrefillPlan {
   int groups;      // row groups a wave
   bool split;
-  bool sort;       // plain: sequences by length
+  int64_t tiles;   // whole: places of a sequence (0: the tiles stand in line)
+  bool sort;       // whole: sequences by length
   int64_t grid;    // workgroups
-  int64_t tiles;   // plain: tiles a sequence
   size_t bytes(int D) const {  // of the workspace
     return split ? grid * (sizeof(i32x4_t) + 2 * 64 * groups * part_floats(D) * sizeof(float)) : 0;
   }
 };
 // How a call is launched, from its sizes alone.
 //
-// Split or whole. Whole, the longest tile sets the time, about 0.65 us a step of its own; split, the
-// steps are spread evenly, for about 8 us of ranges, partial rows and their merge (12 steps) and as much
-// again in proportion (a quarter). In graphs, whole / split, us (Hq 32, Hk 8, D 128 but where noted):
-//   1 draft of 8 behind 500 - 1000 / 2000 - 4000 / 8000 - 16000   16.7 / 15.8, 46.8 / 16.3, 169 / 25.8
-//   8 drafts behind up to 1000 / 2000 / 4000                     21.2 / 17.9, 35.7 / 23.7, 63 / 32.5
-//   32 behind up to 2000, 64 and 128 up to 4000                  37.2 / 40.0, 97 / 99, 181 / 182
-//   1 chunk of 512 behind up to 4000 / 16000                     56.5 / 53.3, 181 / 127
-//   4 chunks of 128 / of 256 behind up to 4000                   90 / 62, 97 / 103
-//   a prompt of 512 / 2048 / 4096                                13.7 / 13.7, 55 / 80, 143 / 194
-//   2 chunks of 400 behind up to 1000, 30 tokens (16, 4, 64)     29.2 / 27.7
+// Split or whole. Whole, the longest tile sets the time, about 0.65 us a step of its own, and the chip is
+// left idle in part; split, the steps are spread evenly, for about 8 us of ranges, partial rows and
+// their merge (12 steps). Tiles that the chip holds at once: split where that idle part (of which a quarter
+// is not had, as other tiles are shorter) is longer. A few more than it holds make a second turn: where their
+// prefixes make them as long as the first, split too; without prefixes, and with more tiles, the order by
+// length fills the gaps. In graphs, whole / split, us (Hq 32, Hk 8, D 128 but where noted):
+//   1 draft of 8 behind 500 - 1000 / 2000 - 4000 / 8000 - 16000   16.7 / 16.7, 47.2 / 15.8, 170 / 25.9
+//   8 drafts behind up to 1000 / 2000 / 4000                     21.2 / 16.8, 35.9 / 20.0, 63.8 / 27.3
+//   32 behind up to 2000, 64 and 128 up to 4000                  37.3 / 35.0, 98 / 95, 183 / 175
+//   1 chunk of 512 behind up to 4000 / 16000, of 1500 up to 6000  56.3 / 52.7, 179 / 124, 191 / 155
+//   4 chunks of 128 / 256 / 300 behind up to 4000                89.8 / 60.2, 98.1 / 93.6, 97.6 / 79.8
+//   8 chunks of 128 behind up to 2000 / 6000                     55.6 / 60.9, 126 / 115
+//   a prompt of 1024 / 2048 / 4096                               23.0 / 34.8, 54.8 / 64.6, 141 / 169
+//   2 chunks of 400 behind up to 1000 / 8000, 30 tokens (16, 4, 64)  28.8 / 26.5, 125 / 58.7
+//   a chunk of 512 behind up to 8000, 30 tokens                  157 / 114
 //
 // Row groups a wave. More of them read, widen and wait for the keys less often; fewer fill the chip
 // sooner. Whole, 1 / 2 / 3 groups, us (Hk 8; workgroups of one group):
@@ -681,8 +722,8 @@ struct ScaledPrefillPlan {
 // At head_dim 64 (four workgroups of one group to a CU, three of two, two of three) 1 / 2 / 3 / 4:
 //   1024 (512)      17.1 / 21.6 / 27.1 / 32.1     4096 (2048)   97 / 92 / 99 / 111
 //   2048 (1024)     35.9 / 39.2 / 48.6 / 56.8     8192 (4096)   357 / 297 / 304 / 300
-// Split, two groups cost less where the tiles are many: 4 chunks of 128 70.6 / 62.3, 1 of 512 behind
-// 16000 155 / 127, but 2 of 64 29.1 / 33.4 and 4 drafts 53.5 / 59.7.
+// Split, two groups cost less where the tiles are many: 4 chunks of 128 66.3 / 59.5, 1 of 512 behind
+// 16000 154 / 122, but 2 of 64 30.5 / 33.6 and 4 drafts 48.3 / 50.9.
 //
 // Order. Workgroups are handed out in turn, the last of them ends alone: longest sequences first, tiles
 // from the last, 342 us for the chunks above and 430 as they come. (Tiles of all sequences in turn: 620,
@@ -698,9 +739,6 @@ static ScaledPrefillPlan scaled_prefill_plan(int64_t n_seqs, int64_t total_q, in
     const int64_t qt = queries(groups);
     return std::min(m.prompts * ((max_q + qt - 1) / qt), m.prompt_rows / qt + m.prompts) + m.rows;
   };
-  const auto launched = [&](int groups) -> int64_t {  // of a plain launch
-    return n_seqs * plain_tiles(n_seqs, max_q, queries(groups)) * Hk;
-  };
   // workgroups that are resident at once: by the ring's LDS (69 KiB, 36 at head_dim 64), or registers
   const auto resident = [&](int groups) { return cus * (D == 128 ? 2 : groups == 1 ? 4 : 3); };
   const int least = g > 64 ? 2 : 1;
@@ -708,23 +746,26 @@ static ScaledPrefillPlan scaled_prefill_plan(int64_t n_seqs, int64_t total_q, in
   p.groups = least;
   const int64_t size = std::min<int64_t>(tiles(least) * Hk, INT32_MAX);
   const int64_t steps = (max_k + kStep - 1) / kStep;
-  p.split = (steps - 12) * resident(least) > 5 * size * steps / 4;
+  const int64_t prefix = max_k > max_q ? (max_k - max_q) / kStep : 0, chip = resident(least);
+  p.split = size <= chip ? 4 * (steps - 12) * chip > 3 * size * steps
+                         : 2 * size <= 3 * chip && (2 * chip - size) * prefix > 24 * chip;
   if (p.split) {
     if (size >= cus / 2 && max_q * g > 64) p.groups = 2;
   } else {
-    if (2 * size > 3 * resident(1) || launched(least) > 24576) p.groups = 2;
+    if (2 * size > 3 * resident(1)) p.groups = 2;
     if (D == 128 && p.groups == 2 && 7 * queries(2) <= 5 * queries(3) &&
-        (2 * tiles(2) * Hk > 5 * resident(2) || launched(2) > 49152))
+        2 * tiles(2) * Hk > 5 * resident(2))
       p.groups = 3;
   }
   const int64_t qt = queries(p.groups);
+  const int64_t most = std::min(n_seqs * ((max_q + qt - 1) / qt), total_q / qt + n_seqs);
   if (p.split)
     p.split = resident(p.groups) >= Hk &&
-              split_fits(n_seqs, std::min(n_seqs * ((max_q + qt - 1) / qt), total_q / qt + n_seqs),
-                         (max_k + kUnitSteps * kStep) * kStep);
-  p.tiles = plain_tiles(n_seqs, max_q, qt);
-  p.grid = p.split ? resident(p.groups) / Hk * Hk : n_seqs * p.tiles * Hk;
-  p.sort = !p.split && n_seqs > 1 && n_seqs <= 64 && p.grid > resident(p.groups);
+              split_fits(n_seqs, most, (max_k + kUnitSteps * kStep) * kStep);
+  const int64_t each = plain_tiles(n_seqs, max_q, qt), line = n_seqs > 64 ? total_q / qt + n_seqs : most;
+  p.sort = !p.split && n_seqs > 1 && n_seqs <= 64 && most * Hk > resident(p.groups);
+  p.tiles = !p.split && !p.sort && n_seqs * each <= line ? each : 0;
+  p.grid = (p.split ? resident(p.groups) / Hk : p.tiles > 0 ? n_seqs * each : line) * Hk;
   return p;
 }
 
@@ -780,7 +821,7 @@ extern "C" int nkv_scaled_prefill(const nkv_scaled_prefill_args* args) {
   NKV_REQUIRE(!p.split || (aligned16(g.workspace) && g.workspace_bytes >= (int64_t)need),
               NKV_EWORKSPACE, "scaled_prefill: workspace needs %zu bytes, 16-byte aligned (got %lld)",
               need, (long long)g.workspace_bytes);
-  NKV_REQUIRE(p.tiles < (1ll << 31) && p.grid < (1ll << 31), NKV_EUNSUPPORTED,
+  NKV_REQUIRE(p.grid < (1ll << 31), NKV_EUNSUPPORTED,
               "scaled_prefill: too many tiles in one call");
   i32x4_t* desc = static_cast<i32x4_t*>(g.workspace);
   const ScaledPrefillArgs a{(const bf16_t*)g.q, g.q_row_stride, (const char*)g.k_cache,

@@ -9,6 +9,7 @@ weights as they are off, move an output by at most r (sum_k p_k |v_k| + |o|) (1 
 u |o|. fp32 sums over the keys and exp2 add less than 2^-16 of sum_k p_k |v_k|.
 """
 import importlib
+import random
 
 import pytest
 import torch
@@ -231,6 +232,17 @@ def test_prefill_row_groups(dev):
 ])
 def test_prefill_more_tiles_than_the_chip_holds(dev, new, lens, Hq, Hk, D):
     check_prefill(dev, make(dev, lens, Hk, D, 64, seed=D + len(new), garbage=False), new, Hq)
+
+
+@pytest.mark.parametrize("n,D", [(65, 128), (70, 64), (200, 64), (4200, 64)])
+def test_prefill_many_sequences_of_few_and_of_many_tiles(dev, n, D):
+    """More sequences than a wave has lanes, some with more tiles than one, some without a query."""
+    rng = random.Random(n)
+    new = [rng.choice([0, 1, 1, 1, 2, 9, rng.randint(1, 30)]) if i % (n // 65) == 0 else rng.choice([0, 0, 1])
+           for i in range(n)]
+    new[-1], new[0] = 25, 17
+    lens = [a + rng.choice([0, 1, 5, 40]) for a in new]
+    check_prefill(dev, make(dev, lens, 1, D, 32, seed=n, garbage=False), new, 8)
 
 
 @pytest.mark.parametrize("new,lens,Hq,Hk,D", [

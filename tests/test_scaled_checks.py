@@ -192,8 +192,7 @@ def test_prefill_maxima_of_any_size():
         assert f(n, tq, 1 << 62, 10 ** 6, 32, 8, 128) == f(n, tq, tq, 10 ** 6, 32, 8, 128) > 0
     assert f(1, 8, 8, 1 << 62, 32, 8, 128) == f(1, 8, 8, (1 << 31) - 1, 32, 8, 128)
     assert f(1, 8, 8, -(1 << 62), 32, 8, 128) == 0 == f((1 << 20) + 1, 8, 8, 9000, 32, 8, 128)
-    for kw in (dict(n=1 << 20, tq=1 << 30, mq=1 << 62), dict(n=1 << 20, tq=1 << 30, mq=1 << 30, hk=512,
-                                                              hq=512, qrs=1 << 15, ors=1 << 15),
+    for kw in (dict(n=1 << 20, tq=1 << 30, mq=1 << 62, hk=512, hq=512, qrs=1 << 15, ors=1 << 15),
                dict(n=(1 << 20) + 1), dict(n=1 << 62)):
         test_entry_points_refuse("nkv_scaled_prefill", PREFILL, kw, -4, b"too many")
 
