@@ -699,7 +699,7 @@ struct ScaledPrefillPlan {
 //
 // Split or whole. Whole, the longest tile sets the time, about 0.65 us a step of its own, and the chip is
 // left idle in part; split, the steps are spread evenly, for about 8 us of ranges, partial rows and
-// their merge (12 steps). Tiles that the chip holds at once: split where that idle part (of which a quarter
+// their merge (12 steps; 18 with two row groups). Tiles that the chip holds at once: split where that idle part (of which a quarter
 // is not had, as other tiles are shorter) is longer. A few more than it holds make a second turn: where their
 // prefixes make them as long as the first, split too; without prefixes, and with more tiles, the order by
 // length fills the gaps. In graphs, whole / split, us (Hq 32, Hk 8, D 128 but where noted):
@@ -707,11 +707,11 @@ struct ScaledPrefillPlan {
 //   8 drafts behind up to 1000 / 2000 / 4000                     21.2 / 16.8, 35.9 / 20.0, 63.8 / 27.3
 //   32 behind up to 2000, 64 and 128 up to 4000                  37.3 / 35.0, 98 / 95, 183 / 175
 //   1 chunk of 512 behind up to 4000 / 16000, of 1500 up to 6000  56.3 / 52.7, 179 / 124, 191 / 155
-//   4 chunks of 128 / 256 / 300 behind up to 4000                89.8 / 60.2, 98.1 / 93.6, 97.6 / 79.8
+//   4 chunks of 128 / 256 / 300 behind up to 4000                89.8 / 60.2, 98.1 / 93.6, 94.7 / 80.3
 //   8 chunks of 128 behind up to 2000 / 6000                     55.6 / 60.9, 126 / 115
 //   a prompt of 1024 / 2048 / 4096                               23.0 / 34.8, 54.8 / 64.6, 141 / 169
-//   2 chunks of 400 behind up to 1000 / 8000, 30 tokens (16, 4, 64)  28.8 / 26.5, 125 / 58.7
-//   a chunk of 512 behind up to 8000, 30 tokens                  157 / 114
+//   2 chunks of 400 behind up to 1000 / 8000, 30 tokens (16, 4, 64)  22.8 / 26.7, 104 / 58.7
+//   a chunk of 512 behind up to 1000 and 40 tokens, 8000 and 30  37.6 / 46.2, 142 / 117
 //
 // Row groups a wave. More of them read, widen and wait for the keys less often; fewer fill the chip
 // sooner. Whole, 1 / 2 / 3 groups, us (Hk 8; workgroups of one group):
@@ -747,10 +747,11 @@ static ScaledPrefillPlan scaled_prefill_plan(int64_t n_seqs, int64_t total_q, in
   const int64_t size = std::min<int64_t>(tiles(least) * Hk, INT32_MAX);
   const int64_t steps = (max_k + kStep - 1) / kStep;
   const int64_t prefix = max_k > max_q ? (max_k - max_q) / kStep : 0, chip = resident(least);
-  p.split = size <= chip ? 4 * (steps - 12) * chip > 3 * size * steps
+  const bool many = size >= cus / 2 && max_q * g > 64;
+  p.split = size <= chip ? 4 * (steps - (many ? 18 : 12)) * chip > 3 * size * steps
                          : 2 * size <= 3 * chip && (2 * chip - size) * prefix > 24 * chip;
   if (p.split) {
-    if (size >= cus / 2 && max_q * g > 64) p.groups = 2;
+    if (many) p.groups = 2;
   } else {
     if (2 * size > 3 * resident(1)) p.groups = 2;
     if (D == 128 && p.groups == 2 && 7 * queries(2) <= 5 * queries(3) &&
