@@ -97,8 +97,8 @@ __device__ __forceinline__ uint32_t put_codes(float a, float b, uint32_t old) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, (int)old, HIGH);
 }
 
-// The codes of the lane's block into the head's tile (or its copy in LDS). SPECIAL: there may be values past +-448 or
-// NaN among them. all: every row of the lane's eight is written.
+// The codes of the lane's block into the head's tile (or its copy in LDS). SPECIAL: there may be
+// values past +-448 or NaN among them. all: every row of the lane's eight is written.
 template <int D, bool SPECIAL>
 __device__ __forceinline__ void write_codes(const Unit<D>& un, const u32x4_t (&row)[8],
                                             const int (&src)[8], bool all, float inv, char* tile) {

@@ -14,9 +14,9 @@
 // v_cvt_scalef32_pk_bf16_fp8 widens two codes and applies the tile's scale, exactly, on the way. The
 // running maximum is only raised when a score exceeds it by more than kLazy (log2), so that most
 // tiles need no exchange between lanes.
-// 64 sequences, 638 MB of codes (Hq 32, Hk 8, D 128): 105 us and 4.7 for the combine, 5.8 TB/s; one of 246
-// MB 41 and 4.6. Loads that the caches keep: 123 us; a ring twice as deep, or K's place refilled before V's
-// products: the same.
+// 64 sequences, 638 MB of codes (Hq 32, Hk 8, D 128): 105 us and 4.7 for the combine, 5.8 TB/s; one of
+// 246 MB 41 and 4.6. Loads that the caches keep: 123 us; a ring twice as deep, or K's place refilled
+// before V's products: the same.
 #include "decode_stream.h"
 #include "scaled_cache.h"
 

@@ -24,10 +24,11 @@
 // 7.1 for one prompt of 77, which q's taking apart costs; not taken.
 //
 // SPLIT: where few tiles would leave the chip idle, the workgroups that fit it at once take equal ranges
-// of all the key steps, and a second launch merges the rows whose keys were cut. Units of few rows (single
-// tokens, drafts) give a wave's rows to two waves, one for each cache tile of a step, joined in LDS at
-// the unit's end: 2 chunks of 400 with 30 tokens behind up to 8000 keys (Hq 16, Hk 4, D 128) 91 us against
-// 109, 4 drafts behind 9000 - 30000 (Hq 32, Hk 8) 50 against 53 (48 now), of which the codes alone take 25.
+// of all the key steps, and a second launch merges the rows whose keys were cut. Units of few rows
+// (single tokens, drafts) give a wave's rows to two waves, one for each cache tile of a step, joined in
+// LDS at the unit's end: 2 chunks of 400 with 30 tokens behind up to 8000 keys (Hq 16, Hk 4, D 128) 91
+// us against 109, 4 drafts behind 9000 - 30000 (Hq 32, Hk 8) 50 against 53 (46 now), of which the codes
+// alone take 25.
 #include "launch_rules.h"
 #include "lds_tiles.h"
 #include "scaled_cache.h"
@@ -80,9 +81,9 @@ struct Cursor {
   int C, T, x, x_end;         // range length, stream length, the range's begin and end
 };
 constexpr int kSnap = 2;        // steps
-// What a unit's start and end cost, counted before its first step. 0 / 2 / 3 / 4 / 6, us: drafts 50.5 / 48.3 /
-// 47.9 / 47.5 / 47.7, 30 tokens and two chunks 36.8 / 34.8 / 34.5 / 34.4 / 36.0, 8 drafts behind up to 4000
-// 29.3 / 27.0 / 27.0 / 26.3 / 26.1, 4 chunks of 128 63.6 / 59.4 / 60.1 / 59.8 / 62.1.
+// What a unit's start and end cost, counted before its first step. 0 / 2 / 3 / 4 / 6, us: drafts 50.5 /
+// 48.3 / 47.9 / 47.5 / 47.7, 30 tokens and two chunks 36.8 / 34.8 / 34.5 / 34.4 / 36.0, 8 drafts behind
+// up to 4000 29.3 / 27.0 / 27.0 / 26.3 / 26.1, 4 chunks of 128 63.6 / 59.4 / 60.1 / 59.8 / 62.1.
 constexpr int kUnitSteps = 3;
 constexpr int kLeastSteps = 4;  // shortest range
 template <int RG>
@@ -149,9 +150,9 @@ __device__ __forceinline__ bool split_begin(const ScaledPrefillArgs& a, int qt, 
 // A whole launch's tile. Either every sequence has n_tiles places (few of them empty), or the tiles stand
 // in line, a sequence's from its last (the longest) on: up to 64 sequences as they come or, if `sort`,
 // the longest first; more at place cu_q[s] / qt + s, which leaves each room for its tiles and is found
-// by trying 64 sequences at a time. A workgroup without a tile keeps its LDS from another for a few
-// us: with as many places for each sequence as the longest needs, a chunk of 512 among 40 single tokens took 79
-// us where this takes 38, and four prompts of 512 among 60 95 and 41 (Hq 32, Hk 8, D 128).
+// by trying 64 sequences at a time. A workgroup without a tile keeps its LDS from another for a few us:
+// with as many places for each sequence as the longest needs, a chunk of 512 among 40 single tokens
+// took 79 us where this takes 38, and four prompts of 512 among 60 95 and 41 (Hq 32, Hk 8, D 128).
 __device__ __forceinline__ bool whole_begin(const ScaledPrefillArgs& a, int qt, Cursor& c) {
   const int lane = threadIdx.x & 63;
   int b = (int)blockIdx.x / a.Hk;
@@ -634,8 +635,8 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
 
 // // Merges the parts of the units that ranges cut: descriptor x (of the workgroup that holds a unit's
 // first part; part p > 0 is in the first slot of the workgroup p * Hk after it), four rows of its tile a
-// wave, 16 lanes each. Lane c of a row owns dims 4 c + 64 i .. + 3, eight parts in flight. (A row a wave: 11
-// us where this takes 6, for the four times as many workgroups to hand out.)
+// wave, 16 lanes each. Lane c of a row owns dims 4 c + 64 i .. + 3, eight parts in flight. (A row a
+// wave: 11 us where this takes 6, for the four times as many workgroups to hand out.)
 template <int D>
 __global__ __launch_bounds__(256) void scaled_merge_kernel(const ScaledPrefillArgs a,
                                                            int32_t tile_rows) {
@@ -699,10 +700,10 @@ struct ScaledPrefillPlan {
 //
 // Split or whole. Whole, the longest tile sets the time, about 0.65 us a step of its own, and the chip is
 // left idle in part; split, the steps are spread evenly, for about 8 us of ranges, partial rows and
-// their merge (12 steps; 18 with two row groups). Tiles that the chip holds at once: split where that idle part (of which a quarter
-// is not had, as other tiles are shorter) is longer. A few more than it holds make a second turn: where their
-// prefixes make them as long as the first, split too; without prefixes, and with more tiles, the order by
-// length fills the gaps. In graphs, whole / split, us (Hq 32, Hk 8, D 128 but where noted):
+// their merge (12 steps; 18 with two row groups). Tiles that the chip holds at once: split where the idle
+// part is longer (tiles taken for three quarters of the longest). A few more than it holds make a
+// second turn: where their prefixes make them as long as the first, split too; without prefixes, and
+// with more tiles, the order by length fills the gaps. In graphs, whole / split, us (Hq 32, Hk 8, D 128 but where noted):
 //   1 draft of 8 behind 500 - 1000 / 2000 - 4000 / 8000 - 16000   16.7 / 16.7, 47.2 / 15.8, 170 / 25.9
 //   8 drafts behind up to 1000 / 2000 / 4000                     21.2 / 16.8, 35.9 / 20.0, 63.8 / 27.3
 //   32 behind up to 2000, 64 and 128 up to 4000                  37.3 / 35.0, 98 / 95, 183 / 175
@@ -829,8 +830,8 @@ extern "C" int nkv_scaled_prefill(const nkv_scaled_prefill_args* args) {
                             (const char*)g.v_cache, g.cu_seqlens_q, g.cu_seqlens_k, g.block_tables,
                             g.bt_row_stride, Hk, group, (int32_t)g.block_size,
                             (int32_t)g.max_blocks_per_seq, (int32_t)g.n_blocks, (int32_t)g.n_seqs,
-                            (int32_t)p.tiles, (int32_t)p.sort, g.total_q, (float)g.scale * kLog2e, (bf16_t*)g.out,
-                            g.out_row_stride, desc,
+                            (int32_t)p.tiles, (int32_t)p.sort, g.total_q,
+                            (float)g.scale * kLog2e, (bf16_t*)g.out, g.out_row_stride, desc,
                             p.split ? reinterpret_cast<float*>(desc + p.grid) : nullptr};
   const dim3 grid((unsigned)p.grid);
 #define NKV_SCALED_PREFILL_S(D, RG, SPLIT)                                                       \
