@@ -210,34 +210,33 @@ __device__ __forceinline__ bool split_next(const ScaledPrefillArgs& a, int qt, i
   return true;
 }
 
-// N KiB (16 bytes a lane each) or 256 bytes (4 a lane) from desc + voff to consecutive LDS bytes (an
-// instruction's offset moves both addresses). Written as asm so that the compiler adds no wait for it
-// before a barrier; the ring's own s_waitcnt does.
+// N KiB (16 bytes a lane each) from desc + code_off to consecutive LDS bytes at codes_at (an
+// instruction's offset moves both addresses) and 256 bytes (4 a lane) from desc + scale_off to scales_at.
+// Written as asm so that the compiler adds no wait for it before a barrier; the ring's own s_waitcnt does.
 template <int N>
-__device__ __forceinline__ void fetch16(i32x4_t desc, uint32_t lds_addr, uint32_t voff) {
+__device__ __forceinline__ void fetch_tile(i32x4_t desc, uint32_t codes_at, uint32_t code_off,
+                                           uint32_t scales_at, uint32_t scale_off) {
   static_assert(N == 2 || N == 4, "a tile of codes");
   if constexpr (N == 2)
-    asm volatile("s_mov_b32 m0, %0\n\t"
+    asm volatile(NKV_LDS_AT
                  "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
-                 "buffer_load_dwordx4 %1, %2, 0 offen offset:0x400 lds"
+                 "buffer_load_dwordx4 %1, %2, 0 offen offset:0x400 lds\n\t"
+                 "s_mov_b32 m0, %3\n\ts_nop 0\n\t"
+                 "buffer_load_dword %4, %2, 0 offen lds"
                  :
-                 : "s"(lds_addr), "v"(voff), "s"(desc)
-                 : "memory");
+                 : "s"(codes_at), "v"(code_off), "s"(desc), "s"(scales_at), "v"(scale_off)
+                 : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\t"
+    asm volatile(NKV_LDS_AT
                  "buffer_load_dwordx4 %1, %2, 0 offen lds\n\t"
                  "buffer_load_dwordx4 %1, %2, 0 offen offset:0x400 lds\n\t"
                  "buffer_load_dwordx4 %1, %2, 0 offen offset:0x800 lds\n\t"
-                 "buffer_load_dwordx4 %1, %2, 0 offen offset:0xc00 lds"
+                 "buffer_load_dwordx4 %1, %2, 0 offen offset:0xc00 lds\n\t"
+                 "s_mov_b32 m0, %3\n\ts_nop 0\n\t"
+                 "buffer_load_dword %4, %2, 0 offen lds"
                  :
-                 : "s"(lds_addr), "v"(voff), "s"(desc)
-                 : "memory");
-}
-__device__ __forceinline__ void fetch4(i32x4_t desc, uint32_t lds_addr, uint32_t voff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-               :
-               : "s"(lds_addr), "v"(voff), "s"(desc)
-               : "memory");
+                 : "s"(codes_at), "v"(code_off), "s"(desc), "s"(scales_at), "v"(scale_off)
+                 : "memory", "m0");
 }
 
 // Zeroes for NaN, and ones where there was one.
@@ -369,8 +368,8 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
     const int64_t at = ((int64_t)(ok ? pb : 0) * tiles_per_block + c_in) * tile_bytes;
     const i32x4_t desc = buffer_desc(cache + at, ok ? (uint32_t)tile_bytes : 0u);
     const uint32_t to = ring_at + (uint32_t)c_stage * kStageB;
-    fetch16<kLoads>(desc, to, code_off);
-    fetch4(desc, to - (uint32_t)wave * kTileB + kCodesB + wave * 256, scale_off & ~3u);
+    fetch_tile<kLoads>(desc, to, code_off, to - (uint32_t)wave * kTileB + kCodesB + wave * 256,
+                       scale_off & ~3u);
     c_stage = c_stage + 1 == kStages ? 0 : c_stage + 1;
     c_left -= kStep;
     c_in += 2;  // at most two blocks on
