@@ -145,6 +145,14 @@ constexpr bool split_fits(int64_t n_seqs, int64_t tiles, int64_t keys) {
   return tiles * steps * kFullStep <= most && n_seqs * ((keys + 15) / 16) <= most;
 }
 
+// The same where the positions count a tile's keys by cost (scaled_prefill.hip), `keys` at most of each
+// of the `tiles` in all, what a tile's start and end count among them. The lengths are not clamped: a
+// tile of 111 million keys is as long as a stream may be.
+constexpr bool key_split_fits(int64_t tiles, int64_t keys) {
+  constexpr int64_t most = 1000000000;
+  return tiles <= 0 || keys <= most / kFullStep / tiles;
+}
+
 // Whether four waves merge the partials of a decode row instead of one: where a row may have more
 // than 24, its sequence's share of the `waves` waves of each KV head and column group, or as many
 // as a full table row makes (ranges of min_chunks of its max_chunks). One wave has 16 partials in

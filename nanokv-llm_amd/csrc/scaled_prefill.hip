@@ -761,8 +761,9 @@ static ScaledPrefillPlan scaled_prefill_plan(int64_t n_seqs, int64_t total_q, in
   const int64_t qt = queries(p.groups);
   const int64_t most = std::min(n_seqs * ((max_q + qt - 1) / qt), total_q / qt + n_seqs);
   if (p.split)
+    // (a tile's keys are its queries' at least, in a sequence of fewer keys too)
     p.split = resident(p.groups) >= Hk &&
-              split_fits(n_seqs, most, (max_k + kUnitSteps * kStep) * kStep);
+              key_split_fits(most, std::max(max_k, max_q) + kUnitSteps * kStep);
   const int64_t each = plain_tiles(n_seqs, max_q, qt), line = n_seqs > 64 ? total_q / qt + n_seqs : most;
   p.sort = !p.split && n_seqs > 1 && n_seqs <= 64 && most * Hk > resident(p.groups);
   p.tiles = !p.split && !p.sort && n_seqs * each <= line ? each : 0;
