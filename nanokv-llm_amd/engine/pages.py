@@ -84,7 +84,7 @@ class PagedSequences:
         self._captured = False
         at = state.data_ptr()
         self._args = _PAGES.pack(kv.data_ptr(), 2 * layers, pages, block,
-                                 kv.stride(3) * kv.element_size(), at, at + 4 * pages,
+                                 kv.shape[4:].numel() * kv.element_size(), at, at + 4 * pages,
                                  at + 4 * (pages + max_seqs), max_blocks_per_seq,
                                  max_blocks_per_seq, max_seqs, self._workspace.data_ptr(), nbytes)
 

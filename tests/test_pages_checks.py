@@ -268,3 +268,25 @@ class OracleAlone:
 
 def test_a_listed_page_that_was_free_keeps_its_new_row():
     free_page_listed(OracleAlone())
+
+
+@pytest.mark.parametrize("shape,swap,row_bytes", [
+    ((2, 2, 5, 16, 3, 64), None, 384), ((2, 2, 1, 5, 3, 64), (2, 3), 384), ((2, 2, 5, 3, 1, 64), (3, 4), 384),
+    ((2, 1, 2, 5, 3, 64), (1, 2), 384)])
+def test_a_row_is_its_heads_whatever_the_strides_of_single_entries(monkeypatch, shape, swap, row_bytes):
+    """A contiguous tensor has any stride in a dimension of size 1 (here block_size, layers)."""
+    monkeypatch.setattr(_lib, "require_device", lambda device, **tensors: None)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0)
+    kv = torch.zeros(shape, dtype=torch.bfloat16)
+    kv = kv if swap is None else kv.transpose(*swap)
+    assert kv.is_contiguous()
+    seqs = pages.PagedSequences(kv, 2, 3)
+    _, planes, n_pages, block, row, *_ = pages._PAGES.unpack(seqs._args)
+    assert (planes, n_pages, block, row) == (2 * kv.size(1), kv.size(2), kv.size(3), row_bytes)
+
+
+def test_a_row_of_a_block_scaled_pool(monkeypatch):
+    monkeypatch.setattr(_lib, "require_device", lambda device, **tensors: None)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0)
+    seqs = pages.PagedSequences(torch.zeros(2, 3, 4, 32, 144, dtype=torch.uint8), 2, 3)
+    assert pages._PAGES.unpack(seqs._args)[1:5] == (6, 4, 32, 144)
