@@ -876,7 +876,7 @@ int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info, 
  * The tokens of a tile must stand next to each other in slot_mapping, in any
  * order, as tokens listed sequence by sequence do, with fewer than 32 skipped ones
  * between any two (of two for one slot the later stays); what a tile holds whose
- * tokens stand in two places is undefined.
+ * tokens stand in two places is undefined. At most 2^27 - 1024 tokens.
  */
 typedef struct nkv_scaled_store_args {
   const void* key;
@@ -946,7 +946,8 @@ int nkv_scaled_decode(const nkv_scaled_decode_args* args);
  * group up to NKV_SCALED_MAX_GROUP. A row that sees no key gives zeros, rows of no
  * sequence stay as they were; keys past the table or in an invalid block are
  * zeros, and keys that a row does not see have no effect on it, whatever they
- * hold. At most 2^20 sequences and 2^30 rows.
+ * hold. At most 2^20 sequences, 2^30 rows, 2^30 keys a sequence, and 2^24 - 1 tiles
+ * of queries and KV heads (64 to 192 rows each, a sequence at least one).
  * No counterpart in the reference (beside nanokvllm/layers/attention.py:96-102).
  */
 #define NKV_SCALED_MAX_GROUP 128

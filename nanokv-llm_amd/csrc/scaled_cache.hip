@@ -402,6 +402,9 @@ extern "C" int nkv_scaled_store(const nkv_scaled_store_args* args) {
   NKV_REQUIRE(g.n_tokens >= 0 && g.n_tokens < (1ll << 31) && g.n_slots >= 0, NKV_EINVAL,
               "scaled_store: bad sizes (%lld tokens, %lld slots)", (long long)g.n_tokens,
               (long long)g.n_slots);
+  // a launch has fewer than 2^32 threads, 256 for each eight tokens
+  NKV_REQUIRE(g.n_tokens <= (1 << 27) - 1024, NKV_EUNSUPPORTED,
+              "scaled_store: at most 2^27 - 1024 tokens (got %lld)", (long long)g.n_tokens);
   if (g.n_tokens == 0) return NKV_OK;
   const int rc = scaled_check("scaled_store", g.k_cache, g.v_cache, g.n_kv_heads, g.head_dim);
   if (rc) return rc;

@@ -823,7 +823,7 @@ extern "C" int nkv_scaled_prefill(const nkv_scaled_prefill_args* args) {
   NKV_REQUIRE(!p.split || (aligned16(g.workspace) && g.workspace_bytes >= (int64_t)need),
               NKV_EWORKSPACE, "scaled_prefill: workspace needs %zu bytes, 16-byte aligned (got %lld)",
               need, (long long)g.workspace_bytes);
-  NKV_REQUIRE(p.grid < (1ll << 31), NKV_EUNSUPPORTED,
+  NKV_REQUIRE(p.grid < (1ll << 24), NKV_EUNSUPPORTED,  // threads of a launch are 32 bits
               "scaled_prefill: too many tiles in one call");
   i32x4_t* desc = static_cast<i32x4_t*>(g.workspace);
   const ScaledPrefillArgs a{(const bf16_t*)g.q, g.q_row_stride, (const char*)g.k_cache,

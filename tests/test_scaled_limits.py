@@ -3,7 +3,7 @@ import struct
 
 import pytest
 
-from test_scaled_checks import L, PREFILL
+from test_scaled_checks import L, P, PREFILL, STORE
 
 
 def _args(base, **kw):
@@ -33,3 +33,18 @@ def test_split_prefill_positions_stay_within_32_bits(n, tq, mq, hq, hk, d):
 def test_split_prefill_takes_long_streams_that_fit():
     f = L.lib().nkv_scaled_prefill_workspace_bytes
     assert f(1, 8, 8, 111_110_000, 4, 1, 64) > 0 == f(1, 8, 8, 111_112_000, 4, 1, 64)
+
+
+@pytest.mark.parametrize("n", [(1 << 27) - 1023, 1 << 27, (1 << 31) - 1])
+def test_store_refuses_more_tokens_than_a_launch_holds(n):
+    """Four waves to a workgroup, a workgroup for eight tokens: threads of a launch are 32 bits."""
+    assert L.lib().nkv_scaled_store(_args(STORE, n=n)) == -4
+    assert b"at most" in L.lib().nkv_last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n=1 << 20, tq=1 << 20, mq=1, hq=16, hk=16, qrs=1024, ors=1024),   # a tile for each row and head
+    dict(n=2, tq=1 << 30, mq=1 << 30, hq=8, hk=8)])
+def test_prefill_refuses_more_tiles_than_a_launch_holds(kw):
+    assert L.lib().nkv_scaled_prefill(_args(PREFILL, **kw)) == -4
+    assert b"too many tiles" in L.lib().nkv_last_error()
