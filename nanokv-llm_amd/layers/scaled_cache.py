@@ -66,9 +66,10 @@ class ScaledKVCachePool:
 
 
 # ---------------------------------------------------------------- checks
-# Each operator passes its arguments by one expression where they are right; only for others does its
-# _refuse_* function look for what is wrong (with messages made and checks by name, they kept the host
-# busy for 8 to 20 us a call, longer than a small call runs).
+# Each operator passes its arguments by one expression where they are right, outputs and workspaces that
+# it is given among them; only for others does its _refuse_* function look for what is wrong (with
+# messages made and checks by name, they kept the host busy for 8 to 20 us a call, longer than a small
+# call runs).
 def _caches(what, k_cache, v_cache, row):
     if not (k_cache.dtype is _U8 and v_cache.dtype is _U8 and k_cache.dim() == 3
             and v_cache.shape == k_cache.shape and k_cache.size(2) == row + ROW_PAD
@@ -191,6 +192,15 @@ def _tables_right(t, shape, di, n):
             and t.get_device() == di and t.stride(1) == 1)
 
 
+def _out_right(t, shape, di):
+    return (t.shape == shape and t.dtype is _BF16 and t.get_device() == di and t.stride(2) == 1
+            and t.stride(1) == shape[2])
+
+
+def _workspace_right(t, di):
+    return t.dtype is _U8 and t.get_device() == di and t.is_contiguous()
+
+
 # ---------------------------------------------------------------- the operators
 def scaled_store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
                          v_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
@@ -237,7 +247,8 @@ def scaled_read_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tabl
             and row % Hk == 0 and n >= 0 and n_tokens >= 0 and _entries_right(cu_seqlens, di)
             and _tables_right(block_tables, bs, di, n)
             and (starts is None or _entries_right(starts, di) and starts.size(0) >= n)
-            and out is None):
+            and (out is None or len(out) == 2 and all(
+                _out_right(t, (n_tokens, Hk, row // Hk), di) and t.is_contiguous() for t in out))):
         _refuse_read(what, k_cache, v_cache, block_tables, cu_seqlens, n_tokens, Hk, starts, out)
     D = row // Hk
     with _lib.device_of(di):
@@ -277,7 +288,8 @@ def scaled_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
             and _caches_right(k_cache, v_cache, cs, di) and cs[2] > ROW_PAD
             and (cs[2] - ROW_PAD) % qs[2] == 0 and _entries_right(context_lens, di)
             and context_lens.size(0) >= qs[0] and _tables_right(block_tables, bs, di, qs[0])
-            and out is None and workspace is None):
+            and (out is None or _out_right(out, qs, di))
+            and (workspace is None or _workspace_right(workspace, di))):
         _refuse_decode(what, q, k_cache, v_cache, context_lens, block_tables, out, workspace)
     n, Hq, D = qs
     lib = _lib.lib()
@@ -337,7 +349,9 @@ def scaled_varlen_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
             and _caches_right(k_cache, v_cache, cs, di) and cs[2] > ROW_PAD
             and (cs[2] - ROW_PAD) % qs[2] == 0 and n >= 0 and _entries_right(cu_seqlens_q, di)
             and _entries_right(cu_seqlens_k, di) and cu_seqlens_k.size(0) == n + 1
-            and _tables_right(block_tables, bs, di, n) and out is None and workspace is None):
+            and _tables_right(block_tables, bs, di, n)
+            and (out is None or _out_right(out, qs, di))
+            and (workspace is None or _workspace_right(workspace, di))):
         _refuse_prefill(what, q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_tables, out,
                         workspace)
     D = qs[2]
