@@ -846,8 +846,10 @@ int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info, 
 
 /*
  * The block-scaled cache: 8-bit codes with a scale for every 32 tokens and head.
- * It needs no calibration, and holds heads and tokens of any magnitude at E4M3's
- * full precision. A cache is uint8 [n_blocks, block_size, n_kv_heads*head_dim +
+ * It needs no calibration: what a tile's 32 tokens hold of a head stands relative to
+ * the largest of it, whatever its magnitude. Values down to 2^-13 of that keep
+ * E4M3's four significant bits, smaller ones fewer, and those below 2^-19 become
+ * zero. A cache is uint8 [n_blocks, block_size, n_kv_heads*head_dim +
  * NKV_SCALED_ROW_PAD], block_size a multiple of 32; its rows stand in tiles of 32,
  * a tile being the heads' codes (32*head_dim bytes each), then n_kv_heads scale
  * bytes, the rest unused. A tile of a head holds code = E4M3(x * 2^-e) and the
@@ -873,6 +875,12 @@ int nkv_pages_compact(const nkv_pages* pages, int32_t max_moves, int32_t* info, 
  * not write lose their values. Else e = max(e_old, need), and where that grows
  * the other rows' codes become E4M3(code * 2^(e_old - e)). Rounding is to nearest
  * even; larger values and infinities become +-448 * 2^e, NaN stays NaN.
+ * So what a tile holds follows from the calls, not from its rows alone: rows are
+ * rounded again at each growth (up to 31 times, by less than one subnormal step,
+ * 2^(e-9), in all), and tokens stored in several calls may hold other codes than
+ * stored in one.
+ * A scale does not shrink: rows that a rollback drops, a rejected draft's, leave the
+ * scale that they raised to the rows that stay, until the tile begins anew.
  * The tokens of a tile must stand next to each other in slot_mapping, in any
  * order, as tokens listed sequence by sequence do, with fewer than 32 skipped ones
  * between any two (of two for one slot the later stays); what a tile holds whose
@@ -916,7 +924,9 @@ int nkv_scaled_read(const nkv_scaled_read_args* args);
  * nkv_paged_decode's; q rows are 16-byte aligned (stride a multiple of 8), out's
  * stride is a multiple of 2. Any GQA group up to 256. A sequence of length 0, or
  * none of whose blocks are valid, gives zeros; what a tile holds behind the
- * sequence's end has no effect.
+ * sequence's end has no effect. Sums of weights (bf16, up to 2^8) times values are
+ * 32-bit floats until they are divided: 2^8 * keys * max |v| stays below 2^128, here
+ * and in nkv_scaled_prefill.
  * No counterpart in the reference (beside nanokvllm/layers/attention.py:104-107).
  */
 typedef struct nkv_scaled_decode_args {

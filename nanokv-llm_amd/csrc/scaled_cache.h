@@ -3,11 +3,13 @@
 //
 // A page's rows stand in tiles of 32 tokens. A tile of a head holds E4M3 codes of x * 2^-e and its e,
 // stored as the byte e + 127. With a power of two both x * 2^-e and code * 2^e are exact (a code has
-// four significant bits: code * 2^e is exact in bf16), so what a cache holds does not depend on how
-// the work was split, and E4M3, being a floating format, loses at most one bit of its 18 binades
-// against a scale that fits exactly.
+// four significant bits: code * 2^e is exact in bf16), so what a call leaves in a cache does not depend on
+// how its work was split, and E4M3, being a floating format, loses at most one bit of its 18 binades
+// against a scale that fits exactly. It does depend on the calls: where a later one raises a tile's scale the
+// rows held are rounded again, in the subnormal range, each time by at most half of its step and by less
+// than one step of the last scale in all.
 //   e: the smallest in [-100, 119] with max |x| <= 448 * 2^e (448: E4M3's largest; the finite x's)
-// Below -100 nothing is left to hold (values under 2^-109 become zero) and every scaled value stays
+// Below -100 nothing is left to hold (values up to 2^-110 become zero) and every scaled value stays
 // a normal number; above 119 a code could reach 2^128. Byte 0: nothing written yet.
 //
 // A tile of a layer's K (or V) is 32 * (Hk * D + 16) bytes: each head's codes (32 * D bytes), then Hk

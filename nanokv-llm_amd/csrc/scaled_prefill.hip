@@ -479,7 +479,8 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
           p[e] = fast_exp2(fmaf(sv[rr][8 * c + e], a.scale_log2, -m_run[rr]));
         pb[rr] = u32x4_t{cvt_pk16<false>(p[0], p[1]), cvt_pk16<false>(p[2], p[3]),
                          cvt_pk16<false>(p[4], p[5]), cvt_pk16<false>(p[6], p[7])};
-        // the sum is that of the rounded weights, which multiply V
+        // weights are rounded to bf16, as the product takes them (2^-9 of each at most); the sum is that
+        // of the rounded ones, which multiply V
 #pragma unroll
         for (int e = 0; e < 4; ++e) l_run[rr] = sum2_16<false>(pb[rr][e], l_run[rr]);
       }
@@ -632,7 +633,7 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
   } while (SPLIT && !cut && split_next(a, QT, u1, cur));
 }
 
-// // Merges the parts of the units that ranges cut: descriptor x (of the workgroup that holds a unit's
+// Merges the parts of the units that ranges cut: descriptor x (of the workgroup that holds a unit's
 // first part; part p > 0 is in the first slot of the workgroup p * Hk after it), four rows of its tile a
 // wave, 16 lanes each. Lane c of a row owns dims 4 c + 64 i .. + 3, eight parts in flight. (A row a
 // wave: 11 us where this takes 6, for the four times as many workgroups to hand out.)
@@ -702,7 +703,8 @@ struct ScaledPrefillPlan {
 // their merge (12 steps; 18 with two row groups). Tiles that the chip holds at once: split where the idle
 // part is longer (tiles taken for three quarters of the longest). A few more than it holds make a
 // second turn: where their prefixes make them as long as the first, split too; without prefixes, and
-// with more tiles, the order by length fills the gaps. In graphs, whole / split, us (Hq 32, Hk 8, D 128 but where noted):
+// with more tiles, the order by length fills the gaps. In graphs, whole / split, us (Hq 32, Hk 8, D 128
+// but where noted):
 //   1 draft of 8 behind 500 - 1000 / 2000 - 4000 / 8000 - 16000   16.7 / 16.7, 47.2 / 15.8, 170 / 25.9
 //   8 drafts behind up to 1000 / 2000 / 4000                     21.2 / 16.8, 35.9 / 20.0, 63.8 / 27.3
 //   32 behind up to 2000, 64 and 128 up to 4000                  37.3 / 35.0, 98 / 95, 183 / 175
@@ -712,6 +714,8 @@ struct ScaledPrefillPlan {
 //   a prompt of 1024 / 2048 / 4096                               23.0 / 34.8, 54.8 / 64.6, 141 / 169
 //   2 chunks of 400 behind up to 1000 / 8000, 30 tokens (16, 4, 64)  22.8 / 26.7, 104 / 58.7
 //   a chunk of 512 behind up to 1000 and 40 tokens, 8000 and 30  37.6 / 46.2, 142 / 117
+//
+// (Two points lie on the slower side: 128 drafts and four chunks of 256 go whole, 183 and 98.1.)
 //
 // Row groups a wave. More of them read, widen and wait for the keys less often; fewer fill the chip
 // sooner. Whole, 1 / 2 / 3 groups, us (Hk 8; workgroups of one group):

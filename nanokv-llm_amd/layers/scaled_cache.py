@@ -2,8 +2,9 @@
 
 The fp8 pool of ``kv_cache`` has one scale per layer, which has to be calibrated. Here a tile of 32 rows
 of one head has a scale of its own, a power of two that follows from what is stored: nothing to
-calibrate, and heads and tokens of any magnitude keep E4M3's full precision, for 16 bytes a token
-(kept beside the codes, so that whoever copies a page copies its scales).
+calibrate, for 16 bytes a token (kept beside the codes, so that whoever copies a page copies its
+scales). Values down to 2^-13 of the largest that the tile's 32 tokens hold of the head keep E4M3's four
+significant bits, whatever its magnitude; smaller ones keep fewer, and those below 2^-19 become zero.
 
     e     the smallest in [-100, 119] with max |x| <= 448 * 2^e over the tile's rows
     code  E4M3(x * 2^-e), read as code * 2^e
@@ -208,7 +209,8 @@ def scaled_store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.
 
     A call that writes a tile's first row begins the tile anew, with the scale of the rows that it
     writes there; otherwise the scale only grows, and the rows held so far are rounded to it where it
-    does. The tokens of one tile must stand next to each other in ``slot_mapping``, as those of a
+    does (also by rows that are dropped later, a rejected draft's, which a rollback does not undo). The
+    tokens of one tile must stand next to each other in ``slot_mapping``, as those of a
     sequence do, fewer than 32 skipped ones between any two.
     """
     what = "scaled_store_kvcache"

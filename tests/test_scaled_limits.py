@@ -1,9 +1,13 @@
-"""Block-scaled caches: sizes at the ends of what the calls take, none of which needs a GPU."""
+"""Block-scaled caches: sizes at the ends of what the calls take and values at the ends of what a tile holds,
+none of which needs a GPU."""
+import math
 import struct
 
 import pytest
+import torch
 
-from test_scaled_checks import L, P, PREFILL, STORE
+from oracle.scaled_ref import PAD, codes_of, exponent, scaled_rows_ref, scaled_store_ref
+from test_scaled_checks import BF, I32, L, P, PREFILL, STORE, U8
 
 
 def _args(base, **kw):
@@ -48,3 +52,41 @@ def test_store_refuses_more_tokens_than_a_launch_holds(n):
 def test_prefill_refuses_more_tiles_than_a_launch_holds(kw):
     assert L.lib().nkv_scaled_prefill(_args(PREFILL, **kw)) == -4
     assert b"too many tiles" in L.lib().nkv_last_error()
+
+
+# ---------------------------------------------------------------- what the header says of precision
+@pytest.mark.parametrize("top", [1.0, 3.5e4, 448.0, 449.0, 1.7e-20, 2.9e38])
+def test_values_far_below_their_tile_s_largest(top):
+    """Down to 2^-13 of it four significant bits are kept (E4M3's normal codes begin at 2^-6 of the scale, the
+    largest value is below 448 of it: 2^-14.9); below 2^-19 nothing is (half of 2^-9, over 224: 2^-17.9)."""
+    top = torch.tensor(top, dtype=BF).item()
+    e = exponent(top)
+    kept = [m * 2.0 ** (math.floor(math.log2(top)) - 3 - k) for m in range(8, 16) for k in range(1, 13)]
+    kept = torch.tensor([v for v in kept if top * 2.0 ** -13 <= v <= top], dtype=torch.float64)
+    assert kept.numel() > 80
+    back = codes_of(kept[:, None], e).view(torch.float8_e4m3fn).double() * 2.0 ** e
+    assert torch.equal(back[:, 0], kept)
+    assert not bool((codes_of(torch.tensor([[top * 2.0 ** -19, -top * 2.0 ** -25]]).double(), e) & 0x7f).any())
+
+
+def test_rows_that_are_rounded_again_at_each_growth():
+    """32 tokens stored one at a time, the scale raised by each: what the first ones hold moves by less than
+    one subnormal step of the last scale. A rollback leaves the scale; the tile's first row takes it back."""
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(32, 1, 64, generator=g).double()
+    x *= 2.0 ** (torch.arange(32).double() * 0.6).view(32, 1, 1)
+    x = x.to(BF)
+    c = torch.zeros(1, 32, 64 + PAD, dtype=U8)
+    held, scales = [], []
+    for i in range(32):
+        scaled_store_ref(x[i:i + 1], x[i:i + 1], c, c.clone(), torch.tensor([i], dtype=I32))
+        held.append(scaled_rows_ref(c, False, [0], i + 1, 1, 64)[i])
+        scales.append(int(c.view(-1)[32 * 64]) - 127)
+    assert len(set(scales)) > 15
+    step = 2.0 ** (scales[-1] - 9)
+    moved = (scaled_rows_ref(c, False, [0], 32, 1, 64) - torch.stack(held)).abs().max().item()
+    assert 0 < moved < step
+    scaled_store_ref(x[3:4], x[3:4], c, c.clone(), torch.tensor([3], dtype=I32))  # rolled back to three
+    assert int(c.view(-1)[32 * 64]) - 127 == scales[-1]
+    scaled_store_ref(x[:1], x[:1], c, c.clone(), torch.tensor([0], dtype=I32))
+    assert int(c.view(-1)[32 * 64]) - 127 == scales[0]
