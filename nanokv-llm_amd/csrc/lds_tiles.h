@@ -33,8 +33,8 @@ __device__ __forceinline__ i32x4_t buffer_desc(const void* base, uint32_t bytes)
 // The start of asm that loads into LDS: m0, which the load takes its LDS address from, and the wait states
 // that the compiler puts before a load of its own but not into asm: one after m0 is written, five after a
 // vector instruction (readfirstlane above, or the reload of a spilled register) wrote a word of the
-// descriptor. Prompts of 1500 and 2900 (Hq 32, Hk 8, D 128) take 35.6 and 79.7 us with the five, 35.1 and
-// 78.7 with the one; four loads under one wait of five take no less than with one each.
+// descriptor. Prompts of 1500 and 2900 (bf16, Hq 32, Hk 8, D 128) take 33.4 and 77.8 us with the five, 33.1
+// and 77.2 with the one alone, 33.2 and 78.6 with four loads in a block behind one wait of five.
 #define NKV_LDS_AT "s_mov_b32 m0, %0\n\ts_nop 4\n\t"
 // 16 bytes per lane from desc+voff into LDS at lds_addr + 16 * lane. Written as
 // asm so that the compiler does not add a wait for it before every barrier;
