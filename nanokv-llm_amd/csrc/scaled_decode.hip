@@ -208,9 +208,9 @@ void scaled_decode_kernel(
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[e] = fast_exp2(sv[e] - mb);
-        // Weights are rounded to bf16, as the product takes them: each is off by 2^-9 at most, outputs by
-        // a tenth more against 64 bits than with weights of 32 bits, since their own bf16 rounding is as
-        // large. The sum is that of the rounded weights, which multiply V.
+        // Weights are rounded to bf16, as the product takes them, each by 2^-8 of it at most. Outputs are
+        // off from 64 bits by 0.0014 - 0.0020 (relative), with weights of 32 bits by 0.0014 - 0.0018: most
+        // of both is their own rounding. The sum is that of the rounded weights, which multiply V.
         const u32x4_t pb = {cvt_pk16<false>(p[0], p[1]), cvt_pk16<false>(p[2], p[3]),
                             cvt_pk16<false>(p[4], p[5]), cvt_pk16<false>(p[6], p[7])};
 #pragma unroll

@@ -479,7 +479,7 @@ __global__ __launch_bounds__(256, 2) void scaled_prefill_kernel(const ScaledPref
           p[e] = fast_exp2(fmaf(sv[rr][8 * c + e], a.scale_log2, -m_run[rr]));
         pb[rr] = u32x4_t{cvt_pk16<false>(p[0], p[1]), cvt_pk16<false>(p[2], p[3]),
                          cvt_pk16<false>(p[4], p[5]), cvt_pk16<false>(p[6], p[7])};
-        // weights are rounded to bf16, as the product takes them (2^-9 of each at most); the sum is that
+        // weights are rounded to bf16, as the product takes them (2^-8 of each at most); the sum is that
         // of the rounded ones, which multiply V
 #pragma unroll
         for (int e = 0; e < 4; ++e) l_run[rr] = sum2_16<false>(pb[rr][e], l_run[rr]);
