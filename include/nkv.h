@@ -925,7 +925,7 @@ int nkv_scaled_read(const nkv_scaled_read_args* args);
  * stride is a multiple of 2. Any GQA group up to 256. A sequence of length 0, or
  * none of whose blocks are valid, gives zeros; what a tile holds behind the
  * sequence's end has no effect. Sums of weights (bf16, up to 2^8) times values are
- * 32-bit floats until they are divided: 2^8 * keys * max |v| stays below 2^128, here
+ * 32-bit floats until they are divided: 2^8 * keys * max |v| must stay below 2^128, here
  * and in nkv_scaled_prefill.
  * No counterpart in the reference (beside nanokvllm/layers/attention.py:104-107).
  */
